@@ -58,6 +58,7 @@ enum NtB200DataType {
 #define NT_B200_ERR_NO_DEVICE 10004        /* no sm_100 device current */
 #define NT_B200_ERR_DEVICE_TIMEOUT 10005   /* a bounded device-side wait gave up */
 #define NT_B200_ERR_WORKSPACE_TOO_LARGE 10006 /* staging exceeds the library's fixed array */
+#define NT_B200_ERR_INDEX_OUT_OF_RANGE 10007 /* a kernel met a position, page or offset outside its array */
 
 /* Library identity and diagnostics. */
 int nt_b200_version(void);
@@ -289,6 +290,88 @@ int nt_b200_jagged_expand(void *values, const int64_t *offsets, int64_t batch, i
                           int64_t values_stride_ragged, int64_t values_stride_inner,
                           const void *src, int64_t src_stride_batch, int64_t src_stride_inner,
                           int dtype, void *stream);
+
+/*
+ * Serving operators: rotary positions, a paged cache of 8-bit keys and values,
+ * attention over it, and causal attention over packed prompts.  They have no
+ * counterpart among the reference's programs.  Each takes its arguments in one
+ * struct of 8-byte fields (sizes, strides and codes are int64; strides count
+ * elements).  Index arrays (positions, offsets, lengths, block tables) live on
+ * the device, all of one call in one dtype, INT32 or INT64 (`index_dtype`).
+ * The kernels check every index they read: one that leaves its array records
+ * NT_B200_ERR_INDEX_OUT_OF_RANGE in the device error word
+ * (nt_b200_device_status) and is not followed.
+ */
+
+/*
+ * Rotary positions of `input` [tokens, heads, head_dim]: the pairs (a, b) among
+ * the first `rotary_dim` elements of each head become (a cos - b sin, b cos +
+ * a sin), the rest is copied.  Half layout: a = x[i], b = x[i + rotary_dim/2];
+ * interleaved: a = x[2i], b = x[2i+1].  cos, sin: fp32 [table_rows,
+ * rotary_dim/2], unit column stride; token t uses row positions[t].  `adjoint`
+ * applies the transposed map (sin -> -sin): the gradient of the rotation.
+ * Products and sums are rounded to fp32 one by one and the result once to
+ * `dtype`.  `output` may be `input`.  A token whose position is outside the
+ * table gets NaN in its rotated part.  dtype: FLOAT16, BFLOAT16, FLOAT32.
+ */
+typedef struct NtB200RotaryArgs {
+    const void *input;
+    const float *cos, *sin;
+    const void *positions;
+    void *output;
+    int64_t tokens, heads, head_dim, rotary_dim, table_rows;
+    int64_t input_strides[3], output_strides[3]; /* token, head, element */
+    int64_t cos_stride, sin_stride, positions_stride;
+    int64_t interleaved, adjoint, dtype, index_dtype;
+} NtB200RotaryArgs;
+int nt_b200_rotary(const NtB200RotaryArgs *args, void *stream);
+
+/*
+ * A paged cache: `pages` pages of `page` tokens each (a multiple of 16), codes
+ * of `code_dtype` (FLOAT8_E4M3FN or INT8) in key and value [pages, kv_heads,
+ * page, head_dim] with unit element stride, head_dim a multiple of 16, every
+ * other stride and both bases multiples of 16; one fp32 scale for each page and
+ * head.  A stored element stands for code * scale.
+ */
+typedef struct NtB200PagedCache {
+    void *key, *value;
+    float *key_scale, *value_scale;
+    int64_t pages, kv_heads, page, head_dim, code_dtype;
+    int64_t key_strides[3], value_strides[3];             /* page, head, token */
+    int64_t key_scale_strides[2], value_scale_strides[2]; /* page, head */
+} NtB200PagedCache;
+
+/*
+ * Appends packed new tokens to a paged cache and rotates queries on the way.
+ * Sequence s (of `batch`) brings the tokens offsets[s] .. offsets[s+1] - 1 of
+ * key and value [tokens, kv_heads, head_dim] and already has past[s] tokens;
+ * its token past[s] + i goes to page block_table[s, (past[s] + i) / page], slot
+ * (past[s] + i) % page.  With tables (cos not null) keys are rotated as by
+ * nt_b200_rotary at those positions before they are stored, and, where given,
+ * `query` [tokens, heads, head_dim] is rotated into `query_out` and the rotated
+ * key stored in `key_out` in `dtype`.
+ *
+ * Scales.  With amax the largest finite magnitude among a page's new elements
+ * of a head: E4M3 codes: s = the least power of two, 2^-126 or more, with
+ * amax <= 448 s; INT8: s = max(amax * fp32(1 / 127), 2^-126).  A page whose first slots
+ * already hold tokens keeps max(its scale, s); where that grows, the held codes
+ * are rounded again by old / new (exact for E4M3 down to its subnormals).  code
+ * = round(x * (1 / s)) to nearest even, saturated; NaN becomes E4M3's NaN, INT8
+ * 0.  A page belongs to one sequence of the call: pages that several sequences
+ * share must be full.  dtype: FLOAT16, BFLOAT16, FLOAT32.
+ */
+typedef struct NtB200PagedAppendArgs {
+    NtB200PagedCache cache;
+    const void *key, *value, *query; /* query may be null */
+    const float *cos, *sin;          /* null: no rotation */
+    const void *offsets, *past, *block_table;
+    void *query_out, *key_out; /* key_out may be null */
+    int64_t tokens, batch, heads, rotary_dim, table_rows, table_columns;
+    int64_t key_strides[3], value_strides[3], query_strides[3], query_out_strides[3], key_out_strides[3];
+    int64_t cos_stride, sin_stride, offsets_stride, past_stride, block_table_strides[2];
+    int64_t interleaved, dtype, index_dtype;
+} NtB200PagedAppendArgs;
+int nt_b200_paged_append(const NtB200PagedAppendArgs *args, void *stream);
 
 /*
  * Failure-detection self-test (no counterpart in the reference): launches one

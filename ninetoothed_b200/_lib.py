@@ -11,6 +11,7 @@ with an error that says how to build it.
 """
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -42,6 +43,7 @@ ERROR_CODES = {
     10004: "NT_B200_ERR_NO_DEVICE",
     10005: "NT_B200_ERR_DEVICE_TIMEOUT",
     10006: "NT_B200_ERR_WORKSPACE_TOO_LARGE",
+    10007: "NT_B200_ERR_INDEX_OUT_OF_RANGE",
 }
 
 _P = ctypes.c_void_p
@@ -49,6 +51,7 @@ _I = ctypes.c_int64
 _C = ctypes.c_int
 _F = ctypes.c_float
 _PI64 = ctypes.POINTER(ctypes.c_int64)
+_S = ctypes.c_char_p  # a packed argument struct
 
 # Every exported entry point with its argument types (in declaration order of
 # include/nt_b200.h).
@@ -91,6 +94,9 @@ SIGNATURES = {
         ctypes.c_int,
         (_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _PI64, _PI64, _PI64, _C, _P),
     ),
+    # argument structs of 8-byte fields, packed by `pack_args`
+    "nt_b200_rotary": (ctypes.c_int, (_S, _P)),
+    "nt_b200_paged_append": (ctypes.c_int, (_S, _P)),
 }
 
 _lock = threading.Lock()
@@ -126,6 +132,12 @@ def int64_array(values):
     """A ctypes int64[] holding `values` (kept alive by the caller)."""
     values = tuple(int(v) for v in values)
     return (ctypes.c_int64 * len(values))(*values)
+
+
+def pack_args(*values):
+    """An argument struct of the C ABI: its 8-byte fields in declaration order
+    (pointers as addresses, None as null)."""
+    return struct.pack(f"={len(values)}q", *[0 if v is None else int(v) for v in values])
 
 
 def error_name(code: int) -> str:

@@ -9,6 +9,8 @@
 #include "pool.cuh"
 #include "copy.cuh"
 #include "contractions.cuh"
+#include "rotary.cuh"
+#include "paged_append.cuh"
 #include "conv_no_alloc.cu"
 
 namespace nt {
@@ -63,6 +65,7 @@ extern "C" const char *nt_b200_error_string(int code) {
     case NT_B200_ERR_NO_DEVICE: return "no sm_100 device";
     case NT_B200_ERR_DEVICE_TIMEOUT: return "a bounded device-side wait timed out";
     case NT_B200_ERR_WORKSPACE_TOO_LARGE: return "conv2d staging exceeds the library's fixed 64 MiB array";
+    case NT_B200_ERR_INDEX_OUT_OF_RANGE: return "an index outside its array met by a kernel";
     default: return cudaGetErrorString(static_cast<cudaError_t>(code));
   }
 }

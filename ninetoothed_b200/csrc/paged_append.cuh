@@ -1,0 +1,449 @@
+// Appending keys and values to a paged 8-bit cache, rotated on the way.
+//
+// A unit of work is one touched page of one sequence, one key/value head, and
+// one of key or value: the new tokens that fall into the page share its scale,
+// so a unit first takes the largest magnitude among them (after the rotation),
+// then settles the scale, rounds the codes the page already held again if the
+// scale grew, and writes the new codes.  No two units share a page and a head,
+// so nothing is atomic and the result does not depend on the order.
+//
+// Bound by memory: key and value are read once and written as a byte each.
+#pragma once
+
+#include "common.cuh"
+#include "rotary.cuh"
+
+namespace nt {
+namespace paged {
+
+// The scale of a block of elements whose largest finite magnitude is `amax`.
+// E4M3 takes a power of two: multiplying and dividing by it is exact, so a
+// block's codes survive a later growth of its scale; a step of INT8 is even,
+// and its scale spends none of the 127 steps.
+constexpr float kLeastScale = 1.1754943508222875e-38f;  // 2^-126
+template <typename C> __device__ __forceinline__ float block_scale(float amax);
+template <> __device__ __forceinline__ float block_scale<int8_t>(float amax) {
+  return fmaxf(__fmul_rn(amax, 1.f / 127.f), kLeastScale);
+}
+template <> __device__ __forceinline__ float block_scale<__nv_fp8_e4m3>(float amax) {
+  // 448 = 1.75 * 2^8: the least k with amax <= 448 * 2^k from amax's exponent
+  // and whether its significand passes 1.75.  Magnitudes under 2^-118 take
+  // the least scale.
+  const uint32_t bits = __float_as_uint(amax);
+  int k = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  if (k < -126) k = -126;
+  return __uint_as_float((uint32_t)(k + 127) << 23);
+}
+
+template <typename C> __device__ __forceinline__ uint8_t encode(float x);
+template <> __device__ __forceinline__ uint8_t encode<__nv_fp8_e4m3>(float x) {
+  return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+}
+template <> __device__ __forceinline__ uint8_t encode<int8_t>(float x) {
+  const int v = __float2int_rn(x);  // NaN converts to 0
+  return (uint8_t)(int8_t)max(-127, min(127, v));
+}
+template <typename C> __device__ __forceinline__ float decode(uint8_t code);
+template <> __device__ __forceinline__ float decode<__nv_fp8_e4m3>(uint8_t code) {
+  __nv_fp8_e4m3 v;
+  v.__x = code;
+  return static_cast<float>(v);
+}
+template <> __device__ __forceinline__ float decode<int8_t>(uint8_t code) { return (float)(int8_t)code; }
+
+// Codes of eight or four values, in memory order.
+template <typename C, int N> __device__ __forceinline__ void store_codes(uint8_t *to, const float (&x)[N], float inv) {
+  uint32_t w[N / 4];
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) {
+    w[i] = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[i] |= (uint32_t)encode<C>(__fmul_rn(x[4 * i + j], inv)) << (8 * j);
+  }
+  if constexpr (N == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t *>(to) = w[0];
+}
+
+__device__ __forceinline__ float finite_magnitude(float x) {
+  const float m = fabsf(x);
+  return m < INFINITY ? m : 0.f;  // NaN compares false
+}
+
+// The largest i in [0, n) with f(i) <= x, for a nondecreasing f with
+// f(0) <= x; all 32 lanes call it and narrow the range 32-fold a step.
+template <typename F> __device__ __forceinline__ int64_t warp_search(int64_t n, int64_t x, F f) {
+  const int lane = threadIdx.x & 31;
+  int64_t low = 0, length = n;
+  while (length > 1) {
+    const int64_t step = (length + 31) / 32, i = lane * step;
+    const bool le = i < length && f(low + i) <= x;
+    const int count = __popc(__ballot_sync(0xffffffffu, le));
+    const int64_t skip = (count > 0 ? count - 1 : 0) * step;
+    low += skip;
+    length = length - skip < step ? length - skip : step;
+  }
+  return low;
+}
+
+struct Side {  // key or value
+  const void *in;
+  uint8_t *codes;
+  float *scales;
+  void *out;  // rotated copy in the input type, or null
+  int64_t in_token, in_head, in_dim, page_stride, head_stride, token_stride, scale_page, scale_head;
+  int64_t out_token, out_head, out_dim;
+};
+
+struct Params {
+  Side side[2];
+  rotary::Params query;  // input null: no queries
+  rotary::Tables tables;
+  IndexArray offsets, past, block_table;
+  int64_t table_row_stride;
+  int64_t tokens, batch, pages, table_columns;
+  int64_t units;  // candidates a head and side: tokens / page + 2 * batch
+  int page, kv_heads, head_dim, chunk_pairs;
+  int unit_blocks;  // blockIdx.x below this: units; the rest: queries
+  int interleaved;
+};
+
+struct Unit {
+  int64_t token0;    // packed index of the first new token in the page
+  int64_t position0; // its position in the sequence
+  int64_t block;     // page in the pool
+  int count, slot0;  // new tokens, first new slot
+};
+
+// The u-th candidate.  Sequence s owns the candidates from offsets[s] / page +
+// 2 s on, at least one for each page it can touch; those past its last page
+// are empty.  All lanes of a warp ask for the same unit.
+__device__ __forceinline__ bool find_unit(const Params &p, int64_t u, Unit &w) {
+  const int64_t s =
+      warp_search(p.batch, u, [&](int64_t i) { return p.offsets[i] / p.page + 2 * i; });
+  const int64_t o0 = p.offsets[s], o1 = p.offsets[s + 1], past = p.past[s];
+  if (o1 <= o0) return false;
+  const int64_t j = u - (o0 / p.page + 2 * s);
+  const int64_t column = past / p.page + j;
+  const int64_t low = max(past, column * p.page), high = min(past + (o1 - o0), (column + 1) * p.page);
+  if (j < 0 || low >= high) return false;
+  if (o0 < 0 || o1 > p.tokens || past < 0 || column >= p.table_columns ||
+      (p.tables.pairs > 0 && high > p.tables.rows)) {
+    record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
+    return false;
+  }
+  w.block = p.block_table.wide
+                ? static_cast<const int64_t *>(p.block_table.data)[s * p.table_row_stride + column * p.block_table.stride]
+                : (int64_t) static_cast<const int32_t *>(
+                      p.block_table.data)[s * p.table_row_stride + column * p.block_table.stride];
+  if (w.block < 0 || w.block >= p.pages) {
+    record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
+    return false;
+  }
+  w.token0 = o0 + (low - past);
+  w.position0 = low;
+  w.count = (int)(high - low);
+  w.slot0 = (int)(low - column * p.page);
+  return true;
+}
+
+constexpr int THREADS = 128;
+
+__device__ __forceinline__ float block_max(float v, float *shared) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = shared[0];
+#pragma unroll
+  for (int i = 1; i < THREADS / 32; ++i) v = fmaxf(v, shared[i]);
+  return v;
+}
+
+// Settles the page's scale and rounds its held codes again where it grew.
+// `scale_at` may be read by every thread before the barrier that the caller
+// has passed; one thread writes it after.
+template <typename C>
+__device__ __forceinline__ float settle_scale(const Params &p, const Side &side, const Unit &w, int h, float amax,
+                                              float held) {
+  float scale = block_scale<C>(amax);
+  if (w.slot0 > 0 && held >= scale) return held;
+  if (w.slot0 > 0) {
+    const float ratio = __fdiv_rn(held, scale);
+    uint8_t *base = side.codes + w.block * side.page_stride + (int64_t)h * side.head_stride;
+    const int words = p.head_dim / 4;
+    for (int i = threadIdx.x; i < w.slot0 * words; i += THREADS) {
+      uint32_t *at = reinterpret_cast<uint32_t *>(base + (int64_t)(i / words) * side.token_stride) + i % words;
+      const uint32_t old = *at;
+      uint32_t moved = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        moved |= (uint32_t)encode<C>(__fmul_rn(decode<C>((uint8_t)(old >> (8 * j))), ratio)) << (8 * j);
+      *at = moved;
+    }
+  }
+  if (threadIdx.x == 0) side.scales[w.block * side.scale_page + (int64_t)h * side.scale_head] = scale;
+  return scale;
+}
+
+// Rotates a block's share of the queries.  Tokens of a block are near one
+// another: a warp searches for the first one's sequence and each thread goes on
+// from there.
+template <typename T, bool VEC>
+__device__ __forceinline__ void rotate_queries(const Params &p, int64_t block) {
+  const rotary::Params &q = p.query;
+  const int64_t per_token = VEC ? (int64_t)q.chunk_pairs * q.head_groups : (int64_t)q.heads;
+  const int64_t first = block * THREADS, i = first + threadIdx.x;
+  int64_t s = warp_search(p.batch, first / per_token, [&](int64_t k) { return p.offsets[k]; });
+  const int64_t token = i / per_token;
+  if (token >= p.tokens) return;
+  while (s + 1 < p.batch && p.offsets[s + 1] <= token) ++s;
+  const int64_t o0 = p.offsets[s];
+  if (token < o0 || token >= p.offsets[s + 1]) return;
+  const int64_t position = p.past[s] + (token - o0);
+  const int r = (int)(i % per_token);
+  if constexpr (VEC) {
+    rotary::rotate_heads<T>(q, token, position, (r / q.chunk_pairs) * rotary::HEADS, r % q.chunk_pairs);
+  } else {
+    const bool known = position >= 0 && position < p.tables.rows;
+    if (!known) record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
+    const T *in = static_cast<const T *>(q.input) + token * q.in_token + (int64_t)r * q.in_head;
+    T *out = static_cast<T *>(q.output) + token * q.out_token + (int64_t)r * q.out_head;
+    for (int e = 0; e < p.tables.pairs; ++e) {
+      const int64_t d0 = q.interleaved ? 2 * e : e, d1 = q.interleaved ? 2 * e + 1 : e + p.tables.pairs;
+      float a = to_f(in[d0 * q.in_dim]), b = to_f(in[d1 * q.in_dim]);
+      rotary::turn(a, b, known ? p.tables.cos[position * p.tables.cos_stride + e] : NAN,
+                   known ? p.tables.sin[position * p.tables.sin_stride + e] : NAN);
+      out[d0 * q.out_dim] = from_f<T>(a);
+      out[d1 * q.out_dim] = from_f<T>(b);
+    }
+    for (int64_t d = 2 * p.tables.pairs; d < q.head_dim; ++d) out[d * q.out_dim] = in[d * q.in_dim];
+  }
+}
+
+// One unit a block: blockIdx.x the candidate, blockIdx.y the head and side.
+template <typename T, typename C>
+__global__ void __launch_bounds__(THREADS) append_kernel(Params p) {
+  __shared__ float shared[THREADS / 32];
+  if ((int)blockIdx.x >= p.unit_blocks) {
+    if (blockIdx.y == 0) rotate_queries<T, true>(p, (int64_t)blockIdx.x - p.unit_blocks);
+    return;
+  }
+  constexpr int N = rotary::Chunk<T>::N;
+  Unit w;
+  if (!find_unit(p, blockIdx.x, w)) return;
+  const int h = (int)blockIdx.y >> 1;
+  const Side &side = p.side[blockIdx.y & 1];
+  const bool turns = p.tables.pairs > 0 && (blockIdx.y & 1) == 0;
+  const int items = w.count * p.chunk_pairs;
+  const float held = side.scales[w.block * side.scale_page + (int64_t)h * side.scale_head];
+  const T *in = static_cast<const T *>(side.in) + (int64_t)h * side.in_head;
+
+  auto load = [&](int i, rotary::Place<T> &at, float(&x)[N], float(&y)[N]) {
+    const int j = i / p.chunk_pairs;
+    at = rotary::place<T>(i % p.chunk_pairs, p.head_dim, turns ? p.tables.pairs : 0, p.interleaved != 0);
+    const T *row = in + (w.token0 + j) * side.in_token;
+    const rotary::Chunk<T> a = *reinterpret_cast<const rotary::Chunk<T> *>(row + at.first);
+    rotary::Chunk<T> b = {};
+    if (at.second >= 0) b = *reinterpret_cast<const rotary::Chunk<T> *>(row + at.second);
+#pragma unroll
+    for (int e = 0; e < N; ++e) { x[e] = to_f(a.v[e]); y[e] = to_f(b.v[e]); }
+    if (turns && at.pair >= 0) {
+      float c[N], s[N];
+      rotary::load_angles<T>(p.tables, w.position0 + j, at.pair, c, s);
+      rotary::turn_chunks<N>(x, y, c, s, p.interleaved != 0, p.tables.pairs - at.pair);
+    }
+  };
+
+  float amax = 0.f;
+  for (int i = threadIdx.x; i < items; i += THREADS) {
+    rotary::Place<T> at;
+    float x[N], y[N];
+    load(i, at, x, y);
+#pragma unroll
+    for (int e = 0; e < N; ++e) amax = fmaxf(amax, fmaxf(finite_magnitude(x[e]), finite_magnitude(y[e])));
+  }
+  const float scale = settle_scale<C>(p, side, w, h, block_max(amax, shared), held);
+  const float inv = __fdiv_rn(1.f, scale);
+  for (int i = threadIdx.x; i < items; i += THREADS) {
+    rotary::Place<T> at;
+    float x[N], y[N];
+    load(i, at, x, y);
+    const int j = i / p.chunk_pairs;
+    uint8_t *codes = side.codes + w.block * side.page_stride + (int64_t)h * side.head_stride +
+                     (int64_t)(w.slot0 + j) * side.token_stride;
+    store_codes<C, N>(codes + at.first, x, inv);
+    if (at.second >= 0) store_codes<C, N>(codes + at.second, y, inv);
+    if (side.out) {
+      T *out = static_cast<T *>(side.out) + (w.token0 + j) * side.out_token + (int64_t)h * side.out_head;
+      rotary::Chunk<T> a, b;
+#pragma unroll
+      for (int e = 0; e < N; ++e) { a.v[e] = from_f<T>(x[e]); b.v[e] = from_f<T>(y[e]); }
+      *reinterpret_cast<rotary::Chunk<T> *>(out + at.first) = a;
+      if (at.second >= 0) *reinterpret_cast<rotary::Chunk<T> *>(out + at.second) = b;
+    }
+  }
+}
+
+// Any strides of the new tokens and any rotary extent: an element or a pair a
+// thread.
+template <typename T, typename C>
+__global__ void __launch_bounds__(THREADS) append_scalar_kernel(Params p) {
+  __shared__ float shared[THREADS / 32];
+  if ((int)blockIdx.x >= p.unit_blocks) {
+    if (blockIdx.y == 0) rotate_queries<T, false>(p, (int64_t)blockIdx.x - p.unit_blocks);
+    return;
+  }
+  Unit w;
+  if (!find_unit(p, blockIdx.x, w)) return;
+  const int h = (int)blockIdx.y >> 1;
+  const Side &side = p.side[blockIdx.y & 1];
+  const int pairs = (blockIdx.y & 1) == 0 ? p.tables.pairs : 0;
+  const int per_token = p.head_dim - pairs;  // pairs, then single elements
+  const int items = w.count * per_token;
+  const float held = side.scales[w.block * side.scale_page + (int64_t)h * side.scale_head];
+  const T *in = static_cast<const T *>(side.in) + (int64_t)h * side.in_head;
+
+  auto load = [&](int i, int &d0, int &d1, float &a, float &b) {
+    const int j = i / per_token, e = i % per_token;
+    const T *row = in + (w.token0 + j) * side.in_token;
+    if (e < pairs) {
+      d0 = p.interleaved ? 2 * e : e;
+      d1 = p.interleaved ? 2 * e + 1 : e + pairs;
+      a = to_f(row[d0 * side.in_dim]);
+      b = to_f(row[d1 * side.in_dim]);
+      const int64_t position = w.position0 + j;
+      rotary::turn(a, b, p.tables.cos[position * p.tables.cos_stride + e], p.tables.sin[position * p.tables.sin_stride + e]);
+    } else {
+      d0 = e + pairs;
+      d1 = -1;
+      a = to_f(row[d0 * side.in_dim]);
+      b = 0.f;
+    }
+  };
+
+  float amax = 0.f;
+  for (int i = threadIdx.x; i < items; i += THREADS) {
+    int d0, d1;
+    float a, b;
+    load(i, d0, d1, a, b);
+    amax = fmaxf(amax, fmaxf(finite_magnitude(a), finite_magnitude(b)));
+  }
+  const float scale = settle_scale<C>(p, side, w, h, block_max(amax, shared), held);
+  const float inv = __fdiv_rn(1.f, scale);
+  for (int i = threadIdx.x; i < items; i += THREADS) {
+    int d0, d1;
+    float a, b;
+    load(i, d0, d1, a, b);
+    const int j = i / per_token;
+    uint8_t *codes = side.codes + w.block * side.page_stride + (int64_t)h * side.head_stride +
+                     (int64_t)(w.slot0 + j) * side.token_stride;
+    codes[d0] = encode<C>(__fmul_rn(a, inv));
+    if (d1 >= 0) codes[d1] = encode<C>(__fmul_rn(b, inv));
+    if (side.out) {
+      T *out = static_cast<T *>(side.out) + (w.token0 + j) * side.out_token + (int64_t)h * side.out_head;
+      out[d0 * side.out_dim] = from_f<T>(a);
+      if (d1 >= 0) out[d1 * side.out_dim] = from_f<T>(b);
+    }
+  }
+}
+
+template <typename T, typename C>
+int launch_append(Params p, cudaStream_t stream) {
+  constexpr int N = rotary::Chunk<T>::N;
+  const int64_t pairs = p.tables.pairs;
+  bool vec = pairs == 0 || rotary::vector_tables(p.tables);
+  for (int i = 0; i < 2; ++i) {
+    const Side &s = p.side[i];
+    const int64_t turned = i == 0 ? pairs : 0;
+    vec = vec && rotary::vector_heads<T>(s.in, s.in_token, s.in_head, s.in_dim, p.head_dim, turned, p.interleaved);
+    if (s.out)
+      vec = vec && rotary::vector_heads<T>(s.out, s.out_token, s.out_head, s.out_dim, p.head_dim, turned, p.interleaved);
+  }
+  rotary::Params &q = p.query;
+  if (q.input)
+    vec = vec && rotary::vector_heads<T>(q.input, q.in_token, q.in_head, q.in_dim, p.head_dim, pairs, p.interleaved) &&
+          rotary::vector_heads<T>(q.output, q.out_token, q.out_head, q.out_dim, p.head_dim, pairs, p.interleaved);
+  p.chunk_pairs = q.chunk_pairs = (p.head_dim + 2 * N - 1) / (2 * N);
+  q.head_groups = (q.heads + rotary::HEADS - 1) / rotary::HEADS;
+  const int64_t threads = q.input ? p.tokens * (vec ? (int64_t)q.chunk_pairs * q.head_groups : (int64_t)q.heads) : 0;
+  const int64_t blocks = p.units + (threads + THREADS - 1) / THREADS;
+  if (blocks > (1LL << 31) - 1 || p.kv_heads > 32767) return NT_B200_ERR_INVALID_ARGUMENT;
+  p.unit_blocks = (int)p.units;
+  const dim3 grid((unsigned)blocks, (unsigned)(p.kv_heads > 0 ? 2 * p.kv_heads : 1));
+  if (vec) append_kernel<T, C><<<grid, THREADS, 0, stream>>>(p);
+  else append_scalar_kernel<T, C><<<grid, THREADS, 0, stream>>>(p);
+  return launch_status();
+}
+
+// Host-side checks of a cache (no launch): 0 or an error code.
+inline int check_cache(const NtB200PagedCache &c) {
+  if (c.pages < 0 || c.kv_heads < 0 || c.page <= 0 || c.head_dim <= 0) return NT_B200_ERR_INVALID_ARGUMENT;
+  if (c.code_dtype != NT_B200_FLOAT8_E4M3FN && c.code_dtype != NT_B200_INT8) return NT_B200_ERR_UNSUPPORTED_DTYPE;
+  if (c.page % 16 != 0 || c.page > (1 << 16) || c.head_dim % 16 != 0 || c.head_dim > (1 << 12))
+    return NT_B200_ERR_SHAPE_MISMATCH;
+  if (!c.key || !c.value || !c.key_scale || !c.value_scale || !rotary::aligned16(c.key) || !rotary::aligned16(c.value))
+    return NT_B200_ERR_INVALID_ARGUMENT;
+  for (int i = 0; i < 3; ++i)
+    if (c.key_strides[i] % 16 != 0 || c.value_strides[i] % 16 != 0) return NT_B200_ERR_INVALID_ARGUMENT;
+  return 0;
+}
+
+}  // namespace paged
+}  // namespace nt
+
+extern "C" int nt_b200_paged_append(const NtB200PagedAppendArgs *a, void *stream) {
+  using namespace nt;
+  if (!a || a->tokens < 0 || a->batch < 0 || a->heads < 0 || a->rotary_dim < 0 || a->rotary_dim % 2 != 0 ||
+      a->table_rows < 0 || a->table_columns < 0)
+    return NT_B200_ERR_INVALID_ARGUMENT;
+  if (!is_float_dtype((int)a->dtype) || !is_index_dtype(a->index_dtype)) return NT_B200_ERR_UNSUPPORTED_DTYPE;
+  if (a->tokens == 0 || a->batch == 0) return 0;
+  const NtB200PagedCache &c = a->cache;
+  const int rc = paged::check_cache(c);
+  if (rc != 0) return rc;
+  const bool turns = a->cos != nullptr;
+  if (turns && (!a->sin || a->rotary_dim > c.head_dim)) return NT_B200_ERR_SHAPE_MISMATCH;
+  if (!a->key || !a->value || !a->offsets || !a->past || !a->block_table || (a->query && (!turns || !a->query_out)))
+    return NT_B200_ERR_INVALID_ARGUMENT;
+  if (c.kv_heads == 0 && !a->query) return 0;
+  paged::Params p{};
+  p.side[0] = {a->key, static_cast<uint8_t *>(c.key), c.key_scale, a->key_out,
+               a->key_strides[0], a->key_strides[1], a->key_strides[2],
+               c.key_strides[0], c.key_strides[1], c.key_strides[2], c.key_scale_strides[0], c.key_scale_strides[1],
+               a->key_out_strides[0], a->key_out_strides[1], a->key_out_strides[2]};
+  p.side[1] = {a->value, static_cast<uint8_t *>(c.value), c.value_scale, nullptr,
+               a->value_strides[0], a->value_strides[1], a->value_strides[2],
+               c.value_strides[0], c.value_strides[1], c.value_strides[2], c.value_scale_strides[0],
+               c.value_scale_strides[1], 0, 0, 0};
+  const int wide = a->index_dtype == NT_B200_INT64;
+  p.tables = {a->cos, a->sin, a->cos_stride, a->sin_stride, a->table_rows, turns ? (int)(a->rotary_dim / 2) : 0, 1.f};
+  p.offsets = {a->offsets, a->offsets_stride, wide};
+  p.past = {a->past, a->past_stride, wide};
+  p.block_table = {a->block_table, a->block_table_strides[1], wide};
+  p.table_row_stride = a->block_table_strides[0];
+  p.tokens = a->tokens;
+  p.batch = a->batch;
+  p.pages = c.pages;
+  p.table_columns = a->table_columns;
+  p.units = c.kv_heads > 0 ? a->tokens / c.page + 2 * a->batch : 0;
+  p.page = (int)c.page;
+  p.kv_heads = (int)c.kv_heads;
+  p.head_dim = (int)c.head_dim;
+  p.interleaved = a->interleaved != 0;
+  if (a->query && a->heads > 0) {
+    p.query.input = a->query;
+    p.query.output = a->query_out;
+    p.query.tables = p.tables;
+    p.query.in_token = a->query_strides[0]; p.query.in_head = a->query_strides[1]; p.query.in_dim = a->query_strides[2];
+    p.query.out_token = a->query_out_strides[0]; p.query.out_head = a->query_out_strides[1];
+    p.query.out_dim = a->query_out_strides[2];
+    p.query.heads = (int)a->heads;
+    p.query.head_dim = (int)c.head_dim;
+    p.query.interleaved = p.interleaved;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return NT_DISPATCH_FLOAT((int)a->dtype, [&] {
+    if (c.code_dtype == NT_B200_INT8) return paged::launch_append<scalar_t, int8_t>(p, s);
+    return paged::launch_append<scalar_t, __nv_fp8_e4m3>(p, s);
+  });
+}

@@ -548,6 +548,15 @@ def copy(dst, src):
     return jagged_expand_kernel(dst, src)
 
 
+# --------------------------------------------------------------------- serving operators
+from ninetoothed_b200.serving import (  # noqa: E402
+    paged_append,
+    paged_append_kernel,
+    rotary,
+    rotary_kernel,
+    rotary_tables,
+)
+
 __all__ = [
     "KernelLaunchError",
     "add",
@@ -572,9 +581,14 @@ __all__ = [
     "matmul_kernel",
     "max_pool2d",
     "max_pool2d_kernels",
+    "paged_append",
+    "paged_append_kernel",
     "pooled_extent",
     "pow",
     "pow_kernel",
+    "rotary",
+    "rotary_kernel",
+    "rotary_tables",
     "softmax",
     "softmax_host",
     "softmax_kernel",

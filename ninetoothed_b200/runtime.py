@@ -44,11 +44,13 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 @dataclass(frozen=True)
 class TensorArg:
-    """Contract of one tensor argument: its rank and the dtypes the kernel takes."""
+    """Contract of one tensor argument: its rank and the dtypes the kernel takes.
+    An optional argument may be None."""
 
     name: str
     ndim: int
     dtypes: tuple = FLOAT_DTYPES
+    optional: bool = False
 
 
 @dataclass(frozen=True)
@@ -118,6 +120,8 @@ class Kernel:
             if not isinstance(arg, TensorArg):
                 continue
             value = values[arg.name]
+            if value is None and arg.optional:
+                continue
             if not isinstance(value, torch.Tensor):
                 raise TypeError(f"Kernel argument `{arg.name}` must be a tensor.")
             if value.dim() != arg.ndim:

@@ -1,0 +1,368 @@
+"""Serving operators on the GPU against plain 64-bit implementations."""
+
+import math
+
+import pytest
+import torch
+
+from ninetoothed_b200 import device_status, programs
+
+pytestmark = pytest.mark.gpu
+
+HALF = {torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8, torch.float32: 2.0**-24}  # half a step, relative
+TINY = {torch.float16: 2.0**-25, torch.bfloat16: 0.0, torch.float32: 0.0}  # half a step among the subnormals
+INDEX_OUT_OF_RANGE = 10007
+
+
+def dev(x):
+    return x.to("cuda")
+
+
+def index(values, dtype=torch.int32):
+    return torch.tensor(values, dtype=dtype, device="cuda")
+
+
+# --------------------------------------------------------------------- rotary
+def turned(x, cos, sin, interleaved, adjoint=False):
+    """The rotation in 64 bits, pair by pair; x [T, H, D], cos and sin [T, R/2]."""
+    out = x.double().clone()
+    r = cos.shape[1]
+    for i in range(r):
+        i0, i1 = (2 * i, 2 * i + 1) if interleaved else (i, i + r)
+        a, b = x[..., i0].double(), x[..., i1].double()
+        c, s = cos[:, i, None].double(), sin[:, i, None].double() * (-1 if adjoint else 1)
+        out[..., i0], out[..., i1] = a * c - b * s, b * c + a * s
+    return out
+
+
+def rotation_error(x, r):
+    """What rounding products and sum to fp32 one by one can add: 2 steps of |a| + |b|."""
+    return 4 * 2.0**-24 * x.double().abs().amax() * torch.ones(())
+
+
+ROTARY_SHAPES = [
+    # tokens, heads, head_dim, rotary_dim
+    (1, 1, 2, 2),
+    (1, 1, 8, 0),
+    (3, 5, 64, 64),
+    (17, 40, 128, 128),
+    (33, 7, 128, 64),
+    (5, 3, 96, 32),
+    (9, 2, 80, 40),
+    (4, 6, 72, 36),
+    (7, 3, 30, 18),
+    (257, 1, 256, 128),
+]
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("interleaved", (False, True))
+@pytest.mark.parametrize("shape", ROTARY_SHAPES)
+def test_rotary(shape, interleaved, dtype):
+    t, h, d, r = shape
+    x = torch.randn(t, h, d).to(dtype)
+    cos, sin = programs.rotary_tables(300, max(r, 2), scaling="ntk" if r > 2 else None, factor=4.0)
+    cos, sin = cos[:, : r // 2].contiguous(), sin[:, : r // 2].contiguous()
+    positions = torch.randint(0, 300, (t,))
+    for adjoint in (False, True):
+        got = programs.rotary(dev(x), dev(cos), dev(sin), dev(positions), interleaved=interleaved, adjoint=adjoint)
+        want = turned(x, cos[positions], sin[positions], interleaved, adjoint)
+        limit = HALF[dtype] * want.abs() + TINY[dtype] + rotation_error(x, r)
+        assert got.dtype == dtype and got.shape == x.shape
+        assert ((got.cpu().double() - want).abs() <= limit).all()
+        assert torch.equal(got.cpu()[..., r:], x[..., r:])
+    assert device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", (torch.float16, torch.float32))
+def test_rotary_strides_and_int64_positions(dtype):
+    """Views of a fused projection, a head-major layout, an element stride, in place."""
+    qkv = torch.randn(21, 9, 64).to(dtype)
+    cos, sin = programs.rotary_tables(64, 64)
+    positions = torch.arange(21, dtype=torch.int64) * 3 % 64
+    want = turned(qkv, cos[positions], sin[positions], False)
+    limit = HALF[dtype] * want.abs() + TINY[dtype] + rotation_error(qkv, 64)
+    tables = dev(cos), dev(sin), dev(positions)
+    inputs = (
+        dev(qkv)[:, 2:7],
+        dev(qkv).transpose(0, 1).contiguous().transpose(0, 1)[:, 2:7],
+        torch.stack((dev(qkv), dev(qkv)), dim=-1)[:, 2:7, :, 0],
+    )
+    for x in inputs:
+        got = programs.rotary(x, *tables)
+        assert ((got.cpu().double() - want[:, 2:7]).abs() <= limit[:, 2:7]).all()
+    spread = torch.zeros(21, 5, 130, dtype=dtype, device="cuda")
+    programs.rotary_kernel(inputs[0], *tables, spread[:, :, 1:129:2])
+    assert torch.equal(spread[:, :, 1:129:2], programs.rotary(inputs[0], *tables))
+    assert not spread[:, :, 0::2].any()
+    whole = dev(qkv)
+    part = whole[:, 2:7]
+    programs.rotary_kernel(part, *tables, part)
+    assert torch.equal(part, programs.rotary(inputs[0], *tables))
+    assert torch.equal(whole[:, :2].cpu(), qkv[:, :2]) and torch.equal(whole[:, 7:].cpu(), qkv[:, 7:])
+
+
+def test_rotary_leaves_copied_elements_alone_when_not_finite():
+    x = torch.randn(2, 2, 64).half()
+    x[..., 8:] = math.inf
+    x[0, 0, 40] = math.nan
+    cos, sin = programs.rotary_tables(8, 8)
+    for interleaved in (False, True):
+        got = programs.rotary(dev(x), dev(cos), dev(sin), index([1, 2]), interleaved=interleaved).cpu()
+        assert torch.equal(got[..., 8:].nan_to_num(7.0), x[..., 8:].nan_to_num(7.0))
+        assert got[..., :8].isfinite().all()
+
+
+def test_rotary_gradient():
+    """The adjoint is the gradient: against the formula (the dot products agree)
+    and against differences of a linear map."""
+    t, h, d, r = 6, 2, 32, 24
+    cos, sin = programs.rotary_tables(16, r, scaling="by_parts", factor=8.0, original_length=16)
+    positions = torch.arange(t)
+    x, g = torch.randn(t, h, d), torch.randn(t, h, d)
+    tables = dev(cos), dev(sin), dev(positions)
+    for interleaved in (False, True):
+        dx = programs.rotary(dev(g), *tables, interleaved=interleaved, adjoint=True).cpu().double()
+        y = programs.rotary(dev(x), *tables, interleaved=interleaved).cpu().double()
+        left, right = (y * g.double()).sum(), (x.double() * dx).sum()
+        # each of the t h d products is off by at most a few steps of its factors
+        assert abs(left - right) <= 16 * 2.0**-24 * t * h * d * 16
+        for at in ((0, 0, 0), (3, 1, r - 1), (5, 0, d - 1), (2, 1, 7)):
+            step = torch.zeros(t, h, d)
+            step[at] = 1.0  # the map is linear: any step is exact up to rounding
+            up = programs.rotary(dev(x + step), *tables, interleaved=interleaved).cpu().double()
+            moved = ((x + step).double()[at] - x.double()[at])
+            assert abs(((up - y) * g.double()).sum() / moved - dx[at]) <= 16 * 2.0**-24 * 16 * 16
+
+
+def test_rotary_position_outside_the_table():
+    cos, sin = programs.rotary_tables(4, 16)
+    x = torch.randn(3, 2, 32).half()
+    got = programs.rotary(dev(x), dev(cos), dev(sin), index([0, 4, -1])).cpu()
+    assert device_status() == INDEX_OUT_OF_RANGE and device_status() == 0
+    assert torch.equal(got[0], programs.rotary(dev(x[:1]), dev(cos), dev(sin), index([0])).cpu()[0])
+    assert got[1:, :, :16].isnan().all() and torch.equal(got[1:, :, 16:], x[1:, :, 16:])
+
+
+# --------------------------------------------------------------------- append
+class Pages:
+    """A cache with shuffled pages and stale contents, and what it should hold, in 64 bits."""
+
+    def __init__(self, lens, page, kv_heads, dim, code, layout="heads"):
+        self.page, self.code = page, code
+        counts = [max(1, -(-n // page)) for n in lens]
+        total = sum(counts) + 2
+        order = torch.randperm(total)
+        self.table = torch.full((len(lens), max(counts) + 1), -1, dtype=torch.int64)
+        at = 0
+        for i, n in enumerate(counts):
+            self.table[i, :n] = order[at : at + n]
+            at += n
+        shape = (total, kv_heads, page, dim)
+        stale = torch.randint(-128, 128, shape, dtype=torch.int8)
+        self.caches = {}
+        for name in ("key", "value"):
+            if layout == "heads":
+                store = stale.cuda().clone()
+            else:  # token-major pages: [pages, page, heads, dim]
+                store = stale.cuda().transpose(1, 2).contiguous().transpose(1, 2)
+            self.caches[name] = store.view(code) if code == torch.int8 or layout == "heads" else (
+                store.transpose(1, 2).view(code).transpose(1, 2))
+        self.scales = {name: torch.full((total, kv_heads), 1e30, device="cuda") for name in ("key", "value")}
+
+    @property
+    def args(self):
+        return self.caches["key"], self.caches["value"], self.scales["key"], self.scales["value"]
+
+    def tokens(self, name, s, length):
+        """(codes, scales) of a sequence's first tokens: [length, H, D] and [length, H], in 64 bits."""
+        pages = self.table[s, : -(-length // self.page)]
+        codes = self.caches[name].cpu()[pages].double().transpose(1, 2).flatten(0, 1)[:length]
+        scales = self.scales[name].cpu()[pages].double().repeat_interleave(self.page, 0)[:length]
+        return codes, scales
+
+
+def least_scale(high, code):
+    """The scale of a block, in 64 bits, from its largest magnitude."""
+    if code == torch.int8:
+        return max(high / 127, 2.0**-126)
+    return 2.0 ** max(-126, math.ceil(math.log2(high / 448))) if high > 0 else 2.0**-126
+
+
+def code_error(x, scale, code):
+    """Half a step of a code that stands for x."""
+    if code == torch.int8:
+        return scale / 2
+    return (x.abs() * 2.0**-4).clamp(min=scale * 2.0**-10)
+
+
+APPENDS = [
+    # past, new, page, heads, kv_heads, dim, rotary
+    ([0], [1], 16, 4, 1, 64, 64),
+    ([15, 16, 17], [1, 1, 1], 16, 8, 2, 128, 128),
+    ([0, 5, 31, 32], [70, 0, 1, 33], 32, 6, 3, 64, 32),
+    ([63, 0, 100], [130, 64, 1], 64, 4, 4, 128, 64),
+    ([3, 0], [200, 129], 128, 2, 1, 96, 96),
+    ([1, 2, 3], [40, 3, 17], 48, 5, 5, 80, 20),
+    ([0] * 40, [1, 0, 2, 3] * 10, 16, 2, 2, 16, 16),
+]
+
+
+@pytest.mark.parametrize("code", (torch.float8_e4m3fn, torch.int8), ids=("e4m3", "int8"))
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("case", APPENDS, ids=range(len(APPENDS)))
+def test_paged_append(case, dtype, code):
+    past, new, page, heads, kv_heads, dim, rotary = case
+    interleaved = heads % 4 == 0
+    total = [p + n for p, n in zip(past, new)]
+    cache = Pages(total, page, kv_heads, dim, code, layout="heads" if dim != 96 else "tokens")
+    cos, sin = programs.rotary_tables(max(total), rotary)
+    held = [(torch.randn(p, kv_heads, dim), torch.randn(p, kv_heads, dim)) for p in past]
+    wide = torch.int64 if page == 64 else torch.int32
+    table = index(cache.table.tolist(), wide)
+
+    def offsets(lens):
+        return index([sum(lens[:i]) for i in range(len(lens) + 1)], wide)
+
+    def append(k, v, lens, before, **kwargs):
+        return programs.paged_append(dev(k), dev(v), offsets(lens), index(before, wide), table, *cache.args, **kwargs)
+
+    # what the sequences hold goes in unrotated, in a call of its own
+    append(torch.cat([k for k, _ in held]).to(dtype), torch.cat([v for _, v in held]).to(dtype), past, [0] * len(past))
+    before = {name: [cache.tokens(name, s, p) for s, p in enumerate(past)] for name in ("key", "value")}
+    stored = cache.caches["key"].view(torch.int8).cpu().clone() if cache.caches["key"].is_contiguous() else None
+    qkv = (torch.randn(sum(new), heads + 2 * kv_heads, dim) * 3).to(dtype)
+    query, key, value = qkv.split((heads, kv_heads, kv_heads), dim=1)
+    query_out, key_out = append(key, value, new, past, query=dev(qkv)[:, :heads], cos=dev(cos), sin=dev(sin),
+                                interleaved=interleaved, return_key=True)
+    assert device_status() == 0
+
+    position = torch.cat([torch.arange(p, p + n) for p, n in zip(past, new)])
+    slack = rotation_error(qkv, rotary)
+    for got, x in ((query_out, query), (key_out, key)):
+        want = turned(x, cos[position], sin[position], interleaved)
+        assert ((got.cpu().double() - want).abs() <= HALF[dtype] * want.abs() + TINY[dtype] + slack).all()
+    rows = {"key": turned(key, cos[position], sin[position], interleaved), "value": value.double()}
+    touched = set()
+    at = 0
+    for s, (p, n) in enumerate(zip(past, new)):
+        for name in ("key", "value"):
+            codes, scales = cache.tokens(name, s, p + n)
+            for j in range(p // page, -(-(p + n) // page)):
+                low, high = max(p, j * page), min(p + n, (j + 1) * page)
+                if low >= high:
+                    continue
+                touched.add(int(cache.table[s, j]))
+                x = rows[name][at + low - p : at + high - p]
+                for h in range(kv_heads):
+                    scale = least_scale(float(x[:, h].abs().max()), code)
+                    first = low > j * page
+                    old_codes, old_scales = before[name][s]
+                    if first:
+                        scale = max(scale, float(old_scales[low - 1, h]))
+                    got = float(scales[low, h])
+                    # int8: two roundings of the scale, and those of the largest magnitude
+                    assert abs(got - scale) <= (4 * 2.0**-24 * scale if code == torch.int8 else 0)
+                    off = (codes[low:high, h] * got - x[:, h]).abs()
+                    assert (off <= code_error(x[:, h], got, code) * (1 + 2.0**-20) + slack).all()
+                    if first:
+                        was = old_codes[j * page : low, h] * old_scales[j * page : low, h, None]
+                        now = codes[j * page : low, h] * got
+                        grew = got > float(old_scales[low - 1, h])
+                        limit = code_error(was, got, code) * (1 + 2.0**-20) if grew else 0 * was
+                        if code != torch.int8:  # a power of two: exact but for subnormals
+                            limit = torch.full_like(was, got * 2.0**-10) if grew else limit
+                        assert ((now - was).abs() <= limit).all()
+        at += n
+    if stored is not None:  # nothing else was written
+        rest = [b for b in range(stored.shape[0]) if b not in touched]
+        assert torch.equal(cache.caches["key"].view(torch.int8).cpu()[rest], stored[rest])
+
+
+@pytest.mark.parametrize("code", (torch.float8_e4m3fn, torch.int8), ids=("e4m3", "int8"))
+def test_paged_append_not_finite_zero_and_large(code):
+    """Infinities saturate and do not set the scale, NaN stays (int8: 0), zeros
+    take the least scale, and the largest values keep theirs."""
+    cache = Pages([4, 16, 2], 16, 1, 16, code)
+    key = torch.ones(22, 1, 16, dtype=torch.bfloat16)
+    key[0, 0, 0], key[1, 0, 1], key[2, 0, 2] = math.inf, -math.inf, math.nan
+    key[4:20] = 0
+    key[20:] = 3e38
+    programs.paged_append(dev(key), dev(key), index([0, 4, 20, 22]), index([0, 0, 0]), index(cache.table.tolist()),
+                          *cache.args)
+    top = 127.0 if code == torch.int8 else 448.0
+    for name in ("key", "value"):
+        codes, scales = cache.tokens(name, 0, 4)
+        assert scales[0, 0] == pytest.approx(least_scale(1.0, code), rel=1e-6)
+        assert codes[0, 0, 0] == top and codes[1, 0, 1] == -top
+        assert codes[2, 0, 2] == 0 if code == torch.int8 else codes[2, 0, 2].isnan()
+        assert ((codes[3] * scales[3, :, None] - 1).abs() <= 2.0**-7).all()
+        codes, scales = cache.tokens(name, 1, 16)
+        assert not codes.any() and (scales == 2.0**-126).all()
+        codes, scales = cache.tokens(name, 2, 2)
+        assert ((codes * scales[..., None] / float(key[20, 0, 0]) - 1).abs() <= 2.0**-4).all()
+    assert device_status() == 0
+
+
+def test_paged_append_bad_indices_are_not_followed():
+    cache = Pages([16, 16], 16, 1, 16, torch.int8)
+    before = cache.caches["key"].clone()
+    key = torch.randn(4, 1, 16).half().cuda()
+    good = cache.table[:, :1].tolist()
+    bad = [
+        ([0, 2, 4], [0, 0], [[-1], [99]]),  # pages outside the pool
+        ([0, 2, 4], [16, 40], good),  # positions past the block table
+        ([0, 2, 9], [0, 0], [[-1], good[1]]),  # tokens that are not there
+        ([0, 2, 4], [-3, -1], good),
+    ]
+    for offsets, past, table in bad:
+        table = [row if isinstance(row, list) else [row] for row in table]
+        programs.paged_append(key, key, index(offsets), index(past), index(table), *cache.args)
+        assert device_status() == INDEX_OUT_OF_RANGE
+        assert torch.equal(cache.caches["key"], before)
+
+
+def test_serving_refusals():
+    x = torch.zeros(4, 2, 32, dtype=torch.float16, device="cuda")
+    cos = torch.zeros(8, 16, device="cuda")
+    at = index([0, 1, 2, 3])
+    with pytest.raises(TypeError, match="rotary shapes"):
+        programs.rotary(x, cos, cos, at[:3])
+    with pytest.raises(TypeError, match="rotary tables"):
+        programs.rotary(x, cos, cos[:, :8], at)
+    with pytest.raises(TypeError, match="rotary tables"):
+        programs.rotary(x[..., :16], cos, cos, at)
+    with pytest.raises(TypeError, match="dtype"):
+        programs.rotary(x, cos.half(), cos.half(), at)
+    with pytest.raises(TypeError, match="dtype"):
+        programs.rotary(x, cos, cos, at.float())
+    with pytest.raises(TypeError, match="unit stride"):
+        programs.rotary(x, cos.repeat(1, 2)[:, ::2], cos.repeat(1, 2)[:, ::2], at)
+    with pytest.raises(TypeError, match="CUDA device"):
+        programs.rotary(x, cos.cpu(), cos, at)
+    codes = torch.zeros(4, 2, 16, 32, dtype=torch.int8, device="cuda")
+    scales = torch.zeros(4, 2, device="cuda")
+    good = dict(key=x, value=x, offsets=index([0, 4]), past=index([0]), block_table=index([[0]]), key_cache=codes,
+                value_cache=codes.clone(), key_scale=scales, value_scale=scales.clone())
+    programs.paged_append(**good)
+    for change, message in (
+        (dict(value=x[:3]), "disagree"),
+        (dict(key=x[:, :1], value=x[:, :1]), "disagree"),
+        (dict(value=x.float()), "share one dtype"),
+        (dict(past=index([0], torch.int64)), "share one dtype"),
+        (dict(offsets=index([0, 2, 4])), "offsets"),
+        (dict(key_scale=scales[:3]), "disagree"),
+        (dict(value_cache=codes[:3]), "disagree"),
+        (dict(key_cache=codes[:, :, :8], value_cache=codes[:, :, :8]), "multiples of 16"),
+        (dict(key_cache=codes.half(), value_cache=codes.half()), "dtype"),
+        (dict(query=x), "needs `cos`"),
+        (dict(cos=cos), "together"),
+    ):
+        with pytest.raises(TypeError, match=message):
+            programs.paged_append(**(good | change))
+    with pytest.raises(TypeError, match="unit stride"):
+        wide = torch.zeros(4, 2, 16, 64, dtype=torch.int8, device="cuda")[..., ::2]
+        programs.paged_append(**(good | dict(key_cache=wide, value_cache=wide)))
+    with pytest.raises(programs.KernelLaunchError):  # a base off the 16-byte grid
+        odd = torch.zeros(4 * 2 * 16 * 32 + 1, dtype=torch.int8, device="cuda")[1:].view(4, 2, 16, 32)
+        programs.paged_append(**(good | dict(key_cache=odd)))
