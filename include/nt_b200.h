@@ -374,6 +374,35 @@ typedef struct NtB200PagedAppendArgs {
 int nt_b200_paged_append(const NtB200PagedAppendArgs *args, void *stream);
 
 /*
+ * Attention of each sequence's last `queries` tokens over a paged cache that
+ * holds them already: query i of `query` [batch, queries, heads, head_dim] sees
+ * the first lengths[b] - queries + 1 + i tokens of sequence b; query head h
+ * reads key/value head h / (heads / kv_heads).  With s = scale * (q . k) over
+ * those tokens, output = softmax(s) v and, where `lse` is not null, lse [batch,
+ * queries, heads] = ln sum exp(s) (fp32); a query that sees nothing gets 0 and
+ * -inf.  Scores, softmax and sums are fp32; the scales must not be negative.
+ * FLOAT16 and BFLOAT16 queries of head_dim up to 128 run on tensor cores
+ * (probabilities rounded to fp16 there), FLOAT32 ones and head_dim up to 256 on
+ * CUDA cores.  `scale` is a double.  `workspace`: 16-byte aligned device memory
+ * of nt_b200_paged_attention_workspace_size() bytes (the current device's), for
+ * this call alone.
+ */
+typedef struct NtB200PagedAttentionArgs {
+    NtB200PagedCache cache;
+    const void *query, *lengths, *block_table;
+    void *output;
+    float *lse;
+    void *workspace;
+    int64_t workspace_bytes, batch, queries, heads, table_columns;
+    int64_t query_strides[4], output_strides[4], lse_strides[3]; /* batch, query, head, element */
+    int64_t lengths_stride, block_table_strides[2];
+    int64_t dtype, index_dtype;
+    double scale;
+} NtB200PagedAttentionArgs;
+int nt_b200_paged_attention(const NtB200PagedAttentionArgs *args, void *stream);
+int64_t nt_b200_paged_attention_workspace_size(void);
+
+/*
  * Failure-detection self-test (no counterpart in the reference): launches one
  * thread that waits on an mbarrier nothing ever arrives on, through the same
  * bounded wait the pipelined kernels use, with a limit of `limit_ns`

@@ -97,6 +97,8 @@ SIGNATURES = {
     # argument structs of 8-byte fields, packed by `pack_args`
     "nt_b200_rotary": (ctypes.c_int, (_S, _P)),
     "nt_b200_paged_append": (ctypes.c_int, (_S, _P)),
+    "nt_b200_paged_attention": (ctypes.c_int, (_S, _P)),
+    "nt_b200_paged_attention_workspace_size": (ctypes.c_int64, ()),
 }
 
 _lock = threading.Lock()
@@ -134,10 +136,11 @@ def int64_array(values):
     return (ctypes.c_int64 * len(values))(*values)
 
 
-def pack_args(*values):
+def pack_args(*values, scale=None):
     """An argument struct of the C ABI: its 8-byte fields in declaration order
-    (pointers as addresses, None as null)."""
-    return struct.pack(f"={len(values)}q", *[0 if v is None else int(v) for v in values])
+    (pointers as addresses), and the double that ends it where it has one."""
+    packed = struct.pack(f"={len(values)}q", *values)
+    return packed if scale is None else packed + struct.pack("=d", scale)
 
 
 def error_name(code: int) -> str:

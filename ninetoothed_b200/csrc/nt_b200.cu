@@ -11,6 +11,7 @@
 #include "contractions.cuh"
 #include "rotary.cuh"
 #include "paged_append.cuh"
+#include "paged_attention.cuh"
 #include "conv_no_alloc.cu"
 
 namespace nt {

@@ -552,6 +552,8 @@ def copy(dst, src):
 from ninetoothed_b200.serving import (  # noqa: E402
     paged_append,
     paged_append_kernel,
+    paged_attention,
+    paged_attention_kernel,
     rotary,
     rotary_kernel,
     rotary_tables,
@@ -583,6 +585,8 @@ __all__ = [
     "max_pool2d_kernels",
     "paged_append",
     "paged_append_kernel",
+    "paged_attention",
+    "paged_attention_kernel",
     "pooled_extent",
     "pow",
     "pow_kernel",

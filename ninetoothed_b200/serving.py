@@ -246,11 +246,85 @@ def paged_append(key, value, offsets, past, block_table, key_cache, value_cache,
     return query_out, key_out
 
 
+# --------------------------------------------------------------------- attention over the cache
+def _launch_paged_attention(v, stream):
+    query, out, lse, lengths, table = v["query"], v["output"], v["lse"], v["lengths"], v["block_table"]
+    check_same_dtype(v, ("query", "output"))
+    check_same_dtype(v, ("lengths", "block_table"))
+    cache = _cache_args(v)
+    batch, queries, heads, dim = query.shape
+    _, kv_heads, _, cache_dim = v["key_cache"].shape
+    if out.shape != query.shape or dim != cache_dim or not kv_heads or heads % kv_heads:
+        raise TypeError(
+            f"paged_attention query {tuple(query.shape)}, cache {tuple(v['key_cache'].shape)} and output "
+            f"{tuple(out.shape)} disagree."
+        )
+    if dim > 256:
+        raise TypeError("Kernel argument `query` has head dimension above the upper bound 256.")
+    if lengths.shape[0] != batch or table.shape[0] != batch:
+        raise TypeError(f"paged_attention needs {batch} lengths and block table rows.")
+    if lse is not None and lse.shape != query.shape[:3]:
+        raise TypeError("paged_attention lse must have the query's shape without the head dimension.")
+    lib = _lib.library()
+    nbytes = lib.nt_b200_paged_attention_workspace_size()
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
+    args = _lib.pack_args(
+        *cache, query.data_ptr(), lengths.data_ptr(), table.data_ptr(), out.data_ptr(),
+        0 if lse is None else lse.data_ptr(), workspace.data_ptr(), nbytes, batch, queries, heads, table.shape[1],
+        *query.stride(), *out.stride(), *((0, 0, 0) if lse is None else lse.stride()), lengths.stride(0),
+        *table.stride(), dtype_code(query.dtype), dtype_code(lengths.dtype), scale=_scale(v["scale"], dim),
+    )
+    return lib.nt_b200_paged_attention(args, stream)
+
+
+def _scale(scale, dim):
+    return dim**-0.5 if scale is None else float(scale)
+
+
+paged_attention_kernel = Kernel(
+    name="paged_attention",
+    args=(
+        TensorArg("query", 4),
+        *_CACHE_ARGS,
+        TensorArg("block_table", 2, INDEX_DTYPES),
+        TensorArg("lengths", 1, INDEX_DTYPES),
+        TensorArg("output", 4),
+        TensorArg("lse", 3, _F32, optional=True),
+    ),
+    outputs=("output",),
+    launch=_launch_paged_attention,
+    meta=("scale",),
+    meta_defaults={"scale": None, "lse": None},
+)
+
+
+def paged_attention(query, key_cache, value_cache, key_scale, value_scale, block_table, lengths, scale=None,
+                    return_lse=False):
+    """Attention of each sequence's newest tokens over the paged 8-bit cache that
+    holds them (`paged_append`).
+
+    `query` [batch, queries, heads, head_dim]: query i of sequence b sees its
+    first lengths[b] - queries + 1 + i tokens (one query: all of them; several,
+    such as drafted tokens: each up to itself).  Query head h reads key/value
+    head h // (heads // kv_heads).  `scale` is 1 / sqrt(head_dim) by default.
+    Returns the output, in the query's shape and dtype, or with `return_lse`
+    (output, lse): the fp32 natural logarithm of each query's sum of exponentials
+    [batch, queries, heads], by which attention over separate keys is joined.  A
+    query that sees no token gets 0, and -inf as its lse."""
+    output = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    lse = torch.empty(query.shape[:3], dtype=torch.float32, device=query.device) if return_lse else None
+    paged_attention_kernel(query, key_cache, value_cache, key_scale, value_scale, block_table, lengths, output, lse,
+                           scale=scale)
+    return (output, lse) if return_lse else output
+
+
 __all__ = [
     "CODE_DTYPES",
     "INDEX_DTYPES",
     "paged_append",
     "paged_append_kernel",
+    "paged_attention",
+    "paged_attention_kernel",
     "rotary",
     "rotary_kernel",
     "rotary_tables",

@@ -35,7 +35,7 @@ def packed(struct, **values):
         value = values.pop(field, 0)
         out += list(value) if count > 1 and value else [value] * count
     assert not values, values
-    return _lib.pack_args(*out)
+    return _lib.pack_args(*out)  # a double 0.0 is eight zero bytes too
 
 
 def test_rotary_tables():
@@ -84,6 +84,18 @@ def test_rotary_tables_refusals(bad):
             ({"cache.page": 0}, 10001), (dict(tokens=0), 0), (dict(batch=0), 0),
             (dict(), 10001),  # null pointers
             ({"cache.key": 16, "cache.value": 24, "cache.key_scale": 16, "cache.value_scale": 16}, 10001),  # off the grid
+        ],
+    ),
+    (
+        "NtB200PagedAttentionArgs", "nt_b200_paged_attention",
+        {"batch": 1, "queries": 1, "heads": 4, "dtype": 9, "index_dtype": 3, "cache.pages": 4, "cache.kv_heads": 2,
+         "cache.page": 16, "cache.head_dim": 64, "cache.code_dtype": 12, "cache.key": 16, "cache.value": 16,
+         "cache.key_scale": 16, "cache.value_scale": 16},
+        [
+            (dict(queries=-1), 10001), (dict(dtype=12), 10002), (dict(index_dtype=8), 10002),
+            ({"cache.code_dtype": 9}, 10002), ({"cache.page": 17}, 10003), ({"cache.head_dim": 272}, 10003),
+            ({"heads": 3}, 10003), ({"cache.kv_heads": 0}, 10003), (dict(batch=0), 0), (dict(heads=0), 0),
+            (dict(), 10001),  # null pointers
         ],
     ),
 ])

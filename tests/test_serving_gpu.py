@@ -322,6 +322,184 @@ def test_paged_append_bad_indices_are_not_followed():
         assert torch.equal(cache.caches["key"], before)
 
 
+# --------------------------------------------------------------------- attention over the cache
+def softmax_rows(q, k, v, scale, limit):
+    """o and lse of one query row over the first `limit` keys, in 64 bits."""
+    if limit <= 0:
+        return torch.zeros(v.shape[-1], dtype=torch.float64), -math.inf
+    s = (k[:limit] @ q) * scale
+    lse = torch.logsumexp(s, 0)
+    return torch.exp(s - lse) @ v[:limit], float(lse)
+
+
+def filled_cache(lens, page, kv_heads, dim, code, spread=1.0):
+    """A cache of random codes with a scale for each page and head; unused slots and pages stay stale."""
+    cache = Pages(lens, page, kv_heads, dim, code, layout="heads" if dim != 96 else "tokens")
+    used = sorted({int(cache.table[s, j]) for s, n in enumerate(lens) for j in range(-(-n // page))})
+    for name in ("key", "value"):
+        top = 127 if code == torch.int8 else 448
+        if used:
+            codes = (torch.randn(len(used), kv_heads, page, dim) * top / 6).clamp(-top, top)
+            codes = codes.round().to(torch.int8) if code == torch.int8 else codes.to(code)
+            view = cache.caches[name].view(torch.int8) if cache.caches[name].is_contiguous() else None
+            if view is not None:
+                view[used] = codes.view(torch.int8).cuda()
+            else:
+                cache.caches[name].transpose(1, 2).view(torch.int8)[used] = codes.transpose(1, 2).contiguous().view(
+                    torch.int8).cuda()
+            scales = 6 / top * torch.exp2(spread * (2 * torch.rand(len(used), kv_heads) - 1))
+            cache.scales[name][used] = scales.cuda()
+    for s, n in enumerate(lens):  # stale NaN codes and scales after the last token
+        if n % page and code != torch.int8:
+            block = cache.table[s, n // page]
+            for name in ("key", "value"):
+                if cache.caches[name].is_contiguous():
+                    cache.caches[name].view(torch.int8)[block, :, n % page :] = 127
+    return cache
+
+
+def check_paged(query, cache, lens, scale, got, lse, dtype):
+    batch, queries, heads, dim = query.shape
+    kv_heads = cache.caches["key"].shape[1]
+    got, lse = got.cpu().double(), lse.cpu().double()
+    for b, n in enumerate(lens):
+        k, v = ((codes * scales[..., None]) for codes, scales in (cache.tokens(name, b, n) for name in ("key", "value")))
+        for i in range(queries):
+            for h in range(heads):
+                g = h // (heads // kv_heads)
+                want, want_lse = softmax_rows(query[b, i, h].double(), k[:, g], v[:, g], scale, n - queries + 1 + i)
+                if want_lse == -math.inf:
+                    assert lse[b, i, h] == -math.inf and not got[b, i, h].any()
+                    continue
+                # scores: fp32 sums of dim products of exact factors, times a factor of a few roundings
+                product = float((k[:, g].abs() @ query[b, i, h].double().abs()).max()) * scale
+                score = (dim + 8) * 2.0**-24 * product
+                assert abs(lse[b, i, h] - want_lse) <= 2 * score + 2.0**-20 * (1 + abs(want_lse))
+                # each weight: the score's error, and half a step of fp16 (half precision inputs)
+                top = float(v[:, g].abs().max())
+                weight = 2 * score + (2.0**-11 if dtype != torch.float32 else 0) + 2.0**-20
+                limit = HALF[dtype] * want.abs() + TINY[dtype] + weight * top
+                assert ((got[b, i, h] - want).abs() <= limit).all(), (b, i, h)
+
+
+PAGED = [
+    # lens, queries, page, heads, kv_heads, dim
+    ([1], 1, 16, 1, 1, 16),
+    ([17, 0, 300], 1, 16, 8, 2, 128),
+    ([257, 1, 64, 1000], 1, 64, 8, 1, 64),
+    ([5, 2, 0, 700], 4, 32, 4, 2, 128),
+    ([513, 3], 7, 48, 6, 2, 96),
+    ([1300, 12], 5, 128, 20, 4, 80),
+    ([40] * 33 + [777, 1200], 1, 16, 3, 3, 112),
+    ([31, 33], 40, 16, 2, 1, 48),
+]
+
+
+@pytest.mark.parametrize("code", (torch.float8_e4m3fn, torch.int8), ids=("e4m3", "int8"))
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("case", PAGED, ids=range(len(PAGED)))
+def test_paged_attention(case, dtype, code):
+    lens, queries, page, heads, kv_heads, dim = case
+    cache = filled_cache(lens, page, kv_heads, dim, code, spread=4.0)
+    query = (torch.randn(len(lens), queries, heads, dim) * 2).to(dtype)
+    wide = torch.int64 if page == 64 else torch.int32
+    scale = 0.7 * dim**-0.5
+    got, lse = programs.paged_attention(dev(query), *cache.args, index(cache.table.tolist(), wide), index(lens, wide),
+                                        scale=scale, return_lse=True)
+    assert device_status() == 0 and got.dtype == dtype
+    check_paged(query, cache, lens, scale, got, lse, dtype)
+    again = programs.paged_attention(dev(query), *cache.args, index(cache.table.tolist(), wide), index(lens, wide), scale)
+    assert torch.equal(again, got)
+
+
+def test_paged_attention_strided_queries_and_output():
+    lens, page, heads, kv_heads, dim = [100, 700], 32, 6, 3, 64
+    cache = filled_cache(lens, page, kv_heads, dim, torch.int8)
+    qkv = torch.randn(2, 1, heads + 2 * kv_heads, 2 * dim).half()
+    spread = torch.zeros(heads, 2, 1, dim + 5, dtype=torch.float16, device="cuda")
+    lse = torch.zeros(heads, 2, 1, device="cuda").permute(1, 2, 0)
+    out = spread.permute(1, 2, 0, 3)[..., 5:]
+    programs.paged_attention_kernel(dev(qkv)[:, :, :heads, ::2], *cache.args, index(cache.table.tolist()), index(lens),
+                                    out, lse)
+    check_paged(qkv[:, :, :heads, ::2], cache, lens, dim**-0.5, out, lse, torch.float16)
+    assert not spread[..., :5].any()
+    part = programs.paged_attention(dev(qkv)[:, :, 2:4, ::2], *(x[:, 1:2] for x in cache.args),
+                                    index(cache.table.tolist()), index(lens))
+    # the heads of one group over a slice of the cache
+    assert torch.allclose(part, out[:, :, 2:4], rtol=2.0**-9, atol=2.0**-9)
+
+
+def test_paged_attention_scales_far_apart():
+    """Weights value_scale * p from blocks of very different scales keep their bits."""
+    lens, page, dim = [640], 16, 64
+    cache = filled_cache(lens, page, 1, dim, torch.float8_e4m3fn, spread=14.0)
+    query = torch.randn(1, 1, 4, dim).bfloat16()
+    cache.scales["key"].fill_(0.02)
+    got, lse = programs.paged_attention(dev(query), *cache.args, index(cache.table.tolist()), index(lens), return_lse=True)
+    check_paged(query, cache, lens, dim**-0.5, got, lse, torch.bfloat16)
+    # a block of zeros with the least scale beside the others, and one of scale 0
+    block = int(cache.table[0, 3])
+    cache.caches["value"].view(torch.int8)[block] = 0
+    cache.scales["value"][block] = 2.0**-126
+    cache.scales["value"][int(cache.table[0, 5])] = 0
+    got, lse = programs.paged_attention(dev(query), *cache.args, index(cache.table.tolist()), index(lens), return_lse=True)
+    check_paged(query, cache, lens, dim**-0.5, got, lse, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", (torch.float16, torch.float32))
+def test_paged_attention_nan_reaches_only_who_sees_it(dtype):
+    lens, queries, dim = [70], 4, 128
+    for heads in (2, 4):
+        cache = filled_cache(lens, 16, 2, dim, torch.float8_e4m3fn)
+        query = torch.randn(1, queries, heads, dim).to(dtype)
+        args = index(cache.table.tolist()), index(lens)
+        clean = programs.paged_attention(dev(query), *cache.args, *args)
+        at = int(cache.table[0, 68 // 16])
+        cache.caches["value"].view(torch.int8)[at, 0, 68 % 16, 5] = 127
+        got = programs.paged_attention(dev(query), *cache.args, *args)
+        bad = got.isnan()
+        group = slice(0, heads // 2)
+        assert bad[:, 2:, group, 5].all() and bad.sum() == 2 * (heads // 2)
+        assert torch.equal(got.nan_to_num(0.0), clean.masked_fill(bad, 0.0))
+
+
+def test_paged_attention_long_and_lengths_out_of_range():
+    cache = filled_cache([5000], 32, 1, 64, torch.int8)
+    query = torch.randn(1, 1, 8, 64).half()
+    table = index(cache.table.tolist())
+    got, lse = programs.paged_attention(dev(query), *cache.args, table, index([5000]), return_lse=True)
+    check_paged(query, cache, [5000], 64**-0.5, got, lse, torch.float16)
+    whole = table[:, :-1]  # 157 pages: 5024 tokens
+    programs.paged_attention(dev(query), *cache.args, whole, index([5025]))
+    assert device_status() == INDEX_OUT_OF_RANGE
+    out = programs.paged_attention(dev(query), *cache.args, whole, index([-1]))
+    assert device_status() == INDEX_OUT_OF_RANGE and not out.any()
+    programs.paged_attention(dev(query), *cache.args, table, index([5056]))  # the last column is page -1
+    assert device_status() == INDEX_OUT_OF_RANGE
+
+
+def test_paged_attention_offsets_past_32_bits():
+    """Pages whose byte offset needs more than 32 bits."""
+    pages, page, dim = 34000, 64, 128
+    cache = torch.zeros(pages, 16, page, dim, dtype=torch.int8, device="cuda")
+    value = torch.zeros(pages, 1, page, dim, dtype=torch.int8, device="cuda")
+    assert cache.numel() > 2**32
+    scales = torch.ones(pages, 16, device="cuda")
+    last = pages - 1
+    value[last, 0, :, :] = 3
+    cache[last, 15, 0, 0] = 100
+    query = torch.zeros(1, 1, 1, dim, dtype=torch.float16, device="cuda")
+    query[..., 0] = 1
+    got, lse = programs.paged_attention(query, cache[:, 15:], value, scales[:, :1], scales[:, :1], index([[0, last]]),
+                                        index([128]), scale=1.0, return_lse=True)
+    assert torch.allclose(got.float(), torch.full_like(got.float(), 3.0), rtol=2.0**-10)
+    assert abs(float(lse) - 100.0) < 1e-4
+    key = torch.full((1, 1, dim), 2.0, dtype=torch.float16, device="cuda")
+    programs.paged_append(key, key, index([0, 1]), index([127]), index([[0, last]]), cache[:, 15:], value,
+                          scales[:, :1], scales[:, 1:2])
+    assert int(cache[last, 15, 63].float().mean()) == 2 and not cache[0].any()
+
+
 def test_serving_refusals():
     x = torch.zeros(4, 2, 32, dtype=torch.float16, device="cuda")
     cos = torch.zeros(8, 16, device="cuda")
@@ -360,6 +538,20 @@ def test_serving_refusals():
     ):
         with pytest.raises(TypeError, match=message):
             programs.paged_append(**(good | change))
+    query = torch.zeros(1, 1, 4, 32, dtype=torch.float16, device="cuda")
+    fine = dict(query=query, lengths=index([0]), **{name: good[name] for name in (
+        "key_cache", "value_cache", "key_scale", "value_scale", "block_table")})
+    assert not programs.paged_attention(**fine).any()
+    for change, message in (
+        (dict(query=query[..., :16]), "disagree"),
+        (dict(query=query[:, :, :3]), "disagree"),
+        (dict(lengths=index([0, 0])), "lengths"),
+        (dict(lengths=index([0], torch.int64)), "share one dtype"),
+        (dict(query=query.double()), "dtype"),
+        (dict(key_scale=scales.half()), "dtype"),
+    ):
+        with pytest.raises(TypeError, match=message):
+            programs.paged_attention(**(fine | change))
     with pytest.raises(TypeError, match="unit stride"):
         wide = torch.zeros(4, 2, 16, 64, dtype=torch.int8, device="cuda")[..., ::2]
         programs.paged_append(**(good | dict(key_cache=wide, value_cache=wide)))
