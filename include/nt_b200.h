@@ -403,6 +403,37 @@ int nt_b200_paged_attention(const NtB200PagedAttentionArgs *args, void *stream);
 int64_t nt_b200_paged_attention_workspace_size(void);
 
 /*
+ * Attention over whole prompts packed one after another: sequence b has the
+ * queries query_offsets[b] .. query_offsets[b+1] - 1 of `query` [query_tokens,
+ * heads, head_dim] and the keys key_offsets[b] .. key_offsets[b+1] - 1 of `key`
+ * and `value` [key_tokens, kv_heads, head_dim]; query head h reads key/value
+ * head h / (heads / kv_heads).  The last query stands at the last key: with
+ * `is_causal`, query i of nq sees the first nk - nq + 1 + i of nk keys.  With s
+ * = scale * (q . k), output = softmax(s) v and, where `lse` is not null, lse
+ * [query_tokens, heads] = ln sum exp(s) (fp32); a query that sees nothing gets 0
+ * and -inf.  Scores, softmax and sums are fp32.  FLOAT16 and BFLOAT16 run on
+ * tcgen05 tensor cores (probabilities rounded to the input type there) for
+ * head_dim up to 128, unit element strides, other strides and bases on the
+ * 16-byte grid and a positive scale; the rest, FLOAT32 and head_dim up to 256,
+ * on CUDA cores.  Tokens that belong to no sequence are not written.
+ * `workspace`: 32-byte aligned device memory of
+ * nt_b200_prompt_attention_workspace_size(...) bytes, for this call alone.
+ */
+typedef struct NtB200PromptAttentionArgs {
+    const void *query, *key, *value, *query_offsets, *key_offsets;
+    void *output;
+    float *lse;
+    void *workspace;
+    int64_t workspace_bytes, query_tokens, key_tokens, batch, heads, kv_heads, head_dim;
+    int64_t query_strides[3], key_strides[3], value_strides[3], output_strides[3]; /* token, head, element */
+    int64_t lse_strides[2], query_offsets_stride, key_offsets_stride;
+    int64_t is_causal, dtype, index_dtype;
+    double scale;
+} NtB200PromptAttentionArgs;
+int nt_b200_prompt_attention(const NtB200PromptAttentionArgs *args, void *stream);
+int64_t nt_b200_prompt_attention_workspace_size(int64_t query_tokens, int64_t batch, int64_t heads, int64_t kv_heads);
+
+/*
  * Failure-detection self-test (no counterpart in the reference): launches one
  * thread that waits on an mbarrier nothing ever arrives on, through the same
  * bounded wait the pipelined kernels use, with a limit of `limit_ns`

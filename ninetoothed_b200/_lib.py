@@ -99,6 +99,8 @@ SIGNATURES = {
     "nt_b200_paged_append": (ctypes.c_int, (_S, _P)),
     "nt_b200_paged_attention": (ctypes.c_int, (_S, _P)),
     "nt_b200_paged_attention_workspace_size": (ctypes.c_int64, ()),
+    "nt_b200_prompt_attention": (ctypes.c_int, (_S, _P)),
+    "nt_b200_prompt_attention_workspace_size": (ctypes.c_int64, (_I, _I, _I, _I)),
 }
 
 _lock = threading.Lock()

@@ -12,6 +12,7 @@
 #include "rotary.cuh"
 #include "paged_append.cuh"
 #include "paged_attention.cuh"
+#include "prompt_attention.cuh"
 #include "conv_no_alloc.cu"
 
 namespace nt {

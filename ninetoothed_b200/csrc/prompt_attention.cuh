@@ -1,0 +1,723 @@
+// Attention over whole prompts packed one after another, grouped heads, causal
+// or not:
+//     s = scale * (q . k),  o = softmax(s) v,  lse = ln sum exp(s)
+// Sequence b has the queries query_offsets[b] .. query_offsets[b+1] - 1 and the
+// keys key_offsets[b] .. key_offsets[b+1] - 1; the last query stands at the
+// last key, so that a causal query i of nq sees the first nk - nq + 1 + i keys.
+// A query that sees none gets o = 0 and lse = -inf.
+//
+// Bound by the tensor cores and, level with them, by the exponentials: a key
+// block of 128 keys costs 256 rows 2048 cycles of dense MMA and 2048 cycles of
+// the SM's 16 exponentials a cycle.
+//
+// Rows of a tile are (query, head of the group) pairs, so that all query heads
+// of a key/value head share one pass over its keys: 128 / group queries a tile.
+// Persistent, one CTA an SM; an item of work is a key/value head and two tiles
+// of 128 rows.  18 warps:
+//   warp 0      TMA: an item's Q tiles, then its key and value blocks through a
+//               ring of 5 shared-memory slots that runs on across items;
+//   warp 1      tensor memory, and the MMAs from one thread: S_t = Q_t K_j^T,
+//               O_t += P_t V_j with P_t read from tensor memory;
+//   warps 2-17  softmax, 8 warps a tile, two threads a row with 64 of a block's
+//               128 keys each.  A row's maximum goes between its two threads
+//               through shared memory and a barrier of their two warps.
+// The two halves of a row are what makes the tile's round trip short: the next
+// Q K^T of a tile waits for its P (S and P share tensor memory, 512 columns
+// hold S and O of two tiles and nothing else), so a block takes one softmax and
+// two MMAs in a row, and half the softmax is off that path this way.
+//
+// The order of items comes from a small kernel before (plan_kernel): longest
+// first over all sequences, dealt out to the CTAs in rounds of alternating
+// direction.
+#pragma once
+
+#include <cuda.h>
+#include "attention_tc.cuh"
+#include "common.cuh"
+#include "paged_attention.cuh"
+#include "ptx.cuh"
+
+namespace nt {
+namespace prompt {
+
+using paged::exp2_fast;
+using paged::kLn2;
+using paged::log2_fast;
+using paged::reference;
+
+struct Problem {
+  const void *q, *k, *v;
+  void *o;
+  float *lse;  // or null
+  IndexArray q_offsets, k_offsets;
+  int64_t q_tokens, k_tokens, batch;
+  int64_t q_token, q_head, q_dim, k_token, k_head, k_dim, v_token, v_head, v_dim, o_token, o_head, o_dim, l_token, l_head;
+  int heads, kv_heads, group, head_dim, causal;
+  float scale;  // softmax scale * log2 e
+  void *workspace;
+};
+
+// A sequence's extents, or false (and the device error word) where its offsets
+// are out of order or leave the tensors.
+__device__ __forceinline__ bool extents(const Problem &p, int64_t b, int64_t &q0, int64_t &nq, int64_t &k0, int64_t &nk) {
+  q0 = p.q_offsets[b];
+  k0 = p.k_offsets[b];
+  nq = p.q_offsets[b + 1] - q0;
+  nk = p.k_offsets[b + 1] - k0;
+  if (q0 < 0 || k0 < 0 || nq < 0 || nk < 0 || q0 + nq > p.q_tokens || k0 + nk > p.k_tokens) {
+    record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
+    return false;
+  }
+  return true;
+}
+
+// ---------------------------------------------------------------- any layout
+// A warp a query row: head elements dealt over the lanes, one key at a time.
+constexpr int kMostDim = 256;
+template <typename T>
+__global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ Problem p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= p.q_tokens * p.heads) return;
+  const int64_t token = row / p.heads;
+  const int h = (int)(row % p.heads);
+  const int64_t b = paged::warp_search(p.batch, token, [&](int64_t i) { return p.q_offsets[i]; });
+  int64_t q0, nq, k0, nk;
+  if (!extents(p, b, q0, nq, k0, nk) || token < q0 || token >= q0 + nq) return;
+  const int64_t limit = p.causal ? nk - nq + 1 + (token - q0) : nk;
+  const T *q = static_cast<const T *>(p.q) + token * p.q_token + h * p.q_head;
+  const int g = h / p.group;
+  constexpr int E = kMostDim / 32;
+  float qv[E], acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int d = lane + 32 * e;
+    qv[e] = d < p.head_dim ? to_f(q[d * p.q_dim]) : 0.f;
+    acc[e] = 0.f;
+  }
+  float m = -INFINITY, l = 0.f;
+  for (int64_t t = 0; t < limit; ++t) {
+    const T *k = static_cast<const T *>(p.k) + (k0 + t) * p.k_token + g * p.k_head;
+    const T *v = static_cast<const T *>(p.v) + (k0 + t) * p.v_token + g * p.v_head;
+    float dot = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (lane + 32 * e < p.head_dim) dot = fmaf(qv[e], to_f(k[(lane + 32 * e) * p.k_dim]), dot);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    const float s = dot * p.scale, m_new = fmaxf(m, s);
+    const float alpha = exp2f(m - reference(m_new)), w = exp2f(s - reference(m_new));
+    l = l * alpha + w;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (lane + 32 * e < p.head_dim) acc[e] = fmaf(w, to_f(v[(lane + 32 * e) * p.v_dim]), acc[e] * alpha);
+    m = m_new;
+  }
+  T *out = static_cast<T *>(p.o) + token * p.o_token + h * p.o_head;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int d = lane + 32 * e;
+    if (d < p.head_dim) out[d * p.o_dim] = from_f<T>(limit > 0 ? acc[e] / l : 0.f);
+  }
+  if (p.lse && lane == 0) p.lse[token * p.l_token + h * p.l_head] = limit > 0 ? (m + log2f(l)) * kLn2 : -INFINITY;
+}
+
+// ---------------------------------------------------------------- plan
+constexpr int BM = 128, BN = 128;  // rows of a tile, keys of a block
+
+// Two tiles of queries of one sequence.
+struct alignas(32) Entry {
+  int32_t q0, queries;  // first packed query, how many (at most two tiles')
+  int32_t k0, keys;     // first packed key, how many the sequence has
+  int32_t limit0;       // keys that the first query sees (causal), else `keys`
+  int32_t pad[3];
+};
+struct Plan {
+  int32_t count, pad[7];
+  // Entry[...] follows
+};
+
+// Key blocks of the tile whose queries are [t * per_tile, ..) of an entry: up
+// to the last key its last query sees, at least one; 0 for a tile without
+// queries.
+__host__ __device__ __forceinline__ int blocks_of(const Entry &e, int t, int per_tile, bool causal) {
+  const int last = (e.queries < (t + 1) * per_tile ? e.queries : (t + 1) * per_tile) - 1;
+  if (last < t * per_tile) return 0;
+  int seen = causal ? e.limit0 + last : e.keys;
+  if (seen > e.keys) seen = e.keys;
+  return seen <= 0 ? 1 : (seen + BN - 1) / BN;
+}
+
+constexpr int PLAN_THREADS = 1024, BINS = 1024;
+
+// The candidate entries: sequence b owns the candidates from query_offsets[b] /
+// pair + b on (pair = queries of two tiles), as many as it can have entries;
+// those past its last are empty.
+__device__ __forceinline__ bool candidate(const Problem &p, int64_t c, int pair, Entry &e) {
+  int64_t low = 0, high = p.batch;  // the largest b whose first candidate is <= c
+  while (high - low > 1) {
+    const int64_t mid = (low + high) / 2;
+    if (p.q_offsets[mid] / pair + mid <= c) low = mid;
+    else high = mid;
+  }
+  int64_t q0, nq, k0, nk;
+  if (!extents(p, low, q0, nq, k0, nk)) return false;
+  const int64_t first = (c - (q0 / pair + low)) * pair;
+  if (first < 0 || first >= nq) return false;
+  e.q0 = (int32_t)(q0 + first);
+  e.queries = (int32_t)(nq - first < pair ? nq - first : pair);
+  e.k0 = (int32_t)k0;
+  e.keys = (int32_t)nk;
+  e.limit0 = (int32_t)(p.causal ? nk - nq + 1 + first : nk);
+  return true;
+}
+
+// Counting sort of the entries by their key blocks, most first (blocks beyond
+// the bins share the first bin: the order is for balance only).
+__global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const __grid_constant__ Problem p, int64_t candidates,
+                                                            int per_tile) {
+  __shared__ int bins[BINS];
+  __shared__ int warp_sums[PLAN_THREADS / 32];
+  static_assert(BINS == PLAN_THREADS, "a thread scans one bin");
+  wait_prior_grid();
+  allow_dependent_launch();
+  bins[threadIdx.x] = 0;
+  __syncthreads();
+  auto bin_of = [&](const Entry &e) {
+    const int n0 = blocks_of(e, 0, per_tile, p.causal), n1 = blocks_of(e, 1, per_tile, p.causal);
+    const int n = n0 + n1;
+    return n >= BINS ? 0 : BINS - 1 - n;
+  };
+  for (int64_t c = threadIdx.x; c < candidates; c += PLAN_THREADS) {
+    Entry e;
+    if (candidate(p, c, 2 * per_tile, e)) atomicAdd(&bins[bin_of(e)], 1);
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = bins[threadIdx.x];
+  int up = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, up, o);
+    if (lane >= o) up += x;
+  }
+  if (lane == 31) warp_sums[warp] = up;
+  __syncthreads();
+  int base = 0;
+  for (int i = 0; i < warp; ++i) base += warp_sums[i];
+  bins[threadIdx.x] = base + up - n;
+  Plan *plan = static_cast<Plan *>(p.workspace);
+  if (threadIdx.x == PLAN_THREADS - 1) plan->count = base + up;
+  __syncthreads();
+  Entry *list = reinterpret_cast<Entry *>(plan + 1);
+  for (int64_t c = threadIdx.x; c < candidates; c += PLAN_THREADS) {
+    Entry e{};
+    if (candidate(p, c, 2 * per_tile, e)) list[atomicAdd(&bins[bin_of(e)], 1)] = e;
+  }
+}
+
+// ---------------------------------------------------------------- tensor cores
+constexpr int TILES = 2, RING = 5;
+constexpr int SOFTMAX_WARPS = 16;
+constexpr int THREADS = (2 + SOFTMAX_WARPS) * 32;
+constexpr int TMEM_COLS = 512;
+
+template <int DP>  // head_dim padded to 64 or 128
+struct Layout {
+  static constexpr int ATOMS = DP / 64;         // 128-byte swizzle atoms along the head
+  static constexpr int Q_BYTES = BM * DP * 2;   // one Q tile
+  static constexpr int KV_BYTES = BN * DP * 2;  // one key or value block
+  static constexpr int RING_OFF = TILES * Q_BYTES;
+  static constexpr int SHARE_OFF = RING_OFF + RING * KV_BYTES;  // float [TILES][2][BM]
+  static constexpr int CTRL_OFF = SHARE_OFF + TILES * 2 * BM * 4;
+  static constexpr int SMEM_BYTES = CTRL_OFF + 256;
+  static_assert(96 + 16 * RING + 32 * TILES <= 240, "barrier slots");
+  static_assert(SMEM_BYTES <= 232448, "shared memory of a CTA");
+};
+
+struct Params {
+  Problem p;
+  int per_tile;  // queries of a tile
+};
+
+// A row's elements [d0, d0 + 64) again, key by key on the CUDA cores, from its
+// final maximum.  An infinity or NaN in the value of a key that the row does
+// not see makes the row's MMA sums NaN (0 * inf): such rows come here.
+template <typename T>
+__device__ __noinline__ void row_again(const Problem &p, int k0, int64_t token, int head, int limit, int d0, int dims,
+                                       float m, float f, T *out) {
+  const T *q = static_cast<const T *>(p.q) + token * p.q_token + head * p.q_head;
+  const int g = head / p.group;
+  for (int c = 0; c < dims; c += 16) {
+    float acc[16] = {};
+    for (int t = 0; t < limit; ++t) {
+      const T *k = static_cast<const T *>(p.k) + (int64_t)(k0 + t) * p.k_token + g * p.k_head;
+      const T *v = static_cast<const T *>(p.v) + (int64_t)(k0 + t) * p.v_token + g * p.v_head;
+      float dot = 0.f;
+      for (int d = 0; d < p.head_dim; ++d) dot = fmaf(to_f(q[d]), to_f(k[d]), dot);
+      const float w = exp2f(dot * p.scale - m);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (c + i < dims) acc[i] = fmaf(w, to_f(v[d0 + c + i]), acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (c + i < dims) out[(d0 + c + i) * p.o_dim] = from_f<T>(acc[i] * f);
+  }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS, 1)
+attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                 const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ Params prm) {
+  using L = Layout<DP>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = ptx::smem_u32(smem);
+  if ((base & 1023u) != 0) {  // the swizzle needs it; there is no room to align by hand
+    record_error(NT_B200_ERR_INVALID_ARGUMENT);
+    return;
+  }
+  const uint32_t ctrl = base + L::CTRL_OFF;
+  // barriers (8 bytes each), per tile t unless noted
+  auto q_full = [&](int t) { return ctrl + 8u * t; };        // Q_t landed
+  auto q_free = [&](int t) { return ctrl + 16 + 8u * t; };   // the item's last Q_t K^T done
+  auto s_full = [&](int t) { return ctrl + 32 + 8u * t; };   // S_t of a key block in tensor memory
+  auto p_full = [&](int t) { return ctrl + 48 + 8u * t; };   // P_t written, O_t rescaled
+  auto o_done = [&](int t) { return ctrl + 64 + 8u * t; };   // the item's last P_t V done
+  auto o_free = [&](int t) { return ctrl + 80 + 8u * t; };   // O_t read out
+  auto slot_full = [&](int s) { return ctrl + 96 + 8u * s; };
+  auto slot_empty = [&](int s) { return ctrl + 96 + 8u * RING + 8u * s; };
+  auto shared_row = [&](int t, int quarter) { return ctrl + 96 + 16u * RING + 8u * (4 * t + quarter); };
+  volatile uint32_t *tmem_base_ptr = reinterpret_cast<volatile uint32_t *>(smem + L::CTRL_OFF + 240);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::CTRL_OFF + 244);
+
+  const Problem &p = prm.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per_tile = prm.per_tile;
+  const Plan *plan = static_cast<const Plan *>(p.workspace);
+  const Entry *list = reinterpret_cast<const Entry *>(plan + 1);
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < TILES; ++t) {
+      ptx::mbar_init(q_full(t), 1);
+      ptx::mbar_init(q_free(t), 1);
+      ptx::mbar_init(s_full(t), 1);
+      ptx::mbar_init(p_full(t), 256);
+      ptx::mbar_init(o_done(t), 1);
+      ptx::mbar_init(o_free(t), 256);
+      for (int w = 0; w < 4; ++w) ptx::mbar_init(shared_row(t, w), 2);  // the two warps of 32 rows
+    }
+    for (int s = 0; s < RING; ++s) {
+      ptx::mbar_init(slot_full(s), 1);
+      ptx::mbar_init(slot_empty(s), 1);
+    }
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tmap(&tmap_q);
+    ptx::prefetch_tmap(&tmap_k);
+    ptx::prefetch_tmap(&tmap_v);
+  }
+  // rows past per_tile * group are never loaded: zeros
+  if (per_tile * p.group < BM) {
+    for (int i = threadIdx.x; i < TILES * L::Q_BYTES / 16; i += THREADS)
+      reinterpret_cast<int4 *>(smem)[i] = make_int4(0, 0, 0, 0);
+    ptx::fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t *>(tmem_base_ptr)), TMEM_COLS);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  wait_prior_grid();
+  const uint32_t tmem_base = *tmem_base_ptr;
+  auto tmem_s = [&](int t) { return tmem_base + (uint32_t)(t * BN); };
+  auto tmem_o = [&](int t) { return tmem_base + (uint32_t)(TILES * BN + t * 128); };
+
+  // Items k = entry * kv_heads + head; the CTA's i-th: the i-th round of
+  // gridDim.x items, in alternating direction.
+  const int64_t num_items = (int64_t)plan->count * p.kv_heads;
+  auto nth_item = [&](int i) -> int64_t {
+    const int64_t g = gridDim.x, c = blockIdx.x;
+    const int64_t k = i * g + ((i & 1) ? g - 1 - c : c);
+    return k < num_items ? k : -1;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      bool ok = true;
+      int r = 0;             // ring items so far
+      int used[TILES] = {};  // items so far that had tile t
+      const uint32_t q_bytes = (uint32_t)(per_tile * p.group * 128 * L::ATOMS);
+      for (int i = 0; ok; ++i) {
+        const int64_t item = nth_item(i);
+        if (item < 0) break;
+        const Entry e = list[item / p.kv_heads];
+        const int h = (int)(item % p.kv_heads);
+        const int n[TILES] = {blocks_of(e, 0, per_tile, p.causal), blocks_of(e, 1, per_tile, p.causal)};
+        const int n_max = max(n[0], n[1]);
+        for (int t = 0; t < TILES && ok; ++t) {
+          if (n[t] == 0) continue;
+          if (used[t] > 0 && !ptx::mbar_wait(q_free(t), (uint32_t)(used[t] - 1) & 1u, abort_flag)) { ok = false; break; }
+          ++used[t];
+          ptx::mbar_arrive_expect_tx(q_full(t), q_bytes);
+          for (int x = 0; x < L::ATOMS; ++x)
+            ptx::tma_load_3d(base + t * L::Q_BYTES + x * (BM * 128), &tmap_q, q_full(t), 64 * x, h * p.group,
+                             e.q0 + t * per_tile);
+        }
+        for (int j = 0; j < 2 * n_max && ok; ++j, ++r) {  // K_0, V_0, K_1, V_1, ...
+          const int slot = r % RING;
+          if (!ptx::mbar_wait(slot_empty(slot), ((uint32_t)(r / RING) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+          ptx::mbar_arrive_expect_tx(slot_full(slot), L::KV_BYTES);
+          const CUtensorMap *map = (j & 1) ? &tmap_v : &tmap_k;
+          for (int x = 0; x < L::ATOMS; ++x)
+            ptx::tma_load_3d(base + L::RING_OFF + slot * L::KV_BYTES + x * (BN * 128), map, slot_full(slot), 64 * x, h,
+                             e.k0 + (j >> 1) * BN);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t fmt = tc::umma_format<T>();
+      constexpr uint32_t idesc_qk = ptx::f16_idesc(fmt, 0, 0, BM, BN);  // B = keys, K-major
+      constexpr uint32_t idesc_pv = ptx::f16_idesc(fmt, 0, 1, BM, DP);  // B = values, MN-major
+      auto slot_addr = [&](int r) { return base + L::RING_OFF + (r % RING) * L::KV_BYTES; };
+      auto wait_slot = [&](int r) { return ptx::mbar_wait(slot_full(r % RING), (uint32_t)(r / RING) & 1u, abort_flag); };
+      auto issue_qk = [&](int t, int r) {
+        const uint32_t kb = slot_addr(r);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint32_t qoff = (kk / 4) * (BM * 128) + (kk % 4) * 32, koff = (kk / 4) * (BN * 128) + (kk % 4) * 32;
+          ptx::mma_f16_ss(tmem_s(t), ptx::sw128_desc(base + t * L::Q_BYTES + qoff, 16, 1024),
+                          ptx::sw128_desc(kb + koff, 16, 1024), idesc_qk, kk > 0 ? 1u : 0u);
+        }
+        ptx::mma_commit(s_full(t));
+      };
+      auto issue_pv = [&](int t, int r, bool first) {
+        const uint32_t vb = slot_addr(r);
+#pragma unroll
+        for (int kk = 0; kk < BN / 16; ++kk)
+          ptx::mma_f16_ts(tmem_o(t), tmem_s(t) + (uint32_t)(kk * 8), ptx::sw128_desc(vb + kk * 16 * 128, BN * 128, 1024),
+                          idesc_pv, (!first || kk > 0) ? 1u : 0u);
+      };
+      bool ok = true;
+      int r = 0;             // ring position of the item's K_0
+      int blk[TILES] = {};   // key blocks of tile t in earlier items
+      int used[TILES] = {};  // earlier items that had tile t
+      for (int i = 0; ok; ++i) {
+        const int64_t item = nth_item(i);
+        if (item < 0) break;
+        const Entry e = list[item / p.kv_heads];
+        const int n[TILES] = {blocks_of(e, 0, per_tile, p.causal), blocks_of(e, 1, per_tile, p.causal)};
+        const int n_max = max(n[0], n[1]);
+        ok = wait_slot(r);  // K_0
+        for (int t = 0; t < TILES && ok; ++t) {
+          if (n[t] == 0) continue;
+          if (!ptx::mbar_wait(q_full(t), (uint32_t)used[t] & 1u, abort_flag)) { ok = false; break; }
+          ptx::tc_fence_after();
+          issue_qk(t, r);
+          if (n[t] == 1) ptx::mma_commit(q_free(t));
+        }
+        if (!ok) break;
+        ptx::mma_commit(slot_empty(r % RING));
+        for (int j = 0; j < n_max && ok; ++j) {
+          const int rv = r + 2 * j + 1, rk = r + 2 * j + 2;
+          if (!wait_slot(rv)) { ok = false; break; }
+          bool next_keys = false;
+          for (int t = 0; t < TILES && ok; ++t) {
+            if (j >= n[t]) continue;
+            // P_t written also means that S_t was read: Q K^T may overwrite it
+            if (!ptx::mbar_wait(p_full(t), (uint32_t)(blk[t] + j) & 1u, abort_flag)) { ok = false; break; }
+            if (j == 0 && used[t] > 0 && !ptx::mbar_wait(o_free(t), (uint32_t)(used[t] - 1) & 1u, abort_flag)) {
+              ok = false;
+              break;
+            }
+            ptx::tc_fence_after();
+            issue_pv(t, rv, j == 0);
+            if (j == n[t] - 1) ptx::mma_commit(o_done(t));
+            if (j + 1 < n[t]) {
+              if (!next_keys) {
+                if (!wait_slot(rk)) { ok = false; break; }
+                next_keys = true;
+                ptx::tc_fence_after();
+              }
+              issue_qk(t, rk);
+              if (j + 2 == n[t]) ptx::mma_commit(q_free(t));
+            }
+          }
+          if (!ok) break;
+          ptx::mma_commit(slot_empty(rv % RING));
+          if (next_keys) ptx::mma_commit(slot_empty(rk % RING));
+        }
+        r += 2 * n_max;
+        for (int t = 0; t < TILES; ++t) {
+          blk[t] += n[t];
+          used[t] += n[t] > 0;
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax, rescaling, output
+    const int t = (warp - 2) / 8, half = (warp - 2) / 4 % 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;  // row of the tile = lane of tensor memory
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const int query_of_row = row / p.group, head_of_row = row % p.group;
+    float *share = reinterpret_cast<float *>(smem + L::SHARE_OFF) + t * 2 * BM + row;
+    bool ok = true;
+    // a value for the row's other thread; the caller sees to it that the last
+    // one was read
+    uint32_t turn = 0;
+    auto meet = [&]() {  // the two warps of 32 rows
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(shared_row(t, quarter));
+      ok = ptx::mbar_wait_warp(shared_row(t, quarter), turn, abort_flag);
+      turn ^= 1;
+    };
+    auto exchange = [&](float mine) {
+      share[half * BM] = mine;
+      meet();
+      return share[(half ^ 1) * BM];
+    };
+    const float c = p.scale;
+    constexpr int HALF_D = DP / 2;
+    int blk = 0, used = 0;
+    for (int i = 0; ok; ++i) {
+      const int64_t item = nth_item(i);
+      if (item < 0) break;
+      const Entry e = list[item / p.kv_heads];
+      const int n_t = blocks_of(e, t, per_tile, p.causal);
+      if (n_t == 0) continue;
+      const int query = t * per_tile + query_of_row;
+      const bool real = query < e.queries && query_of_row < per_tile;
+      const int limit = p.causal ? min(e.limit0 + query, e.keys) : e.keys;
+      const int sure = p.causal ? min(e.limit0 + t * per_tile, e.keys) : e.keys;  // keys that all rows see
+
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < n_t; ++j) {
+        if (!ptx::mbar_wait_warp(s_full(t), (uint32_t)(blk + j) & 1u, abort_flag)) { ok = false; break; }
+        ptx::tc_fence_after();
+        uint32_t sr[64];
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          ptx::tmem_ld_32x32b_x32(tmem_s(t) + lane_base + (uint32_t)(half * 64 + x * 32),
+                                  *reinterpret_cast<uint32_t(*)[32]>(&sr[x * 32]));
+        ptx::tmem_ld_wait();
+        float *s = reinterpret_cast<float *>(sr);
+        if ((j + 1) * BN > sure) {
+          const int seen = limit - j * BN - half * 64;
+#pragma unroll
+          for (int x = 0; x < 64; ++x) s[x] = x < seen ? s[x] : -INFINITY;
+        }
+        float top[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) top[u] = s[u];
+#pragma unroll
+        for (int x = 4; x < 64; ++x) top[x & 3] = fmaxf(top[x & 3], s[x]);
+        float block_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+        // (the last block's maximum was read before its P was reported written,
+        // and this S waited for that)
+        block_top = fmaxf(block_top, exchange(block_top));
+        if (!ok) break;
+        // the maximum moves only when a block passes it by 2^14 (bf16: 2^24):
+        // P stays in its type's range and O is rescaled rarely
+        const bool move = block_top > m + tc::attn::RescaleLog2<T>::value;
+        const float m_new = move ? block_top : m;
+        const float alpha = move ? exp2_fast(m - m_new) : 1.f;
+        const float ref = reference(m_new);
+        float sum[4] = {};
+        uint32_t packed[32];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) {
+          const float p0 = exp2_fast(fmaf(s[2 * x], c, -ref)), p1 = exp2_fast(fmaf(s[2 * x + 1], c, -ref));
+          sum[(2 * x) & 3] += p0;
+          sum[(2 * x + 1) & 3] += p1;
+          packed[x] = tc::attn::pack2<T>(p0, p1);
+        }
+        // both threads of a row have read S: the exchange came after
+        ptx::tmem_st_32x32b_x32(tmem_s(t) + lane_base + (uint32_t)(half * 32), packed);
+        if (j > 0 && __any_sync(0xffffffffu, move)) {
+          // O_t holds P(j-1) V(j-1): the commit of S_t(j) covers it
+#pragma unroll
+          for (int x = 0; x < HALF_D / 32; ++x) {
+            uint32_t o[32];
+            ptx::tmem_ld_32x32b_x32(tmem_o(t) + lane_base + (uint32_t)(half * HALF_D + x * 32), o);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * alpha);
+            ptx::tmem_st_32x32b_x32(tmem_o(t) + lane_base + (uint32_t)(half * HALF_D + x * 32), o);
+          }
+        }
+        m = m_new;
+        l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        ptx::tmem_st_wait();
+        ptx::tc_fence_before();
+        ptx::mbar_arrive(p_full(t));
+      }
+      if (!ok) break;
+      blk += n_t;
+      if (!ptx::mbar_wait_warp(o_done(t), (uint32_t)used & 1u, abort_flag)) {
+        ok = false;
+        break;
+      }
+      ++used;
+      ptx::tc_fence_after();
+      uint32_t o[HALF_D];
+#pragma unroll
+      for (int x = 0; x < HALF_D / 32; ++x)
+        ptx::tmem_ld_32x32b_x32(tmem_o(t) + lane_base + (uint32_t)(half * HALF_D + x * 32),
+                                *reinterpret_cast<uint32_t(*)[32]>(&o[x * 32]));
+      ptx::tmem_ld_wait();
+      ptx::tc_fence_before();
+      ptx::mbar_arrive(o_free(t));
+      l += exchange(l);
+      if (!ok) break;
+      meet();  // read on both sides, before the next item's first maximum
+      if (!ok) break;
+      if (real) {
+        const int64_t token = e.q0 + query;
+        const int head = (int)(item % p.kv_heads) * p.group + head_of_row;
+        const float f = l == 0.f ? 0.f : 1.f / l;
+        T *out = static_cast<T *>(p.o) + token * p.o_token + (int64_t)head * p.o_head;
+        const int d0 = half * HALF_D, dims = min(HALF_D, p.head_dim - d0);
+        float worst = 0.f;  // NaN or infinite if any element is
+#pragma unroll
+        for (int x = 0; x < HALF_D; ++x) worst = fmaf(__uint_as_float(o[x]), 0.f, worst);
+        if (!(worst == 0.f)) {
+          row_again<T>(p, e.k0, token, head, limit, d0, dims, reference(m), f, out);
+        } else if (dims == HALF_D && p.o_dim == 1 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0) {
+#pragma unroll
+          for (int x = 0; x < HALF_D / 8; ++x) {
+            const float *v = reinterpret_cast<const float *>(o + x * 8);
+            *reinterpret_cast<int4 *>(out + d0 + x * 8) =
+                make_int4((int)tc::attn::pack2<T>(v[0] * f, v[1] * f), (int)tc::attn::pack2<T>(v[2] * f, v[3] * f),
+                          (int)tc::attn::pack2<T>(v[4] * f, v[5] * f), (int)tc::attn::pack2<T>(v[6] * f, v[7] * f));
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < HALF_D; ++x)
+            if (x < dims) out[(d0 + x) * p.o_dim] = from_f<T>(__uint_as_float(o[x]) * f);
+        }
+        if (p.lse && half == 0)
+          p.lse[token * p.l_token + (int64_t)head * p.l_head] = l == 0.f ? -INFINITY : (m + log2_fast(l)) * kLn2;
+      }
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// Tensor map over [tokens, heads, head_dim]: box of 64 elements, `box_heads`
+// heads and `box_tokens` tokens, 128-byte swizzle, zeros outside.
+inline bool make_map(CUtensorMap *map, const void *data, CUtensorMapDataType type, int64_t dim, int64_t heads,
+                     int64_t tokens, int64_t head_stride, int64_t token_stride, int box_heads, int box_tokens) {
+  tc::EncodeTiledFn fn = tc::encode_tiled_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)tokens};
+  const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
+  const cuuint32_t ones[3] = {1, 1, 1};
+  return fn(map, type, 3, const_cast<void *>(data), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+inline int64_t candidates_of(int64_t tokens, int64_t batch, int pair) { return tokens / pair + batch; }
+
+template <typename T, int DP>
+int launch_tiles(const Params &prm, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, int64_t candidates,
+                 cudaStream_t stream) {
+  cudaError_t e = smem_optin<attention_kernel<T, DP>>(Layout<DP>::SMEM_BYTES);
+  if (e != cudaSuccess) return (int)e;
+  const int rc = launch_overlapped(plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, stream, prm.p, candidates, prm.per_tile);
+  if (rc != 0) return rc;
+  const int64_t items = candidates * prm.p.kv_heads;
+  const unsigned grid = (unsigned)(items < sm_count() ? items : sm_count());
+  return launch_overlapped(attention_kernel<T, DP>, dim3(grid), dim3(THREADS), Layout<DP>::SMEM_BYTES, stream, tq, tk, tv,
+                           prm);
+}
+
+// tc::kNotEligible where the operands do not meet the tensor-core kernel's layout.
+template <typename T> int try_tiles(const Problem &p, int64_t workspace_bytes, cudaStream_t stream) {
+  if constexpr (sizeof(T) != 2) {
+    return tc::kNotEligible;
+  } else {
+    if (p.head_dim > 128 || p.group > BM || !(p.scale > 0.f) || p.k_tokens == 0) return tc::kNotEligible;
+    if (p.q_dim != 1 || p.k_dim != 1 || p.v_dim != 1) return tc::kNotEligible;
+    if (!rotary::aligned16(p.q) || !rotary::aligned16(p.k) || !rotary::aligned16(p.v)) return tc::kNotEligible;
+    for (int64_t s : {p.q_token, p.q_head, p.k_token, p.k_head, p.v_token, p.v_head})
+      if (s <= 0 || s % 8 != 0) return tc::kNotEligible;
+    if (p.q_tokens > (1 << 30) || p.k_tokens > (1 << 30) || p.batch > (1 << 30)) return tc::kNotEligible;
+    Params prm;
+    prm.p = p;
+    prm.per_tile = BM / p.group;
+    const int64_t candidates = candidates_of(p.q_tokens, p.batch, 2 * prm.per_tile);
+    if ((int64_t)sizeof(Plan) + candidates * (int64_t)sizeof(Entry) > workspace_bytes) return NT_B200_ERR_INVALID_ARGUMENT;
+    CUtensorMap tq, tk, tv;
+    const CUtensorMapDataType type = tc::tmap_dtype<T>();
+    if (!make_map(&tq, p.q, type, p.head_dim, p.heads, p.q_tokens, p.q_head, p.q_token, p.group, prm.per_tile) ||
+        !make_map(&tk, p.k, type, p.head_dim, p.kv_heads, p.k_tokens, p.k_head, p.k_token, 1, BN) ||
+        !make_map(&tv, p.v, type, p.head_dim, p.kv_heads, p.k_tokens, p.v_head, p.v_token, 1, BN))
+      return tc::kNotEligible;
+    if (p.head_dim <= 64) return launch_tiles<T, 64>(prm, tq, tk, tv, candidates, stream);
+    return launch_tiles<T, 128>(prm, tq, tk, tv, candidates, stream);
+  }
+}
+
+}  // namespace prompt
+}  // namespace nt
+
+extern "C" int64_t nt_b200_prompt_attention_workspace_size(int64_t query_tokens, int64_t batch, int64_t heads,
+                                                           int64_t kv_heads) {
+  using namespace nt::prompt;
+  if (query_tokens < 0 || batch < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0) return 0;
+  const int64_t group = heads / kv_heads;
+  const int pair = group > BM ? 2 : 2 * (int)(BM / group);
+  return (int64_t)sizeof(Plan) + candidates_of(query_tokens, batch, pair) * (int64_t)sizeof(Entry);
+}
+
+extern "C" int nt_b200_prompt_attention(const NtB200PromptAttentionArgs *a, void *stream) {
+  using namespace nt;
+  if (!a || a->query_tokens < 0 || a->key_tokens < 0 || a->batch < 0 || a->heads < 0 || a->kv_heads < 0 || a->head_dim < 0)
+    return NT_B200_ERR_INVALID_ARGUMENT;
+  if (!is_float_dtype((int)a->dtype) || !is_index_dtype(a->index_dtype)) return NT_B200_ERR_UNSUPPORTED_DTYPE;
+  if (a->query_tokens == 0 || a->batch == 0 || a->heads == 0 || a->head_dim == 0) return 0;
+  if (a->kv_heads == 0 || a->heads % a->kv_heads != 0 || a->head_dim > prompt::kMostDim) return NT_B200_ERR_SHAPE_MISMATCH;
+  if (!a->query || !a->output || !a->query_offsets || !a->key_offsets || (a->key_tokens > 0 && (!a->key || !a->value)) ||
+      !a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 31u) != 0 || a->heads > (1 << 30) ||
+      !(a->scale == a->scale) ||
+      a->workspace_bytes < nt_b200_prompt_attention_workspace_size(a->query_tokens, a->batch, a->heads, a->kv_heads))
+    return NT_B200_ERR_INVALID_ARGUMENT;
+  const int wide = a->index_dtype == NT_B200_INT64;
+  prompt::Problem p{};
+  p.q = a->query; p.k = a->key; p.v = a->value; p.o = a->output; p.lse = a->lse;
+  p.q_offsets = {a->query_offsets, a->query_offsets_stride, wide};
+  p.k_offsets = {a->key_offsets, a->key_offsets_stride, wide};
+  p.q_tokens = a->query_tokens; p.k_tokens = a->key_tokens; p.batch = a->batch;
+  p.q_token = a->query_strides[0]; p.q_head = a->query_strides[1]; p.q_dim = a->query_strides[2];
+  p.k_token = a->key_strides[0]; p.k_head = a->key_strides[1]; p.k_dim = a->key_strides[2];
+  p.v_token = a->value_strides[0]; p.v_head = a->value_strides[1]; p.v_dim = a->value_strides[2];
+  p.o_token = a->output_strides[0]; p.o_head = a->output_strides[1]; p.o_dim = a->output_strides[2];
+  p.l_token = a->lse_strides[0]; p.l_head = a->lse_strides[1];
+  p.heads = (int)a->heads; p.kv_heads = (int)a->kv_heads; p.group = (int)(a->heads / a->kv_heads);
+  p.head_dim = (int)a->head_dim;
+  p.causal = a->is_causal != 0;
+  p.scale = (float)(a->scale * 1.4426950408889634);
+  p.workspace = a->workspace;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return NT_DISPATCH_FLOAT((int)a->dtype, [&] {
+    const int rc = prompt::try_tiles<scalar_t>(p, a->workspace_bytes, s);
+    if (rc != tc::kNotEligible) return rc;
+    const int64_t blocks = (p.q_tokens * p.heads + 3) / 4;
+    if (blocks > (1LL << 31) - 1) return NT_B200_ERR_INVALID_ARGUMENT;
+    prompt::rows_kernel<scalar_t><<<(unsigned)blocks, 128, 0, s>>>(p);
+    return launch_status();
+  });
+}

@@ -554,6 +554,8 @@ from ninetoothed_b200.serving import (  # noqa: E402
     paged_append_kernel,
     paged_attention,
     paged_attention_kernel,
+    prompt_attention,
+    prompt_attention_kernel,
     rotary,
     rotary_kernel,
     rotary_tables,
@@ -590,6 +592,8 @@ __all__ = [
     "pooled_extent",
     "pow",
     "pow_kernel",
+    "prompt_attention",
+    "prompt_attention_kernel",
     "rotary",
     "rotary_kernel",
     "rotary_tables",

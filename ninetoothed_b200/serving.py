@@ -318,6 +318,77 @@ def paged_attention(query, key_cache, value_cache, key_scale, value_scale, block
     return (output, lse) if return_lse else output
 
 
+# --------------------------------------------------------------------- attention over prompts
+def _launch_prompt_attention(v, stream):
+    query, key, value, out, lse = v["query"], v["key"], v["value"], v["output"], v["lse"]
+    query_offsets, key_offsets = v["query_offsets"], v["key_offsets"]
+    check_same_dtype(v, ("query", "key", "value", "output"))
+    check_same_dtype(v, ("query_offsets", "key_offsets"))
+    tokens, heads, dim = query.shape
+    kv_heads = key.shape[1]
+    if value.shape != key.shape or key.shape[2] != dim or out.shape != query.shape or not kv_heads or heads % kv_heads:
+        raise TypeError(
+            f"prompt_attention query {tuple(query.shape)}, key {tuple(key.shape)}, value {tuple(value.shape)} and "
+            f"output {tuple(out.shape)} disagree."
+        )
+    if dim > 256:
+        raise TypeError("Kernel argument `query` has head dimension above the upper bound 256.")
+    batch = query_offsets.shape[0] - 1
+    if batch < 0 or key_offsets.shape != query_offsets.shape:
+        raise TypeError("prompt_attention needs as many query offsets as key offsets, one more than sequences.")
+    if lse is not None and lse.shape != query.shape[:2]:
+        raise TypeError("prompt_attention lse must have the query's shape without the head dimension.")
+    lib = _lib.library()
+    nbytes = lib.nt_b200_prompt_attention_workspace_size(tokens, batch, heads, kv_heads)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
+    args = _lib.pack_args(
+        query.data_ptr(), key.data_ptr(), value.data_ptr(), query_offsets.data_ptr(), key_offsets.data_ptr(),
+        out.data_ptr(), 0 if lse is None else lse.data_ptr(), workspace.data_ptr(), nbytes, tokens, key.shape[0], batch,
+        heads, kv_heads, dim, *query.stride(), *key.stride(), *value.stride(), *out.stride(),
+        *((0, 0) if lse is None else lse.stride()), query_offsets.stride(0), key_offsets.stride(0),
+        bool(v["is_causal"]), dtype_code(query.dtype), dtype_code(query_offsets.dtype), scale=_scale(v["scale"], dim),
+    )
+    return lib.nt_b200_prompt_attention(args, stream)
+
+
+prompt_attention_kernel = Kernel(
+    name="prompt_attention",
+    args=(
+        TensorArg("query", 3),
+        TensorArg("key", 3),
+        TensorArg("value", 3),
+        TensorArg("query_offsets", 1, INDEX_DTYPES),
+        TensorArg("key_offsets", 1, INDEX_DTYPES),
+        TensorArg("output", 3),
+        TensorArg("lse", 2, _F32, optional=True),
+    ),
+    outputs=("output",),
+    launch=_launch_prompt_attention,
+    meta=("is_causal", "scale"),
+    meta_defaults={"is_causal": True, "scale": None, "lse": None},
+)
+
+
+def prompt_attention(query, key, value, offsets, key_offsets=None, is_causal=True, scale=None, return_lse=False):
+    """Attention over whole prompts packed one after another.
+
+    `query` [tokens, heads, head_dim], `key` and `value` [tokens, kv_heads,
+    head_dim]: sequence s from offsets[s] to offsets[s + 1] (`offsets`: batch + 1
+    entries), its keys from key_offsets[s] to key_offsets[s + 1] where they
+    differ (a prompt's later part against all of its keys: the last query stands
+    at the last key).  Causal queries see the keys up to their own; query head h
+    reads key/value head h // (heads // kv_heads).  `scale` is
+    1 / sqrt(head_dim) by default.  Returns the output, in the query's shape and
+    dtype, or with `return_lse` (output, lse): the fp32 natural logarithm of each
+    query's sum of exponentials [tokens, heads].  A query that sees no key gets
+    0, and -inf as its lse; tokens that belong to no sequence are not written."""
+    output = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    lse = torch.empty(query.shape[:2], dtype=torch.float32, device=query.device) if return_lse else None
+    prompt_attention_kernel(query, key, value, offsets, offsets if key_offsets is None else key_offsets, output, lse,
+                            is_causal=is_causal, scale=scale)
+    return (output, lse) if return_lse else output
+
+
 __all__ = [
     "CODE_DTYPES",
     "INDEX_DTYPES",
@@ -325,6 +396,8 @@ __all__ = [
     "paged_append_kernel",
     "paged_attention",
     "paged_attention_kernel",
+    "prompt_attention",
+    "prompt_attention_kernel",
     "rotary",
     "rotary_kernel",
     "rotary_tables",

@@ -98,6 +98,15 @@ def test_rotary_tables_refusals(bad):
             (dict(), 10001),  # null pointers
         ],
     ),
+    (
+        "NtB200PromptAttentionArgs", "nt_b200_prompt_attention",
+        dict(query_tokens=4, key_tokens=4, batch=1, heads=4, kv_heads=2, head_dim=64, dtype=8, index_dtype=2),
+        [
+            (dict(key_tokens=-1), 10001), (dict(dtype=0), 10002), (dict(index_dtype=0), 10002), (dict(heads=3), 10003),
+            (dict(kv_heads=0), 10003), (dict(head_dim=257), 10003), (dict(query_tokens=0), 0), (dict(batch=0), 0),
+            (dict(heads=0), 0), (dict(head_dim=0), 0), (dict(), 10001),  # null pointers
+        ],
+    ),
 ])
 def test_refused_on_the_host(struct, call, base, cases):
     entry = getattr(_lib.library(), call)

@@ -500,6 +500,171 @@ def test_paged_attention_offsets_past_32_bits():
     assert int(cache[last, 15, 63].float().mean()) == 2 and not cache[0].any()
 
 
+# --------------------------------------------------------------------- attention over prompts
+def check_prompt(q, k, v, q_lens, k_lens, scale, causal, got, lse, dtype):
+    got, lse = got.cpu().double(), lse.cpu().double()
+    q, k, v = q.double(), k.double(), v.double()
+    heads, kv_heads, dim = q.shape[1], k.shape[1], q.shape[2]
+    q0 = k0 = 0
+    for nq, nk in zip(q_lens, k_lens):
+        limit = nk - nq + 1 + torch.arange(nq) if causal else torch.full((nq,), nk)
+        hidden = torch.arange(nk)[None] >= limit[:, None]
+        for h in range(heads):
+            g = h // (heads // kv_heads)
+            rows, keys, values = q[q0 : q0 + nq, h], k[k0 : k0 + nk, g], v[k0 : k0 + nk, g]
+            s = (rows @ keys.T * scale).masked_fill(hidden, -math.inf)
+            want_lse = torch.logsumexp(s, 1)
+            weights = torch.exp(s - want_lse[:, None]).masked_fill(hidden, 0.0)
+            want = weights @ values
+            x, y = got[q0 : q0 + nq, h], lse[q0 : q0 + nq, h]
+            some = (limit > 0) if nk else torch.zeros(nq, dtype=torch.bool)
+            assert not x[~some].any() and (y[~some] == -math.inf).all()
+            if not some.any():
+                continue
+            # scores: fp32 sums of exact products; weights: the scores' error and half a step of the type
+            score = (dim + 8) * 2.0**-24 * float((rows.abs() @ keys.abs().T).max()) * abs(scale)
+            assert ((y - want_lse)[some].abs() <= 2 * score + 2.0**-20 * (1 + want_lse[some].abs())).all()
+            weight = 2 * score + (HALF[dtype] if dtype != torch.float32 else 0) + 2.0**-20
+            top = weights[some] @ values.abs()  # what the weights' relative errors can add up to
+            bound = HALF[dtype] * want[some].abs() + TINY[dtype] + weight * top
+            assert ((x[some] - want[some]).abs() <= bound).all(), (nq, nk, h)
+        q0, k0 = q0 + nq, k0 + nk
+
+
+PROMPTS = [
+    # query lengths, key lengths (None: the same), heads, kv_heads, dim
+    ([1], None, 1, 1, 64),
+    ([1, 0, 17, 100, 3], None, 8, 2, 64),
+    ([300, 129, 128], None, 4, 1, 128),
+    ([257, 5], None, 3, 1, 96),
+    ([64, 200], None, 10, 2, 40),
+    ([700], None, 2, 2, 128),
+    ([90, 31], None, 7, 1, 24),
+    ([5, 60, 0, 33], [300, 60, 7, 40], 6, 3, 80),  # later parts of prompts
+    ([40, 9], [10, 0], 4, 2, 64),  # queries before the first key
+    ([33], [1000], 130, 1, 16),  # a group over 128: CUDA cores
+]
+
+
+@pytest.mark.parametrize("causal", (True, False))
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("case", PROMPTS, ids=range(len(PROMPTS)))
+def test_prompt_attention(case, dtype, causal):
+    q_lens, k_lens, heads, kv_heads, dim = case
+    q = (torch.randn(sum(q_lens), heads, dim) * 2).to(dtype)
+    k, v = (torch.randn(sum(k_lens or q_lens), kv_heads, dim).to(dtype) for _ in range(2))
+    wide = torch.int64 if dim == 64 else torch.int32
+
+    def offsets(lens):
+        return index([sum(lens[:i]) for i in range(len(lens) + 1)], wide)
+
+    scale = 0.6 * dim**-0.5
+    got, lse = programs.prompt_attention(dev(q), dev(k), dev(v), offsets(q_lens), offsets(k_lens) if k_lens else None,
+                                         is_causal=causal, scale=scale, return_lse=True)
+    assert device_status() == 0 and got.dtype == dtype
+    check_prompt(q, k, v, q_lens, k_lens or q_lens, scale, causal, got, lse, dtype)
+    assert torch.equal(programs.prompt_attention(dev(q), dev(k), dev(v), offsets(q_lens),
+                                                 offsets(k_lens) if k_lens else None, causal, scale), got)
+
+
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+def test_prompt_attention_many_sequences_and_scores_far_apart(dtype):
+    """More items than SMs, lengths of every kind, rows whose maximum moves block by block."""
+    lens = [int(n) for n in torch.randint(0, 400, (40,))] + [1500]
+    heads, kv_heads, dim = 8, 4, 128
+    q = torch.randn(sum(lens), heads, dim).to(dtype)
+    k = (torch.randn(sum(lens), kv_heads, dim) * torch.linspace(0.1, 12.0, sum(lens))[:, None, None]).to(dtype)
+    v = torch.randn(sum(lens), kv_heads, dim).to(dtype)
+    offsets = index([sum(lens[:i]) for i in range(len(lens) + 1)])
+    got, lse = programs.prompt_attention(dev(q), dev(k), dev(v), offsets, return_lse=True)
+    check_prompt(q, k, v, lens, lens, dim**-0.5, True, got, lse, dtype)
+
+
+@pytest.mark.parametrize("scale", (0.0, -0.3))
+def test_prompt_attention_scale_not_positive(scale):
+    q, k, v = torch.randn(3, 70, 2, 32).half()
+    got, lse = programs.prompt_attention(dev(q), dev(k), dev(v), index([0, 70]), scale=scale, return_lse=True)
+    check_prompt(q, k, v, [70], [70], scale, True, got, lse, torch.float16)
+
+
+def test_prompt_attention_strides():
+    """Views of a fused projection, an output between other heads, an element stride, a base off the 16-byte grid."""
+    lens, heads, kv_heads, dim = [50, 150], 4, 2, 64
+    qkv = torch.randn(200, heads + 2 * kv_heads, dim).half()
+    q, k, v = qkv.split((heads, kv_heads, kv_heads), 1)
+    offsets = index([0, 50, 200])
+    parts = dev(qkv).split((heads, kv_heads, kv_heads), 1)
+    out = torch.zeros(heads + 2, 200, dim, dtype=torch.float16, device="cuda").transpose(0, 1)
+    lse = torch.zeros(heads, 200, device="cuda").T
+    programs.prompt_attention_kernel(*parts, offsets, offsets, out[:, 1:-1], lse)
+    check_prompt(q, k, v, lens, lens, dim**-0.5, True, out[:, 1:-1], lse, torch.float16)
+    assert not out[:, 0].any() and not out[:, -1].any()
+    spread = torch.stack((dev(qkv), dev(qkv)), dim=-1)[..., 0].split((heads, kv_heads, kv_heads), 1)
+    got, lse = programs.prompt_attention(*spread, offsets, return_lse=True)
+    check_prompt(q, k, v, lens, lens, dim**-0.5, True, got, lse, torch.float16)
+    odd = torch.zeros(qkv.numel() + 1, dtype=torch.float16, device="cuda")[1:].view(qkv.shape).copy_(qkv)
+    got, lse = programs.prompt_attention(*odd.split((heads, kv_heads, kv_heads), 1), offsets, return_lse=True)
+    check_prompt(q, k, v, lens, lens, dim**-0.5, True, got, lse, torch.float16)
+
+
+@pytest.mark.parametrize("dtype", (torch.float16, torch.float32))
+def test_prompt_attention_not_finite_where_it_is_not_seen(dtype):
+    """NaN and infinities in keys and values of later tokens, of the next sequence
+    and of tokens of no sequence reach nobody who does not see them."""
+    lens, heads, kv_heads, dim = [200, 70], 4, 2, 128
+    q, k, v = (torch.randn(300, n, dim).to(dtype) for n in (heads, kv_heads, kv_heads))
+    offsets = index([0, 200, 270])
+    clean = programs.prompt_attention(dev(q), dev(k), dev(v), offsets).cpu()
+    for bad in (math.nan, math.inf):
+        k2, v2 = k.clone(), v.clone()
+        k2[270:], v2[270:] = bad, bad
+        v2[150, 1, 3] = bad
+        v2[190:200, 0] = bad
+        k2[195, 0] = bad
+        got = programs.prompt_attention(dev(q), dev(k2), dev(v2), offsets).cpu()
+        assert not got[150:200, 2:, 3].isfinite().any() and not got[190:200, :2].isfinite().any()
+        same = torch.ones(270, heads, dim, dtype=torch.bool)
+        same[150:200, 2:, 3] = False
+        same[190:200, :2] = False
+        # rows whose sums met the bad values were taken again on other units
+        near = (got[:270] - clean[:270]).abs() <= 2.0**-8 * (1 + clean[:270].abs())
+        assert near[same].all()
+
+
+def test_prompt_attention_offsets_out_of_range():
+    q = torch.randn(64, 2, 64).half().cuda()
+    good = programs.prompt_attention(q, q, q, index([0, 64]))
+    for bad in ([0, 65], [-1, 64], [0, 40, 30]):
+        programs.prompt_attention(q, q, q, index(bad))
+        assert device_status() == INDEX_OUT_OF_RANGE
+        programs.prompt_attention(q.float(), q.float(), q.float(), index(bad))
+        assert device_status() == INDEX_OUT_OF_RANGE
+    assert torch.equal(programs.prompt_attention(q, q, q, index([0, 64])), good)
+
+
+def test_joined_by_lse():
+    """Attention over a cached beginning and over a prompt's rest, joined by
+    their lse, is attention over both."""
+    kept, new, heads, kv_heads, dim = 100, 30, 4, 2, 64
+    cache = filled_cache([kept], 16, kv_heads, dim, torch.int8)
+    q, k, v = (torch.randn(new, n, dim).half() for n in (heads, kv_heads, kv_heads))
+    # every new query sees all that is cached: each as a sequence of its own
+    table = index(cache.table.tolist()).repeat(new, 1)
+    a, la = programs.paged_attention(dev(q)[:, None], *cache.args, table, index([kept] * new), return_lse=True)
+    b, lb = programs.prompt_attention(dev(q), dev(k), dev(v), index([0, new]), return_lse=True)
+    la, lb = la[:, 0].cpu().double(), lb.cpu().double()
+    both = torch.logaddexp(la, lb)
+    joined = (a[:, 0].cpu() * torch.exp(la - both)[..., None] + b.cpu() * torch.exp(lb - both)[..., None])
+    old = [codes * scales[..., None] for codes, scales in (cache.tokens(name, 0, kept) for name in ("key", "value"))]
+    k2, v2 = (torch.cat((x, y.double())) for x, y in zip(old, (k, v)))
+    top = float(v2.abs().max())
+    for i in range(new):
+        for h in range(heads):
+            want, want_lse = softmax_rows(q[i, h].double(), k2[:, h // 2], v2[:, h // 2], dim**-0.5, kept + 1 + i)
+            assert abs(both[i, h] - want_lse) < 1e-4
+            assert ((joined[i, h] - want).abs() <= 2.0**-10 * (top + want.abs())).all()
+
+
 def test_serving_refusals():
     x = torch.zeros(4, 2, 32, dtype=torch.float16, device="cuda")
     cos = torch.zeros(8, 16, device="cuda")
@@ -552,6 +717,20 @@ def test_serving_refusals():
     ):
         with pytest.raises(TypeError, match=message):
             programs.paged_attention(**(fine | change))
+    ok = dict(query=x, key=x, value=x, offsets=index([0, 4]))
+    programs.prompt_attention(**ok)
+    for change, message in (
+        (dict(key=x[:, :1]), "disagree"),
+        (dict(key=x[..., :16], value=x[..., :16]), "disagree"),
+        (dict(query=x[:, :1]), "disagree"),
+        (dict(value=x.float()), "share one dtype"),
+        (dict(offsets=index([])), "offsets"),
+        (dict(key_offsets=index([0, 2, 4])), "offsets"),
+        (dict(key_offsets=index([0, 4], torch.int64)), "share one dtype"),
+        (dict(offsets=index([[0, 4]])), "rank"),
+    ):
+        with pytest.raises(TypeError, match=message):
+            programs.prompt_attention(**(ok | change))
     with pytest.raises(TypeError, match="unit stride"):
         wide = torch.zeros(4, 2, 16, 64, dtype=torch.int8, device="cuda")[..., ::2]
         programs.paged_append(**(good | dict(key_cache=wide, value_cache=wide)))
