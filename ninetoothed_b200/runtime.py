@@ -38,8 +38,11 @@ FP8_DTYPES = tuple(getattr(torch, name) for name in ("float8_e4m3fn", "float8_e5
 GEMM_DTYPES = HALF_DTYPES + FP8_DTYPES + (torch.float32,)
 
 
+_DTYPE_CODES = {getattr(torch, name): code for name, code in _lib.DTYPE_CODES.items() if hasattr(torch, name)}
+
+
 def dtype_code(dtype: torch.dtype) -> int:
-    return _lib.DTYPE_CODES[str(dtype).split(".")[-1]]
+    return _DTYPE_CODES[dtype]
 
 
 @dataclass(frozen=True)
@@ -74,21 +77,25 @@ class Kernel:
     meta: tuple = ()
     meta_defaults: dict = field(default_factory=dict)
 
-    @property
-    def public_args(self) -> tuple:
-        return tuple(arg.name for arg in self.args)
+    def __post_init__(self):
+        # what every call looks up, once
+        self.public_args = tuple(arg.name for arg in self.args)
+        self._tensor_args = tuple(arg for arg in self.args if isinstance(arg, TensorArg))
+        self._accepted = frozenset(self.public_args) | frozenset(self.meta)
+        self._required = self.public_args + tuple(self.meta)
 
     def __call__(self, *args, **kwargs):
         values = self._public_values(args, kwargs)
         device = self._validate(values)
         output = values[self.outputs[0]] if self.outputs else None
-        if any(values[name].numel() == 0 for name in self.outputs):
-            return output
+        for name in self.outputs:
+            if values[name].numel() == 0:
+                return output
         if device.index == torch.cuda.current_device():
-            code = self.launch(values, torch.cuda.current_stream(device).cuda_stream)
+            code = self.launch(values, current_raw_stream(device.index))
         else:
             with torch.cuda.device(device):
-                code = self.launch(values, torch.cuda.current_stream(device).cuda_stream)
+                code = self.launch(values, current_raw_stream(device.index))
         if code != 0:
             raise KernelLaunchError(code)
         return output
@@ -98,27 +105,25 @@ class Kernel:
         public = self.public_args
         if len(args) > len(public):
             raise TypeError(f"Expected at most {len(public)} arguments.")
-        positional = public[: len(args)]
-        duplicates = tuple(name for name in positional if name in kwargs)
-        if duplicates:
-            raise TypeError(f"Kernel arguments passed twice: {', '.join(sorted(duplicates))}.")
-        accepted = set(public) | set(self.meta)
-        unknown = tuple(name for name in kwargs if name not in accepted)
-        if unknown:
-            raise TypeError(f"Unknown kernel arguments: {', '.join(sorted(unknown))}.")
+        if kwargs:
+            positional = public[: len(args)]
+            duplicates = tuple(name for name in positional if name in kwargs)
+            if duplicates:
+                raise TypeError(f"Kernel arguments passed twice: {', '.join(sorted(duplicates))}.")
+            unknown = tuple(name for name in kwargs if name not in self._accepted)
+            if unknown:
+                raise TypeError(f"Unknown kernel arguments: {', '.join(sorted(unknown))}.")
         values = dict(self.meta_defaults)
         values.update(zip(public, args))
         values.update(kwargs)
-        missing = tuple(name for name in public + tuple(self.meta) if name not in values)
-        if missing:
+        if len(values) < len(self._required):
+            missing = tuple(name for name in self._required if name not in values)
             raise TypeError(f"Missing kernel arguments: {', '.join(missing)}.")
         return values
 
     def _validate(self, values) -> torch.device:
         device = None
-        for arg in self.args:
-            if not isinstance(arg, TensorArg):
-                continue
+        for arg in self._tensor_args:
             value = values[arg.name]
             if value is None and arg.optional:
                 continue
@@ -128,11 +133,12 @@ class Kernel:
                 raise TypeError(
                     f"Kernel argument `{arg.name}` has rank {value.dim()}; expected {arg.ndim}."
                 )
-            if value.device.type != "cuda":
-                raise TypeError(f"Kernel argument `{arg.name}` must be on a CUDA device.")
-            if device is not None and value.device != device:
-                raise TypeError("All tensor arguments must use the same CUDA device.")
-            device = value.device
+            if device is None or value.device != device:
+                if value.device.type != "cuda":
+                    raise TypeError(f"Kernel argument `{arg.name}` must be on a CUDA device.")
+                if device is not None:
+                    raise TypeError("All tensor arguments must use the same CUDA device.")
+                device = value.device
             if value.dtype not in arg.dtypes:
                 expected = ", ".join(str(d).split(".")[-1] for d in arg.dtypes)
                 raise TypeError(
@@ -144,13 +150,22 @@ class Kernel:
         return device
 
 
+def _public_raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# The caller's current CUDA stream on a device, as an address.  torch's own
+# lookup of it takes a tenth of the time of building a Stream object.
+current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _public_raw_stream)
+
+
 def ptr(tensor: torch.Tensor) -> int:
     return tensor.data_ptr()
 
 
 def check_same_dtype(values, names):
-    dtypes = {values[name].dtype for name in names}
-    if len(dtypes) != 1:
+    dtype = values[names[0]].dtype
+    if any(values[name].dtype != dtype for name in names):
         listing = ", ".join(f"`{name}`" for name in names)
         raise TypeError(f"Kernel arguments {listing} must share one dtype.")
 

@@ -115,7 +115,7 @@ def rotary(input, cos, sin, positions, interleaved=False, adjoint=False):
     Pairs are (i, i + half) or, interleaved, (2i, 2i + 1).  `adjoint` applies
     the transposed rotation: given the gradient of the output it returns the
     gradient of the input."""
-    output = torch.empty(input.shape, dtype=input.dtype, device=input.device)
+    output = torch.empty_like(input, memory_format=torch.contiguous_format)
     return rotary_kernel(input, cos, sin, positions, output, interleaved=interleaved, adjoint=adjoint)
 
 
@@ -239,8 +239,8 @@ def paged_append(key, value, offsets, past, block_table, key_cache, value_cache,
     rotated too and returned; `return_key` also returns the rotated key in its
     own dtype (a prompt's attention reads it).  What was not asked for is None.
     """
-    query_out = None if query is None else torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    key_out = torch.empty(key.shape, dtype=key.dtype, device=key.device) if return_key else None
+    query_out = None if query is None else torch.empty_like(query, memory_format=torch.contiguous_format)
+    key_out = torch.empty_like(key, memory_format=torch.contiguous_format) if return_key else None
     paged_append_kernel(key, value, offsets, past, block_table, key_cache, value_cache, key_scale, value_scale,
                         query, cos, sin, query_out, key_out, interleaved=interleaved)
     return query_out, key_out
@@ -267,7 +267,7 @@ def _launch_paged_attention(v, stream):
         raise TypeError("paged_attention lse must have the query's shape without the head dimension.")
     lib = _lib.library()
     nbytes = lib.nt_b200_paged_attention_workspace_size()
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
+    workspace = query.new_empty(nbytes, dtype=torch.uint8)
     args = _lib.pack_args(
         *cache, query.data_ptr(), lengths.data_ptr(), table.data_ptr(), out.data_ptr(),
         0 if lse is None else lse.data_ptr(), workspace.data_ptr(), nbytes, batch, queries, heads, table.shape[1],
@@ -311,8 +311,8 @@ def paged_attention(query, key_cache, value_cache, key_scale, value_scale, block
     (output, lse): the fp32 natural logarithm of each query's sum of exponentials
     [batch, queries, heads], by which attention over separate keys is joined.  A
     query that sees no token gets 0, and -inf as its lse."""
-    output = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    lse = torch.empty(query.shape[:3], dtype=torch.float32, device=query.device) if return_lse else None
+    output = torch.empty_like(query, memory_format=torch.contiguous_format)
+    lse = query.new_empty(query.shape[:3], dtype=torch.float32) if return_lse else None
     paged_attention_kernel(query, key_cache, value_cache, key_scale, value_scale, block_table, lengths, output, lse,
                            scale=scale)
     return (output, lse) if return_lse else output
@@ -340,7 +340,7 @@ def _launch_prompt_attention(v, stream):
         raise TypeError("prompt_attention lse must have the query's shape without the head dimension.")
     lib = _lib.library()
     nbytes = lib.nt_b200_prompt_attention_workspace_size(tokens, batch, heads, kv_heads)
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
+    workspace = query.new_empty(nbytes, dtype=torch.uint8)
     args = _lib.pack_args(
         query.data_ptr(), key.data_ptr(), value.data_ptr(), query_offsets.data_ptr(), key_offsets.data_ptr(),
         out.data_ptr(), 0 if lse is None else lse.data_ptr(), workspace.data_ptr(), nbytes, tokens, key.shape[0], batch,
@@ -382,8 +382,8 @@ def prompt_attention(query, key, value, offsets, key_offsets=None, is_causal=Tru
     dtype, or with `return_lse` (output, lse): the fp32 natural logarithm of each
     query's sum of exponentials [tokens, heads].  A query that sees no key gets
     0, and -inf as its lse; tokens that belong to no sequence are not written."""
-    output = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    lse = torch.empty(query.shape[:2], dtype=torch.float32, device=query.device) if return_lse else None
+    output = torch.empty_like(query, memory_format=torch.contiguous_format)
+    lse = query.new_empty(query.shape[:2], dtype=torch.float32) if return_lse else None
     prompt_attention_kernel(query, key, value, offsets, offsets if key_offsets is None else key_offsets, output, lse,
                             is_causal=is_causal, scale=scale)
     return (output, lse) if return_lse else output
