@@ -327,9 +327,9 @@ typedef struct NtB200RotaryArgs {
 int nt_b200_rotary(const NtB200RotaryArgs *args, void *stream);
 
 /*
- * A paged cache: `pages` pages of `page` tokens each (a multiple of 16), codes
- * of `code_dtype` (FLOAT8_E4M3FN or INT8) in key and value [pages, kv_heads,
- * page, head_dim] with unit element stride, head_dim a multiple of 16, every
+ * A paged cache: `pages` pages of `page` tokens each (a multiple of 16, at most
+ * 4096), codes of `code_dtype` (FLOAT8_E4M3FN or INT8) in key and value [pages,
+ * kv_heads, page, head_dim] with unit element stride, head_dim a multiple of 16, every
  * other stride and both bases multiples of 16; one fp32 scale for each page and
  * head.  A stored element stands for code * scale.
  */

@@ -11,10 +11,14 @@
 //
 // The work is one line of 32-token steps: sequence by sequence, within it
 // (kv head, row tile) unit by unit.  The line is cut into equal pieces, one a
-// CTA, so that any mix of lengths keeps every SM busy to the end; a unit that
-// lies in one piece is finished there, the others leave their parts (o, m, l)
-// in a workspace and a second kernel joins them.  Warps of a CTA take the steps
-// of a unit in turn and are joined through shared memory at its end.
+// CTA, and a piece into equal shares, one a warp, so that any mix of lengths
+// keeps every SM busy to the end and no warp waits for another; a unit that
+// lies in one share is finished there.  Of the others, a CTA joins at its end
+// what neighbouring warps hold of one unit, and leaves its parts (o, m, l) in a
+// workspace; a second kernel joins those.  (Warps that took the steps of a unit
+// in turn and joined at the end of every unit took 108 us where this takes
+// DRAFT_US for 256 units of up to 2047 tokens: short units cost a CTA as much as
+// long ones.)
 //
 // A warp's step, S^T = K Q^T and O^T += V^T P^T on 16x8x16 tensor-core
 // instructions with the cached tokens (head elements) as the 16 rows and 8
@@ -66,23 +70,24 @@ struct Attention {
   int64_t table_row_stride;
   int64_t q_batch, q_token, q_head, q_dim, o_batch, o_token, o_head, o_dim, l_batch, l_token, l_head;
   int64_t k_page, k_head, k_token, v_page, v_head, v_token, ks_page, ks_head, vs_page, vs_head;
-  int64_t pages, capacity;  // tokens a block table row can hold
+  int64_t pages;
+  int capacity;  // tokens a block table row can hold
   int batch, queries, heads, kv_heads, group, head_dim, page;
+  int page_groups;          // page / 16
+  uint64_t page_reciprocal; // ceil(2^36 / page_groups)
   int rows, row_tiles;      // queries * group; tiles of them
   float scale;              // softmax scale * log2 e
-  float *parts;             // workspace: two parts a CTA
-  int64_t least;            // fewest steps of a piece
-  int whole;                // one CTA a unit, nothing to join
+  float *parts;             // workspace: two parts a warp
 };
 
 // The cached length of a sequence, in its block table's capacity.
-__device__ __forceinline__ int64_t cached_length(const Attention &a, int64_t b) {
+__device__ __forceinline__ int cached_length(const Attention &a, int64_t b) {
   const int64_t n = a.lengths[b];
   if (n < 0 || n > a.capacity) {
     record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
     return n < 0 ? 0 : a.capacity;
   }
-  return n;
+  return (int)n;
 }
 
 // The page of column `column` of sequence b's block table, or -1.
@@ -149,7 +154,13 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(Attention a) {
 }
 
 // ---------------------------------------------------------------- tensor cores
-constexpr int WARPS = 8, STEP = 32;
+constexpr int STEP = 32;
+constexpr int LEAST_STEPS = 2;  // of a CTA: fewer would be parts to join rather than work
+// A block table row's tokens that are looked at; a page's size.  With them the
+// block table column of a 16-token group is one multiplication: for g < 2^27
+// groups and d = page / 16 <= 2^8, floor(g ceil(2^36 / d) / 2^36) = floor(g / d).
+constexpr int64_t MOST_TOKENS = (1LL << 31) - 64;
+constexpr int MOST_PAGE = 4096;
 
 __device__ __forceinline__ void copy_async16(uint32_t to, const void *from, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid ? 16 : 0) : "memory");
@@ -218,19 +229,20 @@ template <> __device__ __forceinline__ void to_halves<int8_t>(uint32_t w, uint32
 
 template <int DP, int NT> struct Layout {
   static constexpr int ROWS = 8 * NT;
-  static constexpr int STAGES = NT == 1 ? 3 : 2;
+  // One column tile: 12 warps of up to 168 registers, three a scheduler, to
+  // cover each other's load and MMA latency (8 warps: 2.45 TB/s where 12 reach
+  // RATE).  Two column tiles hold twice the accumulators: 8 warps.
+  static constexpr int WARPS = NT == 1 ? 12 : 8;
+  static constexpr int STAGES = DP == 64 ? 4 : NT == 1 ? 2 : 3;
   static constexpr int K_COPIES = DP / 64 * 4;              // 16-byte words a lane and step
   static constexpr int V_WORD = DP / 8;                     // bytes of a token's value a lane takes
   static constexpr int K_BYTES = STEP * DP, V_BYTES = STEP * DP;
   static constexpr int STAGE = K_BYTES + V_BYTES + 32;      // + 2 key scales, 2 value scales
-  static constexpr int RING = WARPS * STAGES * STAGE;
-  static constexpr int PITCH = DP + 4;                      // of a row's partial output, in floats
-  static constexpr int JOIN = WARPS * ROWS * PITCH * 4;
-  static constexpr int STATS = WARPS * ROWS * 3 * 4;
-  static constexpr int SMEM = RING + JOIN + STATS + 64;
+  static constexpr int SMEM = WARPS * STAGES * STAGE;
   // a part in the workspace: o [ROWS][DP], then m, l, mo [ROWS]
   static constexpr int PART = ROWS * (DP + 3);
-  static_assert(SMEM <= 232448, "shared memory of a CTA");
+  static_assert(SMEM + 256 <= 232448, "shared memory of a CTA");
+  static_assert(PART * 4 <= STAGES * STAGE, "a warp's part fits its ring");
 };
 
 // A value's NaN reaches only the rows that see its token, but 0 * NaN in an MMA
@@ -239,7 +251,7 @@ template <int DP, int NT> struct Layout {
 // 8 (i / 2) in v[i], as loaded) and set into the rows' O here.
 template <int DP, int NT>
 __device__ __forceinline__ void separate_nans(uint32_t (&v)[4][DP / 32], float (&o)[NT][DP / 16][4],
-                                              const int64_t (&limit)[NT][2], int64_t token0) {
+                                              const int (&limit)[NT][2], int token0) {
   uint32_t any = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -259,7 +271,7 @@ __device__ __forceinline__ void separate_nans(uint32_t (&v)[4][DP / 32], float (
     }
     for (int c = 0; c < 4; ++c) {
       const uint32_t other = __shfl_sync(0xffffffffu, mask, (lane & ~3) | c);
-      const int64_t token = token0 + 2 * c + (i & 1) + 8 * (i >> 1);
+      const int token = token0 + 2 * c + (i & 1) + 8 * (i >> 1);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -271,215 +283,257 @@ __device__ __forceinline__ void separate_nans(uint32_t (&v)[4][DP / 32], float (
   }
 }
 
-// Where a walk along the line of steps stands: sequence b, `at` steps into its
-// units * n, `left` steps to go in the piece.
+// Where a walk along the line of steps stands: before step s of a unit of
+// sequence b (n steps a unit), `left` steps to go in the piece.
 struct Walk {
-  int64_t at, left, length;
-  int b, n;  // n: steps of one unit of the sequence
+  int64_t left;
+  int b, length, n, unit, s;
 };
 struct Segment {  // steps [s0, s1) of one unit
-  int64_t length;
-  int b, unit, s0, s1, n;
+  int length, b, head, tile, s0, s1, n;
 };
 
-__device__ __forceinline__ int steps_of(int64_t length) { return (int)((length + STEP - 1) / STEP); }
+__host__ __device__ __forceinline__ int steps_of(int64_t length) { return (int)((length + STEP - 1) / STEP); }
 
 __device__ __forceinline__ bool next_segment(const Attention &a, Walk &w, Segment &g) {
   if (w.left <= 0) return false;
-  const int units = a.kv_heads * a.row_tiles;
-  while (w.at >= (int64_t)w.n * units) {
-    w.at -= (int64_t)w.n * units;
+  while (w.n == 0 || w.unit >= a.kv_heads * a.row_tiles) {
     if (++w.b >= a.batch) return false;
     w.length = cached_length(a, w.b);
     w.n = steps_of(w.length);
+    w.unit = w.s = 0;
   }
   g.b = w.b;
   g.length = w.length;
   g.n = w.n;
-  g.unit = (int)(w.at / w.n);
-  g.s0 = (int)(w.at - (int64_t)g.unit * w.n);
-  const int64_t take = w.left < g.n - g.s0 ? w.left : g.n - g.s0;
-  g.s1 = g.s0 + (int)take;
-  w.at += take;
+  g.head = w.unit / a.row_tiles;
+  g.tile = w.unit % a.row_tiles;
+  g.s0 = w.s;
+  const int take = w.left < w.n - w.s ? (int)w.left : w.n - w.s;
+  g.s1 = g.s0 + take;
   w.left -= take;
+  w.s += take;
+  if (w.s == w.n) {
+    w.s = 0;
+    ++w.unit;
+  }
   return true;
 }
 
-// Steps of all sequences below `end`, by a whole block (shared: one int64 a warp).
-template <int THREADS>
-__device__ __forceinline__ int64_t steps_below(const Attention &a, int64_t end, int64_t *shared) {
+// Steps of one unit of sequence b; 0 past the last sequence.
+__device__ __forceinline__ int64_t unit_steps(const Attention &a, int64_t b) {
+  const int64_t n = b < a.batch ? a.lengths[b] : 0;
+  return n <= 0 ? 0 : steps_of(n < a.capacity ? n : a.capacity);
+}
+
+// Steps of the line up to sequence `end`; every lane of a warp gets the sum.
+__device__ __forceinline__ int64_t steps_below(const Attention &a, int64_t end) {
   int64_t sum = 0;
-  for (int64_t b = threadIdx.x; b < end; b += THREADS) {
-    const int64_t n = a.lengths[b];
-    sum += n <= 0 ? 0 : steps_of(n < a.capacity ? n : a.capacity);
-  }
+  for (int64_t b = threadIdx.x & 31; b < end; b += 32) sum += unit_steps(a, b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = sum;
-  __syncthreads();
-  sum = 0;
-#pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i) sum += shared[i];
   return sum * a.kv_heads * a.row_tiles;
 }
 
-// Steps of a piece: total / pieces, at least `least`.
-__device__ __forceinline__ int64_t piece_of(int64_t total, int64_t pieces, int64_t least) {
-  const int64_t q = (total + pieces - 1) / pieces;
-  return q > least ? q : least;
+// The cut of a line of `total` steps: `cta` steps a CTA, `warp` a warp.
+struct Cut {
+  int64_t total, cta, warp;
+};
+__device__ __forceinline__ Cut cut_line(const Attention &a, int64_t ctas, int warps) {
+  Cut c;
+  c.total = steps_below(a, a.batch);
+  c.cta = (c.total + ctas - 1) / ctas;
+  if (c.cta < LEAST_STEPS) c.cta = LEAST_STEPS;
+  c.warp = (c.cta + warps - 1) / warps;
+  return c;
 }
 
-// Four elements of a finished row: o = acc * 2^(mo - m) / l, and its lse.
-template <typename T>
-__device__ __forceinline__ void write_row(const Attention &a, int64_t b, int h, int row, int d, const float (&acc)[4],
+// N neighbouring elements of a finished row: o = acc * 2^(mo - m) / l, and the
+// row's lse.
+template <typename T, int N>
+__device__ __forceinline__ void write_row(const Attention &a, int64_t b, int h, int row, int d, const float (&acc)[N],
                                           float m, float l, float mo) {
   if (row >= a.rows || d >= a.head_dim) return;
   const int i = row / a.group, hq = h * a.group + row % a.group;
   const float f = l == 0.f ? 0.f : exp2_fast(reference(mo) - reference(m)) / l;
-  T *out = static_cast<T *>(a.out) + b * a.o_batch + i * a.o_token + (int64_t)hq * a.o_head;
+  T *out = static_cast<T *>(a.out) + b * a.o_batch + i * a.o_token + (int64_t)hq * a.o_head + d * a.o_dim;
+  if (a.o_dim == 1 && (reinterpret_cast<uintptr_t>(out) & (2 * N - 1)) == 0) {
+    struct alignas(2 * N) Pack { T v[N]; } pack;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) out[(d + e) * a.o_dim] = from_f<T>(acc[e] * f);
+    for (int e = 0; e < N; ++e) pack.v[e] = from_f<T>(acc[e] * f);
+    *reinterpret_cast<Pack *>(out) = pack;
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e * a.o_dim] = from_f<T>(acc[e] * f);
+  }
   if (a.lse && d == 0)
     a.lse[b * a.l_batch + i * a.l_token + (int64_t)hq * a.l_head] = l == 0.f ? -INFINITY : (m + log2_fast(l)) * kLn2;
 }
 
+// A lane's elements of one of its rows, in order.
+template <int DP, int NT>
+__device__ __forceinline__ void row_of(const float (&o)[NT][DP / 16][4], int nt, int u, float (&acc)[DP / 8]) {
+#pragma unroll
+  for (int t = 0; t < DP / 16; ++t) {
+    acc[2 * t] = o[nt][t][u];
+    acc[2 * t + 1] = o[nt][t][u + 2];
+  }
+}
+
+// A warp's part of a unit: o [ROWS][DP], then m, l, mo of each row.
+template <int DP, int NT>
+__device__ __forceinline__ void write_part(float *part, const float (&o)[NT][DP / 16][4], const float (&m)[NT][2],
+                                           const float (&l)[NT][2], const float (&mo)[NT][2]) {
+  const int lane = threadIdx.x & 31, n8 = lane >> 2, c4 = lane & 3;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int row = nt * 8 + 2 * c4 + u;
+      float acc[DP / 8];
+      row_of<DP, NT>(o, nt, u, acc);
+#pragma unroll
+      for (int e = 0; e < DP / 8; e += 4)
+        *reinterpret_cast<float4 *>(part + row * DP + n8 * (DP / 8) + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+      if (n8 == 0) {
+        float *st = part + 8 * NT * DP + row * 3;
+        st[0] = m[nt][u];
+        st[1] = l[nt][u];
+        st[2] = mo[nt][u];
+      }
+    }
+}
+
+// What a warp holds at the end of its share: a part of `unit` (-1: none), and
+// whether that is all the share has.
+struct Held {
+  int64_t unit;
+  bool only;
+};
+
+// The maxima that P is taken against move only when a score passes them by
+// this (base 2): P, up to 2^LEAD, stays in fp16's range and as precise, a step's
+// scores are compared in their own threads, and the reduction over the threads
+// of a row and the rescaling of O happen rarely.
+constexpr float LEAD = 8.f;
+
 template <typename T, typename C, int DP, int NT>
-__global__ void __launch_bounds__(WARPS * 32, 1) attention_kernel(const __grid_constant__ Attention a) {
+__global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kernel(const __grid_constant__ Attention a) {
   using L = Layout<DP, NT>;
+  constexpr int WARPS = L::WARPS;
   constexpr int KS = DP / 16, OT = DP / 16;  // contraction steps of QK; 16-element tiles of O
   extern __shared__ __align__(16) uint8_t smem[];
-  float *join = reinterpret_cast<float *>(smem + L::RING);
-  float *stats = reinterpret_cast<float *>(smem + L::RING + L::JOIN);
-  int64_t *reduce = reinterpret_cast<int64_t *>(smem + L::RING + L::JOIN + L::STATS);
+  __shared__ Held runs[WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n8 = lane >> 2, c4 = lane & 3;
   const uint32_t ring = ptx::smem_u32(smem) + warp * L::STAGES * L::STAGE;
   wait_prior_grid();
   allow_dependent_launch();
 
-  // this CTA's piece of the line
+  // this warp's share of the line
+  const Cut cut = cut_line(a, gridDim.x, WARPS);
+  int64_t first = blockIdx.x * cut.cta + warp * cut.warp;
+  const int64_t end = min(cut.total, min(first + cut.warp, (blockIdx.x + 1) * cut.cta));
   Walk start{};
-  if (a.whole) {
+  start.left = first < end ? end - first : 0;
+  if (start.left > 0) {
+    // the sequence that holds step `first`, 32 sequences at a time
     const int units = a.kv_heads * a.row_tiles;
-    start.b = blockIdx.x / units;
-    start.length = cached_length(a, start.b);
-    start.n = steps_of(start.length);
-    start.at = (int64_t)(blockIdx.x % units) * start.n;
-    start.left = start.n;
-  } else {
-    const int64_t total = steps_below<WARPS * 32>(a, a.batch, reduce);
-    const int64_t piece = piece_of(total, gridDim.x, a.least);
-    int64_t first = blockIdx.x * piece;
-    if (first >= total) return;
-    start.left = total - first < piece ? total - first : piece;
-    // the sequence that holds step `first`: 256 sequences at a time, each
-    // warp's 32 summed, then the lanes of the warp that holds it
-    const int units = a.kv_heads * a.row_tiles;
-    for (int64_t b0 = 0;; b0 += WARPS * 32) {
-      const int64_t b = b0 + threadIdx.x;
-      int64_t n = b < a.batch ? a.lengths[b] : 0;
-      n = n <= 0 ? 0 : (int64_t)steps_of(n < a.capacity ? n : a.capacity) * units;
+    for (int64_t b0 = 0;; b0 += 32) {
+      const int64_t n = unit_steps(a, b0 + lane) * units;
       int64_t up = n;  // inclusive sum over the lanes
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t x = __shfl_up_sync(0xffffffffu, up, o);
         if (lane >= o) up += x;
       }
-      __syncthreads();
-      if (lane == 31) reduce[warp] = up;
-      __syncthreads();
-      int64_t base = 0;
-      int found = -1;
-#pragma unroll
-      for (int i = 0; i < WARPS; ++i) {
-        if (found < 0) {
-          if (first < base + reduce[i]) found = i;
-          else base += reduce[i];
-        }
-      }
-      if (found < 0) {
-        first -= base;
+      const int which = __popc(__ballot_sync(0xffffffffu, up <= first));  // sums are nondecreasing
+      if (which == 32) {
+        first -= __shfl_sync(0xffffffffu, up, 31);
         continue;
       }
-      __syncthreads();
-      if (warp == found) {
-        const unsigned past = __ballot_sync(0xffffffffu, base + up <= first);
-        const int which = __popc(past);  // sums are nondecreasing
-        const int64_t before = __shfl_sync(0xffffffffu, up - n, which);
-        if (lane == 0) {
-          reduce[0] = b0 + warp * 32 + which;
-          reduce[1] = first - base - before;
-        }
-      }
-      __syncthreads();
-      start.b = (int)reduce[0];
-      start.at = reduce[1];
+      first -= __shfl_sync(0xffffffffu, up - n, which);
+      start.b = (int)(b0 + which);
       break;
     }
     start.length = cached_length(a, start.b);
     start.n = steps_of(start.length);
+    start.unit = (int)(first / start.n);
+    start.s = (int)(first - (int64_t)start.unit * start.n);
   }
 
   // ------------------------------------------------------------ loads ahead
   Walk ahead = start;
   Segment lseg{};
-  int lstep = 0;
   bool lmore = next_segment(a, ahead, lseg);
-  lstep = lseg.s0 + warp;
-  int64_t id0 = -1, id1 = -1;  // pages of the next step to load
+  int lstep = lseg.s0;
+  int64_t id0 = -1, id1 = -1;  // pages of the next step's two groups
+  int group0 = 0;              // the first group's place in its page
   auto find_pages = [&]() {
-    while (lmore && lstep >= lseg.s1) {
+    if (lmore && lstep >= lseg.s1) {
       lmore = next_segment(a, ahead, lseg);
-      lstep = lseg.s0 + warp;
+      lstep = lseg.s0;
     }
     if (!lmore) return;
-    const int64_t t = (int64_t)lstep * STEP;
-    const int64_t col = t / a.page;
+    const int g = lstep * (STEP / 16);
+    const int col = (int)(((uint64_t)g * a.page_reciprocal) >> 36);
+    group0 = g - col * a.page_groups;
     id0 = page_of(a, lseg.b, col);
-    const int64_t col1 = t % a.page + 16 == a.page ? col + 1 : col;
-    id1 = t + 16 < lseg.length ? (col1 == col ? id0 : page_of(a, lseg.b, col1)) : -1;
+    id1 = id0;
+    if (group0 + 1 == a.page_groups) id1 = (g + 1) * 16 < lseg.length ? page_of(a, lseg.b, col + 1) : -1;
   };
+  // this lane's share of a 16-token group
+  const int64_t k_lane = n8 * a.k_token + 16 * c4, v_lane = 2 * c4 * a.v_token + n8 * L::V_WORD;
+  const bool full_dim = a.head_dim == DP;
   auto issue = [&](int stage) {
     if (lmore) {
-      const int64_t t0 = (int64_t)lstep * STEP;
-      const int h = lseg.unit / a.row_tiles;
-      const uint32_t to = ring + stage * L::STAGE;
-      const int slot = (int)(t0 % a.page);
+      const uint32_t to = ring + stage * L::STAGE, to_k = to + lane * 16, to_v = to + L::K_BYTES + lane * L::V_WORD;
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        const int64_t base = t0 + 16 * g;
+        int live = lseg.length - (lstep * STEP + 16 * g);  // tokens of the group in the cache
         int64_t id = g == 0 ? id0 : id1;
-        const int64_t live64 = lseg.length - base;
-        int live = live64 > 16 ? 16 : (int)live64;  // tokens of the group in the cache
-        if (live > 0 && id < 0) record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
-        if (id < 0) { live = 0; id = 0; }
-        const int in_page = g == 0 ? slot : (slot + 16 == a.page ? 0 : slot + 16);
-        const uint8_t *k = a.key + id * a.k_page + (int64_t)h * a.k_head + (int64_t)in_page * a.k_token;
-        const uint8_t *v = a.value + id * a.v_page + (int64_t)h * a.v_head + (int64_t)in_page * a.v_token;
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int x = 0; x < DP / 64; ++x) {
-            const int token = n8 + 8 * r, d = x * 64 + 16 * c4;
-            const bool valid = token < live && d < a.head_dim;
-            copy_async16(to + (((g * 2 + r) * (DP / 64) + x) * 32 + lane) * 16, valid ? k + token * a.k_token + d : k, valid);
-          }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int token = 2 * c4 + (i & 1) + 8 * (i >> 1), d = n8 * L::V_WORD;
-          const bool valid = token < live && d < a.head_dim;
-          const uint32_t dst = to + L::K_BYTES + ((g * 4 + i) * 32 + lane) * L::V_WORD;
-          const uint8_t *src = valid ? v + token * a.v_token + d : v;
+        if (id < 0) {
+          if (live > 0) record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
+          live = 0;
+          id = 0;
+        }
+        const int in_page = (g == 0 ? group0 : group0 + 1 == a.page_groups ? 0 : group0 + 1) * 16;
+        const uint8_t *k = a.key + id * a.k_page + lseg.head * a.k_head + in_page * a.k_token + k_lane;
+        const uint8_t *v = a.value + id * a.v_page + lseg.head * a.v_head + in_page * a.v_token + v_lane;
+        const uint32_t tk = to_k + g * (2 * (DP / 64) * 512), tv = to_v + g * (4 * 32 * L::V_WORD);
+        auto copy_v = [&](uint32_t dst, const uint8_t *src, bool valid) {
           if constexpr (DP == 128) copy_async16(dst, src, valid);
           else copy_async8(dst, src, valid);
+        };
+        if (live >= 16 && full_dim) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int x = 0; x < DP / 64; ++x)
+              copy_async16(tk + (r * (DP / 64) + x) * 512, k + r * 8 * a.k_token + x * 64, true);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            copy_v(tv + i * 32 * L::V_WORD, v + ((i & 1) + 8 * (i >> 1)) * a.v_token, true);
+        } else {  // zeros for what is not there; its address stays inside
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int x = 0; x < DP / 64; ++x) {
+              const bool valid = n8 + 8 * r < live && x * 64 + 16 * c4 < a.head_dim;
+              copy_async16(tk + (r * (DP / 64) + x) * 512, valid ? k + r * 8 * a.k_token + x * 64 : a.key, valid);
+            }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool valid = 2 * c4 + (i & 1) + 8 * (i >> 1) < live && n8 * L::V_WORD < a.head_dim;
+            copy_v(tv + i * 32 * L::V_WORD, valid ? v + ((i & 1) + 8 * (i >> 1)) * a.v_token : a.value, valid);
+          }
         }
         if (lane < 2) {
-          const float *src = lane == 0 ? a.key_scale + id * a.ks_page + h * a.ks_head
-                                       : a.value_scale + id * a.vs_page + h * a.vs_head;
+          const float *src = lane == 0 ? a.key_scale + id * a.ks_page + lseg.head * a.ks_head
+                                       : a.value_scale + id * a.vs_page + lseg.head * a.vs_head;
           copy_async4(to + L::K_BYTES + L::V_BYTES + (lane * 2 + g) * 4, src, live > 0);
         }
       }
-      lstep += WARPS;
+      ++lstep;
     }
     copy_commit();
   };
@@ -494,15 +548,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_kernel(const __grid_c
 
   Walk here = start;
   Segment seg;
-  bool empty = a.whole && start.n == 0;  // a unit without keys, to be written all the same
-  while (true) {
-    if (empty) {
-      seg = Segment{0, start.b, (int)(blockIdx.x % (a.kv_heads * a.row_tiles)), 0, 0, 0};
-    } else if (!next_segment(a, here, seg)) {
-      break;
-    }
-    const int h = seg.unit / a.row_tiles, row0 = seg.unit % a.row_tiles * L::ROWS;
-    const bool at_start = seg.s0 == 0, at_end = seg.s1 == seg.n;
+  Held held{-1, false};
+  while (next_segment(a, here, seg)) {
+    const int row0 = seg.tile * L::ROWS;
 
     // Q: lane (n8, c4) holds row n8's elements 16 c4 .. + 15 of each 64, as
     // the B operand of contraction step 4 x + w: bytes 4w .. 4w + 3 of a key's
@@ -513,7 +561,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_kernel(const __grid_c
     for (int nt = 0; nt < NT; ++nt) {
       const int row = row0 + nt * 8 + n8;
       const bool valid = row < a.rows;
-      const int i = valid ? row / a.group : 0, hq = h * a.group + (valid ? row % a.group : 0);
+      const int i = valid ? row / a.group : 0, hq = seg.head * a.group + (valid ? row % a.group : 0);
       const T *q = static_cast<const T *>(a.query) + seg.b * a.q_batch + i * a.q_token + hq * a.q_head;
       float x[DP / 4], top = 0.f;
 #pragma unroll
@@ -535,9 +583,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_kernel(const __grid_c
         qf[nt][s][1] = half2_bits(x[e + 2] * inv, x[e + 3] * inv);
       }
     }
-    // of the rows 2 c4 and 2 c4 + 1 of each tile: score factor, keys seen
+    // of the rows 2 c4 and 2 c4 + 1 of each tile: score factor, maxima, sum,
+    // keys seen
     float factor[NT][2], m[NT][2], mo[NT][2], l[NT][2];
-    int64_t limit[NT][2];
+    int limit[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -547,29 +596,25 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_kernel(const __grid_c
         m[nt][u] = mo[nt][u] = -INFINITY;
         l[nt][u] = 0.f;
       }
-    const int64_t sure = seg.length - a.queries + 1 + row0 / a.group;  // keys that every row sees
+    const int sure = seg.length - a.queries + 1 + row0 / a.group;  // keys that every row sees
     float o[NT][OT][4] = {};
 
-    for (int step = seg.s0 + warp; step < seg.s1; step += WARPS) {
+    for (int step = seg.s0; step < seg.s1; ++step) {
       issue(stage == 0 ? L::STAGES - 1 : stage - 1);  // the stage read one step ago
       find_pages();
       copy_wait<L::STAGES - 1>();
       __syncwarp();  // the scales were copied by two lanes
-      const uint32_t from = ring + stage * L::STAGE;
+      const uint32_t from = ring + stage * L::STAGE, from_k = from + lane * 16, from_v = from + L::K_BYTES + lane * L::V_WORD;
       stage = stage + 1 == L::STAGES ? 0 : stage + 1;
 
       float s[2][NT][4] = {};
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        uint4 k[2][DP / 64];
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int x = 0; x < DP / 64; ++x) k[r][x] = load_shared16(from + (((g * 2 + r) * (DP / 64) + x) * 32 + lane) * 16);
 #pragma unroll
         for (int x = 0; x < DP / 64; ++x) {
-          const uint32_t lo[4] = {k[0][x].x, k[0][x].y, k[0][x].z, k[0][x].w};
-          const uint32_t hi[4] = {k[1][x].x, k[1][x].y, k[1][x].z, k[1][x].w};
+          const uint4 k0 = load_shared16(from_k + ((g * 2) * (DP / 64) + x) * 512);
+          const uint4 k1 = load_shared16(from_k + ((g * 2 + 1) * (DP / 64) + x) * 512);
+          const uint32_t lo[4] = {k0.x, k0.y, k0.z, k0.w}, hi[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             uint32_t a0, a1, a2, a3;
@@ -586,43 +631,51 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_kernel(const __grid_c
         ks[g] = load_shared4(from + L::K_BYTES + L::V_BYTES + g * 4);
         lv[g] = log2_fast(load_shared4(from + L::K_BYTES + L::V_BYTES + 8 + g * 4));
       }
-      const int64_t t0 = (int64_t)step * STEP;
+      const int t0 = step * STEP;
       const bool masked = t0 + STEP > sure;
-      bool grew = false;
-      float alpha[NT][2];
+      bool passed = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int g = 0; g < 2; ++g)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[g][nt][e] *= factor[nt][e & 1] * ks[g];
-            if (masked && t0 + 16 * g + n8 + 8 * (e >> 1) >= limit[nt][e & 1]) s[g][nt][e] = -INFINITY;
-          }
+          for (int e = 0; e < 4; ++e) s[g][nt][e] *= factor[nt][e & 1] * ks[g];
+        if (masked) {
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (t0 + 16 * g + n8 + 8 * (e >> 1) >= limit[nt][e & 1]) s[g][nt][e] = -INFINITY;
+        }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const float b0 = fmaxf(s[0][nt][u], s[0][nt][u + 2]), b1 = fmaxf(s[1][nt][u], s[1][nt][u + 2]);
-          float top = fmaxf(b0, b1), top_o = fmaxf(b0 + lv[0], b1 + lv[1]);
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) {
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-            top_o = fmaxf(top_o, __shfl_xor_sync(0xffffffffu, top_o, x));
-          }
-          const float m_new = fmaxf(m[nt][u], top), mo_new = fmaxf(mo[nt][u], top_o);
-          l[nt][u] *= exp2_fast(m[nt][u] - reference(m_new));
-          alpha[nt][u] = exp2_fast(mo[nt][u] - reference(mo_new));
-          grew |= mo_new > mo[nt][u];
-          m[nt][u] = m_new;
-          mo[nt][u] = mo_new;
+          passed |= fmaxf(b0, b1) > m[nt][u] + LEAD || fmaxf(b0 + lv[0], b1 + lv[1]) > mo[nt][u] + LEAD;
         }
       }
-      if (__any_sync(0xffffffffu, grew)) {
+      if (__any_sync(0xffffffffu, passed)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int t = 0; t < OT; ++t)
+          for (int u = 0; u < 2; ++u) {
+            const float b0 = fmaxf(s[0][nt][u], s[0][nt][u + 2]), b1 = fmaxf(s[1][nt][u], s[1][nt][u + 2]);
+            float top = fmaxf(b0, b1), top_o = fmaxf(b0 + lv[0], b1 + lv[1]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[nt][t][e] *= alpha[nt][e & 1];
+            for (int x = 4; x < 32; x <<= 1) {
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+              top_o = fmaxf(top_o, __shfl_xor_sync(0xffffffffu, top_o, x));
+            }
+            const float m_new = fmaxf(m[nt][u], top), mo_new = fmaxf(mo[nt][u], top_o);
+            l[nt][u] *= exp2_fast(m[nt][u] - reference(m_new));
+            const float alpha = exp2_fast(mo[nt][u] - reference(mo_new));
+            m[nt][u] = m_new;
+            mo[nt][u] = mo_new;
+#pragma unroll
+            for (int t = 0; t < OT; ++t) {
+              o[nt][t][u] *= alpha;
+              o[nt][t][u + 2] *= alpha;
+            }
+          }
       }
       uint32_t pf[2][NT][2];  // P^T: keys 2 c4, 2 c4 + 1 (and + 8) of row n8
 #pragma unroll
@@ -636,7 +689,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_kernel(const __grid_c
             const float x0 = s[g][nt][2 * r], x1 = s[g][nt][2 * r + 1];
             l[nt][0] += exp2_fast(x0 - r0);
             l[nt][1] += exp2_fast(x1 - r1);
-            pf[g][nt][r] = transpose8x8(half2_bits(exp2_fast(x0 + lv[g] - w0), exp2_fast(x1 + lv[g] - w1)));
+            pf[g][nt][r] = transpose8x8(half2_bits(exp2_fast(x0 + (lv[g] - w0)), exp2_fast(x1 + (lv[g] - w1))));
           }
       }
 #pragma unroll
@@ -644,7 +697,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_kernel(const __grid_c
         uint32_t v[4][L::V_WORD / 4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t at = from + L::K_BYTES + ((g * 4 + i) * 32 + lane) * L::V_WORD;
+          const uint32_t at = from_v + (g * 4 + i) * 32 * L::V_WORD;
           if constexpr (DP == 128) {
             const uint4 x = load_shared16(at);
             v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
@@ -667,109 +720,150 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_kernel(const __grid_c
       }
     }
 
-    // ---------------------------------------------------------- join the warps
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float sum = l[nt][u];
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-        const int row = nt * 8 + 2 * c4 + u;
-        if (n8 == 0) {
-          stats[(warp * L::ROWS + row) * 3] = m[nt][u];
-          stats[(warp * L::ROWS + row) * 3 + 1] = sum;
-          stats[(warp * L::ROWS + row) * 3 + 2] = mo[nt][u];
+        for (int x = 4; x < 32; x <<= 1) l[nt][u] += __shfl_xor_sync(0xffffffffu, l[nt][u], x);
+    if (seg.s0 == 0 && seg.s1 == seg.n) {  // a whole unit
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float acc[L::V_WORD];
+          row_of<DP, NT>(o, nt, u, acc);
+          write_row<T>(a, seg.b, seg.head, row0 + nt * 8 + 2 * c4 + u, n8 * L::V_WORD, acc, m[nt][u], l[nt][u], mo[nt][u]);
         }
-        float *to = join + (warp * L::ROWS + row) * L::PITCH + n8 * L::V_WORD;
-#pragma unroll
-        for (int t = 0; t < OT; t += 2)
-          *reinterpret_cast<float4 *>(to + 2 * t) =
-              make_float4(o[nt][t][u], o[nt][t][u + 2], o[nt][t + 1][u], o[nt][t + 1][u + 2]);
-      }
-    __syncthreads();
-    const bool complete = at_start && at_end;
-    float *part = a.parts;
-    if (!complete) part += (2 * (int64_t)blockIdx.x + (here.left + (seg.s1 - seg.s0) == start.left ? 0 : 1)) * L::PART;
-    for (int i = threadIdx.x; i < L::ROWS * (DP / 4); i += WARPS * 32) {
-      const int r = i / (DP / 4), d = i % (DP / 4) * 4;
-      float top = -INFINITY, top_o = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        top = fmaxf(top, stats[(w * L::ROWS + r) * 3]);
-        top_o = fmaxf(top_o, stats[(w * L::ROWS + r) * 3 + 2]);
-      }
-      float sum = 0.f, acc[4] = {};
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float *st = stats + (w * L::ROWS + r) * 3;
-        sum += st[1] * exp2_fast(st[0] - reference(top));
-        const float f = exp2_fast(st[2] - reference(top_o));
-        const float4 x = *reinterpret_cast<const float4 *>(join + (w * L::ROWS + r) * L::PITCH + d);
-        acc[0] = fmaf(x.x, f, acc[0]); acc[1] = fmaf(x.y, f, acc[1]);
-        acc[2] = fmaf(x.z, f, acc[2]); acc[3] = fmaf(x.w, f, acc[3]);
-      }
-      if (complete) {
-        write_row<T>(a, seg.b, h, row0 + r, d, acc, top, sum, top_o);
-      } else {
-        *reinterpret_cast<float4 *>(part + r * DP + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        if (d == 0) {
-          part[L::ROWS * DP + r * 3] = top;
-          part[L::ROWS * DP + r * 3 + 1] = sum;
-          part[L::ROWS * DP + r * 3 + 2] = top_o;
-        }
-      }
+      continue;
     }
-    __syncthreads();
-    if (empty) break;
+    const bool is_first = here.left + (seg.s1 - seg.s0) == start.left;
+    if (here.left > 0) {  // the end of a unit from the share before
+      write_part<DP, NT>(a.parts + (2 * ((int64_t)blockIdx.x * WARPS + warp)) * L::PART, o, m, l, mo);
+      continue;
+    }
+    // the share's last segment: kept for the CTA's join
+    held.unit = ((int64_t)seg.b * a.kv_heads + seg.head) * a.row_tiles + seg.tile;
+    held.only = is_first;
+    write_part<DP, NT>(reinterpret_cast<float *>(smem + warp * L::STAGES * L::STAGE), o, m, l, mo);
+  }
+
+  // ------------------------------------------------------------ the CTA's join
+  // A run: a warp's last segment and the warps after it that have nothing but
+  // the same unit.  Its first warp adds up the others'.
+  if (lane == 0) runs[warp] = held;
+  __syncthreads();
+  if (held.unit < 0 || (warp > 0 && held.only && runs[warp - 1].unit == held.unit)) return;
+  int last = warp;
+  while (last + 1 < WARPS && runs[last + 1].only && runs[last + 1].unit == held.unit) ++last;
+  const int row = lane / (32 / L::ROWS);  // ROWS divides 32: lanes of a row share its elements
+  float *part = a.parts + (2 * ((int64_t)blockIdx.x * WARPS + warp) + (held.only ? 0 : 1)) * L::PART;
+  auto part_of = [&](int w) { return reinterpret_cast<const float *>(smem + w * L::STAGES * L::STAGE); };
+  float top = -INFINITY, top_o = -INFINITY, sum = 0.f;
+  for (int w = warp; w <= last; ++w) {
+    const float *st = part_of(w) + L::ROWS * DP + row * 3;
+    top = fmaxf(top, st[0]);
+    top_o = fmaxf(top_o, st[2]);
+  }
+  for (int w = warp; w <= last; ++w) {
+    const float *st = part_of(w) + L::ROWS * DP + row * 3;
+    sum += st[1] * exp2_fast(st[0] - reference(top));
+  }
+  constexpr int SHARE = DP * L::ROWS / 32;  // a lane's elements of its row
+  const int d0 = lane % (32 / L::ROWS) * 4;
+#pragma unroll 2
+  for (int x = 0; x < SHARE; x += 4) {
+    const int d = d0 + x * (32 / L::ROWS);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = warp; w <= last; ++w) {
+      const float f = exp2_fast(part_of(w)[L::ROWS * DP + row * 3 + 2] - reference(top_o));
+      const float4 v = *reinterpret_cast<const float4 *>(part_of(w) + row * DP + d);
+      acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y);
+      acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+    }
+    *reinterpret_cast<float4 *>(part + row * DP + d) = acc;
+  }
+  if (lane % (32 / L::ROWS) == 0) {
+    part[L::ROWS * DP + row * 3] = top;
+    part[L::ROWS * DP + row * 3 + 1] = sum;
+    part[L::ROWS * DP + row * 3 + 2] = top_o;
   }
 }
 
-// Joins the parts of the units that several CTAs shared, one block a unit, and
-// writes the rows of sequences without keys.
-constexpr int JOIN_THREADS = 128;
+// Joins the parts of the units that several shares held, one block a unit, a
+// warp a row, and writes the rows of sequences without keys.
+constexpr int JOIN_WARPS = 8;
 template <typename T, int DP, int NT>
-__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ Attention a, int64_t pieces) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_constant__ Attention a, int64_t ctas) {
   using L = Layout<DP, NT>;
-  __shared__ int64_t reduce[JOIN_THREADS / 32];
+  const int lane = threadIdx.x & 31;
   wait_prior_grid();
   const int units = a.kv_heads * a.row_tiles;
   const int64_t b = blockIdx.x / units;
   const int unit = (int)(blockIdx.x % units), h = unit / a.row_tiles, row0 = unit % a.row_tiles * L::ROWS;
   const int64_t n = steps_of(cached_length(a, b));
-  const int64_t piece = piece_of(steps_below<JOIN_THREADS>(a, a.batch, reduce), pieces, a.least);
-  const int64_t first = steps_below<JOIN_THREADS>(a, b, reduce) + unit * n;
-  const int64_t c0 = n > 0 ? first / piece : 0, c1 = n > 0 ? (first + n - 1) / piece : 0;
-  if (n > 0 && c0 == c1) return;
-  // the first CTA's part is its first segment only if the unit starts its piece
-  auto part_of = [&](int64_t c) {
-    return a.parts + (2 * c + (c == c0 && first != c0 * piece ? 1 : 0)) * L::PART;
+  const Cut cut = cut_line(a, ctas, L::WARPS);
+  const int64_t first = steps_below(a, b) + unit * n, end = first + n;
+  const int64_t k0 = first / cut.cta, k1 = n > 0 ? (end - 1) / cut.cta : k0;
+  if (n > 0 && k0 == k1 && (first - k0 * cut.cta) / cut.warp == (end - 1 - k0 * cut.cta) / cut.warp) return;
+  // Part j of the unit, or null.  CTA k0 + j / 2 left a run from the warp that
+  // holds the unit's first step there (the warp's second place, unless its
+  // share begins with the unit), and, if the unit ends inside a later warp's
+  // share, that warp's first place.
+  auto part_of = [&](int64_t j) -> const float * {
+    const int64_t k = k0 + j / 2, base = k * cut.cta;
+    if (n == 0 || k > k1) return nullptr;
+    const int64_t lo = max(first, base) - base, hi = min(end, base + cut.cta) - 1 - base;
+    const int64_t w0 = lo / cut.warp, w1 = hi / cut.warp;
+    if (j % 2 == 0) return a.parts + (2 * (k * L::WARPS + w0) + (lo == w0 * cut.warp ? 0 : 1)) * L::PART;
+    const int64_t share_end = min(min((w1 + 1) * cut.warp, cut.cta), cut.total - base);
+    return w1 > w0 && hi + 1 < share_end ? a.parts + 2 * (k * L::WARPS + w1) * L::PART : nullptr;
   };
-  for (int i = threadIdx.x; i < L::ROWS * (DP / 4); i += JOIN_THREADS) {
-    const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+  const int64_t parts = 2 * (k1 - k0 + 1);
+  constexpr int LANES = DP / 4, AT_ONCE = 32 / LANES;  // lanes of a part's row; parts read side by side
+  for (int r = threadIdx.x >> 5; r < L::ROWS; r += JOIN_WARPS) {
     float top = -INFINITY, top_o = -INFINITY, sum = 0.f, acc[4] = {};
-    if (n > 0) {
-      for (int64_t c = c0; c <= c1; ++c) {
-        const float *st = part_of(c) + L::ROWS * DP + r * 3;
-        top = fmaxf(top, st[0]);
-        top_o = fmaxf(top_o, st[2]);
-      }
-      for (int64_t c = c0; c <= c1; ++c) {
-        const float *p = part_of(c), *st = p + L::ROWS * DP + r * 3;
-        sum += st[1] * exp2_fast(st[0] - reference(top));
-        const float f = exp2_fast(st[2] - reference(top_o));
-        const float4 x = *reinterpret_cast<const float4 *>(p + r * DP + d);
-        acc[0] = fmaf(x.x, f, acc[0]); acc[1] = fmaf(x.y, f, acc[1]);
-        acc[2] = fmaf(x.z, f, acc[2]); acc[3] = fmaf(x.w, f, acc[3]);
+    for (int64_t j = lane; j < parts; j += 32) {
+      const float *p = part_of(j);
+      if (p) {
+        top = fmaxf(top, p[L::ROWS * DP + r * 3]);
+        top_o = fmaxf(top_o, p[L::ROWS * DP + r * 3 + 2]);
       }
     }
-    write_row<T>(a, b, h, row0 + r, d, acc, top, sum, top_o);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      top_o = fmaxf(top_o, __shfl_xor_sync(0xffffffffu, top_o, x));
+    }
+    for (int64_t j0 = 0; j0 < parts; j0 += 32) {
+      const float *p = j0 + lane < parts ? part_of(j0 + lane) : nullptr;
+      float f = 0.f;
+      if (p) {
+        sum += p[L::ROWS * DP + r * 3 + 1] * exp2_fast(p[L::ROWS * DP + r * 3] - reference(top));
+        f = exp2_fast(p[L::ROWS * DP + r * 3 + 2] - reference(top_o));
+      }
+      const int count = (int)(parts - j0 < 32 ? parts - j0 : 32);
+#pragma unroll 4
+      for (int j = 0; j < count; j += AT_ONCE) {
+        const int from = j + lane / LANES;
+        const uint64_t at = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(p), from);
+        const float g = __shfl_sync(0xffffffffu, f, from);
+        if (at != 0) {
+          const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(at) + r * DP + lane % LANES * 4);
+          acc[0] = fmaf(v.x, g, acc[0]); acc[1] = fmaf(v.y, g, acc[1]);
+          acc[2] = fmaf(v.z, g, acc[2]); acc[3] = fmaf(v.w, g, acc[3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    if (AT_ONCE == 2) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], 16);
+    }
+    if (lane < LANES) write_row<T>(a, b, h, row0 + r, lane * 4, acc, top, sum, top_o);
   }
 }
-
-// Contexts of at most this many tokens (eight warps' single steps) go one CTA a
-// unit, without a second kernel.
-constexpr int64_t WHOLE_TOKENS = WARPS * STEP;
 
 template <typename T, typename C, int DP, int NT>
 int launch_tiles(Attention a, cudaStream_t stream) {
@@ -779,12 +873,11 @@ int launch_tiles(Attention a, cudaStream_t stream) {
   a.row_tiles = (a.rows + L::ROWS - 1) / L::ROWS;
   const int64_t units = (int64_t)a.batch * a.kv_heads * a.row_tiles;
   if (units > (1LL << 31) - 1) return NT_B200_ERR_INVALID_ARGUMENT;
-  a.whole = a.capacity <= WHOLE_TOKENS;
-  a.least = WARPS;
-  const int64_t grid = a.whole ? units : sm_count();
-  const int rc = launch_overlapped(attention_kernel<T, C, DP, NT>, dim3((unsigned)grid), dim3(WARPS * 32), L::SMEM, stream, a);
-  if (rc != 0 || a.whole) return rc;
-  return launch_overlapped(join_kernel<T, DP, NT>, dim3((unsigned)units), dim3(JOIN_THREADS), 0, stream, a, grid);
+  const int grid = sm_count();
+  const int rc =
+      launch_overlapped(attention_kernel<T, C, DP, NT>, dim3((unsigned)grid), dim3(L::WARPS * 32), L::SMEM, stream, a);
+  if (rc != 0) return rc;
+  return launch_overlapped(join_kernel<T, DP, NT>, dim3((unsigned)units), dim3(JOIN_WARPS * 32), 0, stream, a, (int64_t)grid);
 }
 
 template <typename T, typename C>
@@ -808,8 +901,10 @@ int launch_attention(const Attention &a, cudaStream_t stream) {
 
 extern "C" int64_t nt_b200_paged_attention_workspace_size(void) {
   using namespace nt::paged;
-  // two parts a CTA of the largest layout; the CTAs of a launch are the SMs
-  return 2 * (int64_t)nt::sm_count() * Layout<128, 2>::PART * (int64_t)sizeof(float);
+  // two parts a warp of the largest layout; the CTAs of a launch are the SMs
+  constexpr int64_t one = (int64_t)Layout<128, 1>::WARPS * Layout<128, 1>::PART;
+  constexpr int64_t two = (int64_t)Layout<128, 2>::WARPS * Layout<128, 2>::PART;
+  return 2 * (int64_t)nt::sm_count() * (one > two ? one : two) * (int64_t)sizeof(float);
 }
 
 extern "C" int nt_b200_paged_attention(const NtB200PagedAttentionArgs *a, void *stream) {
@@ -824,7 +919,7 @@ extern "C" int nt_b200_paged_attention(const NtB200PagedAttentionArgs *a, void *
   if (!a->query || !a->output || !a->lengths || (a->table_columns > 0 && !a->block_table) || !a->workspace ||
       (reinterpret_cast<uintptr_t>(a->workspace) & 15u) != 0 ||
       a->workspace_bytes < nt_b200_paged_attention_workspace_size() || a->batch > (1 << 30) ||
-      a->queries * a->heads > (1 << 30) || !(a->scale == a->scale))
+      a->queries > (1 << 30) || a->queries * a->heads > (1 << 30) || a->table_columns > (1LL << 40) || !(a->scale == a->scale))
     return NT_B200_ERR_INVALID_ARGUMENT;
   const int wide = a->index_dtype == NT_B200_INT64;
   paged::Attention p{};
@@ -846,7 +941,10 @@ extern "C" int nt_b200_paged_attention(const NtB200PagedAttentionArgs *a, void *
   p.ks_page = c.key_scale_strides[0]; p.ks_head = c.key_scale_strides[1];
   p.vs_page = c.value_scale_strides[0]; p.vs_head = c.value_scale_strides[1];
   p.pages = c.pages;
-  p.capacity = a->table_columns * c.page;
+  const int64_t capacity = a->table_columns * c.page;
+  p.capacity = (int)(capacity < paged::MOST_TOKENS ? capacity : paged::MOST_TOKENS);
+  p.page_groups = (int)(c.page / 16);
+  p.page_reciprocal = ((1ull << 36) + p.page_groups - 1) / p.page_groups;
   p.batch = (int)a->batch; p.queries = (int)a->queries; p.heads = (int)a->heads; p.kv_heads = (int)c.kv_heads;
   p.group = (int)(a->heads / c.kv_heads);
   p.head_dim = (int)c.head_dim;

@@ -130,8 +130,10 @@ def _cache_args(v):
             f"paged cache shapes {tuple(key.shape)}, {tuple(value.shape)} and scales {tuple(ks.shape)}, "
             f"{tuple(vs.shape)} disagree."
         )
-    if page % 16 or dim % 16:
-        raise TypeError(f"a paged cache needs page size and head dimension in multiples of 16; got {page} and {dim}.")
+    if page % 16 or dim % 16 or page > 4096:
+        raise TypeError(
+            f"a paged cache needs page size (at most 4096) and head dimension in multiples of 16; got {page} and {dim}."
+        )
     if key.stride(3) != 1 or value.stride(3) != 1:
         raise TypeError("Kernel arguments `key_cache`, `value_cache` must have unit stride along their last dimension.")
     return (
