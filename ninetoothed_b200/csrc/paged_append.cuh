@@ -377,7 +377,7 @@ int launch_append(Params p, cudaStream_t stream) {
 
 // Host-side checks of a cache (no launch): 0 or an error code.
 inline int check_cache(const NtB200PagedCache &c) {
-  if (c.pages < 0 || c.kv_heads < 0 || c.page <= 0 || c.head_dim <= 0) return NT_B200_ERR_INVALID_ARGUMENT;
+  if (c.pages < 0 || c.pages >= (1LL << 31) || c.kv_heads < 0 || c.page <= 0 || c.head_dim <= 0) return NT_B200_ERR_INVALID_ARGUMENT;
   if (c.code_dtype != NT_B200_FLOAT8_E4M3FN && c.code_dtype != NT_B200_INT8) return NT_B200_ERR_UNSUPPORTED_DTYPE;
   if (c.page % 16 != 0 || c.page > 4096 || c.head_dim % 16 != 0 || c.head_dim > (1 << 12))
     return NT_B200_ERR_SHAPE_MISMATCH;

@@ -76,6 +76,7 @@ struct Attention {
   int page_groups;          // page / 16
   uint64_t page_reciprocal; // ceil(2^36 / page_groups)
   int rows, row_tiles;      // queries * group; tiles of them
+  int q_vector;             // queries can be read 16 bytes at a time
   float scale;              // softmax scale * log2 e
   float *parts;             // workspace: two parts a warp
 };
@@ -91,11 +92,11 @@ __device__ __forceinline__ int cached_length(const Attention &a, int64_t b) {
 }
 
 // The page of column `column` of sequence b's block table, or -1.
-__device__ __forceinline__ int64_t page_of(const Attention &a, int64_t b, int64_t column) {
+__device__ __forceinline__ int page_of(const Attention &a, int64_t b, int64_t column) {
   const int64_t at = b * a.table_row_stride + column * a.block_table.stride;
   const int64_t id = a.block_table.wide ? static_cast<const int64_t *>(a.block_table.data)[at]
                                         : (int64_t) static_cast<const int32_t *>(a.block_table.data)[at];
-  return id >= 0 && id < a.pages ? id : -1;
+  return id >= 0 && id < a.pages ? (int)id : -1;
 }
 
 // ---------------------------------------------------------------- any type
@@ -121,7 +122,7 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(Attention a) {
   const int g = h / a.group;
   float m = -INFINITY, l = 0.f;
   for (int64_t t = 0; t < limit; ++t) {
-    const int64_t id = page_of(a, b, t / a.page);
+    const int id = page_of(a, b, t / a.page);
     if (id < 0) {
       record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
       continue;
@@ -227,13 +228,18 @@ template <> __device__ __forceinline__ void to_halves<int8_t>(uint32_t w, uint32
   hi = *reinterpret_cast<uint32_t *>(&y);
 }
 
+// Where word w of a token's key lies in its row in shared memory.
+template <int DP> __device__ __forceinline__ int place_of(int token, int w) {
+  return DP == 128 ? w ^ ((token & 1) << 2) : w;
+}
+
 template <int DP, int NT> struct Layout {
   static constexpr int ROWS = 8 * NT;
   // One column tile: 12 warps of up to 168 registers, three a scheduler, to
   // cover each other's load and MMA latency (8 warps: 2.45 TB/s where 12 reach
   // RATE).  Two column tiles hold twice the accumulators: 8 warps.
   static constexpr int WARPS = NT == 1 ? 12 : 8;
-  static constexpr int STAGES = DP == 64 ? 4 : NT == 1 ? 2 : 3;
+  static constexpr int STAGES = 2;
   static constexpr int K_COPIES = DP / 64 * 4;              // 16-byte words a lane and step
   static constexpr int V_WORD = DP / 8;                     // bytes of a token's value a lane takes
   static constexpr int K_BYTES = STEP * DP, V_BYTES = STEP * DP;
@@ -462,87 +468,119 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
   }
 
   // ------------------------------------------------------------ loads ahead
+  // A stage holds a step's keys and one its values; each is loaded again, two
+  // steps on, as soon as it has been read.
   Walk ahead = start;
   Segment lseg{};
   bool lmore = next_segment(a, ahead, lseg);
-  int lstep = lseg.s0;
-  int64_t id0 = -1, id1 = -1;  // pages of the next step's two groups
-  int group0 = 0;              // the first group's place in its page
+  int lstep = lseg.s0;  // the next step to load
+  int id0 = -1, id1 = -1;  // pages of its two 16-token groups
+  int group0 = 0;          // the first group's place in its page
   auto find_pages = [&]() {
-    if (lmore && lstep >= lseg.s1) {
-      lmore = next_segment(a, ahead, lseg);
-      lstep = lseg.s0;
-    }
-    if (!lmore) return;
     const int g = lstep * (STEP / 16);
-    const int col = (int)(((uint64_t)g * a.page_reciprocal) >> 36);
+    const int col = (int)(((uint64_t)(uint32_t)g * a.page_reciprocal) >> 36);
     group0 = g - col * a.page_groups;
     id0 = page_of(a, lseg.b, col);
     id1 = id0;
     if (group0 + 1 == a.page_groups) id1 = (g + 1) * 16 < lseg.length ? page_of(a, lseg.b, col + 1) : -1;
   };
-  // this lane's share of a 16-token group
-  const int64_t k_lane = n8 * a.k_token + 16 * c4, v_lane = 2 * c4 * a.v_token + n8 * L::V_WORD;
-  const bool full_dim = a.head_dim == DP;
-  auto issue = [&](int stage) {
+  // This lane's share of a 16-token group.  Keys are copied four (head_dim up
+  // to 64: eight) whole rows an instruction; a token's 16-byte words change
+  // places in shared memory with its lowest bit, so that reading 8 tokens' words
+  // meets every bank once.  Values are copied as they are read.
+  constexpr int ROW_WORDS = DP / 16, K_COPIES = 16 * ROW_WORDS / 32;
+  const int k_row = lane / ROW_WORDS, k_word = lane % ROW_WORDS;  // of the first copy
+  const uint32_t k_token = (uint32_t)a.k_token, v_token = (uint32_t)a.v_token;
+  const uint8_t *const key_lane = a.key + k_row * k_token + k_word * 16;
+  const uint8_t *const value_lane = a.value + 2 * c4 * v_token + n8 * L::V_WORD;
+  const uint32_t k_place = ring + (uint32_t)(k_row * DP + place_of<DP>(k_row, k_word) * 16);
+  const uint32_t v_place = ring + L::K_BYTES + lane * L::V_WORD;
+  const bool k_in_head = k_word * 16 < a.head_dim, v_in_head = n8 * L::V_WORD < a.head_dim;
+  const uint8_t *key_head = nullptr, *value_head = nullptr;  // of the load segment
+  const float *scale_head = nullptr;                         // lane 0: key scales, lane 1: value scales
+  const uint32_t scale_page = (uint32_t)(lane == 0 ? a.ks_page : a.vs_page);
+  auto enter = [&]() {
+    key_head = key_lane + lseg.head * a.k_head;
+    value_head = value_lane + lseg.head * a.v_head;
+    scale_head = lane == 0 ? a.key_scale + lseg.head * a.ks_head : a.value_scale + lseg.head * a.vs_head;
+    find_pages();
+  };
+  auto next_step = [&]() {
+    if (!lmore) return;
+    if (++lstep < lseg.s1) {
+      find_pages();
+      return;
+    }
+    lmore = next_segment(a, ahead, lseg);
+    lstep = lseg.s0;
+    if (lmore) enter();
+  };
+  // the group's live tokens, its page (0 where it has none) and slot in it
+  auto group_of = [&](int g, int &live, uint32_t &id, uint32_t &slot) {
+    live = lseg.length - (lstep * STEP + 16 * g);
+    const int page = g == 0 ? id0 : id1;
+    if (page < 0) {
+      if (live > 0) record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
+      live = 0;
+    }
+    id = page < 0 ? 0 : page;
+    slot = (g == 0 ? group0 : group0 + 1 == a.page_groups ? 0 : group0 + 1) * 16;
+  };
+  auto load_keys = [&](int stage) {
     if (lmore) {
-      const uint32_t to = ring + stage * L::STAGE, to_k = to + lane * 16, to_v = to + L::K_BYTES + lane * L::V_WORD;
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        int live = lseg.length - (lstep * STEP + 16 * g);  // tokens of the group in the cache
-        int64_t id = g == 0 ? id0 : id1;
-        if (id < 0) {
-          if (live > 0) record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
-          live = 0;
-          id = 0;
-        }
-        const int in_page = (g == 0 ? group0 : group0 + 1 == a.page_groups ? 0 : group0 + 1) * 16;
-        const uint8_t *k = a.key + id * a.k_page + lseg.head * a.k_head + in_page * a.k_token + k_lane;
-        const uint8_t *v = a.value + id * a.v_page + lseg.head * a.v_head + in_page * a.v_token + v_lane;
-        const uint32_t tk = to_k + g * (2 * (DP / 64) * 512), tv = to_v + g * (4 * 32 * L::V_WORD);
-        auto copy_v = [&](uint32_t dst, const uint8_t *src, bool valid) {
-          if constexpr (DP == 128) copy_async16(dst, src, valid);
-          else copy_async8(dst, src, valid);
-        };
-        if (live >= 16 && full_dim) {
+        int live;
+        uint32_t id, slot;
+        group_of(g, live, id, slot);
+        const uint8_t *k = key_head + (uint64_t)id * (uint32_t)a.k_page + (uint64_t)slot * k_token;
+        const uint32_t to = k_place + stage * L::STAGE + g * 16 * DP;
+        if (live >= 16 && a.head_dim == DP) {
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int x = 0; x < DP / 64; ++x)
-              copy_async16(tk + (r * (DP / 64) + x) * 512, k + r * 8 * a.k_token + x * 64, true);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            copy_v(tv + i * 32 * L::V_WORD, v + ((i & 1) + 8 * (i >> 1)) * a.v_token, true);
+          for (int i = 0; i < K_COPIES; ++i)
+            copy_async16(to + i * 512, k + i * (uint64_t)(32 / ROW_WORDS * k_token), true);
         } else {  // zeros for what is not there; its address stays inside
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int x = 0; x < DP / 64; ++x) {
-              const bool valid = n8 + 8 * r < live && x * 64 + 16 * c4 < a.head_dim;
-              copy_async16(tk + (r * (DP / 64) + x) * 512, valid ? k + r * 8 * a.k_token + x * 64 : a.key, valid);
-            }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool valid = 2 * c4 + (i & 1) + 8 * (i >> 1) < live && n8 * L::V_WORD < a.head_dim;
-            copy_v(tv + i * 32 * L::V_WORD, valid ? v + ((i & 1) + 8 * (i >> 1)) * a.v_token : a.value, valid);
+          for (int i = 0; i < K_COPIES; ++i) {
+            const bool valid = k_in_head && k_row + i * (32 / ROW_WORDS) < live;
+            copy_async16(to + i * 512, valid ? k + i * (uint64_t)(32 / ROW_WORDS * k_token) : a.key, valid);
           }
         }
-        if (lane < 2) {
-          const float *src = lane == 0 ? a.key_scale + id * a.ks_page + lseg.head * a.ks_head
-                                       : a.value_scale + id * a.vs_page + lseg.head * a.vs_head;
-          copy_async4(to + L::K_BYTES + L::V_BYTES + (lane * 2 + g) * 4, src, live > 0);
+        if (lane < 2)
+          copy_async4(ring + stage * L::STAGE + L::K_BYTES + L::V_BYTES + (lane * 2 + g) * 4, scale_head + (uint64_t)id * scale_page,
+                      live > 0);
+      }
+    }
+    copy_commit();
+  };
+  auto load_values = [&](int stage) {
+    if (lmore) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        int live;
+        uint32_t id, slot;
+        group_of(g, live, id, slot);
+        const uint8_t *v = value_head + (uint64_t)id * (uint32_t)a.v_page + (uint64_t)slot * v_token;
+        const uint32_t to = v_place + stage * L::STAGE + g * (4 * 32 * L::V_WORD);
+        const bool all = live >= 16 && a.head_dim == DP;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint8_t *src = v + (uint64_t)((uint32_t)((i & 1) + 8 * (i >> 1)) * v_token);
+          const bool valid = all || (v_in_head && 2 * c4 + (i & 1) + 8 * (i >> 1) < live);
+          if constexpr (DP == 128) copy_async16(to + i * 512, valid ? src : a.value, valid);
+          else copy_async8(to + i * 256, valid ? src : a.value, valid);
         }
       }
-      ++lstep;
     }
     copy_commit();
   };
 
-  find_pages();
+  if (lmore) enter();
 #pragma unroll
-  for (int i = 0; i < L::STAGES - 1; ++i) {
-    issue(i);
-    find_pages();
+  for (int i = 0; i < 2; ++i) {
+    load_keys(i);
+    load_values(i);
+    next_step();
   }
   int stage = 0;
 
@@ -564,18 +602,31 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
       const int i = valid ? row / a.group : 0, hq = seg.head * a.group + (valid ? row % a.group : 0);
       const T *q = static_cast<const T *>(a.query) + seg.b * a.q_batch + i * a.q_token + hq * a.q_head;
       float x[DP / 4], top = 0.f;
+      if (a.q_vector) {
 #pragma unroll
-      for (int e = 0; e < DP / 4; ++e) {
-        const int d = (e / 16) * 64 + 16 * c4 + e % 16;
-        x[e] = valid && d < a.head_dim ? to_f(q[d * a.q_dim]) : 0.f;
-        top = fmaxf(top, fabsf(x[e]));
+        for (int e = 0; e < DP / 4; e += 8) {
+          const int d = (e / 16) * 64 + 16 * c4 + e % 16;
+          rotary::Chunk<T> chunk = {};
+          if (valid && d < a.head_dim) chunk = *reinterpret_cast<const rotary::Chunk<T> *>(q + d);
+#pragma unroll
+          for (int y = 0; y < 8; ++y) x[e + y] = to_f(chunk.v[y]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < DP / 4; ++e) {
+          const int d = (e / 16) * 64 + 16 * c4 + e % 16;
+          x[e] = valid && d < a.head_dim ? to_f(q[d * a.q_dim]) : 0.f;
+        }
       }
+#pragma unroll
+      for (int e = 0; e < DP / 4; ++e) top = fmaxf(top, fabsf(x[e]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       int exponent = (int)(__float_as_uint(top) >> 23);  // biased; subnormal and zero rows as 2^-126
       exponent = exponent < 1 ? 1 : exponent > 253 ? 253 : exponent;
       q_unit[nt] = __uint_as_float((uint32_t)exponent << 23);
-      const float inv = __uint_as_float((uint32_t)(254 - exponent) << 23);
+      // with the softmax scale's sign, so that a larger score is a larger weight
+      const float inv = copysignf(__uint_as_float((uint32_t)(254 - exponent) << 23), a.scale);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int e = (s / 4) * 16 + (s % 4) * 4;
@@ -591,7 +642,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        factor[nt][u] = a.scale * __shfl_sync(0xffffffffu, q_unit[nt], (2 * c4 + u) * 4);
+        factor[nt][u] = fabsf(a.scale) * __shfl_sync(0xffffffffu, q_unit[nt], (2 * c4 + u) * 4);
         limit[nt][u] = seg.length - a.queries + 1 + (row0 + nt * 8 + 2 * c4 + u) / a.group;
         m[nt][u] = mo[nt][u] = -INFINITY;
         l[nt][u] = 0.f;
@@ -600,20 +651,17 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
     float o[NT][OT][4] = {};
 
     for (int step = seg.s0; step < seg.s1; ++step) {
-      issue(stage == 0 ? L::STAGES - 1 : stage - 1);  // the stage read one step ago
-      find_pages();
-      copy_wait<L::STAGES - 1>();
-      __syncwarp();  // the scales were copied by two lanes
-      const uint32_t from = ring + stage * L::STAGE, from_k = from + lane * 16, from_v = from + L::K_BYTES + lane * L::V_WORD;
-      stage = stage + 1 == L::STAGES ? 0 : stage + 1;
+      copy_wait<3>();  // all but this step's values and the next step
+      __syncwarp();    // the scales were copied by two lanes
+      const uint32_t from = ring + stage * L::STAGE, from_v = from + L::K_BYTES + lane * L::V_WORD;
 
       float s[2][NT][4] = {};
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
 #pragma unroll
         for (int x = 0; x < DP / 64; ++x) {
-          const uint4 k0 = load_shared16(from_k + ((g * 2) * (DP / 64) + x) * 512);
-          const uint4 k1 = load_shared16(from_k + ((g * 2 + 1) * (DP / 64) + x) * 512);
+          const uint32_t at = from + (g * 16 + n8) * DP + place_of<DP>(n8, 4 * x + c4) * 16;
+          const uint4 k0 = load_shared16(at), k1 = load_shared16(at + 8 * DP);
           const uint32_t lo[4] = {k0.x, k0.y, k0.z, k0.w}, hi[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -625,40 +673,46 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
           }
         }
       }
-      float ks[2], lv[2];
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        ks[g] = load_shared4(from + L::K_BYTES + L::V_BYTES + g * 4);
-        lv[g] = log2_fast(load_shared4(from + L::K_BYTES + L::V_BYTES + 8 + g * 4));
-      }
+      const uint4 scales = load_shared16(from + L::K_BYTES + L::V_BYTES);  // two of the keys, two of the values
+      const float ks[2] = {__uint_as_float(scales.x), __uint_as_float(scales.y)};
+      const float lv[2] = {log2_fast(__uint_as_float(scales.z)), log2_fast(__uint_as_float(scales.w))};
       const int t0 = step * STEP;
       const bool masked = t0 + STEP > sure;
+      // scores in base 2 are s * unit; where some are masked they are multiplied
+      // out first
+      float unit[2][NT][2];
       bool passed = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int g = 0; g < 2; ++g)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[g][nt][e] *= factor[nt][e & 1] * ks[g];
+          for (int u = 0; u < 2; ++u) unit[g][nt][u] = factor[nt][u] * ks[g];
         if (masked) {
 #pragma unroll
           for (int g = 0; g < 2; ++g)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (t0 + 16 * g + n8 + 8 * (e >> 1) >= limit[nt][e & 1]) s[g][nt][e] = -INFINITY;
+              s[g][nt][e] = t0 + 16 * g + n8 + 8 * (e >> 1) < limit[nt][e & 1] ? s[g][nt][e] * unit[g][nt][e & 1] : -INFINITY;
+#pragma unroll
+          for (int g = 0; g < 2; ++g) unit[g][nt][0] = unit[g][nt][1] = 1.f;
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const float b0 = fmaxf(s[0][nt][u], s[0][nt][u + 2]), b1 = fmaxf(s[1][nt][u], s[1][nt][u + 2]);
+          const float b0 = fmaxf(s[0][nt][u], s[0][nt][u + 2]) * unit[0][nt][u];
+          const float b1 = fmaxf(s[1][nt][u], s[1][nt][u + 2]) * unit[1][nt][u];
           passed |= fmaxf(b0, b1) > m[nt][u] + LEAD || fmaxf(b0 + lv[0], b1 + lv[1]) > mo[nt][u] + LEAD;
         }
       }
-      if (__any_sync(0xffffffffu, passed)) {
+      const bool move = __any_sync(0xffffffffu, passed);
+      load_keys(stage);  // every lane has read this step's keys and scales
+      if (move) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const float b0 = fmaxf(s[0][nt][u], s[0][nt][u + 2]), b1 = fmaxf(s[1][nt][u], s[1][nt][u + 2]);
+            const float b0 = fmaxf(s[0][nt][u], s[0][nt][u + 2]) * unit[0][nt][u];
+            const float b1 = fmaxf(s[1][nt][u], s[1][nt][u + 2]) * unit[1][nt][u];
             float top = fmaxf(b0, b1), top_o = fmaxf(b0 + lv[0], b1 + lv[1]);
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) {
@@ -686,12 +740,13 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
         for (int g = 0; g < 2; ++g)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const float x0 = s[g][nt][2 * r], x1 = s[g][nt][2 * r + 1];
-            l[nt][0] += exp2_fast(x0 - r0);
-            l[nt][1] += exp2_fast(x1 - r1);
-            pf[g][nt][r] = transpose8x8(half2_bits(exp2_fast(x0 + (lv[g] - w0)), exp2_fast(x1 + (lv[g] - w1))));
+            const float x0 = s[g][nt][2 * r], x1 = s[g][nt][2 * r + 1], u0 = unit[g][nt][0], u1 = unit[g][nt][1];
+            l[nt][0] += exp2_fast(fmaf(x0, u0, -r0));
+            l[nt][1] += exp2_fast(fmaf(x1, u1, -r1));
+            pf[g][nt][r] = transpose8x8(half2_bits(exp2_fast(fmaf(x0, u0, lv[g] - w0)), exp2_fast(fmaf(x1, u1, lv[g] - w1))));
           }
       }
+      copy_wait<3>();  // all but the next step and the keys after it
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         uint32_t v[4][L::V_WORD / 4];
@@ -718,6 +773,9 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
           for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][t], a0, a1, a2, a3, pf[g][nt][0], pf[g][nt][1]);
         }
       }
+      load_values(stage);
+      next_step();
+      stage ^= 1;
     }
 
 #pragma unroll
@@ -883,7 +941,12 @@ int launch_tiles(Attention a, cudaStream_t stream) {
 template <typename T, typename C>
 int launch_attention(const Attention &a, cudaStream_t stream) {
   if constexpr (sizeof(T) == 2) {
-    if (a.head_dim <= 128) {
+    // 32-bit strides within a pool of pages
+    bool small = true;
+    for (int64_t x : {a.k_page, a.v_page, a.k_token * 32, a.v_token * 32, a.ks_page, a.vs_page})
+      small = small && x >= 0 && x < (1LL << 32);
+    small = small && a.k_token * a.page < (1LL << 32) && a.v_token * a.page < (1LL << 32);
+    if (a.head_dim <= 128 && small) {
       const bool one = a.rows <= 8;
       if (a.head_dim <= 64)
         return one ? launch_tiles<T, C, 64, 1>(a, stream) : launch_tiles<T, C, 64, 2>(a, stream);
@@ -950,6 +1013,7 @@ extern "C" int nt_b200_paged_attention(const NtB200PagedAttentionArgs *a, void *
   p.head_dim = (int)c.head_dim;
   p.page = (int)c.page;
   p.rows = (int)(a->queries * p.group);
+  p.q_vector = p.q_dim == 1 && p.q_batch % 8 == 0 && p.q_token % 8 == 0 && p.q_head % 8 == 0 && rotary::aligned16(p.query);
   p.scale = (float)(a->scale * 1.4426950408889634);
   p.parts = static_cast<float *>(a->workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
