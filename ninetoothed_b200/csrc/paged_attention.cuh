@@ -15,7 +15,9 @@
 // keeps every SM busy to the end and no warp waits for another; a unit that
 // lies in one share is finished there.  Of the others, a CTA joins at its end
 // what neighbouring warps hold of one unit, and leaves its parts (o, m, l) in a
-// workspace; a second kernel joins those.  (Warps that took the steps of a unit
+// workspace; the CTA that brings a unit's last part joins them, always in the
+// line's order.  (A second kernel for that cost 10 to 15 us a call: the first
+// holds all registers, so nothing of the second overlaps it.)  (Warps that took the steps of a unit
 // in turn and joined at the end of every unit took 108 us where this takes
 // DRAFT_US for 256 units of up to 2047 tokens: short units cost a CTA as much as
 // long ones.)
@@ -78,7 +80,9 @@ struct Attention {
   int rows, row_tiles;      // queries * group; tiles of them
   int q_vector;             // queries can be read 16 bytes at a time
   float scale;              // softmax scale * log2 e
-  float *parts;             // workspace: two parts a warp
+  unsigned long long *counters; // workspace: one a warp, then
+  float *parts;                 // two parts a warp
+  unsigned long long tag;       // of this call, 48 bits
 };
 
 // The cached length of a sequence, in its block table's capacity.
@@ -247,7 +251,7 @@ template <int DP, int NT> struct Layout {
   static constexpr int SMEM = WARPS * STAGES * STAGE;
   // a part in the workspace: o [ROWS][DP], then m, l, mo [ROWS]
   static constexpr int PART = ROWS * (DP + 3);
-  static_assert(SMEM + 256 <= 232448, "shared memory of a CTA");
+  static_assert(SMEM + 2048 <= 232448, "shared memory of a CTA");
   static_assert(PART * 4 <= STAGES * STAGE, "a warp's part fits its ring");
 };
 
@@ -292,8 +296,7 @@ __device__ __forceinline__ void separate_nans(uint32_t (&v)[4][DP / 32], float (
 // Where a walk along the line of steps stands: before step s of a unit of
 // sequence b (n steps a unit), `left` steps to go in the piece.
 struct Walk {
-  int64_t left;
-  int b, length, n, unit, s;
+  int left, b, length, n, unit, s;
 };
 struct Segment {  // steps [s0, s1) of one unit
   int length, b, head, tile, s0, s1, n;
@@ -315,7 +318,7 @@ __device__ __forceinline__ bool next_segment(const Attention &a, Walk &w, Segmen
   g.head = w.unit / a.row_tiles;
   g.tile = w.unit % a.row_tiles;
   g.s0 = w.s;
-  const int take = w.left < w.n - w.s ? (int)w.left : w.n - w.s;
+  const int take = min(w.left, w.n - w.s);
   g.s1 = g.s0 + take;
   w.left -= take;
   w.s += take;
@@ -327,29 +330,21 @@ __device__ __forceinline__ bool next_segment(const Attention &a, Walk &w, Segmen
 }
 
 // Steps of one unit of sequence b; 0 past the last sequence.
-__device__ __forceinline__ int64_t unit_steps(const Attention &a, int64_t b) {
+__device__ __forceinline__ int unit_steps(const Attention &a, int b) {
   const int64_t n = b < a.batch ? a.lengths[b] : 0;
   return n <= 0 ? 0 : steps_of(n < a.capacity ? n : a.capacity);
 }
 
-// Steps of the line up to sequence `end`; every lane of a warp gets the sum.
-__device__ __forceinline__ int64_t steps_below(const Attention &a, int64_t end) {
-  int64_t sum = 0;
-  for (int64_t b = threadIdx.x & 31; b < end; b += 32) sum += unit_steps(a, b);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum * a.kv_heads * a.row_tiles;
-}
-
-// The cut of a line of `total` steps: `cta` steps a CTA, `warp` a warp.
+// The cut of a line of `total` steps: `cta` steps a CTA, `warp` a warp.  (The
+// host has seen to it that the line's steps fit 31 bits.)
 struct Cut {
-  int64_t total, cta, warp;
+  int total, cta, warp;
 };
-__device__ __forceinline__ Cut cut_line(const Attention &a, int64_t ctas, int warps) {
-  Cut c;
-  c.total = steps_below(a, a.batch);
-  c.cta = (c.total + ctas - 1) / ctas;
-  if (c.cta < LEAST_STEPS) c.cta = LEAST_STEPS;
+__device__ __forceinline__ Cut cut_line(const Attention &a, int ctas, int warps) {
+  Cut c{0, 0, 0};
+  for (int b = threadIdx.x & 31; b < a.batch; b += 32) c.total += unit_steps(a, b);
+  c.total = __reduce_add_sync(0xffffffffu, c.total) * a.kv_heads * a.row_tiles;
+  c.cta = max((int)(((unsigned)c.total + ctas - 1) / ctas), LEAST_STEPS);
   c.warp = (c.cta + warps - 1) / warps;
   return c;
 }
@@ -410,12 +405,49 @@ __device__ __forceinline__ void write_part(float *part, const float (&o)[NT][DP 
     }
 }
 
-// What a warp holds at the end of its share: a part of `unit` (-1: none), and
-// whether that is all the share has.
-struct Held {
-  int64_t unit;
+// A unit that several shares hold: n steps (0: none) from step `first` of the
+// line; `only`: it is all that the warp's share has.
+struct Shared {
+  int first, b, head, tile, n;
   bool only;
 };
+
+// Where the CTAs' parts of a unit are: the first CTA's run at `head` (the run
+// begins with the warp that holds the unit's first step, in that warp's second
+// place, unless its share begins with the unit), the runs of the CTAs k0 + 1 ..
+// k1 in their first warps' first places, and, if the unit ends inside a later
+// warp's share of CTA k1, that warp's first place (`tail`, else < 0).
+struct Parts {
+  int counter, k0, k1, head, tail;
+  __device__ int count() const { return k1 - k0 + 1 + (tail >= 0); }
+  __device__ int place(int j, int warps) const { return j == 0 ? head : j <= k1 - k0 ? 2 * (k0 + j) * warps : tail; }
+};
+__device__ __forceinline__ Parts parts_of(const Shared &u, const Cut &c, int warps) {
+  Parts p;
+  p.k0 = (unsigned)u.first / (unsigned)c.cta;
+  const int lo = u.first - p.k0 * c.cta, w0 = (unsigned)lo / (unsigned)c.warp, last = u.first + u.n - 1;
+  p.counter = p.k0 * warps + w0;
+  p.head = 2 * p.counter + (lo == w0 * c.warp ? 0 : 1);
+  p.k1 = (unsigned)last / (unsigned)c.cta;
+  const int hi = last - p.k1 * c.cta, w1 = (unsigned)hi / (unsigned)c.warp;
+  const int share_end = min(min((w1 + 1) * c.warp, c.cta), c.total - p.k1 * c.cta);
+  const bool later = w1 > (p.k1 == p.k0 ? w0 : 0);
+  p.tail = later && hi + 1 < share_end ? 2 * (p.k1 * warps + w1) : -1;
+  return p;
+}
+
+// Counts one more of a unit's parts as written; true for the last.  A counter is
+// the call's 48-bit tag and a count; one without the tag, whatever the workspace
+// held, is first set to the tag and zero (once: whoever else tries finds it
+// changed).  The last to come leaves it without the tag, for a graph that
+// replays the call with the same tag.
+__device__ __forceinline__ bool arrive(unsigned long long *counter, unsigned long long tag, int expected) {
+  const unsigned long long now = *reinterpret_cast<volatile unsigned long long *>(counter);
+  if ((now >> 16) != tag) atomicCAS(counter, now, tag << 16);
+  if ((int)(atomicAdd(counter, 1ull) & 0xffffu) + 1 != expected) return false;
+  *reinterpret_cast<volatile unsigned long long *>(counter) = 0;
+  return true;
+}
 
 // The maxima that P is taken against move only when a score passes them by
 // this (base 2): P, up to 2^LEAD, stays in fp16's range and as precise, a step's
@@ -423,13 +455,73 @@ struct Held {
 // of a row and the rescaling of O happen rarely.
 constexpr float LEAD = 8.f;
 
+// Joins a unit's parts and writes its rows; a warp of the block takes a row.
+// (This runs once a call, mostly from a cold instruction cache: small code.)
+template <typename T, int DP, int NT>
+__device__ __forceinline__ void join_unit(const Attention &a, const Shared &u, const Parts &where) {
+  using L = Layout<DP, NT>;
+  const int lane = threadIdx.x & 31, parts = where.count();
+  constexpr int LANES = DP / 4, AT_ONCE = 32 / LANES;  // lanes of a part's row; parts read side by side
+#pragma unroll 1
+  for (int r = threadIdx.x >> 5; r < L::ROWS; r += L::WARPS) {
+    float top = -INFINITY, top_o = -INFINITY, sum = 0.f, acc[4] = {};
+    // 32 parts at a time, each chunk's maxima joined to those before
+#pragma unroll 1
+    for (int j0 = 0; j0 < parts; j0 += 32) {
+      float m = -INFINITY, l = 0.f, mo = -INFINITY;
+      const float *p = nullptr;
+      if (j0 + lane < parts) {
+        p = a.parts + (int64_t)where.place(j0 + lane, L::WARPS) * L::PART;
+        m = __ldcg(p + L::ROWS * DP + r * 3);
+        l = __ldcg(p + L::ROWS * DP + r * 3 + 1);
+        mo = __ldcg(p + L::ROWS * DP + r * 3 + 2);
+        p += r * DP;
+      }
+      float m_new = m, mo_new = mo;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) {
+        m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, x));
+        mo_new = fmaxf(mo_new, __shfl_xor_sync(0xffffffffu, mo_new, x));
+      }
+      m_new = fmaxf(m_new, top);
+      mo_new = fmaxf(mo_new, top_o);
+      sum = sum * exp2_fast(top - reference(m_new)) + l * exp2_fast(m - reference(m_new));
+      const float alpha = exp2_fast(top_o - reference(mo_new)), f = exp2_fast(mo - reference(mo_new));
+      top = m_new;
+      top_o = mo_new;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] *= alpha;
+      const int count = min(parts - j0, 32);
+#pragma unroll 8
+      for (int j = 0; j < count; j += AT_ONCE) {
+        const int from = j + lane / LANES;
+        const uint64_t at = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(p), from);
+        const float g = __shfl_sync(0xffffffffu, f, from);
+        if (at != 0) {
+          const float4 v = __ldcg(reinterpret_cast<const float4 *>(at) + lane % LANES);
+          acc[0] = fmaf(v.x, g, acc[0]); acc[1] = fmaf(v.y, g, acc[1]);
+          acc[2] = fmaf(v.z, g, acc[2]); acc[3] = fmaf(v.w, g, acc[3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    if (AT_ONCE == 2) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], 16);
+    }
+    if (lane < LANES) write_row<T>(a, u.b, u.head, u.tile * L::ROWS + r, lane * 4, acc, top, sum, top_o);
+  }
+}
+
 template <typename T, typename C, int DP, int NT>
 __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kernel(const __grid_constant__ Attention a) {
   using L = Layout<DP, NT>;
   constexpr int WARPS = L::WARPS;
   constexpr int KS = DP / 16, OT = DP / 16;  // contraction steps of QK; 16-element tiles of O
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ Held runs[WARPS];
+  __shared__ Shared runs[WARPS], joins[2 * WARPS];
+  __shared__ Parts places[2 * WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n8 = lane >> 2, c4 = lane & 3;
   const uint32_t ring = ptx::smem_u32(smem) + warp * L::STAGES * L::STAGE;
   wait_prior_grid();
@@ -437,19 +529,19 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
 
   // this warp's share of the line
   const Cut cut = cut_line(a, gridDim.x, WARPS);
-  int64_t first = blockIdx.x * cut.cta + warp * cut.warp;
-  const int64_t end = min(cut.total, min(first + cut.warp, (blockIdx.x + 1) * cut.cta));
+  int first = min((int64_t)blockIdx.x * cut.cta + warp * cut.warp, (int64_t)cut.total);
+  const int end = min((int64_t)cut.total, min((int64_t)first + cut.warp, (int64_t)(blockIdx.x + 1) * cut.cta));
   Walk start{};
-  start.left = first < end ? end - first : 0;
+  start.left = max(end - first, 0);
   if (start.left > 0) {
     // the sequence that holds step `first`, 32 sequences at a time
     const int units = a.kv_heads * a.row_tiles;
-    for (int64_t b0 = 0;; b0 += 32) {
-      const int64_t n = unit_steps(a, b0 + lane) * units;
-      int64_t up = n;  // inclusive sum over the lanes
+    for (int b0 = 0;; b0 += 32) {
+      const int n = unit_steps(a, b0 + lane) * units;
+      int up = n;  // inclusive sum over the lanes
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, up, o);
+        const int x = __shfl_up_sync(0xffffffffu, up, o);
         if (lane >= o) up += x;
       }
       const int which = __popc(__ballot_sync(0xffffffffu, up <= first));  // sums are nondecreasing
@@ -458,13 +550,13 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
         continue;
       }
       first -= __shfl_sync(0xffffffffu, up - n, which);
-      start.b = (int)(b0 + which);
+      start.b = b0 + which;
       break;
     }
     start.length = cached_length(a, start.b);
     start.n = steps_of(start.length);
-    start.unit = (int)(first / start.n);
-    start.s = (int)(first - (int64_t)start.unit * start.n);
+    start.unit = (unsigned)first / (unsigned)start.n;
+    start.s = first - start.unit * start.n;
   }
 
   // ------------------------------------------------------------ loads ahead
@@ -584,9 +676,19 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
   }
   int stage = 0;
 
+  // rows of sequences without keys
+  for (int64_t b = (int64_t)blockIdx.x * WARPS + warp; b < a.batch; b += (int64_t)gridDim.x * WARPS) {
+    if (cached_length(a, b) > 0) continue;
+    const float zero[1] = {0.f};
+    for (int64_t x = lane; x < (int64_t)a.kv_heads * a.rows * a.head_dim; x += 32) {
+      const int64_t r = x / a.head_dim;
+      write_row<T>(a, b, (int)(r / a.rows), (int)(r % a.rows), (int)(x % a.head_dim), zero, -INFINITY, 0.f, -INFINITY);
+    }
+  }
+
   Walk here = start;
   Segment seg;
-  Held held{-1, false};
+  Shared before{}, held{};  // parts of the unit from the share before, and of the last
   while (next_segment(a, here, seg)) {
     const int row0 = seg.tile * L::ROWS;
 
@@ -795,132 +897,77 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
         }
       continue;
     }
-    const bool is_first = here.left + (seg.s1 - seg.s0) == start.left;
-    if (here.left > 0) {  // the end of a unit from the share before
-      write_part<DP, NT>(a.parts + (2 * ((int64_t)blockIdx.x * WARPS + warp)) * L::PART, o, m, l, mo);
-      continue;
+    const Shared unit{end - here.left - seg.s1, seg.b, seg.head, seg.tile, seg.n, here.left + (seg.s1 - seg.s0) == start.left};
+    if (here.left > 0) {
+      before = unit;
+      write_part<DP, NT>(a.parts + 2 * ((int64_t)blockIdx.x * WARPS + warp) * L::PART, o, m, l, mo);
+    } else {  // kept for the CTA's join
+      held = unit;
+      write_part<DP, NT>(reinterpret_cast<float *>(smem + warp * L::STAGES * L::STAGE), o, m, l, mo);
     }
-    // the share's last segment: kept for the CTA's join
-    held.unit = ((int64_t)seg.b * a.kv_heads + seg.head) * a.row_tiles + seg.tile;
-    held.only = is_first;
-    write_part<DP, NT>(reinterpret_cast<float *>(smem + warp * L::STAGES * L::STAGE), o, m, l, mo);
   }
 
   // ------------------------------------------------------------ the CTA's join
   // A run: a warp's last segment and the warps after it that have nothing but
   // the same unit.  Its first warp adds up the others'.
-  if (lane == 0) runs[warp] = held;
+  if (lane == 0) {
+    runs[warp] = held;
+    joins[2 * warp].n = joins[2 * warp + 1].n = 0;
+  }
   __syncthreads();
-  if (held.unit < 0 || (warp > 0 && held.only && runs[warp - 1].unit == held.unit)) return;
-  int last = warp;
-  while (last + 1 < WARPS && runs[last + 1].only && runs[last + 1].unit == held.unit) ++last;
-  const int row = lane / (32 / L::ROWS);  // ROWS divides 32: lanes of a row share its elements
-  float *part = a.parts + (2 * ((int64_t)blockIdx.x * WARPS + warp) + (held.only ? 0 : 1)) * L::PART;
-  auto part_of = [&](int w) { return reinterpret_cast<const float *>(smem + w * L::STAGES * L::STAGE); };
-  float top = -INFINITY, top_o = -INFINITY, sum = 0.f;
-  for (int w = warp; w <= last; ++w) {
-    const float *st = part_of(w) + L::ROWS * DP + row * 3;
-    top = fmaxf(top, st[0]);
-    top_o = fmaxf(top_o, st[2]);
-  }
-  for (int w = warp; w <= last; ++w) {
-    const float *st = part_of(w) + L::ROWS * DP + row * 3;
-    sum += st[1] * exp2_fast(st[0] - reference(top));
-  }
-  constexpr int SHARE = DP * L::ROWS / 32;  // a lane's elements of its row
-  const int d0 = lane % (32 / L::ROWS) * 4;
-#pragma unroll 2
-  for (int x = 0; x < SHARE; x += 4) {
-    const int d = d0 + x * (32 / L::ROWS);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = warp; w <= last; ++w) {
-      const float f = exp2_fast(part_of(w)[L::ROWS * DP + row * 3 + 2] - reference(top_o));
-      const float4 v = *reinterpret_cast<const float4 *>(part_of(w) + row * DP + d);
-      acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y);
-      acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+  const bool leads = held.n > 0 && !(warp > 0 && held.only && runs[warp - 1].n > 0 && runs[warp - 1].first == held.first);
+  if (leads) {
+    int last = warp;
+    while (last + 1 < WARPS && runs[last + 1].n > 0 && runs[last + 1].only && runs[last + 1].first == held.first) ++last;
+    const int row = lane / (32 / L::ROWS);  // ROWS divides 32: lanes of a row share its elements
+    float *part = a.parts + (2 * ((int64_t)blockIdx.x * WARPS + warp) + (held.only ? 0 : 1)) * L::PART;
+    const float *in = reinterpret_cast<const float *>(smem + warp * L::STAGES * L::STAGE);
+    constexpr int NEXT = L::STAGES * L::STAGE / 4, STATS = L::ROWS * DP;
+    float top = -INFINITY, top_o = -INFINITY, sum = 0.f;
+#pragma unroll 1
+    for (int w = 0; w <= last - warp; ++w) {
+      const float *st = in + w * NEXT + STATS + row * 3;
+      const float m_new = fmaxf(top, st[0]);
+      sum = sum * exp2_fast(top - reference(m_new)) + st[1] * exp2_fast(st[0] - reference(m_new));
+      top = m_new;
+      top_o = fmaxf(top_o, st[2]);
     }
-    *reinterpret_cast<float4 *>(part + row * DP + d) = acc;
+#pragma unroll 1
+    for (int d = lane % (32 / L::ROWS) * 4; d < DP; d += 128 / L::ROWS) {
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (int w = 0; w <= last - warp; ++w) {
+        const float f = exp2_fast(in[w * NEXT + STATS + row * 3 + 2] - reference(top_o));
+        const float4 v = *reinterpret_cast<const float4 *>(in + w * NEXT + row * DP + d);
+        acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y);
+        acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+      }
+      *reinterpret_cast<float4 *>(part + row * DP + d) = acc;
+    }
+    if (lane % (32 / L::ROWS) == 0) {
+      part[STATS + row * 3] = top;
+      part[STATS + row * 3 + 1] = sum;
+      part[STATS + row * 3 + 2] = top_o;
+    }
   }
-  if (lane % (32 / L::ROWS) == 0) {
-    part[L::ROWS * DP + row * 3] = top;
-    part[L::ROWS * DP + row * 3 + 1] = sum;
-    part[L::ROWS * DP + row * 3 + 2] = top_o;
-  }
-}
 
-// Joins the parts of the units that several shares held, one block a unit, a
-// warp a row, and writes the rows of sequences without keys.
-constexpr int JOIN_WARPS = 8;
-template <typename T, int DP, int NT>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_constant__ Attention a, int64_t ctas) {
-  using L = Layout<DP, NT>;
-  const int lane = threadIdx.x & 31;
-  wait_prior_grid();
-  const int units = a.kv_heads * a.row_tiles;
-  const int64_t b = blockIdx.x / units;
-  const int unit = (int)(blockIdx.x % units), h = unit / a.row_tiles, row0 = unit % a.row_tiles * L::ROWS;
-  const int64_t n = steps_of(cached_length(a, b));
-  const Cut cut = cut_line(a, ctas, L::WARPS);
-  const int64_t first = steps_below(a, b) + unit * n, end = first + n;
-  const int64_t k0 = first / cut.cta, k1 = n > 0 ? (end - 1) / cut.cta : k0;
-  if (n > 0 && k0 == k1 && (first - k0 * cut.cta) / cut.warp == (end - 1 - k0 * cut.cta) / cut.warp) return;
-  // Part j of the unit, or null.  CTA k0 + j / 2 left a run from the warp that
-  // holds the unit's first step there (the warp's second place, unless its
-  // share begins with the unit), and, if the unit ends inside a later warp's
-  // share, that warp's first place.
-  auto part_of = [&](int64_t j) -> const float * {
-    const int64_t k = k0 + j / 2, base = k * cut.cta;
-    if (n == 0 || k > k1) return nullptr;
-    const int64_t lo = max(first, base) - base, hi = min(end, base + cut.cta) - 1 - base;
-    const int64_t w0 = lo / cut.warp, w1 = hi / cut.warp;
-    if (j % 2 == 0) return a.parts + (2 * (k * L::WARPS + w0) + (lo == w0 * cut.warp ? 0 : 1)) * L::PART;
-    const int64_t share_end = min(min((w1 + 1) * cut.warp, cut.cta), cut.total - base);
-    return w1 > w0 && hi + 1 < share_end ? a.parts + 2 * (k * L::WARPS + w1) * L::PART : nullptr;
-  };
-  const int64_t parts = 2 * (k1 - k0 + 1);
-  constexpr int LANES = DP / 4, AT_ONCE = 32 / LANES;  // lanes of a part's row; parts read side by side
-  for (int r = threadIdx.x >> 5; r < L::ROWS; r += JOIN_WARPS) {
-    float top = -INFINITY, top_o = -INFINITY, sum = 0.f, acc[4] = {};
-    for (int64_t j = lane; j < parts; j += 32) {
-      const float *p = part_of(j);
-      if (p) {
-        top = fmaxf(top, p[L::ROWS * DP + r * 3]);
-        top_o = fmaxf(top_o, p[L::ROWS * DP + r * 3 + 2]);
-      }
+  // ------------------------------------------------------------ the units' join
+  // lanes 0 and 1: the run, the part of the unit from the share before
+  __threadfence();
+  __syncwarp();
+  const Shared mine = lane == 0 ? held : before;
+  if (lane < 2 && mine.n > 0 && (leads || lane == 1)) {
+    const Parts where = parts_of(mine, cut, WARPS);
+    if (arrive(a.counters + where.counter, a.tag, where.count())) {
+      joins[2 * warp + lane] = mine;
+      places[2 * warp + lane] = where;
+      __threadfence();
     }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) {
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      top_o = fmaxf(top_o, __shfl_xor_sync(0xffffffffu, top_o, x));
-    }
-    for (int64_t j0 = 0; j0 < parts; j0 += 32) {
-      const float *p = j0 + lane < parts ? part_of(j0 + lane) : nullptr;
-      float f = 0.f;
-      if (p) {
-        sum += p[L::ROWS * DP + r * 3 + 1] * exp2_fast(p[L::ROWS * DP + r * 3] - reference(top));
-        f = exp2_fast(p[L::ROWS * DP + r * 3 + 2] - reference(top_o));
-      }
-      const int count = (int)(parts - j0 < 32 ? parts - j0 : 32);
-#pragma unroll 4
-      for (int j = 0; j < count; j += AT_ONCE) {
-        const int from = j + lane / LANES;
-        const uint64_t at = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(p), from);
-        const float g = __shfl_sync(0xffffffffu, f, from);
-        if (at != 0) {
-          const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(at) + r * DP + lane % LANES * 4);
-          acc[0] = fmaf(v.x, g, acc[0]); acc[1] = fmaf(v.y, g, acc[1]);
-          acc[2] = fmaf(v.z, g, acc[2]); acc[3] = fmaf(v.w, g, acc[3]);
-        }
-      }
-    }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    if (AT_ONCE == 2) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], 16);
-    }
-    if (lane < LANES) write_row<T>(a, b, h, row0 + r, lane * 4, acc, top, sum, top_o);
   }
+  __syncthreads();
+#pragma unroll 1
+  for (int i = 0; i < 2 * WARPS; ++i)
+    if (joins[i].n > 0) join_unit<T, DP, NT>(a, joins[i], places[i]);
 }
 
 template <typename T, typename C, int DP, int NT>
@@ -929,13 +976,21 @@ int launch_tiles(Attention a, cudaStream_t stream) {
   cudaError_t e = smem_optin<attention_kernel<T, C, DP, NT>>(L::SMEM);
   if (e != cudaSuccess) return (int)e;
   a.row_tiles = (a.rows + L::ROWS - 1) / L::ROWS;
-  const int64_t units = (int64_t)a.batch * a.kv_heads * a.row_tiles;
-  if (units > (1LL << 31) - 1) return NT_B200_ERR_INVALID_ARGUMENT;
-  const int grid = sm_count();
-  const int rc =
-      launch_overlapped(attention_kernel<T, C, DP, NT>, dim3((unsigned)grid), dim3(L::WARPS * 32), L::SMEM, stream, a);
-  if (rc != 0) return rc;
-  return launch_overlapped(join_kernel<T, DP, NT>, dim3((unsigned)units), dim3(JOIN_WARPS * 32), 0, stream, a, (int64_t)grid);
+  return launch_overlapped(attention_kernel<T, C, DP, NT>, dim3((unsigned)sm_count()), dim3(L::WARPS * 32), L::SMEM, stream, a);
+}
+
+// Counters of a workspace: one for each warp of up to 512 SMs.
+constexpr int64_t COUNTERS = 512 * 12;
+
+// A tag that no other call of the process has: a counter through an invertible
+// mix, so that it looks like nothing that a workspace may have held before.
+inline unsigned long long call_tag() {
+  static std::atomic<unsigned long long> calls{0};
+  constexpr unsigned long long mask = (1ull << 48) - 1;
+  unsigned long long x = calls.fetch_add(1, std::memory_order_relaxed) + 1;
+  x = (x * 0x9e3779b97f4a7c15ull) & mask;
+  x ^= x >> 25;
+  return (x * 0xbf58476d1ce4e5b9ull) & mask;
 }
 
 template <typename T, typename C>
@@ -946,7 +1001,9 @@ int launch_attention(const Attention &a, cudaStream_t stream) {
     for (int64_t x : {a.k_page, a.v_page, a.k_token * 32, a.v_token * 32, a.ks_page, a.vs_page})
       small = small && x >= 0 && x < (1LL << 32);
     small = small && a.k_token * a.page < (1LL << 32) && a.v_token * a.page < (1LL << 32);
-    if (a.head_dim <= 128 && small) {
+    // and a line of steps that 31 bits count
+    small = small && (double)a.batch * a.kv_heads * ((a.rows + 7) / 8) * (a.capacity / STEP + 1) < 2e9;
+    if (a.head_dim <= 128 && small && sm_count() <= 512) {
       const bool one = a.rows <= 8;
       if (a.head_dim <= 64)
         return one ? launch_tiles<T, C, 64, 1>(a, stream) : launch_tiles<T, C, 64, 2>(a, stream);
@@ -967,7 +1024,7 @@ extern "C" int64_t nt_b200_paged_attention_workspace_size(void) {
   // two parts a warp of the largest layout; the CTAs of a launch are the SMs
   constexpr int64_t one = (int64_t)Layout<128, 1>::WARPS * Layout<128, 1>::PART;
   constexpr int64_t two = (int64_t)Layout<128, 2>::WARPS * Layout<128, 2>::PART;
-  return 2 * (int64_t)nt::sm_count() * (one > two ? one : two) * (int64_t)sizeof(float);
+  return COUNTERS * 8 + 2 * (int64_t)nt::sm_count() * (one > two ? one : two) * (int64_t)sizeof(float);
 }
 
 extern "C" int nt_b200_paged_attention(const NtB200PagedAttentionArgs *a, void *stream) {
@@ -1015,7 +1072,9 @@ extern "C" int nt_b200_paged_attention(const NtB200PagedAttentionArgs *a, void *
   p.rows = (int)(a->queries * p.group);
   p.q_vector = p.q_dim == 1 && p.q_batch % 8 == 0 && p.q_token % 8 == 0 && p.q_head % 8 == 0 && rotary::aligned16(p.query);
   p.scale = (float)(a->scale * 1.4426950408889634);
-  p.parts = static_cast<float *>(a->workspace);
+  p.counters = static_cast<unsigned long long *>(a->workspace);
+  p.parts = reinterpret_cast<float *>(p.counters + paged::COUNTERS);
+  p.tag = paged::call_tag();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return NT_DISPATCH_FLOAT((int)a->dtype, [&] {
     if (c.code_dtype == NT_B200_INT8) return paged::launch_attention<scalar_t, int8_t>(p, s);
