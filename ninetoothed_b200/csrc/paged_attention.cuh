@@ -29,8 +29,8 @@
 // elements is as good as another, so each lane takes 16 neighbouring bytes of a
 // key as its share of the head, and 16 neighbouring elements of four tokens'
 // values: loads are whole 16-byte words and bytes are paired with one permute.
-// A lane reads from shared memory just what it copied there itself
-// (cp.async), so the ring of stages needs no barrier.
+// Each warp copies for itself (cp.async) through a ring of its own, so nothing
+// waits for another warp.
 //
 // Codes become fp16 (exact for both types).  A query row is scaled by a power
 // of two to a largest element in [1, 2), so that bfloat16 rows fit too; P is
@@ -79,6 +79,7 @@ struct Attention {
   uint64_t page_reciprocal; // ceil(2^36 / page_groups)
   int rows, row_tiles;      // queries * group; tiles of them
   int q_vector;             // queries can be read 16 bytes at a time
+  int bf16;                 // query and output elements: bfloat16, else fp16
   float scale;              // softmax scale * log2 e
   unsigned long long *counters; // workspace: one a warp, then
   float *parts;                 // two parts a warp
@@ -170,9 +171,6 @@ constexpr int MOST_PAGE = 4096;
 __device__ __forceinline__ void copy_async16(uint32_t to, const void *from, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void copy_async8(uint32_t to, const void *from, bool valid) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(valid ? 8 : 0) : "memory");
-}
 __device__ __forceinline__ void copy_async4(uint32_t to, const void *from, bool valid) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(valid ? 4 : 0) : "memory");
 }
@@ -232,33 +230,44 @@ template <> __device__ __forceinline__ void to_halves<int8_t>(uint32_t w, uint32
   hi = *reinterpret_cast<uint32_t *>(&y);
 }
 
-// Where word w of a token's key lies in its row in shared memory.
-template <int DP> __device__ __forceinline__ int place_of(int token, int w) {
-  return DP == 128 ? w ^ ((token & 1) << 2) : w;
+// Tokens of a 16-token group in the order of the MMAs' rows: row r holds token
+// r / 2 (even r) or 4 + r / 2 (odd r), and so on from 8.  A lane's four values
+// (rows 2 c4, 2 c4 + 1, 2 c4 + 8, 2 c4 + 9) are then those of the tokens c4, 4 +
+// c4, 8 + c4 and 12 + c4: four neighbouring rows of shared memory a load.
+__device__ __forceinline__ int token_of(int row) { return (row >> 1 & 3) + 4 * (row & 1) + (row & 8); }
+__device__ __forceinline__ int row_at(int token) { return 2 * (token & 3) + (token >> 2 & 1) + (token & 8); }
+// Where a row's 16-byte word w lies in shared memory: moved so that a quarter
+// warp's (8-byte words: half a warp's) loads meet every bank once.  Keys are
+// kept in MMA order and read 8 rows by 4 words, values in token order and read
+// 4 rows by 2 words.
+template <int DP> __device__ __forceinline__ int key_place(int row, int w) { return DP == 128 ? w ^ ((row & 1) << 2) : w; }
+template <int DP> __device__ __forceinline__ int value_place(int token, int w) {
+  return DP == 128 ? w ^ ((token & 3) << 1) : w ^ (token & 2);
 }
 
 template <int DP, int NT> struct Layout {
   static constexpr int ROWS = 8 * NT;
-  // One column tile: 12 warps of up to 168 registers, three a scheduler, to
-  // cover each other's load and MMA latency (8 warps: 2.45 TB/s where 12 reach
-  // RATE).  Two column tiles hold twice the accumulators: 8 warps.
+  // One column tile: 12 warps of up to 168 registers, three a scheduler, to cover
+  // each other's latencies, each with two steps in flight (8 warps reach 0.8 of
+  // their rate; 16 warps of 128 registers spill and have room for a step and a
+  // half each: 0.88).  Two column tiles hold twice the accumulators: 8 warps.
   static constexpr int WARPS = NT == 1 ? 12 : 8;
-  static constexpr int STAGES = 2;
-  static constexpr int K_COPIES = DP / 64 * 4;              // 16-byte words a lane and step
-  static constexpr int V_WORD = DP / 8;                     // bytes of a token's value a lane takes
-  static constexpr int K_BYTES = STEP * DP, V_BYTES = STEP * DP;
-  static constexpr int STAGE = K_BYTES + V_BYTES + 32;      // + 2 key scales, 2 value scales
-  static constexpr int SMEM = WARPS * STAGES * STAGE;
+  static constexpr int V_WORD = DP / 8;           // bytes of a token's value a lane takes
+  static constexpr int SLOTS = 4;                 // of a warp's ring: keys, values of a step, of the next
+  static constexpr int CODES = STEP * DP;
+  static constexpr int SLOT = CODES + 16;         // + the step's scales (two of keys, two of values), with the keys
+  static constexpr int RING = SLOTS * SLOT;
+  static constexpr int SMEM = WARPS * RING;
   // a part in the workspace: o [ROWS][DP], then m, l, mo [ROWS]
   static constexpr int PART = ROWS * (DP + 3);
-  static_assert(SMEM + 2048 <= 232448, "shared memory of a CTA");
-  static_assert(PART * 4 <= STAGES * STAGE, "a warp's part fits its ring");
+  static_assert(SMEM + 3072 <= 232448, "shared memory of a CTA");
+  static_assert(PART * 4 <= RING, "a warp's part fits its ring");
 };
 
 // A value's NaN reaches only the rows that see its token, but 0 * NaN in an MMA
 // would reach every row.  In steps where rows differ in what they see, NaN
-// codes are taken out of a 16-token group's value words (token 2 c4 + i % 2 +
-// 8 (i / 2) in v[i], as loaded) and set into the rows' O here.
+// codes are taken out of a 16-token group's value words (token 4 i + c4 in v[i],
+// as loaded) and set into the rows' O here.
 template <int DP, int NT>
 __device__ __forceinline__ void separate_nans(uint32_t (&v)[4][DP / 32], float (&o)[NT][DP / 16][4],
                                               const int (&limit)[NT][2], int token0) {
@@ -281,7 +290,7 @@ __device__ __forceinline__ void separate_nans(uint32_t (&v)[4][DP / 32], float (
     }
     for (int c = 0; c < 4; ++c) {
       const uint32_t other = __shfl_sync(0xffffffffu, mask, (lane & ~3) | c);
-      const int token = token0 + 2 * c + (i & 1) + 8 * (i >> 1);
+      const int token = token0 + 4 * i + c;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -349,23 +358,32 @@ __device__ __forceinline__ Cut cut_line(const Attention &a, int ctas, int warps)
   return c;
 }
 
+// Query and output elements are fp16 or, with `bf16`, bfloat16: a run-time flag,
+// as only the ends of a unit depend on it.
+__device__ __forceinline__ float element(uint16_t bits, int bf16) {
+  return bf16 ? __uint_as_float((uint32_t)bits << 16) : __half2float(__ushort_as_half(bits));
+}
+__device__ __forceinline__ uint16_t element_bits(float x, int bf16) {
+  return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x)) : __half_as_ushort(__float2half_rn(x));
+}
+
 // N neighbouring elements of a finished row: o = acc * 2^(mo - m) / l, and the
 // row's lse.
-template <typename T, int N>
+template <int N>
 __device__ __forceinline__ void write_row(const Attention &a, int64_t b, int h, int row, int d, const float (&acc)[N],
                                           float m, float l, float mo) {
   if (row >= a.rows || d >= a.head_dim) return;
   const int i = row / a.group, hq = h * a.group + row % a.group;
   const float f = l == 0.f ? 0.f : exp2_fast(reference(mo) - reference(m)) / l;
-  T *out = static_cast<T *>(a.out) + b * a.o_batch + i * a.o_token + (int64_t)hq * a.o_head + d * a.o_dim;
+  uint16_t *out = static_cast<uint16_t *>(a.out) + b * a.o_batch + i * a.o_token + (int64_t)hq * a.o_head + d * a.o_dim;
   if (a.o_dim == 1 && (reinterpret_cast<uintptr_t>(out) & (2 * N - 1)) == 0) {
-    struct alignas(2 * N) Pack { T v[N]; } pack;
+    struct alignas(2 * N < 16 ? 2 * N : 16) Pack { uint16_t v[N]; } pack;
 #pragma unroll
-    for (int e = 0; e < N; ++e) pack.v[e] = from_f<T>(acc[e] * f);
+    for (int e = 0; e < N; ++e) pack.v[e] = element_bits(acc[e] * f, a.bf16);
     *reinterpret_cast<Pack *>(out) = pack;
   } else {
 #pragma unroll
-    for (int e = 0; e < N; ++e) out[e * a.o_dim] = from_f<T>(acc[e] * f);
+    for (int e = 0; e < N; ++e) out[e * a.o_dim] = element_bits(acc[e] * f, a.bf16);
   }
   if (a.lse && d == 0)
     a.lse[b * a.l_batch + i * a.l_token + (int64_t)hq * a.l_head] = l == 0.f ? -INFINITY : (m + log2_fast(l)) * kLn2;
@@ -457,7 +475,7 @@ constexpr float LEAD = 8.f;
 
 // Joins a unit's parts and writes its rows; a warp of the block takes a row.
 // (This runs once a call, mostly from a cold instruction cache: small code.)
-template <typename T, int DP, int NT>
+template <int DP, int NT>
 __device__ __forceinline__ void join_unit(const Attention &a, const Shared &u, const Parts &where) {
   using L = Layout<DP, NT>;
   const int lane = threadIdx.x & 31, parts = where.count();
@@ -510,11 +528,13 @@ __device__ __forceinline__ void join_unit(const Attention &a, const Shared &u, c
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], 16);
     }
-    if (lane < LANES) write_row<T>(a, u.b, u.head, u.tile * L::ROWS + r, lane * 4, acc, top, sum, top_o);
+    if (lane < LANES) write_row(a, u.b, u.head, u.tile * L::ROWS + r, lane * 4, acc, top, sum, top_o);
   }
 }
 
-template <typename T, typename C, int DP, int NT>
+// SPLIT: pages of an odd number of 16-token groups, so that a step may lie in
+// two pages with a scale each.
+template <typename C, int DP, int NT, bool SPLIT>
 __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kernel(const __grid_constant__ Attention a) {
   using L = Layout<DP, NT>;
   constexpr int WARPS = L::WARPS;
@@ -523,7 +543,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
   __shared__ Shared runs[WARPS], joins[2 * WARPS];
   __shared__ Parts places[2 * WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n8 = lane >> 2, c4 = lane & 3;
-  const uint32_t ring = ptx::smem_u32(smem) + warp * L::STAGES * L::STAGE;
+  const uint32_t ring = ptx::smem_u32(smem) + warp * L::RING;
   wait_prior_grid();
   allow_dependent_launch();
 
@@ -560,41 +580,45 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
   }
 
   // ------------------------------------------------------------ loads ahead
-  // A stage holds a step's keys and one its values; each is loaded again, two
-  // steps on, as soon as it has been read.
+  // A ring of four slots, keys and values of two steps; each is loaded again,
+  // two steps on, as soon as it has been read.
   Walk ahead = start;
   Segment lseg{};
   bool lmore = next_segment(a, ahead, lseg);
-  int lstep = lseg.s0;  // the next step to load
+  int lstep = lseg.s0;     // the step to load
   int id0 = -1, id1 = -1;  // pages of its two 16-token groups
   int group0 = 0;          // the first group's place in its page
+  // This lane's share of a 16-token group: whole rows, neighbouring words by
+  // neighbouring lanes, four (head_dim up to 64: eight) tokens an instruction.
+  // (Copied as the lanes read them, by lanes of four tokens in turn, values came
+  // from memory in 32-byte pieces: 318 us where this takes LONG_US for 6 x 131072
+  // tokens.)
+  constexpr int ROW_WORDS = DP / 16, COPIES = 16 * ROW_WORDS / 32;
+  const int k_row = lane / ROW_WORDS, k_word = lane % ROW_WORDS;  // of the first copy
+  const uint32_t k_token = (uint32_t)a.k_token, v_token = (uint32_t)a.v_token;
+  auto k_place = [&](int i) {
+    const int row = row_at(k_row + i * (32 / ROW_WORDS));
+    return ring + (uint32_t)(row * DP + key_place<DP>(row, k_word) * 16);
+  };
+  const uint32_t k_even = k_place(0), k_odd = k_place(1);  // places of copies 0 and 1; two copies on, eight rows on
+  const uint32_t v_place = ring + (uint32_t)(k_row * DP + value_place<DP>(k_row, k_word) * 16);
+  const uint8_t *key_head = nullptr, *value_head = nullptr;  // of the load segment
+  const float *scale_head = nullptr;                         // even lanes: key scales, odd: value scales
+  const uint32_t scale_page = (uint32_t)(lane & 1 ? a.vs_page : a.ks_page);
   auto find_pages = [&]() {
     const int g = lstep * (STEP / 16);
     const int col = (int)(((uint64_t)(uint32_t)g * a.page_reciprocal) >> 36);
     group0 = g - col * a.page_groups;
     id0 = page_of(a, lseg.b, col);
-    id1 = id0;
-    if (group0 + 1 == a.page_groups) id1 = (g + 1) * 16 < lseg.length ? page_of(a, lseg.b, col + 1) : -1;
+    if (SPLIT) {
+      id1 = id0;
+      if (group0 + 1 == a.page_groups) id1 = (g + 1) * 16 < lseg.length ? page_of(a, lseg.b, col + 1) : -1;
+    }
   };
-  // This lane's share of a 16-token group.  Keys are copied four (head_dim up
-  // to 64: eight) whole rows an instruction; a token's 16-byte words change
-  // places in shared memory with its lowest bit, so that reading 8 tokens' words
-  // meets every bank once.  Values are copied as they are read.
-  constexpr int ROW_WORDS = DP / 16, K_COPIES = 16 * ROW_WORDS / 32;
-  const int k_row = lane / ROW_WORDS, k_word = lane % ROW_WORDS;  // of the first copy
-  const uint32_t k_token = (uint32_t)a.k_token, v_token = (uint32_t)a.v_token;
-  const uint8_t *const key_lane = a.key + k_row * k_token + k_word * 16;
-  const uint8_t *const value_lane = a.value + 2 * c4 * v_token + n8 * L::V_WORD;
-  const uint32_t k_place = ring + (uint32_t)(k_row * DP + place_of<DP>(k_row, k_word) * 16);
-  const uint32_t v_place = ring + L::K_BYTES + lane * L::V_WORD;
-  const bool k_in_head = k_word * 16 < a.head_dim, v_in_head = n8 * L::V_WORD < a.head_dim;
-  const uint8_t *key_head = nullptr, *value_head = nullptr;  // of the load segment
-  const float *scale_head = nullptr;                         // lane 0: key scales, lane 1: value scales
-  const uint32_t scale_page = (uint32_t)(lane == 0 ? a.ks_page : a.vs_page);
   auto enter = [&]() {
-    key_head = key_lane + lseg.head * a.k_head;
-    value_head = value_lane + lseg.head * a.v_head;
-    scale_head = lane == 0 ? a.key_scale + lseg.head * a.ks_head : a.value_scale + lseg.head * a.vs_head;
+    key_head = a.key + lseg.head * a.k_head + k_row * k_token + k_word * 16;
+    value_head = a.value + lseg.head * a.v_head + k_row * v_token + k_word * 16;
+    scale_head = lane & 1 ? a.value_scale + lseg.head * a.vs_head : a.key_scale + lseg.head * a.ks_head;
     find_pages();
   };
   auto next_step = [&]() {
@@ -607,60 +631,61 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
     lstep = lseg.s0;
     if (lmore) enter();
   };
-  // the group's live tokens, its page (0 where it has none) and slot in it
+  // the live tokens of a group, its page (0 where it has none) and slot in it
   auto group_of = [&](int g, int &live, uint32_t &id, uint32_t &slot) {
     live = lseg.length - (lstep * STEP + 16 * g);
-    const int page = g == 0 ? id0 : id1;
+    const int page = SPLIT && g == 1 ? id1 : id0;
     if (page < 0) {
       if (live > 0) record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
       live = 0;
     }
     id = page < 0 ? 0 : page;
-    slot = (g == 0 ? group0 : group0 + 1 == a.page_groups ? 0 : group0 + 1) * 16;
+    slot = (g == 0 ? group0 : SPLIT && group0 + 1 == a.page_groups ? 0 : group0 + 1) * 16;
   };
-  auto load_keys = [&](int stage) {
+  auto load_keys = [&](int at) {
     if (lmore) {
+      constexpr int EIGHT = DP == 128 ? 2 : 1;  // copies for eight tokens
+      auto to = [&](int g, int i) {
+        return (EIGHT == 2 && (i & 1) ? k_odd : k_even) + at * L::SLOT + g * 16 * DP + i / EIGHT * 8 * DP;
+      };
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         int live;
         uint32_t id, slot;
         group_of(g, live, id, slot);
         const uint8_t *k = key_head + (uint64_t)id * (uint32_t)a.k_page + (uint64_t)slot * k_token;
-        const uint32_t to = k_place + stage * L::STAGE + g * 16 * DP;
         if (live >= 16 && a.head_dim == DP) {
 #pragma unroll
-          for (int i = 0; i < K_COPIES; ++i)
-            copy_async16(to + i * 512, k + i * (uint64_t)(32 / ROW_WORDS * k_token), true);
+          for (int i = 0; i < COPIES; ++i)
+            copy_async16(to(g, i), k + i * (uint64_t)(32 / ROW_WORDS * k_token), true);
         } else {  // zeros for what is not there; its address stays inside
 #pragma unroll
-          for (int i = 0; i < K_COPIES; ++i) {
-            const bool valid = k_in_head && k_row + i * (32 / ROW_WORDS) < live;
-            copy_async16(to + i * 512, valid ? k + i * (uint64_t)(32 / ROW_WORDS * k_token) : a.key, valid);
+          for (int i = 0; i < COPIES; ++i) {
+            const bool valid = k_word * 16 < a.head_dim && k_row + i * (32 / ROW_WORDS) < live;
+            copy_async16(to(g, i), valid ? k + i * (uint64_t)(32 / ROW_WORDS * k_token) : a.key, valid);
           }
         }
-        if (lane < 2)
-          copy_async4(ring + stage * L::STAGE + L::K_BYTES + L::V_BYTES + (lane * 2 + g) * 4, scale_head + (uint64_t)id * scale_page,
-                      live > 0);
+        if ((SPLIT || g == 0) && lane < 2)
+          copy_async4(ring + at * L::SLOT + L::CODES + (lane * 2 + g) * 4, scale_head + (uint64_t)id * scale_page, live > 0);
       }
     }
     copy_commit();
   };
-  auto load_values = [&](int stage) {
+  auto load_values = [&](int at) {
     if (lmore) {
+      const uint32_t to = v_place + at * L::SLOT;
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         int live;
         uint32_t id, slot;
         group_of(g, live, id, slot);
         const uint8_t *v = value_head + (uint64_t)id * (uint32_t)a.v_page + (uint64_t)slot * v_token;
-        const uint32_t to = v_place + stage * L::STAGE + g * (4 * 32 * L::V_WORD);
         const bool all = live >= 16 && a.head_dim == DP;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint8_t *src = v + (uint64_t)((uint32_t)((i & 1) + 8 * (i >> 1)) * v_token);
-          const bool valid = all || (v_in_head && 2 * c4 + (i & 1) + 8 * (i >> 1) < live);
-          if constexpr (DP == 128) copy_async16(to + i * 512, valid ? src : a.value, valid);
-          else copy_async8(to + i * 256, valid ? src : a.value, valid);
+        for (int i = 0; i < COPIES; ++i) {
+          const uint8_t *src = v + i * (uint64_t)(32 / ROW_WORDS * v_token);
+          const bool valid = all || (k_word * 16 < a.head_dim && k_row + i * (32 / ROW_WORDS) < live);
+          copy_async16(to + g * 16 * DP + i * 512, valid ? src : a.value, valid);
         }
       }
     }
@@ -668,13 +693,16 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
   };
 
   if (lmore) enter();
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < 2; ++i) {
-    load_keys(i);
-    load_values(i);
+    load_keys(2 * i);
+    load_values(2 * i + 1);
     next_step();
   }
-  int stage = 0;
+  int at = 0;  // slot of the step's keys; its values are in the next
+  // this lane's elements (V_WORD from n8 V_WORD on) of token c4
+  const uint32_t v_read =
+      ring + (uint32_t)(c4 * DP + value_place<DP>(c4, n8 * L::V_WORD / 16) * 16 + n8 * L::V_WORD % 16);
 
   // rows of sequences without keys
   for (int64_t b = (int64_t)blockIdx.x * WARPS + warp; b < a.batch; b += (int64_t)gridDim.x * WARPS) {
@@ -682,7 +710,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
     const float zero[1] = {0.f};
     for (int64_t x = lane; x < (int64_t)a.kv_heads * a.rows * a.head_dim; x += 32) {
       const int64_t r = x / a.head_dim;
-      write_row<T>(a, b, (int)(r / a.rows), (int)(r % a.rows), (int)(x % a.head_dim), zero, -INFINITY, 0.f, -INFINITY);
+      write_row(a, b, (int)(r / a.rows), (int)(r % a.rows), (int)(x % a.head_dim), zero, -INFINITY, 0.f, -INFINITY);
     }
   }
 
@@ -702,22 +730,26 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
       const int row = row0 + nt * 8 + n8;
       const bool valid = row < a.rows;
       const int i = valid ? row / a.group : 0, hq = seg.head * a.group + (valid ? row % a.group : 0);
-      const T *q = static_cast<const T *>(a.query) + seg.b * a.q_batch + i * a.q_token + hq * a.q_head;
+      const uint16_t *q = static_cast<const uint16_t *>(a.query) + seg.b * a.q_batch + i * a.q_token + hq * a.q_head;
       float x[DP / 4], top = 0.f;
       if (a.q_vector) {
 #pragma unroll
         for (int e = 0; e < DP / 4; e += 8) {
           const int d = (e / 16) * 64 + 16 * c4 + e % 16;
-          rotary::Chunk<T> chunk = {};
-          if (valid && d < a.head_dim) chunk = *reinterpret_cast<const rotary::Chunk<T> *>(q + d);
+          uint4 chunk = make_uint4(0, 0, 0, 0);
+          if (valid && d < a.head_dim) chunk = *reinterpret_cast<const uint4 *>(q + d);
+          const uint32_t w[4] = {chunk.x, chunk.y, chunk.z, chunk.w};
 #pragma unroll
-          for (int y = 0; y < 8; ++y) x[e + y] = to_f(chunk.v[y]);
+          for (int y = 0; y < 4; ++y) {
+            x[e + 2 * y] = element((uint16_t)w[y], a.bf16);
+            x[e + 2 * y + 1] = element((uint16_t)(w[y] >> 16), a.bf16);
+          }
         }
       } else {
 #pragma unroll
         for (int e = 0; e < DP / 4; ++e) {
           const int d = (e / 16) * 64 + 16 * c4 + e % 16;
-          x[e] = valid && d < a.head_dim ? to_f(q[d * a.q_dim]) : 0.f;
+          x[e] = valid && d < a.head_dim ? element(q[d * a.q_dim], a.bf16) : 0.f;
         }
       }
 #pragma unroll
@@ -754,16 +786,16 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
 
     for (int step = seg.s0; step < seg.s1; ++step) {
       copy_wait<3>();  // all but this step's values and the next step
-      __syncwarp();    // the scales were copied by two lanes
-      const uint32_t from = ring + stage * L::STAGE, from_v = from + L::K_BYTES + lane * L::V_WORD;
+      __syncwarp();    // other lanes' copies
+      const uint32_t from = ring + at * L::SLOT, from_v = v_read + (at + 1) * L::SLOT;
 
       float s[2][NT][4] = {};
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
 #pragma unroll
         for (int x = 0; x < DP / 64; ++x) {
-          const uint32_t at = from + (g * 16 + n8) * DP + place_of<DP>(n8, 4 * x + c4) * 16;
-          const uint4 k0 = load_shared16(at), k1 = load_shared16(at + 8 * DP);
+          const uint32_t word = from + (g * 16 + n8) * DP + key_place<DP>(n8, 4 * x + c4) * 16;
+          const uint4 k0 = load_shared16(word), k1 = load_shared16(word + 8 * DP);
           const uint32_t lo[4] = {k0.x, k0.y, k0.z, k0.w}, hi[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -775,9 +807,12 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
           }
         }
       }
-      const uint4 scales = load_shared16(from + L::K_BYTES + L::V_BYTES);  // two of the keys, two of the values
-      const float ks[2] = {__uint_as_float(scales.x), __uint_as_float(scales.y)};
-      const float lv[2] = {log2_fast(__uint_as_float(scales.z)), log2_fast(__uint_as_float(scales.w))};
+      // scales: two of the keys, two of the values
+      const uint4 scales = load_shared16(from + L::CODES);
+      const float ks[2] = {__uint_as_float(scales.x), __uint_as_float(SPLIT ? scales.y : scales.x)};
+      float lv[2];
+      lv[0] = log2_fast(__uint_as_float(scales.z));
+      lv[1] = SPLIT ? log2_fast(__uint_as_float(scales.w)) : lv[0];
       const int t0 = step * STEP;
       const bool masked = t0 + STEP > sure;
       // scores in base 2 are s * unit; where some are masked they are multiplied
@@ -795,7 +830,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
           for (int g = 0; g < 2; ++g)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              s[g][nt][e] = t0 + 16 * g + n8 + 8 * (e >> 1) < limit[nt][e & 1] ? s[g][nt][e] * unit[g][nt][e & 1] : -INFINITY;
+              s[g][nt][e] = t0 + 16 * g + token_of(n8) + 8 * (e >> 1) < limit[nt][e & 1] ? s[g][nt][e] * unit[g][nt][e & 1] : -INFINITY;
 #pragma unroll
           for (int g = 0; g < 2; ++g) unit[g][nt][0] = unit[g][nt][1] = 1.f;
         }
@@ -807,7 +842,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
         }
       }
       const bool move = __any_sync(0xffffffffu, passed);
-      load_keys(stage);  // every lane has read this step's keys and scales
+      load_keys(at);  // every lane has read this step's keys and scales
       if (move) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -833,7 +868,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
             }
           }
       }
-      uint32_t pf[2][NT][2];  // P^T: keys 2 c4, 2 c4 + 1 (and + 8) of row n8
+      uint32_t pf[2][NT][2];  // P^T: MMA rows 2 c4, 2 c4 + 1 (and + 8) of query row n8
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float r0 = reference(m[nt][0]), r1 = reference(m[nt][1]);
@@ -849,17 +884,18 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
           }
       }
       copy_wait<3>();  // all but the next step and the keys after it
+      __syncwarp();
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         uint32_t v[4][L::V_WORD / 4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t at = from_v + (g * 4 + i) * 32 * L::V_WORD;
+          const uint32_t word = from_v + (g * 4 + i) * 4 * DP;
           if constexpr (DP == 128) {
-            const uint4 x = load_shared16(at);
+            const uint4 x = load_shared16(word);
             v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
           } else {
-            const uint2 x = load_shared8(at);
+            const uint2 x = load_shared8(word);
             v[i][0] = x.x; v[i][1] = x.y;
           }
         }
@@ -875,9 +911,10 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
           for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][t], a0, a1, a2, a3, pf[g][nt][0], pf[g][nt][1]);
         }
       }
-      load_values(stage);
+      __syncwarp();  // every lane has read this step's values
+      load_values(at + 1);
       next_step();
-      stage ^= 1;
+      at ^= 2;
     }
 
 #pragma unroll
@@ -893,7 +930,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
         for (int u = 0; u < 2; ++u) {
           float acc[L::V_WORD];
           row_of<DP, NT>(o, nt, u, acc);
-          write_row<T>(a, seg.b, seg.head, row0 + nt * 8 + 2 * c4 + u, n8 * L::V_WORD, acc, m[nt][u], l[nt][u], mo[nt][u]);
+          write_row(a, seg.b, seg.head, row0 + nt * 8 + 2 * c4 + u, n8 * L::V_WORD, acc, m[nt][u], l[nt][u], mo[nt][u]);
         }
       continue;
     }
@@ -903,7 +940,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
       write_part<DP, NT>(a.parts + 2 * ((int64_t)blockIdx.x * WARPS + warp) * L::PART, o, m, l, mo);
     } else {  // kept for the CTA's join
       held = unit;
-      write_part<DP, NT>(reinterpret_cast<float *>(smem + warp * L::STAGES * L::STAGE), o, m, l, mo);
+      write_part<DP, NT>(reinterpret_cast<float *>(smem + warp * L::RING), o, m, l, mo);
     }
   }
 
@@ -921,8 +958,8 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
     while (last + 1 < WARPS && runs[last + 1].n > 0 && runs[last + 1].only && runs[last + 1].first == held.first) ++last;
     const int row = lane / (32 / L::ROWS);  // ROWS divides 32: lanes of a row share its elements
     float *part = a.parts + (2 * ((int64_t)blockIdx.x * WARPS + warp) + (held.only ? 0 : 1)) * L::PART;
-    const float *in = reinterpret_cast<const float *>(smem + warp * L::STAGES * L::STAGE);
-    constexpr int NEXT = L::STAGES * L::STAGE / 4, STATS = L::ROWS * DP;
+    const float *in = reinterpret_cast<const float *>(smem + warp * L::RING);
+    constexpr int NEXT = L::RING / 4, STATS = L::ROWS * DP;
     float top = -INFINITY, top_o = -INFINITY, sum = 0.f;
 #pragma unroll 1
     for (int w = 0; w <= last - warp; ++w) {
@@ -967,16 +1004,21 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
   __syncthreads();
 #pragma unroll 1
   for (int i = 0; i < 2 * WARPS; ++i)
-    if (joins[i].n > 0) join_unit<T, DP, NT>(a, joins[i], places[i]);
+    if (joins[i].n > 0) join_unit<DP, NT>(a, joins[i], places[i]);
 }
 
-template <typename T, typename C, int DP, int NT>
-int launch_tiles(Attention a, cudaStream_t stream) {
+template <typename C, int DP, int NT, bool SPLIT>
+int launch_split(Attention a, cudaStream_t stream) {
   using L = Layout<DP, NT>;
-  cudaError_t e = smem_optin<attention_kernel<T, C, DP, NT>>(L::SMEM);
+  cudaError_t e = smem_optin<attention_kernel<C, DP, NT, SPLIT>>(L::SMEM);
   if (e != cudaSuccess) return (int)e;
   a.row_tiles = (a.rows + L::ROWS - 1) / L::ROWS;
-  return launch_overlapped(attention_kernel<T, C, DP, NT>, dim3((unsigned)sm_count()), dim3(L::WARPS * 32), L::SMEM, stream, a);
+  return launch_overlapped(attention_kernel<C, DP, NT, SPLIT>, dim3((unsigned)sm_count()), dim3(L::WARPS * 32), L::SMEM, stream,
+                           a);
+}
+template <typename C, int DP, int NT>
+int launch_tiles(const Attention &a, cudaStream_t stream) {
+  return a.page_groups % 2 ? launch_split<C, DP, NT, true>(a, stream) : launch_split<C, DP, NT, false>(a, stream);
 }
 
 // Counters of a workspace: one for each warp of up to 512 SMs.
@@ -1006,8 +1048,8 @@ int launch_attention(const Attention &a, cudaStream_t stream) {
     if (a.head_dim <= 128 && small && sm_count() <= 512) {
       const bool one = a.rows <= 8;
       if (a.head_dim <= 64)
-        return one ? launch_tiles<T, C, 64, 1>(a, stream) : launch_tiles<T, C, 64, 2>(a, stream);
-      return one ? launch_tiles<T, C, 128, 1>(a, stream) : launch_tiles<T, C, 128, 2>(a, stream);
+        return one ? launch_tiles<C, 64, 1>(a, stream) : launch_tiles<C, 64, 2>(a, stream);
+      return one ? launch_tiles<C, 128, 1>(a, stream) : launch_tiles<C, 128, 2>(a, stream);
     }
   }
   const int64_t blocks = ((int64_t)a.batch * a.queries * a.heads + 3) / 4;
@@ -1070,6 +1112,7 @@ extern "C" int nt_b200_paged_attention(const NtB200PagedAttentionArgs *a, void *
   p.head_dim = (int)c.head_dim;
   p.page = (int)c.page;
   p.rows = (int)(a->queries * p.group);
+  p.bf16 = a->dtype == NT_B200_BFLOAT16;
   p.q_vector = p.q_dim == 1 && p.q_batch % 8 == 0 && p.q_token % 8 == 0 && p.q_head % 8 == 0 && rotary::aligned16(p.query);
   p.scale = (float)(a->scale * 1.4426950408889634);
   p.counters = static_cast<unsigned long long *>(a->workspace);
