@@ -162,6 +162,11 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(Attention a) {
 // ---------------------------------------------------------------- tensor cores
 constexpr int STEP = 32;
 constexpr int LEAST_STEPS = 2;  // of a CTA: fewer would be parts to join rather than work
+// A unit's start and end (its queries, its output) take a warp about two steps'
+// time, and count as that in the line where shares are long (BUSY_STEPS): a share
+// of nine short units took 113 us beside 80 of long ones.  Short shares are bound
+// by latency and are cut by what there is to read.
+constexpr int UNIT_STEPS = 2, BUSY_STEPS = 8;
 // A block table row's tokens that are looked at; a page's size.  With them the
 // block table column of a 16-token group is one multiplication: for g < 2^27
 // groups and d = page / 16 <= 2^8, floor(g ceil(2^36 / d) / 2^36) = floor(g / d).
@@ -302,23 +307,31 @@ __device__ __forceinline__ void separate_nans(uint32_t (&v)[4][DP / 32], float (
   }
 }
 
-// Where a walk along the line of steps stands: before step s of a unit of
-// sequence b (n steps a unit), `left` steps to go in the piece.
+// The cut of a line of `total` steps: `cta` steps a CTA, `warp` a warp; `extra`
+// steps of each unit stand for its start and end.  (The host has seen to it that
+// the line's steps fit 31 bits.)
+struct Cut {
+  int total, cta, warp, extra;
+};
+// Where a walk along the line stands: before step s of a unit of sequence b (n
+// steps a unit, `extra` among them), `left` steps to go in the share.
 struct Walk {
   int left, b, length, n, unit, s;
 };
-struct Segment {  // steps [s0, s1) of one unit
-  int length, b, head, tile, s0, s1, n;
+// Steps [s0, s1) of one unit; those from `real` on are extra.
+struct Segment {
+  int length, b, head, tile, s0, s1, n, real;
 };
 
 __host__ __device__ __forceinline__ int steps_of(int64_t length) { return (int)((length + STEP - 1) / STEP); }
+__device__ __forceinline__ int line_steps(int length, int extra) { return length > 0 ? steps_of(length) + extra : 0; }
 
-__device__ __forceinline__ bool next_segment(const Attention &a, Walk &w, Segment &g) {
+__device__ __forceinline__ bool next_segment(const Attention &a, int extra, Walk &w, Segment &g) {
   if (w.left <= 0) return false;
   while (w.n == 0 || w.unit >= a.kv_heads * a.row_tiles) {
     if (++w.b >= a.batch) return false;
     w.length = cached_length(a, w.b);
-    w.n = steps_of(w.length);
+    w.n = line_steps(w.length, extra);
     w.unit = w.s = 0;
   }
   g.b = w.b;
@@ -329,6 +342,7 @@ __device__ __forceinline__ bool next_segment(const Attention &a, Walk &w, Segmen
   g.s0 = w.s;
   const int take = min(w.left, w.n - w.s);
   g.s1 = g.s0 + take;
+  g.real = min(g.s1, g.n - extra);
   w.left -= take;
   w.s += take;
   if (w.s == w.n) {
@@ -339,20 +353,25 @@ __device__ __forceinline__ bool next_segment(const Attention &a, Walk &w, Segmen
 }
 
 // Steps of one unit of sequence b; 0 past the last sequence.
-__device__ __forceinline__ int unit_steps(const Attention &a, int b) {
+__device__ __forceinline__ int unit_steps(const Attention &a, int b, int extra) {
   const int64_t n = b < a.batch ? a.lengths[b] : 0;
-  return n <= 0 ? 0 : steps_of(n < a.capacity ? n : a.capacity);
+  return n <= 0 ? 0 : line_steps((int)(n < a.capacity ? n : a.capacity), extra);
 }
 
-// The cut of a line of `total` steps: `cta` steps a CTA, `warp` a warp.  (The
-// host has seen to it that the line's steps fit 31 bits.)
-struct Cut {
-  int total, cta, warp;
-};
 __device__ __forceinline__ Cut cut_line(const Attention &a, int ctas, int warps) {
-  Cut c{0, 0, 0};
-  for (int b = threadIdx.x & 31; b < a.batch; b += 32) c.total += unit_steps(a, b);
-  c.total = __reduce_add_sync(0xffffffffu, c.total) * a.kv_heads * a.row_tiles;
+  Cut c{0, 0, 0, 0};
+  int some = 0;  // sequences with keys
+  for (int b = threadIdx.x & 31; b < a.batch; b += 32) {
+    const int n = unit_steps(a, b, 0);
+    c.total += n;
+    some += n > 0;
+  }
+  const int units = a.kv_heads * a.row_tiles;
+  c.total = __reduce_add_sync(0xffffffffu, c.total) * units;
+  if (c.total / (ctas * warps) >= BUSY_STEPS) {
+    c.extra = UNIT_STEPS;
+    c.total += UNIT_STEPS * units * (int)__reduce_add_sync(0xffffffffu, some);
+  }
   c.cta = max((int)(((unsigned)c.total + ctas - 1) / ctas), LEAST_STEPS);
   c.warp = (c.cta + warps - 1) / warps;
   return c;
@@ -557,7 +576,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
     // the sequence that holds step `first`, 32 sequences at a time
     const int units = a.kv_heads * a.row_tiles;
     for (int b0 = 0;; b0 += 32) {
-      const int n = unit_steps(a, b0 + lane) * units;
+      const int n = unit_steps(a, b0 + lane, cut.extra) * units;
       int up = n;  // inclusive sum over the lanes
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -574,7 +593,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
       break;
     }
     start.length = cached_length(a, start.b);
-    start.n = steps_of(start.length);
+    start.n = line_steps(start.length, cut.extra);
     start.unit = (unsigned)first / (unsigned)start.n;
     start.s = first - start.unit * start.n;
   }
@@ -584,8 +603,8 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
   // two steps on, as soon as it has been read.
   Walk ahead = start;
   Segment lseg{};
-  bool lmore = next_segment(a, ahead, lseg);
-  int lstep = lseg.s0;     // the step to load
+  bool lmore = true;
+  int lstep = 0;           // the step to load
   int id0 = -1, id1 = -1;  // pages of its two 16-token groups
   int group0 = 0;          // the first group's place in its page
   // This lane's share of a 16-token group: whole rows, neighbouring words by
@@ -615,7 +634,12 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
       if (group0 + 1 == a.page_groups) id1 = (g + 1) * 16 < lseg.length ? page_of(a, lseg.b, col + 1) : -1;
     }
   };
-  auto enter = [&]() {
+  auto enter = [&]() {  // the next segment with something to load
+    do {
+      lmore = next_segment(a, cut.extra, ahead, lseg);
+      if (!lmore) return;
+      lstep = lseg.s0;
+    } while (lstep >= lseg.real);
     key_head = a.key + lseg.head * a.k_head + k_row * k_token + k_word * 16;
     value_head = a.value + lseg.head * a.v_head + k_row * v_token + k_word * 16;
     scale_head = lane & 1 ? a.value_scale + lseg.head * a.vs_head : a.key_scale + lseg.head * a.ks_head;
@@ -623,13 +647,8 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
   };
   auto next_step = [&]() {
     if (!lmore) return;
-    if (++lstep < lseg.s1) {
-      find_pages();
-      return;
-    }
-    lmore = next_segment(a, ahead, lseg);
-    lstep = lseg.s0;
-    if (lmore) enter();
+    if (++lstep < lseg.real) find_pages();
+    else enter();
   };
   // the live tokens of a group, its page (0 where it has none) and slot in it
   auto group_of = [&](int g, int &live, uint32_t &id, uint32_t &slot) {
@@ -692,7 +711,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
     copy_commit();
   };
 
-  if (lmore) enter();
+  enter();
 #pragma unroll 1
   for (int i = 0; i < 2; ++i) {
     load_keys(2 * i);
@@ -717,7 +736,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
   Walk here = start;
   Segment seg;
   Shared before{}, held{};  // parts of the unit from the share before, and of the last
-  while (next_segment(a, here, seg)) {
+  while (next_segment(a, cut.extra, here, seg)) {
     const int row0 = seg.tile * L::ROWS;
 
     // Q: lane (n8, c4) holds row n8's elements 16 c4 .. + 15 of each 64, as
@@ -784,7 +803,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
     const int sure = seg.length - a.queries + 1 + row0 / a.group;  // keys that every row sees
     float o[NT][OT][4] = {};
 
-    for (int step = seg.s0; step < seg.s1; ++step) {
+    for (int step = seg.s0; step < seg.real; ++step) {
       copy_wait<3>();  // all but this step's values and the next step
       __syncwarp();    // other lanes' copies
       const uint32_t from = ring + at * L::SLOT, from_v = v_read + (at + 1) * L::SLOT;
@@ -1044,7 +1063,7 @@ int launch_attention(const Attention &a, cudaStream_t stream) {
       small = small && x >= 0 && x < (1LL << 32);
     small = small && a.k_token * a.page < (1LL << 32) && a.v_token * a.page < (1LL << 32);
     // and a line of steps that 31 bits count
-    small = small && (double)a.batch * a.kv_heads * ((a.rows + 7) / 8) * (a.capacity / STEP + 1) < 2e9;
+    small = small && (double)a.batch * a.kv_heads * ((a.rows + 7) / 8) * (a.capacity / STEP + 1 + UNIT_STEPS) < 2e9;
     if (a.head_dim <= 128 && small && sm_count() <= 512) {
       const bool one = a.rows <= 8;
       if (a.head_dim <= 64)
