@@ -103,7 +103,7 @@ struct Params {
   int64_t tokens, batch, pages, table_columns;
   int64_t units;  // candidates a head and side: tokens / page + 2 * batch
   int page, kv_heads, head_dim, chunk_pairs;
-  int unit_blocks;  // blockIdx.x below this: units; the rest: queries
+  uint32_t unit_blocks;  // blockIdx.x below this: a unit, head and side each; the rest: queries
   int interleaved;
 };
 
@@ -220,20 +220,21 @@ __device__ __forceinline__ void rotate_queries(const Params &p, int64_t block) {
   }
 }
 
-// One unit a block: blockIdx.x the candidate, blockIdx.y the head and side.
+// One unit, head and side a block, heads and sides innermost.
 template <typename T, typename C>
 __global__ void __launch_bounds__(THREADS) append_kernel(Params p) {
   __shared__ float shared[THREADS / 32];
-  if ((int)blockIdx.x >= p.unit_blocks) {
-    if (blockIdx.y == 0) rotate_queries<T, true>(p, (int64_t)blockIdx.x - p.unit_blocks);
+  if (blockIdx.x >= p.unit_blocks) {
+    rotate_queries<T, true>(p, blockIdx.x - p.unit_blocks);
     return;
   }
+  const uint32_t which = blockIdx.x % (uint32_t)(2 * p.kv_heads);  // head and side
   constexpr int N = rotary::Chunk<T>::N;
   Unit w;
-  if (!find_unit(p, blockIdx.x, w)) return;
-  const int h = (int)blockIdx.y >> 1;
-  const Side &side = p.side[blockIdx.y & 1];
-  const bool turns = p.tables.pairs > 0 && (blockIdx.y & 1) == 0;
+  if (!find_unit(p, blockIdx.x / (uint32_t)(2 * p.kv_heads), w)) return;
+  const int h = (int)which >> 1;
+  const Side &side = p.side[which & 1];
+  const bool turns = p.tables.pairs > 0 && (which & 1) == 0;
   const int items = w.count * p.chunk_pairs;
   const float held = side.scales[w.block * side.scale_page + (int64_t)h * side.scale_head];
   const T *in = static_cast<const T *>(side.in) + (int64_t)h * side.in_head;
@@ -289,15 +290,16 @@ __global__ void __launch_bounds__(THREADS) append_kernel(Params p) {
 template <typename T, typename C>
 __global__ void __launch_bounds__(THREADS) append_scalar_kernel(Params p) {
   __shared__ float shared[THREADS / 32];
-  if ((int)blockIdx.x >= p.unit_blocks) {
-    if (blockIdx.y == 0) rotate_queries<T, false>(p, (int64_t)blockIdx.x - p.unit_blocks);
+  if (blockIdx.x >= p.unit_blocks) {
+    rotate_queries<T, false>(p, blockIdx.x - p.unit_blocks);
     return;
   }
+  const uint32_t which = blockIdx.x % (uint32_t)(2 * p.kv_heads);  // head and side
   Unit w;
-  if (!find_unit(p, blockIdx.x, w)) return;
-  const int h = (int)blockIdx.y >> 1;
-  const Side &side = p.side[blockIdx.y & 1];
-  const int pairs = (blockIdx.y & 1) == 0 ? p.tables.pairs : 0;
+  if (!find_unit(p, blockIdx.x / (uint32_t)(2 * p.kv_heads), w)) return;
+  const int h = (int)which >> 1;
+  const Side &side = p.side[which & 1];
+  const int pairs = (which & 1) == 0 ? p.tables.pairs : 0;
   const int per_token = p.head_dim - pairs;  // pairs, then single elements
   const int items = w.count * per_token;
   const float held = side.scales[w.block * side.scale_page + (int64_t)h * side.scale_head];
@@ -366,10 +368,10 @@ int launch_append(Params p, cudaStream_t stream) {
   p.chunk_pairs = q.chunk_pairs = (p.head_dim + 2 * N - 1) / (2 * N);
   q.head_groups = (q.heads + rotary::HEADS - 1) / rotary::HEADS;
   const int64_t threads = q.input ? p.tokens * (vec ? (int64_t)q.chunk_pairs * q.head_groups : (int64_t)q.heads) : 0;
-  const int64_t blocks = p.units + (threads + THREADS - 1) / THREADS;
-  if (blocks > (1LL << 31) - 1 || p.kv_heads > 32767) return NT_B200_ERR_INVALID_ARGUMENT;
-  p.unit_blocks = (int)p.units;
-  const dim3 grid((unsigned)blocks, (unsigned)(p.kv_heads > 0 ? 2 * p.kv_heads : 1));
+  const int64_t units = p.units * 2 * p.kv_heads, blocks = units + (threads + THREADS - 1) / THREADS;
+  if (blocks > (1LL << 31) - 1) return NT_B200_ERR_INVALID_ARGUMENT;
+  p.unit_blocks = (uint32_t)units;
+  const dim3 grid((unsigned)blocks);
   if (vec) append_kernel<T, C><<<grid, THREADS, 0, stream>>>(p);
   else append_scalar_kernel<T, C><<<grid, THREADS, 0, stream>>>(p);
   return launch_status();
