@@ -42,6 +42,27 @@ template <typename T> struct alignas(16) Chunk {
   T v[N];
 };
 
+// Elements of a chunk from fp32 values, two a conversion.
+template <typename T> __device__ __forceinline__ Chunk<T> to_chunk(const float (&x)[Chunk<T>::N]) {
+  Chunk<T> c;
+#pragma unroll
+  for (int i = 0; i < Chunk<T>::N; i += 2) {
+    if constexpr (sizeof(T) == 4) {
+      c.v[i] = x[i];
+      c.v[i + 1] = x[i + 1];
+    } else if constexpr (Elem<T>::is_f16) {
+      const __half2 h = __floats2half2_rn(x[i], x[i + 1]);
+      c.v[i] = h.x;
+      c.v[i + 1] = h.y;
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[i], x[i + 1]);
+      c.v[i] = h.x;
+      c.v[i + 1] = h.y;
+    }
+  }
+  return c;
+}
+
 struct Tables {
   const float *cos, *sin;
   int64_t cos_stride, sin_stride, rows;
@@ -124,26 +145,34 @@ struct Params {
 };
 
 // A thread takes one chunk pair of HEADS heads of a token, so a table entry is
-// read once for all of them and 2 HEADS 16-byte loads are in flight.
-constexpr int HEADS = 4, THREADS = 128;
+// read once for all of them and 2 HEADS 16-byte loads are in flight.  Two heads
+// (64 registers, 32 warps an SM) take ROT_US for 16384 tokens of 40 heads of 128
+// bfloat16 elements, four (96 registers, 20 warps) 82 us, one 76 us.
+constexpr int HEADS = 2, THREADS = 128;
 
-template <typename T>
-__device__ __forceinline__ void rotate_heads(const Params &p, int64_t token, int64_t position, int h0, int cpair) {
+// Rotates chunk pair `cpair` of the heads h0 .. h0 + HEADS - 1 of a token.
+// `position_of` gives its position (or says with a value below kNone that the
+// token is not to be written) and is asked only after the loads: a wait for it
+// before them would put its latency in front of theirs.
+constexpr int64_t kNone = INT64_MIN / 2;
+template <typename T, typename F>
+__device__ __forceinline__ void rotate_heads(const Params &p, int64_t token, bool valid, int h0, int cpair, F position_of) {
   constexpr int N = Chunk<T>::N;
   const Place<T> at = place<T>(cpair, p.head_dim, p.tables.pairs, p.interleaved != 0);
-  const bool known = position >= 0 && position < p.tables.rows;
-  if (!known) record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
   const T *in = static_cast<const T *>(p.input) + token * p.in_token;
-  T *out = static_cast<T *>(p.output) + token * p.out_token;
   Chunk<T> a[HEADS] = {}, b[HEADS] = {};
 #pragma unroll
   for (int i = 0; i < HEADS; ++i) {
-    if (h0 + i >= p.heads) break;
+    if (!valid || h0 + i >= p.heads) break;
     const T *row = in + (int64_t)(h0 + i) * p.in_head;
     a[i] = *reinterpret_cast<const Chunk<T> *>(row + at.first);
     if (at.second >= 0) b[i] = *reinterpret_cast<const Chunk<T> *>(row + at.second);
   }
+  const int64_t position = position_of();
+  if (!valid || position < kNone) return;
   if (at.pair >= 0) {
+    const bool known = position >= 0 && position < p.tables.rows;
+    if (!known) record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
     float c[N], s[N];
     if (known) {
       load_angles<T>(p.tables, position, at.pair, c, s);
@@ -157,10 +186,11 @@ __device__ __forceinline__ void rotate_heads(const Params &p, int64_t token, int
 #pragma unroll
       for (int j = 0; j < N; ++j) { x[j] = to_f(a[i].v[j]); y[j] = to_f(b[i].v[j]); }
       turn_chunks<N>(x, y, c, s, p.interleaved != 0, p.tables.pairs - at.pair);
-#pragma unroll
-      for (int j = 0; j < N; ++j) { a[i].v[j] = from_f<T>(x[j]); b[i].v[j] = from_f<T>(y[j]); }
+      a[i] = to_chunk<T>(x);
+      b[i] = to_chunk<T>(y);
     }
   }
+  T *out = static_cast<T *>(p.output) + token * p.out_token;
 #pragma unroll
   for (int i = 0; i < HEADS; ++i) {
     if (h0 + i >= p.heads) break;
@@ -176,7 +206,7 @@ __global__ void __launch_bounds__(THREADS) chunk_kernel(Params p, uint32_t total
   if (i >= total) return;
   const uint32_t c = i % (uint32_t)p.chunk_pairs, r = i / (uint32_t)p.chunk_pairs;
   const uint32_t g = r % (uint32_t)p.head_groups, token = r / (uint32_t)p.head_groups;
-  rotate_heads<T>(p, token, p.positions[token], (int)g * HEADS, (int)c);
+  rotate_heads<T>(p, token, true, (int)g * HEADS, (int)c, [&] { return p.positions[token]; });
 }
 
 // Any strides, any head and rotary extents: a thread per pair or copied element.
