@@ -18,17 +18,17 @@
 //               ring of 5 shared-memory slots that runs on across items;
 //   warp 1      tensor memory, and the MMAs from one thread: S_t = Q_t K_j^T,
 //               O_t += P_t V_j with P_t read from tensor memory;
-//   warps 2-17  softmax, 8 warps a tile, two threads a row with 64 of a block's
-//               128 keys each.  A row's maximum goes between its two threads
-//               through shared memory and a barrier of their two warps.
-// The two halves of a row are what makes the tile's round trip short: the next
-// Q K^T of a tile waits for its P (S and P share tensor memory, 512 columns
-// hold S and O of two tiles and nothing else), so a block takes one softmax and
-// two MMAs in a row, and half the softmax is off that path this way.
+//   warps 2-9   softmax, 4 warps a tile, a thread a row.
+// (Eight warps a tile, two threads a row of 64 keys each with their maxima
+// exchanged through shared memory, took 1160 us where this takes NONCAUSAL_US for
+// four sequences of 4096 tokens, 32 heads of 128, not causal: at 96 registers a
+// thread they spill.)
 //
-// The order of items comes from a small kernel before (plan_kernel): longest
-// first over all sequences, dealt out to the CTAs in rounds of alternating
-// direction.
+// The order of items comes from a small kernel before (plan_kernel): sequences
+// longest first, all tiles of a key/value head together, so that its keys and
+// values stay in L2 while they are used, later queries first.  CTAs take the
+// next item when they are done with one (a counter; warp 0 fetches it an item
+// ahead and hands it to the other warps through shared memory).
 #pragma once
 
 #include <cuda.h>
@@ -125,16 +125,18 @@ __global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ Probl
 // ---------------------------------------------------------------- plan
 constexpr int BM = 128, BN = 128;  // rows of a tile, keys of a block
 
-// Two tiles of queries of one sequence.
+// Two tiles of queries of one sequence: entry `first` + i of `total` that the
+// sequence has, latest queries first.
 struct alignas(32) Entry {
   int32_t q0, queries;  // first packed query, how many (at most two tiles')
   int32_t k0, keys;     // first packed key, how many the sequence has
   int32_t limit0;       // keys that the first query sees (causal), else `keys`
-  int32_t pad[3];
+  int32_t first, total;
+  int32_t head;         // of an item; unused in the list
 };
+// The workspace: Plan, the entries, then an int32 for each sequence.
 struct Plan {
-  int32_t count, pad[7];
-  // Entry[...] follows
+  int32_t count, next, pad[6];  // entries; the next item
 };
 
 // Key blocks of the tile whose queries are [t * per_tile, ..) of an entry: up
@@ -152,28 +154,9 @@ constexpr int PLAN_THREADS = 1024, BINS = 1024;
 
 // The candidate entries: sequence b owns the candidates from query_offsets[b] /
 // pair + b on (pair = queries of two tiles), as many as it can have entries;
-// those past its last are empty.
-__device__ __forceinline__ bool candidate(const Problem &p, int64_t c, int pair, Entry &e) {
-  int64_t low = 0, high = p.batch;  // the largest b whose first candidate is <= c
-  while (high - low > 1) {
-    const int64_t mid = (low + high) / 2;
-    if (p.q_offsets[mid] / pair + mid <= c) low = mid;
-    else high = mid;
-  }
-  int64_t q0, nq, k0, nk;
-  if (!extents(p, low, q0, nq, k0, nk)) return false;
-  const int64_t first = (c - (q0 / pair + low)) * pair;
-  if (first < 0 || first >= nq) return false;
-  e.q0 = (int32_t)(q0 + first);
-  e.queries = (int32_t)(nq - first < pair ? nq - first : pair);
-  e.k0 = (int32_t)k0;
-  e.keys = (int32_t)nk;
-  e.limit0 = (int32_t)(p.causal ? nk - nq + 1 + first : nk);
-  return true;
-}
-
-// Counting sort of the entries by their key blocks, most first (blocks beyond
-// the bins share the first bin: the order is for balance only).
+// those past its last are empty.  Counting sort of the sequences by the key
+// blocks of their last queries, most first (beyond the bins in the first one:
+// the order is for balance only), then the entries at their sequence's place.
 __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const __grid_constant__ Problem p, int64_t candidates,
                                                             int per_tile) {
   __shared__ int bins[BINS];
@@ -181,44 +164,70 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const __grid_constan
   static_assert(BINS == PLAN_THREADS, "a thread scans one bin");
   wait_prior_grid();
   allow_dependent_launch();
+  const int pair = 2 * per_tile;
+  Plan *plan = static_cast<Plan *>(p.workspace);
+  Entry *list = reinterpret_cast<Entry *>(plan + 1);
+  int32_t *first_of = reinterpret_cast<int32_t *>(list + candidates);  // a sequence's first entry; -1: none
   bins[threadIdx.x] = 0;
   __syncthreads();
-  auto bin_of = [&](const Entry &e) {
-    const int n0 = blocks_of(e, 0, per_tile, p.causal), n1 = blocks_of(e, 1, per_tile, p.causal);
-    const int n = n0 + n1;
-    return n >= BINS ? 0 : BINS - 1 - n;
-  };
-  for (int64_t c = threadIdx.x; c < candidates; c += PLAN_THREADS) {
-    Entry e;
-    if (candidate(p, c, 2 * per_tile, e)) atomicAdd(&bins[bin_of(e)], 1);
-  }
-  __syncthreads();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n = bins[threadIdx.x];
-  int up = n;
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int64_t b = threadIdx.x; b < p.batch; b += PLAN_THREADS) {
+      int64_t q0, nq, k0, nk;
+      if (!extents(p, b, q0, nq, k0, nk)) nq = 0;
+      const int total = (int)((nq + pair - 1) / pair);
+      const int64_t blocks = (nk + BN - 1) / BN;
+      int *bin = &bins[blocks >= BINS ? 0 : BINS - 1 - (int)blocks];
+      if (total == 0) first_of[b] = -1;
+      else if (pass == 0) atomicAdd(bin, total);
+      else first_of[b] = atomicAdd(bin, total);
+    }
+    __syncthreads();
+    if (pass == 1) break;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int n = bins[threadIdx.x];
+    int up = n;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, up, o);
-    if (lane >= o) up += x;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += x;
+    }
+    if (lane == 31) warp_sums[warp] = up;
+    __syncthreads();
+    int base = 0;
+    for (int i = 0; i < warp; ++i) base += warp_sums[i];
+    bins[threadIdx.x] = base + up - n;
+    if (threadIdx.x == PLAN_THREADS - 1) {
+      plan->count = base + up;
+      plan->next = 0;
+    }
+    __syncthreads();
   }
-  if (lane == 31) warp_sums[warp] = up;
-  __syncthreads();
-  int base = 0;
-  for (int i = 0; i < warp; ++i) base += warp_sums[i];
-  bins[threadIdx.x] = base + up - n;
-  Plan *plan = static_cast<Plan *>(p.workspace);
-  if (threadIdx.x == PLAN_THREADS - 1) plan->count = base + up;
-  __syncthreads();
-  Entry *list = reinterpret_cast<Entry *>(plan + 1);
   for (int64_t c = threadIdx.x; c < candidates; c += PLAN_THREADS) {
+    int64_t low = 0, high = p.batch;  // the largest b whose first candidate is <= c
+    while (high - low > 1) {
+      const int64_t mid = (low + high) / 2;
+      if (p.q_offsets[mid] / pair + mid <= c) low = mid;
+      else high = mid;
+    }
+    int64_t q0, nq, k0, nk;
+    if (first_of[low] < 0 || !extents(p, low, q0, nq, k0, nk)) continue;
+    const int64_t i = c - (q0 / pair + low), first = i * pair;
+    if (i < 0 || first >= nq) continue;
     Entry e{};
-    if (candidate(p, c, 2 * per_tile, e)) list[atomicAdd(&bins[bin_of(e)], 1)] = e;
+    e.q0 = (int32_t)(q0 + first);
+    e.queries = (int32_t)(nq - first < pair ? nq - first : pair);
+    e.k0 = (int32_t)k0;
+    e.keys = (int32_t)nk;
+    e.limit0 = (int32_t)(p.causal ? nk - nq + 1 + first : nk);
+    e.first = first_of[low];
+    e.total = (int32_t)((nq + pair - 1) / pair);
+    list[e.first + e.total - 1 - (int)i] = e;
   }
 }
 
 // ---------------------------------------------------------------- tensor cores
 constexpr int TILES = 2, RING = 5;
-constexpr int SOFTMAX_WARPS = 16;
+constexpr int SOFTMAX_WARPS = 8;
 constexpr int THREADS = (2 + SOFTMAX_WARPS) * 32;
 constexpr int TMEM_COLS = 512;
 
@@ -228,10 +237,9 @@ struct Layout {
   static constexpr int Q_BYTES = BM * DP * 2;   // one Q tile
   static constexpr int KV_BYTES = BN * DP * 2;  // one key or value block
   static constexpr int RING_OFF = TILES * Q_BYTES;
-  static constexpr int SHARE_OFF = RING_OFF + RING * KV_BYTES;  // float [TILES][2][BM]
-  static constexpr int CTRL_OFF = SHARE_OFF + TILES * 2 * BM * 4;
-  static constexpr int SMEM_BYTES = CTRL_OFF + 256;
-  static_assert(96 + 16 * RING + 32 * TILES <= 240, "barrier slots");
+  static constexpr int CTRL_OFF = RING_OFF + RING * KV_BYTES;
+  static constexpr int SMEM_BYTES = CTRL_OFF + 384;
+  static_assert(96 + 16 * RING <= 240, "barrier slots");
   static_assert(SMEM_BYTES <= 232448, "shared memory of a CTA");
 };
 
@@ -240,15 +248,15 @@ struct Params {
   int per_tile;  // queries of a tile
 };
 
-// A row's elements [d0, d0 + 64) again, key by key on the CUDA cores, from its
-// final maximum.  An infinity or NaN in the value of a key that the row does
-// not see makes the row's MMA sums NaN (0 * inf): such rows come here.
+// A row again, key by key on the CUDA cores, from its final maximum.  An
+// infinity or NaN in the value of a key that the row does not see makes the
+// row's MMA sums NaN (0 * inf): such rows come here.
 template <typename T>
-__device__ __noinline__ void row_again(const Problem &p, int k0, int64_t token, int head, int limit, int d0, int dims,
-                                       float m, float f, T *out) {
+__device__ __noinline__ void row_again(const Problem &p, int k0, int64_t token, int head, int limit, float m, float f,
+                                       T *out) {
   const T *q = static_cast<const T *>(p.q) + token * p.q_token + head * p.q_head;
   const int g = head / p.group;
-  for (int c = 0; c < dims; c += 16) {
+  for (int c = 0; c < p.head_dim; c += 16) {
     float acc[16] = {};
     for (int t = 0; t < limit; ++t) {
       const T *k = static_cast<const T *>(p.k) + (int64_t)(k0 + t) * p.k_token + g * p.k_head;
@@ -258,11 +266,11 @@ __device__ __noinline__ void row_again(const Problem &p, int k0, int64_t token, 
       const float w = exp2f(dot * p.scale - m);
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (c + i < dims) acc[i] = fmaf(w, to_f(v[d0 + c + i]), acc[i]);
+        if (c + i < p.head_dim) acc[i] = fmaf(w, to_f(v[c + i]), acc[i]);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (c + i < dims) out[(d0 + c + i) * p.o_dim] = from_f<T>(acc[i] * f);
+      if (c + i < p.head_dim) out[(c + i) * p.o_dim] = from_f<T>(acc[i] * f);
   }
 }
 
@@ -287,25 +295,29 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
   auto o_free = [&](int t) { return ctrl + 80 + 8u * t; };   // O_t read out
   auto slot_full = [&](int s) { return ctrl + 96 + 8u * s; };
   auto slot_empty = [&](int s) { return ctrl + 96 + 8u * RING + 8u * s; };
-  auto shared_row = [&](int t, int quarter) { return ctrl + 96 + 16u * RING + 8u * (4 * t + quarter); };
+  // items, two in turn: handed over, taken by the MMA issuer and the softmax warps
+  auto item_full = [&](int s) { return ctrl + 248 + 8u * s; };
+  auto item_empty = [&](int s) { return ctrl + 264 + 8u * s; };
+  volatile int4 *item_slots = reinterpret_cast<volatile int4 *>(smem + L::CTRL_OFF + 288);
   volatile uint32_t *tmem_base_ptr = reinterpret_cast<volatile uint32_t *>(smem + L::CTRL_OFF + 240);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::CTRL_OFF + 244);
 
   const Problem &p = prm.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per_tile = prm.per_tile;
-  const Plan *plan = static_cast<const Plan *>(p.workspace);
-  const Entry *list = reinterpret_cast<const Entry *>(plan + 1);
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < TILES; ++t) {
       ptx::mbar_init(q_full(t), 1);
       ptx::mbar_init(q_free(t), 1);
       ptx::mbar_init(s_full(t), 1);
-      ptx::mbar_init(p_full(t), 256);
+      ptx::mbar_init(p_full(t), 4);  // a warp's lanes arrive as one
       ptx::mbar_init(o_done(t), 1);
-      ptx::mbar_init(o_free(t), 256);
-      for (int w = 0; w < 4; ++w) ptx::mbar_init(shared_row(t, w), 2);  // the two warps of 32 rows
+      ptx::mbar_init(o_free(t), 4);
+    }
+    for (int s = 0; s < 2; ++s) {
+      ptx::mbar_init(item_full(s), 1);
+      ptx::mbar_init(item_empty(s), 1 + SOFTMAX_WARPS);
     }
     for (int s = 0; s < RING; ++s) {
       ptx::mbar_init(slot_full(s), 1);
@@ -335,13 +347,14 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
   auto tmem_s = [&](int t) { return tmem_base + (uint32_t)(t * BN); };
   auto tmem_o = [&](int t) { return tmem_base + (uint32_t)(TILES * BN + t * 128); };
 
-  // Items k = entry * kv_heads + head; the CTA's i-th: the i-th round of
-  // gridDim.x items, in alternating direction.
-  const int64_t num_items = (int64_t)plan->count * p.kv_heads;
-  auto nth_item = [&](int i) -> int64_t {
-    const int64_t g = gridDim.x, c = blockIdx.x;
-    const int64_t k = i * g + ((i & 1) ? g - 1 - c : c);
-    return k < num_items ? k : -1;
+  // The CTA's i-th item (queries 0: no more), once it was handed over; false
+  // where the wait gave up.  The caller then lets go of it.
+  auto take_item = [&](int i, Entry &e) {
+    if (!ptx::mbar_wait(item_full(i & 1), (uint32_t)(i >> 1) & 1u, abort_flag)) return false;
+    const volatile int4 *at = item_slots + 2 * (i & 1);
+    e.q0 = at[0].x; e.queries = at[0].y; e.k0 = at[0].z; e.keys = at[0].w;
+    e.limit0 = at[1].x; e.head = at[1].w;
+    return true;
   };
 
   if (warp == 0) {
@@ -351,11 +364,32 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       int r = 0;             // ring items so far
       int used[TILES] = {};  // items so far that had tile t
       const uint32_t q_bytes = (uint32_t)(per_tile * p.group * 128 * L::ATOMS);
+      // Items count sequence by sequence (all entries of one together), in it
+      // head by head, in it entry by entry.
+      Plan *plan = static_cast<Plan *>(p.workspace);
+      const Entry *list = reinterpret_cast<const Entry *>(plan + 1);
+      const int64_t num_items = (int64_t)plan->count * p.kv_heads;
+      auto next_item = [&]() {
+        const int64_t k = atomicAdd(&plan->next, 1);
+        Entry e{};
+        if (k >= num_items) return e;
+        const Entry any = list[k / p.kv_heads];  // of the same sequence
+        const int r = (int)(k - (int64_t)any.first * p.kv_heads), h = r / any.total;
+        e = list[any.first + r - h * any.total];
+        e.head = h;
+        return e;
+      };
+      Entry ahead = next_item();
       for (int i = 0; ok; ++i) {
-        const int64_t item = nth_item(i);
-        if (item < 0) break;
-        const Entry e = list[item / p.kv_heads];
-        const int h = (int)(item % p.kv_heads);
+        const Entry e = ahead;
+        if (!ptx::mbar_wait(item_empty(i & 1), ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag)) break;
+        volatile int4 *to = item_slots + 2 * (i & 1);
+        to[0].x = e.q0; to[0].y = e.queries; to[0].z = e.k0; to[0].w = e.keys;
+        to[1].x = e.limit0; to[1].w = e.head;
+        ptx::mbar_arrive(item_full(i & 1));
+        if (e.queries == 0) break;
+        ahead = next_item();
+        const int h = e.head;
         const int n[TILES] = {blocks_of(e, 0, per_tile, p.causal), blocks_of(e, 1, per_tile, p.causal)};
         const int n_max = max(n[0], n[1]);
         for (int t = 0; t < TILES && ok; ++t) {
@@ -408,9 +442,9 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       int blk[TILES] = {};   // key blocks of tile t in earlier items
       int used[TILES] = {};  // earlier items that had tile t
       for (int i = 0; ok; ++i) {
-        const int64_t item = nth_item(i);
-        if (item < 0) break;
-        const Entry e = list[item / p.kv_heads];
+        Entry e;
+        if (!take_item(i, e) || e.queries == 0) break;
+        ptx::mbar_arrive(item_empty(i & 1));
         const int n[TILES] = {blocks_of(e, 0, per_tile, p.causal), blocks_of(e, 1, per_tile, p.causal)};
         const int n_max = max(n[0], n[1]);
         ok = wait_slot(r);  // K_0
@@ -461,33 +495,21 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
     }
   } else {
     // ------------------------------------------------------------ softmax, rescaling, output
-    const int t = (warp - 2) / 8, half = (warp - 2) / 4 % 2, quarter = warp & 3;
+    const int t = (warp - 2) / 4, quarter = warp & 3;
     const int row = quarter * 32 + lane;  // row of the tile = lane of tensor memory
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const int query_of_row = row / p.group, head_of_row = row % p.group;
-    float *share = reinterpret_cast<float *>(smem + L::SHARE_OFF) + t * 2 * BM + row;
     bool ok = true;
-    // a value for the row's other thread; the caller sees to it that the last
-    // one was read
-    uint32_t turn = 0;
-    auto meet = [&]() {  // the two warps of 32 rows
+    auto arrive_warp = [&](uint32_t bar) {
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(shared_row(t, quarter));
-      ok = ptx::mbar_wait_warp(shared_row(t, quarter), turn, abort_flag);
-      turn ^= 1;
-    };
-    auto exchange = [&](float mine) {
-      share[half * BM] = mine;
-      meet();
-      return share[(half ^ 1) * BM];
+      if (lane == 0) ptx::mbar_arrive(bar);
     };
     const float c = p.scale;
-    constexpr int HALF_D = DP / 2;
     int blk = 0, used = 0;
     for (int i = 0; ok; ++i) {
-      const int64_t item = nth_item(i);
-      if (item < 0) break;
-      const Entry e = list[item / p.kv_heads];
+      Entry e;
+      if (!__all_sync(0xffffffffu, take_item(i, e)) || e.queries == 0) break;
+      arrive_warp(item_empty(i & 1));
       const int n_t = blocks_of(e, t, per_tile, p.causal);
       if (n_t == 0) continue;
       const int query = t * per_tile + query_of_row;
@@ -499,62 +521,69 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       for (int j = 0; j < n_t; ++j) {
         if (!ptx::mbar_wait_warp(s_full(t), (uint32_t)(blk + j) & 1u, abort_flag)) { ok = false; break; }
         ptx::tc_fence_after();
-        uint32_t sr[64];
+        uint32_t sr[BN];
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-          ptx::tmem_ld_32x32b_x32(tmem_s(t) + lane_base + (uint32_t)(half * 64 + x * 32),
-                                  *reinterpret_cast<uint32_t(*)[32]>(&sr[x * 32]));
+        for (int x = 0; x < BN / 32; ++x)
+          ptx::tmem_ld_32x32b_x32(tmem_s(t) + lane_base + (uint32_t)(x * 32), *reinterpret_cast<uint32_t(*)[32]>(&sr[x * 32]));
         ptx::tmem_ld_wait();
         float *s = reinterpret_cast<float *>(sr);
         if ((j + 1) * BN > sure) {
-          const int seen = limit - j * BN - half * 64;
+          const int seen = limit - j * BN;
 #pragma unroll
-          for (int x = 0; x < 64; ++x) s[x] = x < seen ? s[x] : -INFINITY;
+          for (int x = 0; x < BN; ++x) s[x] = x < seen ? s[x] : -INFINITY;
         }
-        float top[4];
+        float top[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) top[u] = s[u];
+        for (int u = 0; u < 8; ++u) top[u] = s[u];
 #pragma unroll
-        for (int x = 4; x < 64; ++x) top[x & 3] = fmaxf(top[x & 3], s[x]);
-        float block_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-        // (the last block's maximum was read before its P was reported written,
-        // and this S waited for that)
-        block_top = fmaxf(block_top, exchange(block_top));
-        if (!ok) break;
+        for (int x = 8; x < BN; ++x) top[x & 7] = fmaxf(top[x & 7], s[x]);
+#pragma unroll
+        for (int u = 4; u > 0; u >>= 1)
+#pragma unroll
+          for (int v = 0; v < u; ++v) top[v] = fmaxf(top[v], top[v + u]);
+        const float block_top = top[0] * c;
         // the maximum moves only when a block passes it by 2^14 (bf16: 2^24):
         // P stays in its type's range and O is rescaled rarely
         const bool move = block_top > m + tc::attn::RescaleLog2<T>::value;
         const float m_new = move ? block_top : m;
         const float alpha = move ? exp2_fast(m - m_new) : 1.f;
         const float ref = reference(m_new);
-        float sum[4] = {};
-        uint32_t packed[32];
+        float sum[8] = {};
 #pragma unroll
-        for (int x = 0; x < 32; ++x) {
-          const float p0 = exp2_fast(fmaf(s[2 * x], c, -ref)), p1 = exp2_fast(fmaf(s[2 * x + 1], c, -ref));
-          sum[(2 * x) & 3] += p0;
-          sum[(2 * x + 1) & 3] += p1;
-          packed[x] = tc::attn::pack2<T>(p0, p1);
+        for (int half = 0; half < 2; ++half) {
+          uint32_t packed[32];
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            const int k = half * 64 + 2 * x;
+            const float p0 = exp2_fast(fmaf(s[k], c, -ref)), p1 = exp2_fast(fmaf(s[k + 1], c, -ref));
+            sum[(2 * x) & 7] += p0;
+            sum[(2 * x + 1) & 7] += p1;
+            packed[x] = tc::attn::pack2<T>(p0, p1);
+          }
+          ptx::tmem_st_32x32b_x32(tmem_s(t) + lane_base + (uint32_t)(half * 32), packed);
         }
-        // both threads of a row have read S: the exchange came after
-        ptx::tmem_st_32x32b_x32(tmem_s(t) + lane_base + (uint32_t)(half * 32), packed);
+#pragma unroll
+        for (int u = 4; u > 0; u >>= 1)
+#pragma unroll
+          for (int v = 0; v < u; ++v) sum[v] += sum[v + u];
         if (j > 0 && __any_sync(0xffffffffu, move)) {
           // O_t holds P(j-1) V(j-1): the commit of S_t(j) covers it
+          uint32_t o[DP];
 #pragma unroll
-          for (int x = 0; x < HALF_D / 32; ++x) {
-            uint32_t o[32];
-            ptx::tmem_ld_32x32b_x32(tmem_o(t) + lane_base + (uint32_t)(half * HALF_D + x * 32), o);
-            ptx::tmem_ld_wait();
+          for (int x = 0; x < DP / 32; ++x)
+            ptx::tmem_ld_32x32b_x32(tmem_o(t) + lane_base + (uint32_t)(x * 32), *reinterpret_cast<uint32_t(*)[32]>(&o[x * 32]));
+          ptx::tmem_ld_wait();
 #pragma unroll
-            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * alpha);
-            ptx::tmem_st_32x32b_x32(tmem_o(t) + lane_base + (uint32_t)(half * HALF_D + x * 32), o);
-          }
+          for (int y = 0; y < DP; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * alpha);
+#pragma unroll
+          for (int x = 0; x < DP / 32; ++x)
+            ptx::tmem_st_32x32b_x32(tmem_o(t) + lane_base + (uint32_t)(x * 32), *reinterpret_cast<uint32_t(*)[32]>(&o[x * 32]));
         }
         m = m_new;
-        l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        l = l * alpha + sum[0];
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
-        ptx::mbar_arrive(p_full(t));
+        arrive_warp(p_full(t));
       }
       if (!ok) break;
       blk += n_t;
@@ -564,43 +593,37 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       }
       ++used;
       ptx::tc_fence_after();
-      uint32_t o[HALF_D];
+      uint32_t o[DP];
 #pragma unroll
-      for (int x = 0; x < HALF_D / 32; ++x)
-        ptx::tmem_ld_32x32b_x32(tmem_o(t) + lane_base + (uint32_t)(half * HALF_D + x * 32),
-                                *reinterpret_cast<uint32_t(*)[32]>(&o[x * 32]));
+      for (int x = 0; x < DP / 32; ++x)
+        ptx::tmem_ld_32x32b_x32(tmem_o(t) + lane_base + (uint32_t)(x * 32), *reinterpret_cast<uint32_t(*)[32]>(&o[x * 32]));
       ptx::tmem_ld_wait();
       ptx::tc_fence_before();
-      ptx::mbar_arrive(o_free(t));
-      l += exchange(l);
-      if (!ok) break;
-      meet();  // read on both sides, before the next item's first maximum
-      if (!ok) break;
+      arrive_warp(o_free(t));
       if (real) {
         const int64_t token = e.q0 + query;
-        const int head = (int)(item % p.kv_heads) * p.group + head_of_row;
+        const int head = e.head * p.group + head_of_row;
         const float f = l == 0.f ? 0.f : 1.f / l;
         T *out = static_cast<T *>(p.o) + token * p.o_token + (int64_t)head * p.o_head;
-        const int d0 = half * HALF_D, dims = min(HALF_D, p.head_dim - d0);
         float worst = 0.f;  // NaN or infinite if any element is
 #pragma unroll
-        for (int x = 0; x < HALF_D; ++x) worst = fmaf(__uint_as_float(o[x]), 0.f, worst);
+        for (int x = 0; x < DP; ++x) worst = fmaf(__uint_as_float(o[x]), 0.f, worst);
         if (!(worst == 0.f)) {
-          row_again<T>(p, e.k0, token, head, limit, d0, dims, reference(m), f, out);
-        } else if (dims == HALF_D && p.o_dim == 1 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0) {
+          row_again<T>(p, e.k0, token, head, limit, reference(m), f, out);
+        } else if (p.head_dim == DP && p.o_dim == 1 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0) {
 #pragma unroll
-          for (int x = 0; x < HALF_D / 8; ++x) {
+          for (int x = 0; x < DP / 8; ++x) {
             const float *v = reinterpret_cast<const float *>(o + x * 8);
-            *reinterpret_cast<int4 *>(out + d0 + x * 8) =
+            *reinterpret_cast<int4 *>(out + x * 8) =
                 make_int4((int)tc::attn::pack2<T>(v[0] * f, v[1] * f), (int)tc::attn::pack2<T>(v[2] * f, v[3] * f),
                           (int)tc::attn::pack2<T>(v[4] * f, v[5] * f), (int)tc::attn::pack2<T>(v[6] * f, v[7] * f));
           }
         } else {
 #pragma unroll
-          for (int x = 0; x < HALF_D; ++x)
-            if (x < dims) out[(d0 + x) * p.o_dim] = from_f<T>(__uint_as_float(o[x]) * f);
+          for (int x = 0; x < DP; ++x)
+            if (x < p.head_dim) out[x * p.o_dim] = from_f<T>(__uint_as_float(o[x]) * f);
         }
-        if (p.lse && half == 0)
+        if (p.lse)
           p.lse[token * p.l_token + (int64_t)head * p.l_head] = l == 0.f ? -INFINITY : (m + log2_fast(l)) * kLn2;
       }
     }
@@ -630,6 +653,9 @@ inline bool make_map(CUtensorMap *map, const void *data, CUtensorMapDataType typ
 }
 
 inline int64_t candidates_of(int64_t tokens, int64_t batch, int pair) { return tokens / pair + batch; }
+inline int64_t plan_bytes(int64_t candidates, int64_t batch) {
+  return (int64_t)sizeof(Plan) + candidates * (int64_t)sizeof(Entry) + batch * 4;
+}
 
 template <typename T, int DP>
 int launch_tiles(const Params &prm, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, int64_t candidates,
@@ -659,7 +685,7 @@ template <typename T> int try_tiles(const Problem &p, int64_t workspace_bytes, c
     prm.p = p;
     prm.per_tile = BM / p.group;
     const int64_t candidates = candidates_of(p.q_tokens, p.batch, 2 * prm.per_tile);
-    if ((int64_t)sizeof(Plan) + candidates * (int64_t)sizeof(Entry) > workspace_bytes) return NT_B200_ERR_INVALID_ARGUMENT;
+    if (candidates * p.kv_heads > (1 << 30) || plan_bytes(candidates, p.batch) > workspace_bytes) return NT_B200_ERR_INVALID_ARGUMENT;
     CUtensorMap tq, tk, tv;
     const CUtensorMapDataType type = tc::tmap_dtype<T>();
     if (!make_map(&tq, p.q, type, p.head_dim, p.heads, p.q_tokens, p.q_head, p.q_token, p.group, prm.per_tile) ||
@@ -680,7 +706,7 @@ extern "C" int64_t nt_b200_prompt_attention_workspace_size(int64_t query_tokens,
   if (query_tokens < 0 || batch < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0) return 0;
   const int64_t group = heads / kv_heads;
   const int pair = group > BM ? 2 : 2 * (int)(BM / group);
-  return (int64_t)sizeof(Plan) + candidates_of(query_tokens, batch, pair) * (int64_t)sizeof(Entry);
+  return plan_bytes(candidates_of(query_tokens, batch, pair), batch);
 }
 
 extern "C" int nt_b200_prompt_attention(const NtB200PromptAttentionArgs *a, void *stream) {
