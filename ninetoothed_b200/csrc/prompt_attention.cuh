@@ -24,11 +24,13 @@
 // four sequences of 4096 tokens, 32 heads of 128, not causal: at 96 registers a
 // thread they spill.)
 //
-// The order of items comes from a small kernel before (plan_kernel): sequences
-// longest first, all tiles of a key/value head together, so that its keys and
-// values stay in L2 while they are used, later queries first.  CTAs take the
+// The order of items comes from a small kernel before (plan_kernel): items of
+// more than half, a quarter, an eighth of the longest item's key blocks, and the
+// rest; in each class sequence by sequence, longest first, and head by head, so
+// that a head's keys and values stay in L2 while they are used.  CTAs take the
 // next item when they are done with one (a counter; warp 0 fetches it an item
-// ahead and hands it to the other warps through shared memory).
+// ahead and hands it to the other warps through shared memory), and the last to
+// be taken are short.
 #pragma once
 
 #include <cuda.h>
@@ -125,8 +127,8 @@ __global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ Probl
 // ---------------------------------------------------------------- plan
 constexpr int BM = 128, BN = 128;  // rows of a tile, keys of a block
 
-// Two tiles of queries of one sequence: entry `first` + i of `total` that the
-// sequence has, latest queries first.
+// Two tiles of queries of one sequence.  A sequence's entries of one class are
+// `total` from `first` on in the list, latest queries first.
 struct alignas(32) Entry {
   int32_t q0, queries;  // first packed query, how many (at most two tiles')
   int32_t k0, keys;     // first packed key, how many the sequence has
@@ -134,7 +136,7 @@ struct alignas(32) Entry {
   int32_t first, total;
   int32_t head;         // of an item; unused in the list
 };
-// The workspace: Plan, the entries, then an int32 for each sequence.
+// The workspace: Plan, the entries, then an int32 for each sequence and class.
 struct Plan {
   int32_t count, next, pad[6];  // entries; the next item
 };
@@ -150,36 +152,63 @@ __host__ __device__ __forceinline__ int blocks_of(const Entry &e, int t, int per
   return seen <= 0 ? 1 : (seen + BN - 1) / BN;
 }
 
-constexpr int PLAN_THREADS = 1024, BINS = 1024;
+constexpr int PLAN_THREADS = 1024, CLASSES = 4, BINS = PLAN_THREADS / CLASSES;
+
+// A sequence in the plan: `total` entries, entry i the queries from i * pair on.
+struct Span {
+  int64_t q0, nq, k0, nk;
+  int total, blocks;  // entries; key blocks of the last
+  __device__ bool load(const Problem &p, int64_t b, int pair) {
+    if (!extents(p, b, q0, nq, k0, nk)) nq = 0;
+    total = (int)((nq + pair - 1) / pair);
+    blocks = (int)((nk + BN - 1) / BN);
+    return total > 0;
+  }
+  // the first entry of class `c` or a lower one, for a longest item of `most`
+  // key blocks: those with more than most / 2^(c + 1)
+  __device__ int from(const Problem &p, int c, int most, int pair) const {
+    if (c == CLASSES - 1) return 0;
+    const int least = most >> (c + 1);
+    if (!p.causal) return blocks > least ? 0 : total;
+    const int64_t i = ((int64_t)least * BN - (nk - nq)) / pair;
+    return (int64_t)least * BN < nk - nq ? 0 : i < total ? (int)i : total;
+  }
+};
 
 // The candidate entries: sequence b owns the candidates from query_offsets[b] /
 // pair + b on (pair = queries of two tiles), as many as it can have entries;
-// those past its last are empty.  Counting sort of the sequences by the key
-// blocks of their last queries, most first (beyond the bins in the first one:
-// the order is for balance only), then the entries at their sequence's place.
+// those past its last are empty.  Counting sort of the sequences' classes by
+// class and key blocks, then the entries at their class's place.
 __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const __grid_constant__ Problem p, int64_t candidates,
                                                             int per_tile) {
-  __shared__ int bins[BINS];
+  __shared__ int bins[CLASSES * BINS];
   __shared__ int warp_sums[PLAN_THREADS / 32];
-  static_assert(BINS == PLAN_THREADS, "a thread scans one bin");
+  __shared__ int most_shared;
   wait_prior_grid();
   allow_dependent_launch();
   const int pair = 2 * per_tile;
   Plan *plan = static_cast<Plan *>(p.workspace);
   Entry *list = reinterpret_cast<Entry *>(plan + 1);
-  int32_t *first_of = reinterpret_cast<int32_t *>(list + candidates);  // a sequence's first entry; -1: none
+  int32_t *first_of = reinterpret_cast<int32_t *>(list + candidates);  // [batch][CLASSES]
   bins[threadIdx.x] = 0;
+  if (threadIdx.x == 0) most_shared = 1;
   __syncthreads();
+  Span w;
+  for (int64_t b = threadIdx.x; b < p.batch; b += PLAN_THREADS)
+    if (w.load(p, b, pair)) atomicMax(&most_shared, w.blocks);
+  __syncthreads();
+  const int most = most_shared;
   for (int pass = 0; pass < 2; ++pass) {
     for (int64_t b = threadIdx.x; b < p.batch; b += PLAN_THREADS) {
-      int64_t q0, nq, k0, nk;
-      if (!extents(p, b, q0, nq, k0, nk)) nq = 0;
-      const int total = (int)((nq + pair - 1) / pair);
-      const int64_t blocks = (nk + BN - 1) / BN;
-      int *bin = &bins[blocks >= BINS ? 0 : BINS - 1 - (int)blocks];
-      if (total == 0) first_of[b] = -1;
-      else if (pass == 0) atomicAdd(bin, total);
-      else first_of[b] = atomicAdd(bin, total);
+      if (!w.load(p, b, pair)) continue;
+      int end = w.total;
+      for (int c = 0; c < CLASSES; ++c) {
+        const int from = w.from(p, c, most, pair);
+        int *bin = &bins[c * BINS + (int)((int64_t)(most - w.blocks) * (BINS - 1) / most)];
+        if (pass == 0) atomicAdd(bin, end - from);
+        else first_of[b * CLASSES + c] = atomicAdd(bin, end - from);
+        end = from;
+      }
     }
     __syncthreads();
     if (pass == 1) break;
@@ -202,26 +231,31 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const __grid_constan
     }
     __syncthreads();
   }
-  for (int64_t c = threadIdx.x; c < candidates; c += PLAN_THREADS) {
-    int64_t low = 0, high = p.batch;  // the largest b whose first candidate is <= c
+  for (int64_t x = threadIdx.x; x < candidates; x += PLAN_THREADS) {
+    int64_t low = 0, high = p.batch;  // the largest b whose first candidate is <= x
     while (high - low > 1) {
       const int64_t mid = (low + high) / 2;
-      if (p.q_offsets[mid] / pair + mid <= c) low = mid;
+      if (p.q_offsets[mid] / pair + mid <= x) low = mid;
       else high = mid;
     }
-    int64_t q0, nq, k0, nk;
-    if (first_of[low] < 0 || !extents(p, low, q0, nq, k0, nk)) continue;
-    const int64_t i = c - (q0 / pair + low), first = i * pair;
-    if (i < 0 || first >= nq) continue;
+    if (!w.load(p, low, pair)) continue;
+    const int64_t i = x - (w.q0 / pair + low);
+    if (i < 0 || i >= w.total) continue;
+    int c = 0, end = w.total, from = w.from(p, 0, most, pair);
+    while (i < from) {
+      end = from;
+      from = w.from(p, ++c, most, pair);
+    }
+    const int64_t first = i * pair;
     Entry e{};
-    e.q0 = (int32_t)(q0 + first);
-    e.queries = (int32_t)(nq - first < pair ? nq - first : pair);
-    e.k0 = (int32_t)k0;
-    e.keys = (int32_t)nk;
-    e.limit0 = (int32_t)(p.causal ? nk - nq + 1 + first : nk);
-    e.first = first_of[low];
-    e.total = (int32_t)((nq + pair - 1) / pair);
-    list[e.first + e.total - 1 - (int)i] = e;
+    e.q0 = (int32_t)(w.q0 + first);
+    e.queries = (int32_t)(w.nq - first < pair ? w.nq - first : pair);
+    e.k0 = (int32_t)w.k0;
+    e.keys = (int32_t)w.nk;
+    e.limit0 = (int32_t)(p.causal ? w.nk - w.nq + 1 + first : w.nk);
+    e.first = first_of[low * CLASSES + c];
+    e.total = end - from;
+    list[e.first + end - 1 - (int)i] = e;
   }
 }
 
@@ -238,7 +272,8 @@ struct Layout {
   static constexpr int KV_BYTES = BN * DP * 2;  // one key or value block
   static constexpr int RING_OFF = TILES * Q_BYTES;
   static constexpr int CTRL_OFF = RING_OFF + RING * KV_BYTES;
-  static constexpr int SMEM_BYTES = CTRL_OFF + 384;
+  static constexpr int ROWS_OFF = CTRL_OFF + 384;  // ushort2 [BM]: a row's query and head in its tile
+  static constexpr int SMEM_BYTES = ROWS_OFF + BM * 4;
   static_assert(96 + 16 * RING <= 240, "barrier slots");
   static_assert(SMEM_BYTES <= 232448, "shared memory of a CTA");
 };
@@ -329,6 +364,9 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
     ptx::prefetch_tmap(&tmap_k);
     ptx::prefetch_tmap(&tmap_v);
   }
+  ushort2 *rows = reinterpret_cast<ushort2 *>(smem + L::ROWS_OFF);
+  if (threadIdx.x < BM)
+    rows[threadIdx.x] = make_ushort2((unsigned short)(threadIdx.x / p.group), (unsigned short)(threadIdx.x % p.group));
   // rows past per_tile * group are never loaded: zeros
   if (per_tile * p.group < BM) {
     for (int i = threadIdx.x; i < TILES * L::Q_BYTES / 16; i += THREADS)
@@ -364,22 +402,31 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       int r = 0;             // ring items so far
       int used[TILES] = {};  // items so far that had tile t
       const uint32_t q_bytes = (uint32_t)(per_tile * p.group * 128 * L::ATOMS);
-      // Items count sequence by sequence (all entries of one together), in it
-      // head by head, in it entry by entry.
+      // Items count along the list by a sequence's entries of one class, among
+      // them head by head, in it entry by entry.
       Plan *plan = static_cast<Plan *>(p.workspace);
       const Entry *list = reinterpret_cast<const Entry *>(plan + 1);
       const int64_t num_items = (int64_t)plan->count * p.kv_heads;
-      auto next_item = [&]() {
-        const int64_t k = atomicAdd(&plan->next, 1);
-        Entry e{};
-        if (k >= num_items) return e;
-        const Entry any = list[k / p.kv_heads];  // of the same sequence
-        const int r = (int)(k - (int64_t)any.first * p.kv_heads), h = r / any.total;
-        e = list[any.first + r - h * any.total];
-        e.head = h;
-        return e;
+      // The next item is fetched in three steps, each waiting for the one before
+      // only when it comes to its turn among this item's loads.
+      int64_t next = 0;
+      Entry any{}, ahead{};
+      auto fetch = [&](int step) {
+        if (step == 0) {
+          next = atomicAdd(&plan->next, 1);
+        } else if (step == 1) {
+          any = Entry{};
+          if (next < num_items) any = list[next / p.kv_heads];  // of the same sequence and class
+        } else {
+          ahead = Entry{};
+          if (next < num_items) {
+            const int r = (int)(next - (int64_t)any.first * p.kv_heads), h = r / any.total;
+            ahead = list[any.first + r - h * any.total];
+            ahead.head = h;
+          }
+        }
       };
-      Entry ahead = next_item();
+      for (int x = 0; x < 3; ++x) fetch(x);
       for (int i = 0; ok; ++i) {
         const Entry e = ahead;
         if (!ptx::mbar_wait(item_empty(i & 1), ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag)) break;
@@ -388,7 +435,7 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         to[1].x = e.limit0; to[1].w = e.head;
         ptx::mbar_arrive(item_full(i & 1));
         if (e.queries == 0) break;
-        ahead = next_item();
+        fetch(0);
         const int h = e.head;
         const int n[TILES] = {blocks_of(e, 0, per_tile, p.causal), blocks_of(e, 1, per_tile, p.causal)};
         const int n_max = max(n[0], n[1]);
@@ -409,7 +456,11 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
           for (int x = 0; x < L::ATOMS; ++x)
             ptx::tma_load_3d(base + L::RING_OFF + slot * L::KV_BYTES + x * (BN * 128), map, slot_full(slot), 64 * x, h,
                              e.k0 + (j >> 1) * BN);
+          if (j == 4) fetch(1);
+          if (j == 8) fetch(2);
         }
+        if (2 * n_max <= 4) fetch(1);
+        if (2 * n_max <= 8) fetch(2);
       }
     }
   } else if (warp == 1) {
@@ -498,28 +549,33 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
     const int t = (warp - 2) / 4, quarter = warp & 3;
     const int row = quarter * 32 + lane;  // row of the tile = lane of tensor memory
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const int query_of_row = row / p.group, head_of_row = row % p.group;
     bool ok = true;
     auto arrive_warp = [&](uint32_t bar) {
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar);
     };
     const float c = p.scale;
-    int blk = 0, used = 0;
+    uint32_t s_turn = 0, o_turn = 0;
+    // A block's scores fill a thread's registers: what an item's end needs is
+    // read again there, and the item let go only then.
     for (int i = 0; ok; ++i) {
-      Entry e;
-      if (!__all_sync(0xffffffffu, take_item(i, e)) || e.queries == 0) break;
-      arrive_warp(item_empty(i & 1));
-      const int n_t = blocks_of(e, t, per_tile, p.causal);
-      if (n_t == 0) continue;
-      const int query = t * per_tile + query_of_row;
-      const bool real = query < e.queries && query_of_row < per_tile;
-      const int limit = p.causal ? min(e.limit0 + query, e.keys) : e.keys;
-      const int sure = p.causal ? min(e.limit0 + t * per_tile, e.keys) : e.keys;  // keys that all rows see
+      int n_t, limit, sure;  // key blocks; keys that the row sees; keys that all rows see
+      {
+        Entry e;
+        if (!__all_sync(0xffffffffu, take_item(i, e)) || e.queries == 0) break;
+        n_t = blocks_of(e, t, per_tile, p.causal);
+        limit = p.causal ? min(e.limit0 + t * per_tile + rows[row].x, e.keys) : e.keys;
+        sure = p.causal ? min(e.limit0 + t * per_tile, e.keys) : e.keys;
+      }
+      if (n_t == 0) {
+        arrive_warp(item_empty(i & 1));
+        continue;
+      }
 
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n_t; ++j) {
-        if (!ptx::mbar_wait_warp(s_full(t), (uint32_t)(blk + j) & 1u, abort_flag)) { ok = false; break; }
+        if (!ptx::mbar_wait_warp(s_full(t), s_turn, abort_flag)) { ok = false; break; }
+        s_turn ^= 1;
         ptx::tc_fence_after();
         uint32_t sr[BN];
 #pragma unroll
@@ -585,13 +641,8 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         ptx::tc_fence_before();
         arrive_warp(p_full(t));
       }
-      if (!ok) break;
-      blk += n_t;
-      if (!ptx::mbar_wait_warp(o_done(t), (uint32_t)used & 1u, abort_flag)) {
-        ok = false;
-        break;
-      }
-      ++used;
+      if (!ok || !ptx::mbar_wait_warp(o_done(t), o_turn, abort_flag)) break;
+      o_turn ^= 1;
       ptx::tc_fence_after();
       uint32_t o[DP];
 #pragma unroll
@@ -600,9 +651,13 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       ptx::tmem_ld_wait();
       ptx::tc_fence_before();
       arrive_warp(o_free(t));
-      if (real) {
+      Entry e;
+      take_item(i, e);
+      arrive_warp(item_empty(i & 1));
+      const int query = t * per_tile + rows[row].x;
+      if (query < e.queries && rows[row].x < per_tile) {
         const int64_t token = e.q0 + query;
-        const int head = e.head * p.group + head_of_row;
+        const int head = e.head * p.group + rows[row].y;
         const float f = l == 0.f ? 0.f : 1.f / l;
         T *out = static_cast<T *>(p.o) + token * p.o_token + (int64_t)head * p.o_head;
         float worst = 0.f;  // NaN or infinite if any element is
@@ -654,7 +709,7 @@ inline bool make_map(CUtensorMap *map, const void *data, CUtensorMapDataType typ
 
 inline int64_t candidates_of(int64_t tokens, int64_t batch, int pair) { return tokens / pair + batch; }
 inline int64_t plan_bytes(int64_t candidates, int64_t batch) {
-  return (int64_t)sizeof(Plan) + candidates * (int64_t)sizeof(Entry) + batch * 4;
+  return (int64_t)sizeof(Plan) + candidates * (int64_t)sizeof(Entry) + batch * 4 * CLASSES;
 }
 
 template <typename T, int DP>
