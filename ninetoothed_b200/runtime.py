@@ -80,7 +80,9 @@ class Kernel:
     def __post_init__(self):
         # what every call looks up, once
         self.public_args = tuple(arg.name for arg in self.args)
-        self._tensor_args = tuple(arg for arg in self.args if isinstance(arg, TensorArg))
+        self._tensor_args = tuple(
+            (arg.name, arg.ndim, frozenset(arg.dtypes), arg) for arg in self.args if isinstance(arg, TensorArg)
+        )
         self._accepted = frozenset(self.public_args) | frozenset(self.meta)
         self._required = self.public_args + tuple(self.meta)
 
@@ -123,26 +125,24 @@ class Kernel:
 
     def _validate(self, values) -> torch.device:
         device = None
-        for arg in self._tensor_args:
-            value = values[arg.name]
+        for name, ndim, dtypes, arg in self._tensor_args:
+            value = values[name]
             if value is None and arg.optional:
                 continue
             if not isinstance(value, torch.Tensor):
-                raise TypeError(f"Kernel argument `{arg.name}` must be a tensor.")
-            if value.dim() != arg.ndim:
-                raise TypeError(
-                    f"Kernel argument `{arg.name}` has rank {value.dim()}; expected {arg.ndim}."
-                )
-            if device is None or value.device != device:
+                raise TypeError(f"Kernel argument `{name}` must be a tensor.")
+            if value.dim() != ndim:
+                raise TypeError(f"Kernel argument `{name}` has rank {value.dim()}; expected {ndim}.")
+            if value.device != device:
                 if value.device.type != "cuda":
-                    raise TypeError(f"Kernel argument `{arg.name}` must be on a CUDA device.")
+                    raise TypeError(f"Kernel argument `{name}` must be on a CUDA device.")
                 if device is not None:
                     raise TypeError("All tensor arguments must use the same CUDA device.")
                 device = value.device
-            if value.dtype not in arg.dtypes:
+            if value.dtype not in dtypes:
                 expected = ", ".join(str(d).split(".")[-1] for d in arg.dtypes)
                 raise TypeError(
-                    f"Kernel argument `{arg.name}` has dtype {str(value.dtype).split('.')[-1]}; "
+                    f"Kernel argument `{name}` has dtype {str(value.dtype).split('.')[-1]}; "
                     f"expected one of {expected}."
                 )
         if device is None:
@@ -165,9 +165,10 @@ def ptr(tensor: torch.Tensor) -> int:
 
 def check_same_dtype(values, names):
     dtype = values[names[0]].dtype
-    if any(values[name].dtype != dtype for name in names):
-        listing = ", ".join(f"`{name}`" for name in names)
-        raise TypeError(f"Kernel arguments {listing} must share one dtype.")
+    for name in names:
+        if values[name].dtype != dtype:
+            listing = ", ".join(f"`{name}`" for name in names)
+            raise TypeError(f"Kernel arguments {listing} must share one dtype.")
 
 
 def device_status(stream: int = None) -> int:
