@@ -108,12 +108,11 @@ class Kernel:
         if len(args) > len(public):
             raise TypeError(f"Expected at most {len(public)} arguments.")
         if kwargs:
-            positional = public[: len(args)]
-            duplicates = tuple(name for name in positional if name in kwargs)
+            duplicates = tuple(name for name in kwargs if name in public and public.index(name) < len(args))
             if duplicates:
                 raise TypeError(f"Kernel arguments passed twice: {', '.join(sorted(duplicates))}.")
-            unknown = tuple(name for name in kwargs if name not in self._accepted)
-            if unknown:
+            if not self._accepted.issuperset(kwargs):
+                unknown = tuple(name for name in kwargs if name not in self._accepted)
                 raise TypeError(f"Unknown kernel arguments: {', '.join(sorted(unknown))}.")
         values = dict(self.meta_defaults)
         values.update(zip(public, args))

@@ -14,6 +14,7 @@ an index outside its array is not followed and shows in
 """
 
 import math
+from operator import itemgetter
 
 import torch
 
@@ -120,9 +121,12 @@ def rotary(input, cos, sin, positions, interleaved=False, adjoint=False):
 
 
 # --------------------------------------------------------------------- paged cache
+_cache_values = itemgetter("key_cache", "value_cache", "key_scale", "value_scale")
+
+
 def _cache_args(v):
     """The fields of NtB200PagedCache, with the checks that need no device."""
-    key, value, ks, vs = v["key_cache"], v["value_cache"], v["key_scale"], v["value_scale"]
+    key, value, ks, vs = _cache_values(v)
     check_same_dtype(v, ("key_cache", "value_cache"))
     pages, heads, page, dim = key.shape
     if value.shape != key.shape or ks.shape != (pages, heads) or vs.shape != (pages, heads):
@@ -134,11 +138,13 @@ def _cache_args(v):
         raise TypeError(
             f"a paged cache needs page size (at most 4096) and head dimension in multiples of 16; got {page} and {dim}."
         )
-    if key.stride(3) != 1 or value.stride(3) != 1:
+    k0, k1, k2, k3 = key.stride()
+    v0, v1, v2, v3 = value.stride()
+    if k3 != 1 or v3 != 1:
         raise TypeError("Kernel arguments `key_cache`, `value_cache` must have unit stride along their last dimension.")
     return (
         key.data_ptr(), value.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, heads, page, dim,
-        dtype_code(key.dtype), *key.stride()[:3], *value.stride()[:3], *ks.stride(), *vs.stride(),
+        dtype_code(key.dtype), k0, k1, k2, v0, v1, v2, *ks.stride(), *vs.stride(),
     )
 
 
@@ -150,24 +156,26 @@ _CACHE_ARGS = (
 )
 
 
+_append_values = itemgetter("key", "value", "query", "offsets", "past", "block_table", "query_out", "key_out", "cos",
+                            "sin")
+
+
 def _launch_paged_append(v, stream):
-    key, value, query = v["key"], v["value"], v["query"]
-    offsets, past, table = v["offsets"], v["past"], v["block_table"]
-    query_out, key_out = v["query_out"], v["key_out"]
+    key, value, query, offsets, past, table, query_out, key_out, cos, sin = _append_values(v)
     check_same_dtype(v, ("key", "value"))
     check_same_dtype(v, ("offsets", "past", "block_table"))
     cache = _cache_args(v)
     tokens, kv_heads, dim = key.shape
     batch = past.shape[0]
-    if value.shape != key.shape or (kv_heads, dim) != (v["key_cache"].shape[1], v["key_cache"].shape[3]):
+    if value.shape != key.shape or (kv_heads, dim) != (cache[5], cache[7]):
         raise TypeError(
             f"paged_append key {tuple(key.shape)}, value {tuple(value.shape)} and cache "
             f"{tuple(v['key_cache'].shape)} disagree."
         )
     if offsets.shape[0] != batch + 1 or table.shape[0] != batch:
         raise TypeError(f"paged_append needs {batch + 1} offsets and {batch} block table rows.")
-    turns = v["cos"] is not None
-    if turns != (v["sin"] is not None):
+    turns = cos is not None
+    if turns != (sin is not None):
         raise TypeError("Kernel arguments `cos`, `sin` must be given together.")
     if turns:
         _check_tables(v, dim)
@@ -183,7 +191,6 @@ def _launch_paged_append(v, stream):
         if key_out.shape != key.shape:
             raise TypeError("paged_append key_out must have the key's shape.")
     none3 = (0, 0, 0)
-    cos, sin = v["cos"], v["sin"]
     args = _lib.pack_args(
         *cache, key.data_ptr(), value.data_ptr(), query.data_ptr() if query is not None else 0,
         cos.data_ptr() if turns else 0, sin.data_ptr() if turns else 0, offsets.data_ptr(), past.data_ptr(),
@@ -249,13 +256,16 @@ def paged_append(key, value, offsets, past, block_table, key_cache, value_cache,
 
 
 # --------------------------------------------------------------------- attention over the cache
+_attention_values = itemgetter("query", "output", "lse", "lengths", "block_table")
+
+
 def _launch_paged_attention(v, stream):
-    query, out, lse, lengths, table = v["query"], v["output"], v["lse"], v["lengths"], v["block_table"]
+    query, out, lse, lengths, table = _attention_values(v)
     check_same_dtype(v, ("query", "output"))
     check_same_dtype(v, ("lengths", "block_table"))
     cache = _cache_args(v)
     batch, queries, heads, dim = query.shape
-    _, kv_heads, _, cache_dim = v["key_cache"].shape
+    kv_heads, cache_dim = cache[5], cache[7]
     if out.shape != query.shape or dim != cache_dim or not kv_heads or heads % kv_heads:
         raise TypeError(
             f"paged_attention query {tuple(query.shape)}, cache {tuple(v['key_cache'].shape)} and output "
