@@ -415,7 +415,8 @@ int64_t nt_b200_paged_attention_workspace_size(void);
  * tcgen05 tensor cores (probabilities rounded to the input type there) for
  * head_dim up to 128, unit element strides, other strides and bases on the
  * 16-byte grid and a positive scale; the rest, FLOAT32 and head_dim up to 256,
- * on CUDA cores.  Tokens that belong to no sequence are not written.
+ * on CUDA cores.  Tokens that belong to no sequence are not written, and none
+ * are on tensor cores where any offsets are out of order or leave the tensors.
  * `workspace`: 32-byte aligned device memory of
  * nt_b200_prompt_attention_workspace_size(...) bytes, for this call alone.
  */

@@ -549,7 +549,7 @@ extern "C" int nt_b200_paged_append(const NtB200PagedAppendArgs *a, void *stream
   const bool turns = a->cos != nullptr;
   if (turns && (!a->sin || a->rotary_dim > c.head_dim)) return NT_B200_ERR_SHAPE_MISMATCH;
   if (!a->key || !a->value || !a->offsets || !a->past || !a->block_table || (a->query && (!turns || !a->query_out)) ||
-      a->tokens > (1 << 30) || a->batch > (1 << 28) || a->heads > (1 << 20))
+      a->tokens > (1 << 30) || a->batch > (1 << 28) || a->heads > (1 << 20) || a->table_columns > (1LL << 31))
     return NT_B200_ERR_INVALID_ARGUMENT;
   if (c.kv_heads == 0 && !a->query) return 0;
   paged::Params p{};

@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const __grid_constan
                                                             int per_tile) {
   __shared__ int bins[CLASSES * BINS];
   __shared__ int warp_sums[PLAN_THREADS / 32];
-  __shared__ int most_shared;
+  __shared__ int most_shared, out_of_order;
   wait_prior_grid();
   allow_dependent_launch();
   const int pair = 2 * per_tile;
@@ -191,12 +191,21 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const __grid_constan
   Entry *list = reinterpret_cast<Entry *>(plan + 1);
   int32_t *first_of = reinterpret_cast<int32_t *>(list + candidates);  // [batch][CLASSES]
   bins[threadIdx.x] = 0;
-  if (threadIdx.x == 0) most_shared = 1;
+  if (threadIdx.x == 0) {
+    most_shared = 1;
+    out_of_order = 0;
+  }
   __syncthreads();
   Span w;
-  for (int64_t b = threadIdx.x; b < p.batch; b += PLAN_THREADS)
-    if (w.load(p, b, pair)) atomicMax(&most_shared, w.blocks);
+  for (int64_t b = threadIdx.x; b < p.batch; b += PLAN_THREADS) {
+    if (!extents(p, b, w.q0, w.nq, w.k0, w.nk)) out_of_order = 1;
+    else if (w.load(p, b, pair)) atomicMax(&most_shared, w.blocks);
+  }
   __syncthreads();
+  if (out_of_order) {  // sequences may overlap and outnumber the candidates: none is taken
+    if (threadIdx.x == 0) plan->count = plan->next = 0;
+    return;
+  }
   const int most = most_shared;
   for (int pass = 0; pass < 2; ++pass) {
     for (int64_t b = threadIdx.x; b < p.batch; b += PLAN_THREADS) {

@@ -220,7 +220,7 @@ paged_append_kernel = Kernel(
         TensorArg("query_out", 3, optional=True),
         TensorArg("key_out", 3, optional=True),
     ),
-    outputs=("key_cache",),
+    outputs=(),  # the cache is updated in place; the kernel returns None
     launch=_launch_paged_append,
     meta=("interleaved",),
     meta_defaults={"interleaved": False, "query": None, "cos": None, "sin": None, "query_out": None, "key_out": None},

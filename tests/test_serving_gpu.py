@@ -634,12 +634,34 @@ def test_prompt_attention_not_finite_where_it_is_not_seen(dtype):
 def test_prompt_attention_offsets_out_of_range():
     q = torch.randn(64, 2, 64).half().cuda()
     good = programs.prompt_attention(q, q, q, index([0, 64]))
-    for bad in ([0, 65], [-1, 64], [0, 40, 30]):
+    # the last: overlapping sequences, more of their tiles than tokens have room for
+    for bad in ([0, 65], [-1, 64], [0, 40, 30], [0, 64] * 300):
         programs.prompt_attention(q, q, q, index(bad))
         assert device_status() == INDEX_OUT_OF_RANGE
         programs.prompt_attention(q.float(), q.float(), q.float(), index(bad))
         assert device_status() == INDEX_OUT_OF_RANGE
     assert torch.equal(programs.prompt_attention(q, q, q, index([0, 64])), good)
+
+
+@pytest.mark.parametrize("dtype", (torch.float16, torch.float32))
+def test_prompt_attention_without_keys_or_queries(dtype):
+    q = torch.randn(5, 2, 64).to(dtype).cuda()
+    none = q[:0, :1]
+    got, lse = programs.prompt_attention(q, none, none, index([0, 3, 5]), index([0, 0, 0]), return_lse=True)
+    assert not got.any() and (lse == -math.inf).all()
+    got, lse = programs.prompt_attention(q[:0], q[:, :1], q[:, :1], index([0, 0]), index([0, 5]), return_lse=True)
+    assert got.shape == (0, 2, 64) and lse.shape == (0, 2)
+    assert device_status() == 0
+
+
+@pytest.mark.parametrize("heads, kv_heads", ((4, 4), (6, 2)))
+def test_prompt_attention_head_major(heads, kv_heads):
+    """[heads, tokens, head_dim] in memory."""
+    lens = [200, 60]
+    q, k, v = (torch.randn(n, 260, 64).bfloat16().transpose(0, 1) for n in (heads, kv_heads, kv_heads))
+    got, lse = programs.prompt_attention(dev(q), dev(k), dev(v), index([0, 200, 260]), return_lse=True)
+    assert not dev(q).is_contiguous()
+    check_prompt(q, k, v, lens, lens, 64**-0.5, True, got, lse, torch.bfloat16)
 
 
 def test_joined_by_lse():
