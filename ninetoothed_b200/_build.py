@@ -4,16 +4,22 @@ The library is one translation unit (`csrc/nt_b200.cu` includes every kernel
 family), compiled with `-gencode arch=compute_100a,code=sm_100a`.  It links only
 the CUDA runtime; the TMA tensor-map encoder is fetched from the driver at run
 time with `cudaGetDriverEntryPoint`, so no `-lcuda` is needed.
+
+Beside it, `_binding.so` (`csrc/binding.cpp`, g++ against torch's headers) binds
+the serving operators' calls in C++; without it they take their Python path.
 """
 
 import os
 import shutil
 import subprocess
+import sysconfig
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
 SOURCE_DIR = PACKAGE_DIR / "csrc"
 LIBRARY = PACKAGE_DIR / "libnt_b200.so"
+BINDING = PACKAGE_DIR / "_binding.so"
+BINDING_SOURCE = SOURCE_DIR / "binding.cpp"
 MAIN_SOURCE = SOURCE_DIR / "nt_b200.cu"
 INCLUDE_DIR = PACKAGE_DIR.parent / "include"
 
@@ -56,16 +62,47 @@ def sources() -> list[Path]:
     )
 
 
+def _older(built: Path, paths) -> bool:
+    return not built.is_file() or any(path.stat().st_mtime > built.stat().st_mtime for path in paths)
+
+
+def binding_is_stale() -> bool:
+    return _older(BINDING, [BINDING_SOURCE, *INCLUDE_DIR.glob("*.h"), Path(__file__).resolve()])
+
+
 def is_stale(library: Path = LIBRARY) -> bool:
-    if not library.is_file():
-        return True
-    built = library.stat().st_mtime
-    return any(path.stat().st_mtime > built for path in sources())
+    return _older(library, sources()) or binding_is_stale()
+
+
+def build_binding(verbose: bool = False) -> Path:
+    """Compile the C++ binding against the installed torch."""
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(find_nvcc()).resolve().parent.parent
+    temporary = BINDING.with_name(f".{BINDING.name}.{os.getpid()}.tmp")
+    command = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden"]
+    command += [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
+    command += [f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include", f"-I{cuda}/include"]
+    command += [f"-I{sysconfig.get_paths()['include']}", "-o", str(temporary), str(BINDING_SOURCE), f"-L{root}/lib"]
+    command += ["-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(command))
+    try:
+        subprocess.run(command, check=True)
+        os.replace(temporary, BINDING)
+    finally:
+        if temporary.exists():
+            temporary.unlink()
+    return BINDING
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the library if it is missing or older than its sources."""
-    if not force and not is_stale():
+    """Compile the library and the binding where they are missing or older than
+    their sources."""
+    if force or binding_is_stale():
+        build_binding(verbose)
+    if not force and not _older(LIBRARY, sources()):
         return LIBRARY
     temporary = LIBRARY.with_name(f".{LIBRARY.name}.{os.getpid()}.tmp")
     command = [find_nvcc(), *NVCC_FLAGS]

@@ -132,6 +132,29 @@ def library():
     return _library
 
 
+_binding = None  # the C++ binding; False: there is none
+
+
+def binding():
+    """The serving operators' calls in C++ (csrc/binding.cpp), bound to the
+    library once per process, or None where the binding is not built."""
+    global _binding
+    if _binding is None:
+        lib = library()
+        with _lock:
+            if _binding is None:
+                try:
+                    from ninetoothed_b200 import _binding as module
+                except ImportError:
+                    _binding = False
+                else:
+                    names = ("rotary", "paged_append", "paged_attention", "prompt_attention",
+                             "paged_attention_workspace_size", "prompt_attention_workspace_size")
+                    module.bind(*(ctypes.cast(getattr(lib, f"nt_b200_{name}"), _P).value for name in names))
+                    _binding = module
+    return _binding or None
+
+
 def int64_array(values):
     """A ctypes int64[] holding `values` (kept alive by the caller)."""
     values = tuple(int(v) for v in values)

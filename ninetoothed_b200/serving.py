@@ -19,11 +19,24 @@ from operator import itemgetter
 import torch
 
 from ninetoothed_b200 import _lib
-from ninetoothed_b200.runtime import Kernel, TensorArg, check_same_dtype, dtype_code
+from ninetoothed_b200.runtime import Kernel, KernelLaunchError, TensorArg, check_same_dtype, dtype_code
 
 INDEX_DTYPES = (torch.int32, torch.int64)
 CODE_DTYPES = (torch.float8_e4m3fn, torch.int8)
 _F32 = (torch.float32,)
+
+
+def _bound(name, *args):
+    """The call made by the C++ binding, which checks it, allocates its outputs and
+    launches it; None where there is no binding or it left the call alone (one
+    that is not as it should be, for which the kernel object below says why)."""
+    binding = _lib.binding()
+    if binding is None:
+        return None
+    result = getattr(binding, name)(*args)
+    if result.__class__ is int:
+        raise KernelLaunchError(result)
+    return result
 
 
 def _check_tables(v, head_dim):
@@ -116,6 +129,9 @@ def rotary(input, cos, sin, positions, interleaved=False, adjoint=False):
     Pairs are (i, i + half) or, interleaved, (2i, 2i + 1).  `adjoint` applies
     the transposed rotation: given the gradient of the output it returns the
     gradient of the input."""
+    result = _bound("rotary", input, cos, sin, positions, interleaved, adjoint)
+    if result is not None:
+        return result
     output = torch.empty_like(input, memory_format=torch.contiguous_format)
     return rotary_kernel(input, cos, sin, positions, output, interleaved=interleaved, adjoint=adjoint)
 
@@ -248,6 +264,10 @@ def paged_append(key, value, offsets, past, block_table, key_cache, value_cache,
     rotated too and returned; `return_key` also returns the rotated key in its
     own dtype (a prompt's attention reads it).  What was not asked for is None.
     """
+    result = _bound("paged_append", key, value, offsets, past, block_table, key_cache, value_cache, key_scale,
+                    value_scale, query, cos, sin, interleaved, return_key)
+    if result is not None:
+        return result
     query_out = None if query is None else torch.empty_like(query, memory_format=torch.contiguous_format)
     key_out = torch.empty_like(key, memory_format=torch.contiguous_format) if return_key else None
     paged_append_kernel(key, value, offsets, past, block_table, key_cache, value_cache, key_scale, value_scale,
@@ -323,6 +343,10 @@ def paged_attention(query, key_cache, value_cache, key_scale, value_scale, block
     (output, lse): the fp32 natural logarithm of each query's sum of exponentials
     [batch, queries, heads], by which attention over separate keys is joined.  A
     query that sees no token gets 0, and -inf as its lse."""
+    result = _bound("paged_attention", query, key_cache, value_cache, key_scale, value_scale, block_table, lengths,
+                    scale, return_lse)
+    if result is not None:
+        return result
     output = torch.empty_like(query, memory_format=torch.contiguous_format)
     lse = query.new_empty(query.shape[:3], dtype=torch.float32) if return_lse else None
     paged_attention_kernel(query, key_cache, value_cache, key_scale, value_scale, block_table, lengths, output, lse,
@@ -394,6 +418,10 @@ def prompt_attention(query, key, value, offsets, key_offsets=None, is_causal=Tru
     dtype, or with `return_lse` (output, lse): the fp32 natural logarithm of each
     query's sum of exponentials [tokens, heads].  A query that sees no key gets
     0, and -inf as its lse; tokens that belong to no sequence are not written."""
+    result = _bound("prompt_attention", query, key, value, offsets, offsets if key_offsets is None else key_offsets,
+                    is_causal, scale, return_lse)
+    if result is not None:
+        return result
     output = torch.empty_like(query, memory_format=torch.contiguous_format)
     lse = query.new_empty(query.shape[:2], dtype=torch.float32) if return_lse else None
     prompt_attention_kernel(query, key, value, offsets, offsets if key_offsets is None else key_offsets, output, lse,
