@@ -160,8 +160,8 @@ struct Span {
   int total, blocks;  // entries; key blocks of the last
   __device__ bool load(const Problem &p, int64_t b, int pair) {
     if (!extents(p, b, q0, nq, k0, nk)) nq = 0;
-    total = (int)((nq + pair - 1) / pair);
-    blocks = (int)((nk + BN - 1) / BN);
+    total = (int)((uint32_t)(nq + pair - 1) / (uint32_t)pair);  // (at most 2^30 tokens)
+    blocks = (int)((uint32_t)(nk + BN - 1) / BN);
     return total > 0;
   }
   // the first entry of class `c` or a lower one, for a longest item of `most`
@@ -170,8 +170,8 @@ struct Span {
     if (c == CLASSES - 1) return 0;
     const int least = most >> (c + 1);
     if (!p.causal) return blocks > least ? 0 : total;
-    const int64_t i = ((int64_t)least * BN - (nk - nq)) / pair;
-    return (int64_t)least * BN < nk - nq ? 0 : i < total ? (int)i : total;
+    const int64_t before = (int64_t)least * BN - (nk - nq);  // queries that see no more
+    return before < 0 ? 0 : before > nq ? total : min((int)((uint32_t)before / (uint32_t)pair), total);
   }
 };
 
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const __grid_constan
       int end = w.total;
       for (int c = 0; c < CLASSES; ++c) {
         const int from = w.from(p, c, most, pair);
-        int *bin = &bins[c * BINS + (int)((int64_t)(most - w.blocks) * (BINS - 1) / most)];
+        int *bin = &bins[c * BINS + (int)((uint32_t)(most - w.blocks) * (BINS - 1) / (uint32_t)most)];
         if (pass == 0) atomicAdd(bin, end - from);
         else first_of[b * CLASSES + c] = atomicAdd(bin, end - from);
         end = from;
@@ -244,11 +244,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const __grid_constan
     int64_t low = 0, high = p.batch;  // the largest b whose first candidate is <= x
     while (high - low > 1) {
       const int64_t mid = (low + high) / 2;
-      if (p.q_offsets[mid] / pair + mid <= x) low = mid;
+      if ((uint32_t)p.q_offsets[mid] / (uint32_t)pair + mid <= x) low = mid;
       else high = mid;
     }
     if (!w.load(p, low, pair)) continue;
-    const int64_t i = x - (w.q0 / pair + low);
+    const int64_t i = x - ((uint32_t)w.q0 / (uint32_t)pair + low);
     if (i < 0 || i >= w.total) continue;
     int c = 0, end = w.total, from = w.from(p, 0, most, pair);
     while (i < from) {
