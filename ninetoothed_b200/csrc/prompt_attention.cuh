@@ -8,12 +8,14 @@
 //
 // Bound by the tensor cores and, level with them, by the exponentials: a key
 // block of 128 keys costs 256 rows 2048 cycles of dense MMA and 2048 cycles of
-// the SM's 16 exponentials a cycle.
+// the SM's 16 exponentials a cycle.  Now by a tile's round trip, softmax, then P V
+// and the next Q K^T: four causal sequences of 4096 tokens, 32 heads on 8, 128
+// bfloat16 elements: 600-640 us, 860-915 TFLOP/s.
 //
 // Rows of a tile are (query, head of the group) pairs, so that all query heads
 // of a key/value head share one pass over its keys: 128 / group queries a tile.
 // Persistent, one CTA an SM; an item of work is a key/value head and two tiles
-// of 128 rows.  18 warps:
+// of 128 rows.  10 warps:
 //   warp 0      TMA: an item's Q tiles, then its key and value blocks through a
 //               ring of 5 shared-memory slots that runs on across items;
 //   warp 1      tensor memory, and the MMAs from one thread: S_t = Q_t K_j^T,
