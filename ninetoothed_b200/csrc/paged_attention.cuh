@@ -18,11 +18,11 @@
 // workspace; the CTA that brings a unit's last part joins them, always in the
 // line's order.  A second kernel for that cost 3 us of the device's time and 6 us
 // of the host's a call.  Warps that took the steps of a unit in turn and joined
-// at the end of every unit took 108 us where this takes 31 us for 256 units of up
+// at the end of every unit took 108 us where this takes 27 us for 256 units of up
 // to 2047 tokens: short units cost a CTA as much as long ones.
 //
 // Measured (32 query heads on 8 key/value heads of 128 e4m3 elements, 64-token
-// pages): 6 x 131072 tokens 283-298 us, 5.4-5.7 TB/s of the cache; 64 sequences of 1
+// pages): 6 x 131072 tokens 275-290 us, 5.6-5.8 TB/s of the cache; 64 sequences of 1
 // to 8192 tokens 121 us, 4.7 TB/s; one of 1023 tokens 14 us.  Loads alone, without
 // the arithmetic, take 266 us for the first.
 //
@@ -165,12 +165,17 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(Attention a) {
 
 // ---------------------------------------------------------------- tensor cores
 constexpr int STEP = 32;
-constexpr int LEAST_STEPS = 2;  // of a CTA: fewer would be parts to join rather than work
-// A unit's start and end (its queries, its output) take a warp about two steps'
-// time, and count as that in the line where shares are long (BUSY_STEPS): a share
-// of nine short units took 113 us beside 80 of long ones.  Short shares are bound
-// by latency and are cut by what there is to read.
-constexpr int UNIT_STEPS = 2, BUSY_STEPS = 8;
+// Steps of a CTA at least: fewer would be parts to join rather than work.  One
+// sequence of 1023 e4m3 tokens, 8 key/value heads of 128: 14.6 us at 2, 13.9 at 4,
+// 15.4 at 6.
+constexpr int LEAST_STEPS = 4;
+// A unit's start and end (its queries, its output) take a warp about three steps'
+// time, and count as that in the line where a warp's share is BUSY_STEPS or more:
+// a share of nine short units took 113 us beside 80 of long ones.  With 4 queries
+// each of 16 sequences of up to 2047 tokens, 16 heads of 64, at (UNIT_STEPS,
+// BUSY_STEPS) of (2, 8) 31.2 us, (2, 2) 29.6, (3, 2) 26.9.  Shares below that are
+// bound by latency and are cut by what there is to read.
+constexpr int UNIT_STEPS = 3, BUSY_STEPS = 2;
 // A block table row's tokens that are looked at; a page's size.  With them the
 // block table column of a 16-token group is one multiplication: for g < 2^27
 // groups and d = page / 16 <= 2^8, floor(g ceil(2^36 / d) / 2^36) = floor(g / d).
