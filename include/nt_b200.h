@@ -377,8 +377,8 @@ int nt_b200_paged_append(const NtB200PagedAppendArgs *args, void *stream);
  * Attention of each sequence's last `queries` tokens over a paged cache that
  * holds them already: query i of `query` [batch, queries, heads, head_dim] sees
  * the first lengths[b] - queries + 1 + i tokens of sequence b; query head h
- * reads key/value head h / (heads / kv_heads).  With s = scale * (q . k) over
- * those tokens, output = softmax(s) v and, where `lse` is not null, lse [batch,
+ * reads key/value head h / (heads / kv_heads).  Nobody sees the tokens of a page
+ * outside the pool.  With s = scale * (q . k) over the tokens seen, output = softmax(s) v and, where `lse` is not null, lse [batch,
  * queries, heads] = ln sum exp(s) (fp32); a query that sees nothing gets 0 and
  * -inf.  Scores, softmax and sums are fp32; the scales must not be negative.
  * FLOAT16 and BFLOAT16 queries of head_dim up to 128 run on tensor cores

@@ -158,9 +158,9 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(Attention a) {
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int d = lane + 32 * e;
-    if (d < a.head_dim) out[d * a.o_dim] = from_f<T>(limit > 0 ? acc[e] / l : 0.f);
+    if (d < a.head_dim) out[d * a.o_dim] = from_f<T>(l == 0.f ? 0.f : acc[e] / l);
   }
-  if (a.lse && lane == 0) a.lse[b * a.l_batch + i * a.l_token + h * a.l_head] = limit > 0 ? (m + log2f(l)) * kLn2 : -INFINITY;
+  if (a.lse && lane == 0) a.lse[b * a.l_batch + i * a.l_token + h * a.l_head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 // ---------------------------------------------------------------- tensor cores
@@ -201,10 +201,8 @@ __device__ __forceinline__ uint2 load_shared8(uint32_t from) {
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(from) : "memory");
   return v;
 }
-__device__ __forceinline__ float load_shared4(uint32_t from) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(from) : "memory");
-  return v;
+__device__ __forceinline__ void store_shared4(uint32_t to, uint32_t v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(v) : "memory");
 }
 
 // D[16 x 8] += A[16 x 16] B[16 x 8], fp16 in, fp32 accumulator.
@@ -243,6 +241,10 @@ template <> __device__ __forceinline__ void to_halves<int8_t>(uint32_t w, uint32
   lo = *reinterpret_cast<uint32_t *>(&x);
   hi = *reinterpret_cast<uint32_t *>(&y);
 }
+
+// Stands for the key scale of a page outside the pool (a NaN that no scale is):
+// nobody sees its tokens.
+constexpr uint32_t kNoPage = 0xffffffffu;
 
 // Tokens of a 16-token group in the order of the MMAs' rows: row r holds token
 // r / 2 (even r) or 4 + r / 2 (odd r), and so on from 8.  A lane's four values
@@ -659,6 +661,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
     if (++lstep < lseg.real) find_pages();
     else enter();
   };
+  auto page_known = [&](int g) { return (SPLIT && g == 1 ? id1 : id0) >= 0; };
   // the live tokens of a group, its page (0 where it has none) and slot in it
   auto group_of = [&](int g, int &live, uint32_t &id, uint32_t &slot) {
     live = lseg.length - (lstep * STEP + 16 * g);
@@ -693,8 +696,11 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
             copy_async16(to(g, i), valid ? k + i * (uint64_t)(32 / ROW_WORDS * k_token) : a.key, valid);
           }
         }
-        if ((SPLIT || g == 0) && lane < 2)
-          copy_async4(ring + at * L::SLOT + L::CODES + (lane * 2 + g) * 4, scale_head + (uint64_t)id * scale_page, live > 0);
+        if ((SPLIT || g == 0) && lane < 2) {
+          const uint32_t place = ring + at * L::SLOT + L::CODES + (lane * 2 + g) * 4;
+          if (lane == 0 && !page_known(g)) store_shared4(place, kNoPage);
+          else copy_async4(place, scale_head + (uint64_t)id * scale_page, live > 0);
+        }
       }
     }
     copy_commit();
@@ -843,6 +849,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
       lv[1] = SPLIT ? log2_fast(__uint_as_float(scales.w)) : lv[0];
       const int t0 = step * STEP;
       const bool masked = t0 + STEP > sure;
+      const bool gone[2] = {scales.x == kNoPage, (SPLIT ? scales.y : scales.x) == kNoPage};
       // scores in base 2 are s * unit; where some are masked they are multiplied
       // out first
       float unit[2][NT][2];
@@ -861,6 +868,15 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
               s[g][nt][e] = t0 + 16 * g + token_of(n8) + 8 * (e >> 1) < limit[nt][e & 1] ? s[g][nt][e] * unit[g][nt][e & 1] : -INFINITY;
 #pragma unroll
           for (int g = 0; g < 2; ++g) unit[g][nt][0] = unit[g][nt][1] = 1.f;
+        }
+        if (gone[0] || gone[1]) {
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (!gone[g]) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[g][nt][e] = -INFINITY;
+            unit[g][nt][0] = unit[g][nt][1] = 1.f;
+          }
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
