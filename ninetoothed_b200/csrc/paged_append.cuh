@@ -260,7 +260,7 @@ __device__ __forceinline__ void rotate_queries(const Params &p, uint32_t block) 
   } else {
     const int64_t position = position_of();
     if (!valid || position < rotary::kNone) return;
-    const bool known = position >= 0 && position < p.tables.rows;
+    const bool known = p.tables.pairs == 0 || (position >= 0 && position < p.tables.rows);
     if (!known) record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
     const T *in = static_cast<const T *>(q.input) + token * q.in_token + (int64_t)r * q.in_head;
     T *out = static_cast<T *>(q.output) + token * q.out_token + (int64_t)r * q.out_head;
@@ -548,8 +548,8 @@ extern "C" int nt_b200_paged_append(const NtB200PagedAppendArgs *a, void *stream
   if (rc != 0) return rc;
   const bool turns = a->cos != nullptr;
   if (turns && (!a->sin || a->rotary_dim > c.head_dim)) return NT_B200_ERR_SHAPE_MISMATCH;
-  if (!a->key || !a->value || !a->offsets || !a->past || !a->block_table || (a->query && (!turns || !a->query_out)) ||
-      a->tokens > (1 << 30) || a->batch > (1 << 28) || a->heads > (1 << 20) || a->table_columns > (1LL << 31))
+  if (!a->key || !a->value || !a->offsets || !a->past || !a->block_table ||
+      (a->query && ((!turns && a->rotary_dim > 0) || !a->query_out)) || a->tokens > (1 << 30) || a->batch > (1 << 28) || a->heads > (1 << 20) || a->table_columns > (1LL << 31))
     return NT_B200_ERR_INVALID_ARGUMENT;
   if (c.kv_heads == 0 && !a->query) return 0;
   paged::Params p{};

@@ -1,0 +1,37 @@
+"""paged_append at the edges of its arguments: tables without columns."""
+
+import pytest
+import torch
+
+from ninetoothed_b200 import _lib, device_status, programs
+from tests.test_serving_gpu import index
+
+pytestmark = pytest.mark.gpu
+
+
+def empty_cache(pages, kv_heads=2, page=16, dim=32):
+    caches = [torch.zeros(pages, kv_heads, page, dim, dtype=torch.int8, device="cuda") for _ in range(2)]
+    return *caches, *(torch.zeros(pages, kv_heads, device="cuda") for _ in range(2))
+
+
+@pytest.fixture(params=(True, False), ids=("binding", "python"))
+def path(request, monkeypatch):
+    if not request.param:
+        monkeypatch.setattr(_lib, "binding", lambda: None)
+
+
+@pytest.mark.parametrize("dim", (32, 48))
+@pytest.mark.parametrize("spread", (False, True))
+def test_tables_without_columns_copy_the_query(path, dim, spread):
+    """No rotated pairs: the query and the stored key are as they came, wherever the tokens stand."""
+    q, k = torch.randn(20, 4, dim).half().cuda(), torch.randn(20, 2, dim).half().cuda()
+    if spread:  # strides off the vector grid
+        q = torch.stack((q, q), dim=-1)[..., 0]
+    none = torch.zeros(3, 0, device="cuda")  # rows: fewer than tokens
+    cache, plain = empty_cache(2, dim=dim), empty_cache(2, dim=dim)
+    where = index([0, 20]), index([0]), index([[1, 0]])
+    query, key = programs.paged_append(k, k, *where, *cache, query=q, cos=none, sin=none, return_key=True)
+    programs.paged_append(k, k, *where, *plain)
+    assert device_status() == 0
+    assert torch.equal(query, q) and torch.equal(key, k)
+    assert all(torch.equal(a, b) for a, b in zip(cache, plain))
