@@ -67,7 +67,8 @@ at::Tensor like(const at::Tensor &t) { return at::empty(t.sizes(), t.options());
 
 bool good_tables(const at::Tensor &cos, const at::Tensor &sin, int64_t dim) {
   return cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat && cos.sizes() == sin.sizes() &&
-         2 * cos.size(1) <= dim && (cos.size(1) <= 1 || (cos.stride(1) == 1 && sin.stride(1) == 1));
+         2 * cos.size(1) <= dim && (cos.size(0) > 0 || cos.size(1) == 0) &&
+         (cos.size(1) <= 1 || (cos.stride(1) == 1 && sin.stride(1) == 1));
 }
 
 bool cache_of(Call &call, PyObject *const *o, NtB200PagedCache &c) {

@@ -195,6 +195,9 @@ def _launch_paged_append(v, stream):
         raise TypeError("Kernel arguments `cos`, `sin` must be given together.")
     if turns:
         _check_tables(v, dim)
+        if tokens and cos.shape[1] and not cos.shape[0]:
+            # their address is null, which would mean that nothing is rotated
+            raise TypeError("Kernel arguments `cos`, `sin` have no rows: every position is outside them.")
     if query is not None:
         check_same_dtype(v, ("key", "query"))
         if not turns or query_out is None:

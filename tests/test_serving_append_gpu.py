@@ -1,4 +1,4 @@
-"""paged_append at the edges of its arguments: tables without columns."""
+"""paged_append at the edges of its arguments: tables without columns or rows."""
 
 import pytest
 import torch
@@ -35,3 +35,13 @@ def test_tables_without_columns_copy_the_query(path, dim, spread):
     assert device_status() == 0
     assert torch.equal(query, q) and torch.equal(key, k)
     assert all(torch.equal(a, b) for a, b in zip(cache, plain))
+
+
+def test_tables_without_rows_are_refused(path):
+    """Every position is outside them: nothing may be stored as if there were no tables."""
+    k = torch.randn(3, 2, 32).half().cuda()
+    none = torch.zeros(0, 16, device="cuda")
+    cache = empty_cache(1)
+    with pytest.raises(TypeError, match="row"):
+        programs.paged_append(k, k, index([0, 3]), index([0]), index([[0]]), *cache, cos=none, sin=none)
+    assert not any(t.any() for t in cache)
