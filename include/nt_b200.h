@@ -300,7 +300,8 @@ int nt_b200_jagged_expand(void *values, const int64_t *offsets, int64_t batch, i
  * the device, all of one call in one dtype, INT32 or INT64 (`index_dtype`).
  * The kernels check every index they read: one that leaves its array records
  * NT_B200_ERR_INDEX_OUT_OF_RANGE in the device error word
- * (nt_b200_device_status) and is not followed.
+ * (nt_b200_device_status) and is not followed; offsets out of order record it
+ * too, and leave out some or all tokens of the call.
  */
 
 /*

@@ -126,6 +126,16 @@ struct Params {
   int interleaved;
 };
 
+// Where offsets are out of order the search can miss sequences, and with them
+// tokens.  The grid's last block looks for that and does nothing else (in the
+// others it took a step of 32 sequences from 3.9 to 4.2 us).
+__device__ __forceinline__ bool checks_order(const Params &p) {
+  if (blockIdx.x != gridDim.x - 1) return false;
+  for (int64_t i = threadIdx.x; i < p.batch; i += blockDim.x)
+    if (p.offsets[i + 1] < p.offsets[i]) record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
+  return true;
+}
+
 struct Unit {
   int64_t token0;    // packed index of the first new token in the page
   int64_t position0; // its position in the sequence
@@ -289,6 +299,7 @@ template <typename T, typename C>
 __global__ void __launch_bounds__(THREADS, 8) append_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) float4 kept[];  // [KEPT][chunk pair / 4][THREADS]
   __shared__ float shared[THREADS / 32];
+  if (checks_order(p)) return;
   if (blockIdx.x >= p.unit_blocks) {
     rotate_queries<T, true>(p, blockIdx.x - p.unit_blocks);
     return;
@@ -422,6 +433,7 @@ __global__ void __launch_bounds__(THREADS, 8) append_kernel(const __grid_constan
 template <typename T, typename C>
 __global__ void __launch_bounds__(THREADS) append_scalar_kernel(const __grid_constant__ Params p) {
   __shared__ float shared[THREADS / 32];
+  if (checks_order(p)) return;
   if (blockIdx.x >= p.unit_blocks) {
     rotate_queries<T, false>(p, blockIdx.x - p.unit_blocks);
     return;
@@ -510,7 +522,7 @@ int launch_append(Params p, cudaStream_t stream) {
   while (p.team_warps < THREADS / 32 && p.team_warps * 32 * KEPT < p.page * p.chunk_pairs) p.team_warps *= 2;
   const int teams = vec ? THREADS / 32 / p.team_warps : 1;
   p.groups = (uint32_t)((2 * p.kv_heads + teams - 1) / teams);
-  const int64_t units = p.units * p.groups, blocks = units + (threads + THREADS - 1) / THREADS;
+  const int64_t units = p.units * p.groups, blocks = units + (threads + THREADS - 1) / THREADS + 1;
   if (blocks > (1LL << 31) - 1 || threads >= (1LL << 32)) return NT_B200_ERR_INVALID_ARGUMENT;
   p.unit_blocks = (uint32_t)units;
   const dim3 grid((unsigned)blocks);

@@ -10,7 +10,8 @@ through `libnt_b200.so`.
 Index tensors (positions, offsets, past, lengths, block_table) are int32 or
 int64 CUDA tensors, one dtype a call.  Their values are checked by the kernels:
 an index outside its array is not followed and shows in
-`ninetoothed_b200.device_status()` as NT_B200_ERR_INDEX_OUT_OF_RANGE.
+`ninetoothed_b200.device_status()` as NT_B200_ERR_INDEX_OUT_OF_RANGE.  So do
+offsets out of order, with which some or all tokens of the call are left out.
 """
 
 import math

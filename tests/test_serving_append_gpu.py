@@ -1,10 +1,10 @@
-"""paged_append at the edges of its arguments: tables without columns or rows."""
+"""paged_append at the edges of its arguments: tables without columns or rows, offsets out of order."""
 
 import pytest
 import torch
 
 from ninetoothed_b200 import _lib, device_status, programs
-from tests.test_serving_gpu import index
+from tests.test_serving_gpu import INDEX_OUT_OF_RANGE, index
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +45,20 @@ def test_tables_without_rows_are_refused(path):
     with pytest.raises(TypeError, match="row"):
         programs.paged_append(k, k, index([0, 3]), index([0]), index([[0]]), *cache, cos=none, sin=none)
     assert not any(t.any() for t in cache)
+
+
+@pytest.mark.parametrize("batch, step", ((3, 40), (80, 5)))
+def test_offsets_out_of_order_are_recorded(batch, step):
+    """A step back by more than two pages hides a sequence from the search by candidates."""
+    k = torch.randn(400, 2, 32).half().cuda()
+    good = [step * i for i in range(batch + 1)]
+    table = index([[8 * s + c for c in range(8)] for s in range(batch)])  # 128 tokens each
+    past = index([0] * batch)
+    programs.paged_append(k, k, index(good), past, table, *empty_cache(8 * batch))
+    assert device_status() == 0
+    for at, value in ((1, 100), (batch - 1, good[-1] - 120), (batch, 0)):
+        offsets = list(good)
+        offsets[at] = value
+        assert any(a > b for a, b in zip(offsets, offsets[1:])) and max(b - a for a, b in zip(offsets, offsets[1:])) <= 128
+        programs.paged_append(k, k, index(offsets), past, table, *empty_cache(8 * batch))
+        assert device_status() == INDEX_OUT_OF_RANGE, (at, value)
