@@ -90,10 +90,20 @@ bool cache_of(Call &call, PyObject *const *o, NtB200PagedCache &c) {
 
 PyObject *none() { Py_RETURN_NONE; }
 
+// Whether an object has a truth value, and which.  One that has none is an odd
+// call too: Python's own path raises for it.
+bool flag(PyObject *o, bool &value) {
+  const int truth = PyObject_IsTrue(o);
+  if (truth < 0) PyErr_Clear();
+  value = truth > 0;
+  return truth >= 0;
+}
+
 // rotary(input, cos, sin, positions, interleaved, adjoint)
 PyObject *rotary(PyObject *, PyObject *const *o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 6 || !rotary_entry) return none();
+  bool interleaved, adjoint;
+  if (n != 6 || !rotary_entry || !flag(o[4], interleaved) || !flag(o[5], adjoint)) return none();
   Call call;
   const at::Tensor &x = call.tensor(o[0], 3), &cos = call.tensor(o[1], 2), &sin = call.tensor(o[2], 2);
   const at::Tensor &at = call.tensor(o[3], 1);
@@ -107,7 +117,7 @@ PyObject *rotary(PyObject *, PyObject *const *o, Py_ssize_t n) {
   a.tokens = x.size(0); a.heads = x.size(1); a.head_dim = x.size(2); a.rotary_dim = 2 * cos.size(1); a.table_rows = cos.size(0);
   strides(x, a.input_strides); strides(out, a.output_strides);
   a.cos_stride = cos.stride(0); a.sin_stride = sin.stride(0); a.positions_stride = at.stride(0);
-  a.interleaved = PyObject_IsTrue(o[4]); a.adjoint = PyObject_IsTrue(o[5]);
+  a.interleaved = interleaved; a.adjoint = adjoint;
   a.dtype = code_of(x); a.index_dtype = code_of(at);
   const int code = rotary_entry(&a, call.stream());
   return code ? PyLong_FromLong(code) : THPVariable_Wrap(out);
@@ -118,7 +128,8 @@ PyObject *rotary(PyObject *, PyObject *const *o, Py_ssize_t n) {
 // key_scale, value_scale, query, cos, sin, interleaved, return_key)
 PyObject *paged_append(PyObject *, PyObject *const *o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 14 || !append_entry) return none();
+  bool interleaved, return_key;
+  if (n != 14 || !append_entry || !flag(o[12], interleaved) || !flag(o[13], return_key)) return none();
   Call call;
   const bool asks = o[9] != Py_None, turns = o[10] != Py_None;
   if (turns != (o[11] != Py_None) || (asks && !turns)) return none();
@@ -145,7 +156,7 @@ PyObject *paged_append(PyObject *, PyObject *const *o, Py_ssize_t n) {
     a.query = q.data_ptr(); a.query_out = query_out.data_ptr(); a.heads = q.size(1);
     strides(q, a.query_strides); strides(query_out, a.query_out_strides);
   }
-  if (PyObject_IsTrue(o[13])) {
+  if (return_key) {
     key_out = like(k);
     a.key_out = key_out.data_ptr();
     strides(key_out, a.key_out_strides);
@@ -155,7 +166,7 @@ PyObject *paged_append(PyObject *, PyObject *const *o, Py_ssize_t n) {
   a.tokens = k.size(0); a.batch = past.size(0); a.table_columns = table.size(1);
   strides(k, a.key_strides); strides(v, a.value_strides); strides(table, a.block_table_strides);
   a.offsets_stride = offsets.stride(0); a.past_stride = past.stride(0);
-  a.interleaved = PyObject_IsTrue(o[12]); a.dtype = code_of(k); a.index_dtype = code_of(offsets);
+  a.interleaved = interleaved; a.dtype = code_of(k); a.index_dtype = code_of(offsets);
   const int code = append_entry(&a, call.stream());
   if (code) return PyLong_FromLong(code);
   PyObject *q = asks ? THPVariable_Wrap(query_out) : Py_NewRef(Py_None);
@@ -191,7 +202,8 @@ PyObject *with_lse(const at::Tensor &out, const at::Tensor &lse) {
 // block_table, lengths, scale, return_lse)
 PyObject *paged_attention(PyObject *, PyObject *const *o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 9 || !paged_entry) return none();
+  bool return_lse;
+  if (n != 9 || !paged_entry || !flag(o[8], return_lse)) return none();
   Call call;
   const at::Tensor &q = call.tensor(o[0], 4), &table = call.tensor(o[5], 2), &lengths = call.tensor(o[6], 1);
   NtB200PagedAttentionArgs a{};
@@ -200,7 +212,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *o, Py_ssize_t n) {
       lengths.size(0) != q.size(0) || table.size(0) != q.size(0) || !scale_of(o[7], q.size(3), a.scale))
     return none();
   at::Tensor out = like(q), lse;
-  if (PyObject_IsTrue(o[8])) {
+  if (return_lse) {
     lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
     a.lse = static_cast<float *>(lse.data_ptr());
     strides(lse, a.lse_strides);
@@ -221,7 +233,8 @@ PyObject *paged_attention(PyObject *, PyObject *const *o, Py_ssize_t n) {
 // return_lse)
 PyObject *prompt_attention(PyObject *, PyObject *const *o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 8 || !prompt_entry) return none();
+  bool is_causal, return_lse;
+  if (n != 8 || !prompt_entry || !flag(o[5], is_causal) || !flag(o[7], return_lse)) return none();
   Call call;
   const at::Tensor &q = call.tensor(o[0], 3), &k = call.tensor(o[1], 3), &v = call.tensor(o[2], 3);
   const at::Tensor &qo = call.tensor(o[3], 1), &ko = call.tensor(o[4], 1);
@@ -232,7 +245,7 @@ PyObject *prompt_attention(PyObject *, PyObject *const *o, Py_ssize_t n) {
       ko.sizes() != qo.sizes() || !scale_of(o[6], q.size(2), a.scale))
     return none();
   at::Tensor out = like(q), lse;
-  if (PyObject_IsTrue(o[7])) {
+  if (return_lse) {
     lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
     a.lse = static_cast<float *>(lse.data_ptr());
     strides(lse, a.lse_strides);
@@ -246,7 +259,7 @@ PyObject *prompt_attention(PyObject *, PyObject *const *o, Py_ssize_t n) {
   a.output = out.data_ptr(); a.workspace = workspace.data_ptr();
   strides(q, a.query_strides); strides(k, a.key_strides); strides(v, a.value_strides); strides(out, a.output_strides);
   a.query_offsets_stride = qo.stride(0); a.key_offsets_stride = ko.stride(0);
-  a.is_causal = PyObject_IsTrue(o[5]); a.dtype = code_of(q); a.index_dtype = code_of(qo);
+  a.is_causal = is_causal; a.dtype = code_of(q); a.index_dtype = code_of(qo);
   const int code = prompt_entry(&a, call.stream());
   return code ? PyLong_FromLong(code) : with_lse(out, lse);
   END_HANDLE_TH_ERRORS
