@@ -5,20 +5,22 @@ family), compiled with `-gencode arch=compute_100a,code=sm_100a`.  It links only
 the CUDA runtime; the TMA tensor-map encoder is fetched from the driver at run
 time with `cudaGetDriverEntryPoint`, so no `-lcuda` is needed.
 
-Beside it, `_binding.so` (`csrc/binding.cpp`, g++ against torch's headers) binds
-the serving operators' calls in C++; without it they take their Python path.
+Beside it, a binding (`csrc/binding.cpp`, g++ against torch's headers) makes the
+serving operators' calls in C++; without it they take their Python path.  It is
+good for the Python and the torch that it was compiled against alone, and its
+file's name says which.
 """
 
 import os
 import shutil
 import subprocess
+import sys
 import sysconfig
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
 SOURCE_DIR = PACKAGE_DIR / "csrc"
 LIBRARY = PACKAGE_DIR / "libnt_b200.so"
-BINDING = PACKAGE_DIR / "_binding.so"
 BINDING_SOURCE = SOURCE_DIR / "binding.cpp"
 MAIN_SOURCE = SOURCE_DIR / "nt_b200.cu"
 INCLUDE_DIR = PACKAGE_DIR.parent / "include"
@@ -66,8 +68,16 @@ def _older(built: Path, paths) -> bool:
     return not built.is_file() or any(path.stat().st_mtime > built.stat().st_mtime for path in paths)
 
 
+def binding_path() -> Path:
+    """The binding's file for this Python and this torch."""
+    import torch
+
+    build = (getattr(torch.version, "git_version", None) or "")[:8]
+    return PACKAGE_DIR / f"_binding.{sys.implementation.cache_tag}-torch-{torch.__version__}-{build}.so"
+
+
 def binding_is_stale() -> bool:
-    return _older(BINDING, [BINDING_SOURCE, *INCLUDE_DIR.glob("*.h"), Path(__file__).resolve()])
+    return _older(binding_path(), [BINDING_SOURCE, *INCLUDE_DIR.glob("*.h"), Path(__file__).resolve()])
 
 
 def is_stale(library: Path = LIBRARY) -> bool:
@@ -80,7 +90,8 @@ def build_binding(verbose: bool = False) -> Path:
 
     root = Path(torch.__file__).resolve().parent
     cuda = Path(find_nvcc()).resolve().parent.parent
-    temporary = BINDING.with_name(f".{BINDING.name}.{os.getpid()}.tmp")
+    binding = binding_path()
+    temporary = binding.with_name(f".{binding.name}.{os.getpid()}.tmp")
     command = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden"]
     command += [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
     command += [f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include", f"-I{cuda}/include"]
@@ -90,11 +101,11 @@ def build_binding(verbose: bool = False) -> Path:
         print(" ".join(command))
     try:
         subprocess.run(command, check=True)
-        os.replace(temporary, BINDING)
+        os.replace(temporary, binding)
     finally:
         if temporary.exists():
             temporary.unlink()
-    return BINDING
+    return binding
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:

@@ -11,9 +11,12 @@ with an error that says how to build it.
 """
 
 import ctypes
+import importlib.util
 import struct
 import threading
 from pathlib import Path
+
+from ninetoothed_b200 import _build
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "libnt_b200.so"
 
@@ -135,17 +138,30 @@ def library():
 _binding = None  # the C++ binding; False: there is none
 
 
+def _load_binding():
+    path = _build.binding_path()
+    if not path.is_file():
+        return None
+    spec = importlib.util.spec_from_file_location("ninetoothed_b200._binding", path)
+    try:
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+    except ImportError:
+        return None
+    return module
+
+
 def binding():
     """The serving operators' calls in C++ (csrc/binding.cpp), bound to the
-    library once per process, or None where the binding is not built."""
+    library once per process, or None where there is none built for this Python
+    and this torch."""
     global _binding
     if _binding is None:
         lib = library()
         with _lock:
             if _binding is None:
-                try:
-                    from ninetoothed_b200 import _binding as module
-                except ImportError:
+                module = _load_binding()
+                if module is None:
                     _binding = False
                 else:
                     names = ("rotary", "paged_append", "paged_attention", "prompt_attention",
