@@ -16,6 +16,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -108,13 +109,8 @@ def build_binding(verbose: bool = False) -> Path:
     return binding
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the library and the binding where they are missing or older than
-    their sources."""
-    if force or binding_is_stale():
-        build_binding(verbose)
-    if not force and not _older(LIBRARY, sources()):
-        return LIBRARY
+def build_library(verbose: bool = False) -> Path:
+    """Compile the library."""
     temporary = LIBRARY.with_name(f".{LIBRARY.name}.{os.getpid()}.tmp")
     command = [find_nvcc(), *NVCC_FLAGS]
     if verbose:
@@ -126,6 +122,20 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     finally:
         if temporary.exists():
             temporary.unlink()
+    return LIBRARY
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the library and the binding where they are missing or older than
+    their sources.  A binding that cannot be compiled is a warning: its calls take
+    their Python path."""
+    if force or _older(LIBRARY, sources()):
+        build_library(verbose)
+    if force or binding_is_stale():
+        try:
+            build_binding(verbose)
+        except (OSError, subprocess.CalledProcessError) as error:
+            warnings.warn(f"the C++ binding of the serving calls was not built: {error}", stacklevel=2)
     return LIBRARY
 
 
