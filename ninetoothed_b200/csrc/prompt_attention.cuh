@@ -657,6 +657,13 @@ __device__ __noinline__ void give_back(T *out, int64_t stride, int head_dim, con
   }
 }
 
+// A row's maximum moves only when a block passes it by 2^kLead, so that O is
+// rescaled rarely; P, up to 2^kLead, keeps its relative precision (bfloat16: 8
+// bits, float16: 11, to which it is rounded for the MMA).  float16: P has to stay
+// in its range, and values of up to 65504 cannot bring O out of fp32's.  bfloat16:
+// values can, so the lead that adds to them is kept small (2^24 took as long).
+template <typename T> constexpr float kLead = Elem<T>::is_f16 ? 14.f : 8.f;
+
 template <typename T, int DP, bool AGAIN>
 __device__ __forceinline__ void attend(const Control<DP> &c, uint32_t tmem_base, const Params &prm, const ushort2 *rows,
                                        Standing &at) {
@@ -717,9 +724,7 @@ __device__ __forceinline__ void attend(const Control<DP> &c, uint32_t tmem_base,
 #pragma unroll
         for (int v = 0; v < u; ++v) top[v] = fmaxf(top[v], top[v + u]);
       const float block_top = top[0] * scale;
-      // the maximum moves only when a block passes it by 2^14 (bf16: 2^24):
-      // P stays in its type's range and O is rescaled rarely
-      const bool move = block_top > m + tc::attn::RescaleLog2<T>::value;
+      const bool move = block_top > m + kLead<T>;
       const float m_new = move ? block_top : m;
       const float alpha = move ? exp2_fast(m - m_new) : 1.f;
       const float ref = reference(m_new);
