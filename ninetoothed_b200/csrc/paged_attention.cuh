@@ -37,9 +37,12 @@
 // waits for another warp.
 //
 // Codes become fp16 (exact for both types).  A query row is scaled by a power
-// of two to a largest element in [1, 2), so that bfloat16 rows fit too; P is
-// rounded to fp16 relative to the largest weight value_scale * p of its row, so
-// neither scales far apart nor a long tail lose bits that count.
+// of two to a largest element in [2^14, 2^15): bfloat16 rows fit, and elements
+// down to 2^-28 of the largest keep all their bits (scaled to [1, 2), elements
+// beside an outlier of 60000 lost theirs).  P is rounded to fp16 (11 bits; the
+// MMA takes its two operands in one type, and the codes are in fp16) relative to
+// the largest weight value_scale * p of its row, so neither scales far apart nor a
+// long tail lose bits that count.
 #pragma once
 
 #include <type_traits>
@@ -165,6 +168,7 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(Attention a) {
 
 // ---------------------------------------------------------------- tensor cores
 constexpr int STEP = 32;
+constexpr int Q_TOP = 14;  // a query row's largest element, as a power of two
 // Steps of a CTA at least: fewer would be parts to join rather than work.  One
 // sequence of 1023 e4m3 tokens, 8 key/value heads of 128: 14.6 us at 2, 13.9 at 4,
 // 15.4 at 6.
@@ -790,7 +794,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
       for (int e = 0; e < DP / 4; ++e) top = fmaxf(top, fabsf(x[e]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      int exponent = (int)(__float_as_uint(top) >> 23);  // biased; subnormal and zero rows as 2^-126
+      int exponent = (int)(__float_as_uint(top) >> 23) - Q_TOP;  // biased, of the power
       exponent = exponent < 1 ? 1 : exponent > 253 ? 253 : exponent;
       q_unit[nt] = __uint_as_float((uint32_t)exponent << 23);
       // with the softmax scale's sign, so that a larger score is a larger weight
