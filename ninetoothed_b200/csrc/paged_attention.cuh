@@ -401,14 +401,26 @@ __device__ __forceinline__ uint16_t element_bits(float x, int bf16) {
   return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x)) : __half_as_ushort(__float2half_rn(x));
 }
 
-// N neighbouring elements of a finished row: o = acc * 2^(mo - m) / l, and the
+// The maxima that P is taken against move only when a score passes them by LEAD
+// (base 2): a step's scores are compared in their own threads, and the reduction
+// over the threads of a row and the rescaling of O happen rarely.  P is kept RISE
+// above them, so that its largest, 2^(LEAD + RISE), stays in fp16's range and what
+// a long tail adds does not fall among fp16's subnormals: tokens with 2^-25.5 of
+// the largest weight were lost in the share that holds it at (8, 0), 15 % of what
+// 65536 of them give.
+constexpr float LEAD = 6.f, RISE = 9.f;
+// A lane's sum of weights goes over to a second one every FAR_STEPS steps: beside
+// a weight of 1, weights of 2^-25 and less added one by one are lost.
+constexpr int FAR_STEPS = 64;
+
+// N neighbouring elements of a finished row: o = acc * 2^(mo - RISE - m) / l, and the
 // row's lse.
 template <int N>
 __device__ __forceinline__ void write_row(const Attention &a, int64_t b, int h, int row, int d, const float (&acc)[N],
                                           float m, float l, float mo) {
   if (row >= a.rows || d >= a.head_dim) return;
   const int i = row / a.group, hq = h * a.group + row % a.group;
-  const float f = l == 0.f ? 0.f : exp2_fast(reference(mo) - reference(m)) / l;
+  const float f = l == 0.f ? 0.f : exp2_fast(reference(mo) - RISE - reference(m)) / l;
   uint16_t *out = static_cast<uint16_t *>(a.out) + b * a.o_batch + i * a.o_token + (int64_t)hq * a.o_head + d * a.o_dim;
   if (a.o_dim == 1 && (reinterpret_cast<uintptr_t>(out) & (2 * N - 1)) == 0) {
     struct alignas(2 * N < 16 ? 2 * N : 16) Pack { uint16_t v[N]; } pack;
@@ -500,12 +512,6 @@ __device__ __forceinline__ bool arrive(unsigned long long *counter, unsigned lon
   *reinterpret_cast<volatile unsigned long long *>(counter) = 0;
   return true;
 }
-
-// The maxima that P is taken against move only when a score passes them by
-// this (base 2): P, up to 2^LEAD, stays in fp16's range and as precise, a step's
-// scores are compared in their own threads, and the reduction over the threads
-// of a row and the rescaling of O happen rarely.
-constexpr float LEAD = 8.f;
 
 // Joins a unit's parts and writes its rows; a warp of the block takes a row.
 // (This runs once a call, mostly from a cold instruction cache: small code.)
@@ -808,7 +814,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
     }
     // of the rows 2 c4 and 2 c4 + 1 of each tile: score factor, maxima, sum,
     // keys seen
-    float factor[NT][2], m[NT][2], mo[NT][2], l[NT][2];
+    float factor[NT][2], m[NT][2], mo[NT][2], l[NT][2], l_far[NT][2];
     int limit[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -817,7 +823,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
         factor[nt][u] = fabsf(a.scale) * __shfl_sync(0xffffffffu, q_unit[nt], (2 * c4 + u) * 4);
         limit[nt][u] = seg.length - a.queries + 1 + (row0 + nt * 8 + 2 * c4 + u) / a.group;
         m[nt][u] = mo[nt][u] = -INFINITY;
-        l[nt][u] = 0.f;
+        l[nt][u] = l_far[nt][u] = 0.f;
       }
     const int sure = seg.length - a.queries + 1 + row0 / a.group;  // keys that every row sees
     float o[NT][OT][4] = {};
@@ -905,7 +911,9 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
               top_o = fmaxf(top_o, __shfl_xor_sync(0xffffffffu, top_o, x));
             }
             const float m_new = fmaxf(m[nt][u], top), mo_new = fmaxf(mo[nt][u], top_o);
-            l[nt][u] *= exp2_fast(m[nt][u] - reference(m_new));
+            const float fade = exp2_fast(m[nt][u] - reference(m_new));
+            l[nt][u] *= fade;
+            l_far[nt][u] *= fade;
             const float alpha = exp2_fast(mo[nt][u] - reference(mo_new));
             m[nt][u] = m_new;
             mo[nt][u] = mo_new;
@@ -920,7 +928,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float r0 = reference(m[nt][0]), r1 = reference(m[nt][1]);
-        const float w0 = reference(mo[nt][0]), w1 = reference(mo[nt][1]);
+        const float w0 = reference(mo[nt][0]) - RISE, w1 = reference(mo[nt][1]) - RISE;
 #pragma unroll
         for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -963,14 +971,25 @@ __global__ void __launch_bounds__(Layout<DP, NT>::WARPS * 32, 1) attention_kerne
       load_values(at + 1);
       next_step();
       at ^= 2;
+      if (step % FAR_STEPS == FAR_STEPS - 1) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            l_far[nt][u] += l[nt][u];
+            l[nt][u] = 0.f;
+          }
+      }
     }
 
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u) {
+        l[nt][u] += l_far[nt][u];
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[nt][u] += __shfl_xor_sync(0xffffffffu, l[nt][u], x);
+      }
     if (seg.s0 == 0 && seg.s1 == seg.n) {  // a whole unit
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)

@@ -1,0 +1,41 @@
+"""One key that takes nearly all of the weight, and a long tail of equal values."""
+
+import math
+
+import pytest
+import torch
+
+from ninetoothed_b200 import device_status, programs
+from tests.test_serving_gpu import index
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dim", (64, 128))
+@pytest.mark.parametrize("queries", (1, 12))
+def test_tail_of_a_paged_sequence(dim, queries):
+    """65536 tokens with 2^-25.5 of the first one's weight, which is all that has a
+    value, in one warp's share (as many sequences as warps, all of the same pages)."""
+    length, page, batch = 65536, 4096, 2048 // queries
+    caches = [torch.zeros(length // page, 1, page, dim, dtype=torch.int8, device="cuda") for _ in range(2)]
+    caches[0][0, 0, 0, 0] = 64
+    caches[1].fill_(100)
+    caches[1][0, 0, 0] = 0
+    scales = [torch.full((length // page, 1), 1 / 64, device="cuda") for _ in range(2)]
+    query = torch.zeros(batch, queries, 1, dim, dtype=torch.float16, device="cuda")
+    query[..., 0] = 25.5
+    table = index([list(range(length // page))]).expand(batch, -1)
+    got, lse = programs.paged_attention(query, *caches, *scales, table, index([length] * batch), scale=math.log(2.0),
+                                        return_lse=True)
+    assert device_status() == 0
+    for i in (0, queries - 1):
+        n = length - queries + 1 + i
+        tail = (n - 1) * 2.0**-25.5
+        want = tail * 100 / 64 / (1 + tail)
+        # relative to the output: a tail weight that is kept 2^9 above the largest is
+        # 2^-16.5, where half a step of fp16 is 2^-25; 2 n / 32 sums of 16 terms, each
+        # off by two units in the last of 24 bits; the output's half step
+        limit = (2.0**-8.5 + 2 * n / 32 * 2.0**-22 + 2.0**-11) * want
+        assert float((got[:, i].double() - want).abs().max()) <= limit
+        # the lanes' sums: n / 8 terms, in blocks of 256, of which the first's tail is lost
+        assert float((lse[:, i].double() - math.log(1 + tail) - 25.5 * math.log(2.0)).abs().max()) <= 2.0**-16
