@@ -658,11 +658,14 @@ __device__ __noinline__ void give_back(T *out, int64_t stride, int head_dim, con
 }
 
 // A row's maximum moves only when a block passes it by 2^kLead, so that O is
-// rescaled rarely; P, up to 2^kLead, keeps its relative precision (bfloat16: 8
-// bits, float16: 11, to which it is rounded for the MMA).  float16: P has to stay
-// in its range, and values of up to 65504 cannot bring O out of fp32's.  bfloat16:
-// values can, so the lead that adds to them is kept small (2^24 took as long).
-template <typename T> constexpr float kLead = Elem<T>::is_f16 ? 14.f : 8.f;
+// rescaled rarely, and P is kept 2^kRise above it.  P is rounded to the operands'
+// type for the MMA, 8 bits (bfloat16) or 11 (float16).  float16: its largest, 2^15,
+// stays in range, and what a long tail adds out of the subnormals: of 131072 keys
+// with 2^-25.5 of the largest weight all was lost at (14, 0); values of up to 65504
+// cannot bring O out of fp32's range.  bfloat16: values can, so the lead that adds
+// to them is kept small (2^24 took as long), and its range needs no rise.
+template <typename T> constexpr float kLead = Elem<T>::is_f16 ? 6.f : 8.f;
+template <typename T> constexpr float kRise = Elem<T>::is_f16 ? 9.f : 0.f;
 
 template <typename T, int DP, bool AGAIN>
 __device__ __forceinline__ void attend(const Control<DP> &c, uint32_t tmem_base, const Params &prm, const ushort2 *rows,
@@ -727,7 +730,7 @@ __device__ __forceinline__ void attend(const Control<DP> &c, uint32_t tmem_base,
       const bool move = block_top > m + kLead<T>;
       const float m_new = move ? block_top : m;
       const float alpha = move ? exp2_fast(m - m_new) : 1.f;
-      const float ref = reference(m_new);
+      const float ref = reference(m_new) - kRise<T>;
       float sum[8] = {};
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -798,7 +801,7 @@ __device__ __forceinline__ void attend(const Control<DP> &c, uint32_t tmem_base,
           if (x < p.head_dim) out[x * p.o_dim] = from_f<T>(__uint_as_float(o[x]) * f);
       }
       if (p.lse)
-        p.lse[token * p.l_token + (int64_t)head * p.l_head] = l == 0.f ? -INFINITY : (m + log2_fast(l)) * kLn2;
+        p.lse[token * p.l_token + (int64_t)head * p.l_head] = l == 0.f ? -INFINITY : (m - kRise<T> + log2_fast(l)) * kLn2;
       if (!AGAIN) {
         float worst[8] = {};  // a sum is NaN if any element is NaN or infinite
 #pragma unroll

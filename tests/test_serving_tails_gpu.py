@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from ninetoothed_b200 import device_status, programs
-from tests.test_serving_gpu import index
+from tests.test_serving_gpu import HALF, index
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +39,27 @@ def test_tail_of_a_paged_sequence(dim, queries):
         assert float((got[:, i].double() - want).abs().max()) <= limit
         # the lanes' sums: n / 8 terms, in blocks of 256, of which the first's tail is lost
         assert float((lse[:, i].double() - math.log(1 + tail) - 25.5 * math.log(2.0)).abs().max()) <= 2.0**-16
+
+
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+@pytest.mark.parametrize("dim", (64, 128))
+def test_tail_of_a_prompt(dim, dtype):
+    """The same over the last four queries of 131072 keys."""
+    length, queries = 131072, 4
+    q = torch.zeros(queries, 2, dim, dtype=dtype, device="cuda")
+    q[..., 0] = 25.5
+    k, v = torch.zeros(length, 1, dim), torch.full((length, 1, dim), 100 / 64)
+    k[0, 0, 0], v[0] = 1.0, 0.0
+    got, lse = programs.prompt_attention(q, k.to(dtype).cuda(), v.to(dtype).cuda(), index([0, queries]), index([0, length]),
+                                         scale=math.log(2.0), return_lse=True)
+    assert device_status() == 0
+    for i in range(queries):
+        n = length - queries + 1 + i
+        tail = (n - 1) * 2.0**-25.5
+        want = tail * 100 / 64 / (1 + tail)
+        # as above; bfloat16 weights keep 8 bits wherever they are
+        half = 2.0**-8.5 if dtype == torch.float16 else 2.0**-9
+        limit = (half + n / 16 * 2.0**-22 + HALF[dtype]) * want
+        assert float((got[i].double() - want).abs().max()) <= limit
+        # n / 128 blocks are added to the sum one by one
+        assert float((lse[i].double() - math.log(1 + tail) - 25.5 * math.log(2.0)).abs().max()) <= 2.0**-14 + 2.0**-18
