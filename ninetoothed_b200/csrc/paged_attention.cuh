@@ -113,7 +113,9 @@ __device__ __forceinline__ int page_of(const Attention &a, int64_t b, int64_t co
 
 // ---------------------------------------------------------------- any type
 // A warp a query row: head elements dealt over the lanes, one key at a time.
-constexpr int kMostDim = 256;
+// Every FAR_KEYS keys the sums go over to others: beside a weight of 1, what weights
+// of 2^-25 and less add one by one is lost.
+constexpr int kMostDim = 256, FAR_KEYS = 256;
 template <typename T, typename C>
 __global__ void __launch_bounds__(128) attention_rows_kernel(Attention a) {
   const int lane = threadIdx.x & 31;
@@ -124,15 +126,15 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(Attention a) {
   const int64_t limit = cached_length(a, b) - a.queries + 1 + i;
   const T *q = static_cast<const T *>(a.query) + b * a.q_batch + i * a.q_token + h * a.q_head;
   constexpr int E = kMostDim / 32;
-  float qv[E], acc[E];
+  float qv[E], acc[E], far[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int d = lane + 32 * e;
     qv[e] = d < a.head_dim ? to_f(q[d * a.q_dim]) : 0.f;
-    acc[e] = 0.f;
+    acc[e] = far[e] = 0.f;
   }
   const int g = h / a.group;
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f, l_far = 0.f;
   for (int64_t t = 0; t < limit; ++t) {
     const int id = page_of(a, b, t / a.page);
     if (id < 0) {
@@ -149,19 +151,38 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(Attention a) {
     for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
     const float s = dot * (a.scale * a.key_scale[id * a.ks_page + g * a.ks_head]);
     const float vs = a.value_scale[id * a.vs_page + g * a.vs_head];
-    const float m_new = fmaxf(m, s);
-    const float alpha = exp2f(m - reference(m_new)), p = exp2f(s - reference(m_new));
-    l = l * alpha + p;
+    if (s > m) {
+      const float alpha = exp2f(m - s);
+      m = s;
+      l *= alpha;
+      l_far *= alpha;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        acc[e] *= alpha;
+        far[e] *= alpha;
+      }
+    }
+    const float p = exp2f(s - reference(m));
+    l += p;
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      if (lane + 32 * e < a.head_dim) acc[e] = fmaf(p, decode<C>(v[lane + 32 * e]) * vs, acc[e] * alpha);
-    m = m_new;
+      if (lane + 32 * e < a.head_dim) acc[e] = fmaf(p, decode<C>(v[lane + 32 * e]) * vs, acc[e]);
+    if (t % FAR_KEYS == FAR_KEYS - 1) {
+      l_far += l;
+      l = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        far[e] += acc[e];
+        acc[e] = 0.f;
+      }
+    }
   }
+  l += l_far;
   T *out = static_cast<T *>(a.out) + b * a.o_batch + i * a.o_token + h * a.o_head;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int d = lane + 32 * e;
-    if (d < a.head_dim) out[d * a.o_dim] = from_f<T>(l == 0.f ? 0.f : acc[e] / l);
+    if (d < a.head_dim) out[d * a.o_dim] = from_f<T>(l == 0.f ? 0.f : (acc[e] + far[e]) / l);
   }
   if (a.lse && lane == 0) a.lse[b * a.l_batch + i * a.l_token + h * a.l_head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }

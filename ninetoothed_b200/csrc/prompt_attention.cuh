@@ -92,14 +92,14 @@ __global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ Probl
   const T *q = static_cast<const T *>(p.q) + token * p.q_token + h * p.q_head;
   const int g = h / p.group;
   constexpr int E = kMostDim / 32;
-  float qv[E], acc[E];
+  float qv[E], acc[E], far[E];  // (sums in two levels, as in the paged kernel)
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int d = lane + 32 * e;
     qv[e] = d < p.head_dim ? to_f(q[d * p.q_dim]) : 0.f;
-    acc[e] = 0.f;
+    acc[e] = far[e] = 0.f;
   }
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f, l_far = 0.f;
   for (int64_t t = 0; t < limit; ++t) {
     const T *k = static_cast<const T *>(p.k) + (k0 + t) * p.k_token + g * p.k_head;
     const T *v = static_cast<const T *>(p.v) + (k0 + t) * p.v_token + g * p.v_head;
@@ -109,19 +109,39 @@ __global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ Probl
       if (lane + 32 * e < p.head_dim) dot = fmaf(qv[e], to_f(k[(lane + 32 * e) * p.k_dim]), dot);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    const float s = dot * p.scale, m_new = fmaxf(m, s);
-    const float alpha = exp2f(m - reference(m_new)), w = exp2f(s - reference(m_new));
-    l = l * alpha + w;
+    const float s = dot * p.scale;
+    if (s > m) {
+      const float alpha = exp2f(m - s);
+      m = s;
+      l *= alpha;
+      l_far *= alpha;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        acc[e] *= alpha;
+        far[e] *= alpha;
+      }
+    }
+    const float w = exp2f(s - reference(m));
+    l += w;
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      if (lane + 32 * e < p.head_dim) acc[e] = fmaf(w, to_f(v[(lane + 32 * e) * p.v_dim]), acc[e] * alpha);
-    m = m_new;
+      if (lane + 32 * e < p.head_dim) acc[e] = fmaf(w, to_f(v[(lane + 32 * e) * p.v_dim]), acc[e]);
+    if (t % paged::FAR_KEYS == paged::FAR_KEYS - 1) {
+      l_far += l;
+      l = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        far[e] += acc[e];
+        acc[e] = 0.f;
+      }
+    }
   }
+  l += l_far;
   T *out = static_cast<T *>(p.o) + token * p.o_token + h * p.o_head;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int d = lane + 32 * e;
-    if (d < p.head_dim) out[d * p.o_dim] = from_f<T>(limit > 0 ? acc[e] / l : 0.f);
+    if (d < p.head_dim) out[d * p.o_dim] = from_f<T>(limit > 0 ? (acc[e] + far[e]) / l : 0.f);
   }
   if (p.lse && lane == 0) p.lse[token * p.l_token + h * p.l_head] = limit > 0 ? (m + log2f(l)) * kLn2 : -INFINITY;
 }

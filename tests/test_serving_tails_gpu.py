@@ -63,3 +63,32 @@ def test_tail_of_a_prompt(dim, dtype):
         assert float((got[i].double() - want).abs().max()) <= limit
         # n / 128 blocks are added to the sum one by one
         assert float((lse[i].double() - math.log(1 + tail) - 25.5 * math.log(2.0)).abs().max()) <= 2.0**-14 + 2.0**-18
+
+
+@pytest.mark.parametrize("dim", (64, 160))
+@pytest.mark.parametrize("paged", (True, False))
+def test_tail_in_float32(paged, dim):
+    """On CUDA cores, with a value at the first key too: a thread's sums go over to
+    others every 256 keys."""
+    n = 65536
+    q = torch.zeros(1, 1, 2, dim, device="cuda")
+    q[..., 0] = 25.5
+    if paged:
+        caches = [torch.zeros(n // 4096, 1, 4096, dim, dtype=torch.int8, device="cuda") for _ in range(2)]
+        caches[0][0, 0, 0, 0] = 64
+        caches[1].fill_(100)
+        caches[1][0, 0, 0] = 1
+        scales = [torch.full((n // 4096, 1), 1 / 64, device="cuda") for _ in range(2)]
+        got, lse = programs.paged_attention(q, *caches, *scales, index([list(range(n // 4096))]), index([n]),
+                                            scale=math.log(2.0), return_lse=True)
+    else:
+        k, v = torch.zeros(n, 1, dim, device="cuda"), torch.full((n, 1, dim), 100 / 64, device="cuda")
+        k[0, 0, 0], v[0] = 1.0, 1 / 64
+        got, lse = programs.prompt_attention(q[0], k, v, index([0, 1]), index([0, n]), scale=math.log(2.0), return_lse=True)
+    assert device_status() == 0
+    tail = (n - 1) * 2.0**-25.5
+    want = (1 / 64 + tail * 100 / 64) / (1 + tail)
+    # 256 terms, then n / 256 sums; scores of 25.5 in base 2 with a few roundings, in each weight
+    weight = (256 + n / 256) * 2.0**-24 + 8 * 2.0**-24 * 25.5
+    assert float((got.double() - want).abs().max()) <= 2 * weight * want
+    assert float((lse.double() - math.log(1 + tail) - 25.5 * math.log(2.0)).abs().max()) <= weight + 2.0**-19
