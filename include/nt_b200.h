@@ -351,6 +351,8 @@ typedef struct NtB200PagedCache {
  * nt_b200_rotary at those positions before they are stored, and, where given,
  * `query` [tokens, heads, head_dim] is rotated into `query_out` and the rotated
  * key stored in `key_out` in `dtype`.  A query needs tables unless rotary_dim is 0.
+ * Tokens that belong to no sequence are written in neither, nor keys that an index
+ * out of range keeps from the cache.
  *
  * Scales.  With amax the largest finite magnitude among a page's new elements
  * of a head: E4M3 codes: s = the least power of two, 2^-126 or more, with

