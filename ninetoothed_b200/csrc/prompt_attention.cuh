@@ -686,6 +686,7 @@ __device__ __noinline__ void give_back(T *out, int64_t stride, int head_dim, con
 // to them is kept small (2^24 took as long), and its range needs no rise.
 template <typename T> constexpr float kLead = Elem<T>::is_f16 ? 6.f : 8.f;
 template <typename T> constexpr float kRise = Elem<T>::is_f16 ? 9.f : 0.f;
+template <typename T> constexpr float kFall = Elem<T>::is_f16 ? 1.f / 512.f : 1.f;  // 2^-kRise
 
 template <typename T, int DP, bool AGAIN>
 __device__ __forceinline__ void attend(const Control<DP> &c, uint32_t tmem_base, const Params &prm, const ushort2 *rows,
@@ -821,7 +822,7 @@ __device__ __forceinline__ void attend(const Control<DP> &c, uint32_t tmem_base,
           if (x < p.head_dim) out[x * p.o_dim] = from_f<T>(__uint_as_float(o[x]) * f);
       }
       if (p.lse)
-        p.lse[token * p.l_token + (int64_t)head * p.l_head] = l == 0.f ? -INFINITY : (m - kRise<T> + log2_fast(l)) * kLn2;
+        p.lse[token * p.l_token + (int64_t)head * p.l_head] = l == 0.f ? -INFINITY : (m + log2_fast(l * kFall<T>)) * kLn2;
       if (!AGAIN) {
         float worst[8] = {};  // a sum is NaN if any element is NaN or infinite
 #pragma unroll

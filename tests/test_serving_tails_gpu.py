@@ -92,3 +92,14 @@ def test_tail_in_float32(paged, dim):
     weight = (256 + n / 256) * 2.0**-24 + 8 * 2.0**-24 * 25.5
     assert float((got.double() - want).abs().max()) <= 2 * weight * want
     assert float((lse.double() - math.log(1 + tail) - 25.5 * math.log(2.0)).abs().max()) <= weight + 2.0**-19
+
+
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+def test_lse_of_one_key_is_its_score(dtype):
+    """However small: what P is kept above the maximum does not show."""
+    q, k = (torch.randn(200, 1, 64).to(dtype).cuda() * 0.1 for _ in range(2))
+    _, lse = programs.prompt_attention(q, k, k, index(list(range(201))), return_lse=True)
+    score = (q.double() * k.double()).sum(-1) / 8
+    # 64 exact products added in fp32, a factor of a few roundings
+    limit = 72 * 2.0**-24 * (q.double() * k.double()).abs().sum(-1) / 8
+    assert device_status() == 0 and ((lse.double() - score).abs() <= limit).all()
