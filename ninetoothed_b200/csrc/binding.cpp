@@ -60,6 +60,17 @@ bool is_float(const at::Tensor &t) {
 }
 bool is_index(const at::Tensor &t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
 
+// Lets other Python threads run: allocations and launches can wait for the device
+// (a full launch queue), and what they wait for may need the interpreter.
+struct Released {
+  PyThreadState *state = PyEval_SaveThread();
+  void reset() {
+    if (state) PyEval_RestoreThread(state);
+    state = nullptr;
+  }
+  ~Released() { reset(); }
+};
+
 template <int N> void strides(const at::Tensor &t, int64_t (&to)[N]) {
   for (int i = 0; i < N; ++i) to[i] = t.stride(i);
 }
@@ -110,6 +121,7 @@ PyObject *rotary(PyObject *, PyObject *const *o, Py_ssize_t n) {
   if (!call.good || !is_float(x) || !is_index(at) || at.size(0) != x.size(0) || x.numel() == 0 ||
       !good_tables(cos, sin, x.size(2)))
     return none();
+  Released released;
   at::Tensor out = like(x);
   NtB200RotaryArgs a{};
   a.input = x.data_ptr(); a.output = out.data_ptr(); a.positions = at.data_ptr();
@@ -120,6 +132,7 @@ PyObject *rotary(PyObject *, PyObject *const *o, Py_ssize_t n) {
   a.interleaved = interleaved; a.adjoint = adjoint;
   a.dtype = code_of(x); a.index_dtype = code_of(at);
   const int code = rotary_entry(&a, call.stream());
+  released.reset();
   return code ? PyLong_FromLong(code) : THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
@@ -142,6 +155,7 @@ PyObject *paged_append(PyObject *, PyObject *const *o, Py_ssize_t n) {
       offsets.size(0) != past.size(0) + 1 || table.size(0) != past.size(0))
     return none();
   at::Tensor query_out, key_out;
+  const at::Tensor *query = nullptr;
   if (turns) {
     const at::Tensor &cos = call.tensor(o[10], 2), &sin = call.tensor(o[11], 2);
     if (!call.good || !good_tables(cos, sin, k.size(2))) return none();
@@ -152,9 +166,13 @@ PyObject *paged_append(PyObject *, PyObject *const *o, Py_ssize_t n) {
   if (asks) {
     const at::Tensor &q = call.tensor(o[9], 3);
     if (!call.good || q.scalar_type() != k.scalar_type() || q.size(0) != k.size(0) || q.size(2) != k.size(2)) return none();
-    query_out = like(q);
-    a.query = q.data_ptr(); a.query_out = query_out.data_ptr(); a.heads = q.size(1);
-    strides(q, a.query_strides); strides(query_out, a.query_out_strides);
+    query = &q;
+  }
+  Released released;
+  if (query) {
+    query_out = like(*query);
+    a.query = query->data_ptr(); a.query_out = query_out.data_ptr(); a.heads = query->size(1);
+    strides(*query, a.query_strides); strides(query_out, a.query_out_strides);
   }
   if (return_key) {
     key_out = like(k);
@@ -168,6 +186,7 @@ PyObject *paged_append(PyObject *, PyObject *const *o, Py_ssize_t n) {
   a.offsets_stride = offsets.stride(0); a.past_stride = past.stride(0);
   a.interleaved = interleaved; a.dtype = code_of(k); a.index_dtype = code_of(offsets);
   const int code = append_entry(&a, call.stream());
+  released.reset();
   if (code) return PyLong_FromLong(code);
   PyObject *q = asks ? THPVariable_Wrap(query_out) : Py_NewRef(Py_None);
   PyObject *r = a.key_out ? THPVariable_Wrap(key_out) : Py_NewRef(Py_None);
@@ -211,6 +230,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *o, Py_ssize_t n) {
       q.size(2) % a.cache.kv_heads || !is_index(lengths) || table.scalar_type() != lengths.scalar_type() ||
       lengths.size(0) != q.size(0) || table.size(0) != q.size(0) || !scale_of(o[7], q.size(3), a.scale))
     return none();
+  Released released;
   at::Tensor out = like(q), lse;
   if (return_lse) {
     lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
@@ -225,6 +245,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *o, Py_ssize_t n) {
   strides(q, a.query_strides); strides(out, a.output_strides); strides(table, a.block_table_strides);
   a.lengths_stride = lengths.stride(0); a.dtype = code_of(q); a.index_dtype = code_of(lengths);
   const int code = paged_entry(&a, call.stream());
+  released.reset();
   return code ? PyLong_FromLong(code) : with_lse(out, lse);
   END_HANDLE_TH_ERRORS
 }
@@ -244,6 +265,7 @@ PyObject *prompt_attention(PyObject *, PyObject *const *o, Py_ssize_t n) {
       q.size(1) % k.size(1) || !is_index(qo) || ko.scalar_type() != qo.scalar_type() || qo.size(0) < 1 ||
       ko.sizes() != qo.sizes() || !scale_of(o[6], q.size(2), a.scale))
     return none();
+  Released released;
   at::Tensor out = like(q), lse;
   if (return_lse) {
     lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
@@ -261,6 +283,7 @@ PyObject *prompt_attention(PyObject *, PyObject *const *o, Py_ssize_t n) {
   a.query_offsets_stride = qo.stride(0); a.key_offsets_stride = ko.stride(0);
   a.is_causal = is_causal; a.dtype = code_of(q); a.index_dtype = code_of(qo);
   const int code = prompt_entry(&a, call.stream());
+  released.reset();
   return code ? PyLong_FromLong(code) : with_lse(out, lse);
   END_HANDLE_TH_ERRORS
 }
