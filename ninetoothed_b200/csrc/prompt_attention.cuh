@@ -307,7 +307,7 @@ struct Layout {
   static constexpr int ROWS_OFF = CTRL_OFF + 384;  // ushort2 [BM]: a row's query and head in its tile
   static constexpr int NOTES_OFF = ROWS_OFF + BM * 4;  // uint32 [2][128], see take_out
   static constexpr int SMEM_BYTES = NOTES_OFF + 2 * 128 * 4;
-  static_assert(96 + 16 * RING + 16 <= 240, "barrier slots");
+  static_assert(120 + 16 * RING <= 240, "barrier slots");
   static_assert(SMEM_BYTES <= 232448, "shared memory of a CTA");
 };
 
@@ -449,6 +449,8 @@ template <int DP> struct Control {
   // of items, two in turn: the notes of a second pass are complete; handed over;
   // taken by the MMA issuer and the softmax warps
   NT_BARRIER item_clean(int s) const { return ctrl + 96 + 16u * RING + 8u * s; }
+  // after a wait gave up: the MMAs in flight are done
+  NT_BARRIER settled() const { return ctrl + 112 + 16u * RING; }
   NT_BARRIER item_full(int s) const { return ctrl + 248 + 8u * s; }
   NT_BARRIER item_empty(int s) const { return ctrl + 264 + 8u * s; }
 #undef NT_BARRIER
@@ -848,7 +850,7 @@ __device__ __forceinline__ void attend(const Control<DP> &c, uint32_t tmem_base,
 // code it took registers and time from the first (packed prompts of up to 2048
 // tokens: 147 us beside 139).
 template <typename T, int DP>
-__device__ __noinline__ void second_pass(uint8_t *smem, uint32_t tmem_base, const Params &prm, const CUtensorMap *tmap_q,
+__device__ __noinline__ Standing second_pass(uint8_t *smem, uint32_t tmem_base, const Params &prm, const CUtensorMap *tmap_q,
                                          const CUtensorMap *tmap_k, const CUtensorMap *tmap_v, Standing at) {
   const Control<DP> c(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -864,6 +866,24 @@ __device__ __noinline__ void second_pass(uint8_t *smem, uint32_t tmem_base, cons
     issue<T, DP, true>(c, tmem_base, prm, at);
   } else {
     attend<T, DP, true>(c, tmem_base, prm, reinterpret_cast<const ushort2 *>(smem + Layout<DP>::ROWS_OFF), at);
+  }
+  return at;
+}
+
+// After a wait gave up: the copies and MMAs that a thread has in flight, so that the
+// CTA's shared and tensor memory are at rest when it ends.
+template <int DP> __device__ __noinline__ void settle(uint8_t *smem, Standing at) {
+  constexpr uint64_t limit_ns = 1000000000ull;
+  const Control<DP> c(smem);
+  volatile int over = 0;
+  if (threadIdx.x == 0) {
+    for (int r = max(at.r - RING, 0); r < at.r; ++r)
+      ptx::mbar_wait(c.slot_full(r % RING), (uint32_t)(r / RING) & 1u, &over, limit_ns);
+    for (int t = 0; t < TILES; ++t)
+      if (at.used[t] > 0) ptx::mbar_wait(c.q_full(t), (uint32_t)(at.used[t] - 1) & 1u, &over, limit_ns);
+  } else if (threadIdx.x == 32) {
+    ptx::mma_commit(c.settled());
+    ptx::mbar_wait(c.settled(), 0, &over, limit_ns);
   }
 }
 
@@ -901,6 +921,7 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       ptx::mbar_init(c.slot_full(s), 1);
       ptx::mbar_init(c.slot_empty(s), 1);
     }
+    ptx::mbar_init(c.settled(), 1);
     *c.abort_flag = 0;
     *c.again = kEnd;
     ptx::fence_mbar_init();
@@ -939,8 +960,12 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
   __syncthreads();
   if (*c.again != kEnd && !*c.abort_flag) {
     ptx::tc_fence_after();
-    second_pass<T, DP>(smem, tmem_base, prm, &tmap_q, &tmap_k, &tmap_v, at);
+    at = second_pass<T, DP>(smem, tmem_base, prm, &tmap_q, &tmap_k, &tmap_v, at);
     ptx::tc_fence_before();
+    __syncthreads();
+  }
+  if (*c.abort_flag) {
+    settle<DP>(smem, at);
     __syncthreads();
   }
   if (warp == 1) {
