@@ -48,8 +48,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 }
 
 // Wall-clock bound of any single wait.  The longest legitimate wait is one
-// output tile's main loop (tens of microseconds), so this only ends waits that
-// would never complete.
+// output tile's main loop (tens of microseconds; for an attention tile about a
+// microsecond per 128 keys), so this only ends waits that would never complete.
 constexpr uint64_t kWaitLimitNs = 4000000000ull;
 
 // Waits until the barrier's phase with the given parity has completed.
