@@ -438,6 +438,55 @@ int nt_b200_prompt_attention(const NtB200PromptAttentionArgs *args, void *stream
 int64_t nt_b200_prompt_attention_workspace_size(int64_t query_tokens, int64_t batch, int64_t heads, int64_t kv_heads);
 
 /*
+ * Root-mean-square norm of the rows of `input` [rows, width], after the addition
+ * of `residual` where it is not null: t = input + residual, rounded to `dtype` and
+ * stored in `total` (which may be `residual` or `input`), or t = input; y = (t * r)
+ * * weight with r = 1 / sqrt(mean(t^2) + eps).  The mean and its root are taken in
+ * 64 bits and r is rounded to fp32, as is each product.  weight: [width], of
+ * weight_dtype, `dtype` or FLOAT32.  output_dtype = dtype: output = round(y), and it
+ * may be `input`.  output_dtype FLOAT8_E4M3FN or INT8: codes round(y * (1 / s)) with
+ * one fp32 scale s in `scale` [rows, ceil(width / group)] for each `group` elements
+ * of a row (the last group may be shorter), by the rules of a paged cache's pages
+ * (nt_b200_paged_append).  `group`: the width or more, or a multiple of 16; width at
+ * most 131072.  dtype: FLOAT16, BFLOAT16, FLOAT32.
+ */
+typedef struct NtB200RmsNormArgs {
+    const void *input, *residual, *weight; /* residual may be null */
+    void *output, *total;                  /* total: with a residual */
+    float *scale;                          /* with codes */
+    int64_t rows, width, group;
+    int64_t input_strides[2], residual_strides[2], weight_stride, output_strides[2], total_strides[2],
+        scale_strides[2]; /* row, element */
+    int64_t dtype, weight_dtype, output_dtype;
+    double eps;
+} NtB200RmsNormArgs;
+int nt_b200_rms_norm(const NtB200RmsNormArgs *args, void *stream);
+
+/*
+ * output[m, n] = input_scale[m] * sum_k input[m, k] (q[n, k] - z[n, k / group])
+ * scales[n, k / group] for input [rows, inner] and 4-bit weights q, two a byte of
+ * `codes` [outer, inner / 2], the even k in the low half.  z = 8 where `zeros` is
+ * null, else the low four bits of zeros (uint8) [outer, inner / group]; scales
+ * [outer, inner / group] of scales_dtype; input_scale (fp32, [rows]) may be null.
+ * `group` is a multiple of 32 and divides inner.  Products and sums are fp32, the
+ * result is rounded once to output_dtype.  dtype: FLOAT16, BFLOAT16, FLOAT32,
+ * FLOAT8_E4M3FN or INT8; scales and output: FLOAT16, BFLOAT16, FLOAT32.  Tensor
+ * cores take all but FLOAT32 inputs where element strides are 1, rows of input and
+ * codes (and both bases) on the 16-byte grid and the bases of scales and zeros on
+ * the 4-byte one; the rest runs on CUDA cores.
+ */
+typedef struct NtB200Int4MatmulArgs {
+    const void *input, *codes, *scales, *zeros; /* zeros may be null */
+    const float *input_scale;                   /* or null */
+    void *output;
+    int64_t rows, inner, outer, group;
+    int64_t input_strides[2], codes_strides[2], scales_strides[2], zeros_strides[2], input_scale_stride,
+        output_strides[2];
+    int64_t dtype, scales_dtype, output_dtype;
+} NtB200Int4MatmulArgs;
+int nt_b200_int4_matmul(const NtB200Int4MatmulArgs *args, void *stream);
+
+/*
  * Failure-detection self-test (no counterpart in the reference): launches one
  * thread that waits on an mbarrier nothing ever arrives on, through the same
  * bounded wait the pipelined kernels use, with a limit of `limit_ns`

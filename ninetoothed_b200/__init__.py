@@ -15,12 +15,15 @@ from ninetoothed_b200.programs import (
     attention,
     conv2d,
     dropout,
+    int4_matmul,
+    int4_quantize,
     matmul,
     max_pool2d,
     paged_append,
     paged_attention,
     pow,
     prompt_attention,
+    rms_norm,
     rotary,
     rotary_tables,
     softmax,
@@ -36,6 +39,8 @@ __all__ = [
     "conv2d",
     "device_status",
     "dropout",
+    "int4_matmul",
+    "int4_quantize",
     "matmul",
     "max_pool2d",
     "paged_append",
@@ -43,6 +48,7 @@ __all__ = [
     "pow",
     "programs",
     "prompt_attention",
+    "rms_norm",
     "rotary",
     "rotary_tables",
     "softmax",

@@ -64,6 +64,10 @@ template <> struct Elem<__nv_fp8_e5m2> {
   static __device__ __forceinline__ float to_f(__nv_fp8_e5m2 v) { return static_cast<float>(v); }
   static __device__ __forceinline__ __nv_fp8_e5m2 from_f(float v) { return __nv_fp8_e5m2(v); }
 };
+template <> struct Elem<int8_t> {
+  static constexpr bool is_f16 = false;
+  static __device__ __forceinline__ float to_f(int8_t v) { return (float)v; }
+};
 
 template <typename T> __device__ __forceinline__ float to_f(T v) { return Elem<T>::to_f(v); }
 template <typename T> __device__ __forceinline__ T from_f(float v) { return Elem<T>::from_f(v); }

@@ -550,12 +550,17 @@ def copy(dst, src):
 
 # --------------------------------------------------------------------- serving operators
 from ninetoothed_b200.serving import (  # noqa: E402
+    int4_matmul,
+    int4_matmul_kernel,
+    int4_quantize,
     paged_append,
     paged_append_kernel,
     paged_attention,
     paged_attention_kernel,
     prompt_attention,
     prompt_attention_kernel,
+    rms_norm,
+    rms_norm_kernel,
     rotary,
     rotary_kernel,
     rotary_tables,
@@ -581,6 +586,9 @@ __all__ = [
     "conv2d_max_pool2d",
     "dropout",
     "dropout_kernel",
+    "int4_matmul",
+    "int4_matmul_kernel",
+    "int4_quantize",
     "matmul",
     "matmul_kernel",
     "max_pool2d",
@@ -594,6 +602,8 @@ __all__ = [
     "pow_kernel",
     "prompt_attention",
     "prompt_attention_kernel",
+    "rms_norm",
+    "rms_norm_kernel",
     "rotary",
     "rotary_kernel",
     "rotary_tables",

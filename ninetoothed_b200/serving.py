@@ -20,7 +20,7 @@ from operator import itemgetter
 import torch
 
 from ninetoothed_b200 import _lib
-from ninetoothed_b200.runtime import Kernel, KernelLaunchError, TensorArg, check_same_dtype, dtype_code
+from ninetoothed_b200.runtime import FLOAT_DTYPES, Kernel, KernelLaunchError, TensorArg, check_same_dtype, dtype_code
 
 INDEX_DTYPES = (torch.int32, torch.int64)
 CODE_DTYPES = (torch.float8_e4m3fn, torch.int8)
@@ -34,7 +34,10 @@ def _bound(name, *args):
     binding = _lib.binding()
     if binding is None:
         return None
-    result = getattr(binding, name)(*args)
+    call = getattr(binding, name, None)
+    if call is None:
+        return None
+    result = call(*args)
     if result.__class__ is int:
         raise KernelLaunchError(result)
     return result
@@ -435,15 +438,211 @@ def prompt_attention(query, key, value, offsets, key_offsets=None, is_causal=Tru
     return (output, lse) if return_lse else output
 
 
+# --------------------------------------------------------------------- norm
+_norm_values = itemgetter("input", "residual", "weight", "output", "total", "scale")
+
+
+def _launch_rms_norm(v, stream):
+    x, residual, weight, out, total, scale = _norm_values(v)
+    rows, width = x.shape
+    codes, group = out.dtype in CODE_DTYPES, v["group"]
+    if weight.dtype not in (x.dtype, torch.float32) or not (codes or out.dtype == x.dtype):
+        raise TypeError(
+            "rms_norm takes a weight of the input's dtype or float32, and an output of the input's dtype, "
+            "float8_e4m3fn or int8."
+        )
+    if weight.shape[0] != width or out.shape != x.shape:
+        raise TypeError(f"rms_norm shapes {tuple(x.shape)}, weight {tuple(weight.shape)} -> {tuple(out.shape)} disagree.")
+    if width > 131072:
+        raise TypeError("Kernel argument `input` has rows above the upper bound 131072.")
+    if (residual is None) != (total is None):
+        raise TypeError("Kernel arguments `residual`, `total` must be given together.")
+    if residual is not None:
+        check_same_dtype(v, ("input", "residual", "total"))
+        if residual.shape != x.shape or total.shape != x.shape:
+            raise TypeError("rms_norm residual and total must have the input's shape.")
+    if codes != (scale is not None):
+        raise TypeError("rms_norm needs `scale` with an 8-bit output, and with no other.")
+    if codes:
+        group = _norm_group(width, group)
+        if scale.shape != (rows, -(-width // group)):
+            raise TypeError(f"rms_norm scale must be {(rows, -(-width // group))}; got {tuple(scale.shape)}.")
+    elif group is not None:
+        raise TypeError("rms_norm has groups with an 8-bit output only.")
+    eps = float(v["eps"])
+    if not eps >= 0.0:
+        raise TypeError(f"rms_norm needs an eps of 0 or more; got {eps}.")
+    none2 = (0, 0)
+    args = _lib.pack_args(
+        x.data_ptr(), 0 if residual is None else residual.data_ptr(), weight.data_ptr(), out.data_ptr(),
+        0 if total is None else total.data_ptr(), 0 if scale is None else scale.data_ptr(), rows, width, group or width,
+        *x.stride(), *(none2 if residual is None else residual.stride()), weight.stride(0), *out.stride(),
+        *(none2 if total is None else total.stride()), *(none2 if scale is None else scale.stride()),
+        dtype_code(x.dtype), dtype_code(weight.dtype), dtype_code(out.dtype), scale=eps,
+    )
+    return _lib.library().nt_b200_rms_norm(args, stream)
+
+
+def _norm_group(width, group):
+    """Elements of a row that share a scale."""
+    if group is None or group >= width:
+        return max(width, 1)
+    if group <= 0 or group % 16:
+        raise TypeError(f"rms_norm needs groups of a multiple of 16 elements; got {group}.")
+    return int(group)
+
+
+rms_norm_kernel = Kernel(
+    name="rms_norm",
+    args=(
+        TensorArg("input", 2),
+        TensorArg("weight", 1),
+        TensorArg("output", 2, FLOAT_DTYPES + CODE_DTYPES),
+        TensorArg("residual", 2, optional=True),
+        TensorArg("total", 2, optional=True),
+        TensorArg("scale", 2, _F32, optional=True),
+    ),
+    outputs=("output",),
+    launch=_launch_rms_norm,
+    meta=("eps", "group"),
+    meta_defaults={"eps": 1e-6, "group": None, "residual": None, "total": None, "scale": None},
+)
+
+
+def rms_norm(input, weight, residual=None, eps=1e-6, code_dtype=None, group=None):
+    """Root-mean-square norm of the rows of `input` [rows, width]: with t = input
+    + residual (or input), t / sqrt(mean(t^2) + eps) * weight (`weight`: [width],
+    in the input's dtype or float32).
+
+    Returns the output in the input's dtype, or with `code_dtype` (float8_e4m3fn
+    or int8) two tensors: codes round(y / scale), and fp32 scales [rows, groups],
+    one for each `group` elements of a row (a multiple of 16; the last may be
+    shorter; one for the row by default).  E4M3 scales are the least power of two
+    that brings a group's largest element to 448 or less, int8 ones that element /
+    127.  With a `residual` the last of the outputs is the sum t in the input's
+    dtype, the next residual; the norm is that of t as it is stored."""
+    result = _bound("rms_norm", input, weight, residual, eps, code_dtype, group)
+    if result is not None:
+        return result
+    total = None if residual is None else torch.empty_like(input, memory_format=torch.contiguous_format)
+    output = torch.empty_like(input, dtype=code_dtype, memory_format=torch.contiguous_format)
+    scale = None
+    if code_dtype is not None:
+        rows, width = input.shape
+        scale = input.new_empty((rows, -(-width // _norm_group(width, group))), dtype=torch.float32)
+    rms_norm_kernel(input, weight, output, residual, total, scale, eps=eps, group=group)
+    outputs = (output,) + (() if scale is None else (scale,)) + (() if total is None else (total,))
+    return outputs if len(outputs) > 1 else output
+
+
+# --------------------------------------------------------------------- 4-bit weights
+def int4_quantize(weight, group=128, symmetric=True):
+    """4-bit weights for `int4_matmul` from `weight` [outer, inner]: (codes, scales,
+    zeros).  Each `group` elements of a row (a multiple of 32 that divides inner)
+    share a scale, in the weight's dtype, and without `symmetric` a zero point:
+    element = (code - zero) * scale with codes from 0 to 15; symmetric groups are
+    centred at 8 and have no zeros (None)."""
+    outer, inner = weight.shape
+    if group <= 0 or group % 32 or inner % group:
+        raise ValueError(f"group must be a multiple of 32 that divides {inner}; got {group}.")
+    w = weight.float().view(outer, -1, group) if weight.is_contiguous() else weight.float().reshape(outer, -1, group)
+    if symmetric:
+        scales = (w.abs().amax(dim=2) / 7).to(weight.dtype)
+        zero = torch.full_like(scales, 8, dtype=torch.float32)
+    else:
+        low, high = w.amin(dim=2).clamp(max=0), w.amax(dim=2).clamp(min=0)
+        scales = ((high - low) / 15).to(weight.dtype)
+        step = scales.float()
+        zero = torch.where(step > 0, torch.round(-low / step), 8.0).clamp(0, 15)
+    step = scales.float()[:, :, None]
+    codes = torch.where(step > 0, torch.round(w / step), 0.0).add_(zero[:, :, None]).clamp_(0, 15).to(torch.uint8)
+    codes = codes.view(outer, inner)
+    return codes[:, 0::2] | codes[:, 1::2] << 4, scales, None if symmetric else zero.to(torch.uint8)
+
+
+_int4_values = itemgetter("input", "codes", "scales", "output", "zeros", "input_scale")
+
+
+def _launch_int4_matmul(v, stream):
+    x, codes, scales, out, zeros, input_scale = _int4_values(v)
+    rows, inner = x.shape
+    outer, groups = scales.shape
+    if out.dtype != (scales.dtype if x.dtype in CODE_DTYPES else x.dtype):
+        raise TypeError("int4_matmul's output has the input's dtype, or the scales' where the input has 8 bits.")
+    if codes.shape != (outer, inner // 2) or out.shape != (rows, outer):
+        raise TypeError(
+            f"int4_matmul input {tuple(x.shape)}, codes {tuple(codes.shape)}, scales {tuple(scales.shape)} and output "
+            f"{tuple(out.shape)} disagree."
+        )
+    group = inner // groups if groups else 0
+    if not group or group * groups != inner or group % 32:
+        raise TypeError(f"int4_matmul needs groups of a multiple of 32 elements; got {groups} groups of {inner}.")
+    if zeros is not None and zeros.shape != scales.shape:
+        raise TypeError("int4_matmul zeros must have the scales' shape.")
+    if input_scale is not None and input_scale.shape != (rows,):
+        raise TypeError(f"int4_matmul needs one input scale for each of {rows} rows; got {tuple(input_scale.shape)}.")
+    none2 = (0, 0)
+    args = _lib.pack_args(
+        x.data_ptr(), codes.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(),
+        0 if input_scale is None else input_scale.data_ptr(), out.data_ptr(), rows, inner, outer, group, *x.stride(),
+        *codes.stride(), *scales.stride(), *(none2 if zeros is None else zeros.stride()),
+        0 if input_scale is None else input_scale.stride(0), *out.stride(), dtype_code(x.dtype),
+        dtype_code(scales.dtype), dtype_code(out.dtype),
+    )
+    return _lib.library().nt_b200_int4_matmul(args, stream)
+
+
+int4_matmul_kernel = Kernel(
+    name="int4_matmul",
+    args=(
+        TensorArg("input", 2, FLOAT_DTYPES + CODE_DTYPES),
+        TensorArg("codes", 2, (torch.uint8,)),
+        TensorArg("scales", 2),
+        TensorArg("output", 2),
+        TensorArg("zeros", 2, (torch.uint8,), optional=True),
+        TensorArg("input_scale", 1, _F32, optional=True),
+    ),
+    outputs=("output",),
+    launch=_launch_int4_matmul,
+    meta_defaults={"zeros": None, "input_scale": None},
+)
+
+
+def int4_matmul(input, codes, scales, zeros=None, input_scale=None):
+    """input [rows, inner] times the transpose of a matrix [outer, inner] of 4-bit
+    weights (code - zero) * scale: `codes` uint8 [outer, inner / 2], two a byte with
+    the even element in the low half; `scales` [outer, groups], each for inner /
+    groups neighbouring elements (a multiple of 32); `zeros` uint8 [outer, groups],
+    0 to 15, or 8 throughout (`int4_quantize` makes all three).  Made for the few
+    rows of a decoding step: every 32 rows read the weights once.
+
+    The input is float16, bfloat16 or float32, and so is the output; or
+    float8_e4m3fn or int8 with `input_scale` fp32 [rows] or [rows, 1] (`rms_norm`'s
+    codes with one scale a row), with an output in the scales' dtype."""
+    result = _bound("int4_matmul", input, codes, scales, zeros, input_scale)
+    if result is not None:
+        return result
+    if isinstance(input_scale, torch.Tensor) and input_scale.dim() == 2 and input_scale.shape[1] == 1:
+        input_scale = input_scale[:, 0]
+    dtype = scales.dtype if input.dtype in CODE_DTYPES else input.dtype
+    output = input.new_empty((input.shape[0], scales.shape[0]), dtype=dtype)
+    return int4_matmul_kernel(input, codes, scales, output, zeros, input_scale)
+
+
 __all__ = [
     "CODE_DTYPES",
     "INDEX_DTYPES",
+    "int4_matmul",
+    "int4_matmul_kernel",
+    "int4_quantize",
     "paged_append",
     "paged_append_kernel",
     "paged_attention",
     "paged_attention_kernel",
     "prompt_attention",
     "prompt_attention_kernel",
+    "rms_norm",
+    "rms_norm_kernel",
     "rotary",
     "rotary_kernel",
     "rotary_tables",
