@@ -438,6 +438,38 @@ int nt_b200_prompt_attention(const NtB200PromptAttentionArgs *args, void *stream
 int64_t nt_b200_prompt_attention_workspace_size(int64_t query_tokens, int64_t batch, int64_t heads, int64_t kv_heads);
 
 /*
+ * Causal attention of the next pieces of prompts, packed one after another, over a
+ * paged cache that holds them already: sequence b has the queries offsets[b] ..
+ * offsets[b+1] - 1 of `query` [tokens, heads, head_dim], the last of its lengths[b]
+ * cached tokens; query i of n sees the first lengths[b] - n + 1 + i of them.  Query
+ * head h reads key/value head h / (heads / kv_heads); nobody sees the tokens of a page
+ * outside the pool.  With s = scale * (q . k) over the tokens seen, output = softmax(s)
+ * v and, where `lse` is not null, lse [tokens, heads] = ln sum exp(s) (fp32); a query
+ * that sees nothing gets 0 and -inf.  Scores, softmax and sums are fp32; the cache's
+ * scales must not be negative.  FLOAT16 and BFLOAT16 queries run on tcgen05 tensor cores
+ * (probabilities rounded to fp16 there) for head_dim up to 128, up to 128 query heads to
+ * a key/value head and a positive scale; the rest, FLOAT32 and head_dim up to 256, on
+ * CUDA cores.  Tokens that belong to no sequence are not written, nor those of a sequence
+ * whose offsets are out of order or leave the tensors.  `workspace`: 16-byte aligned
+ * device memory of nt_b200_chunk_attention_workspace_size() bytes (the current
+ * device's), for this call alone.
+ */
+typedef struct NtB200ChunkAttentionArgs {
+    NtB200PagedCache cache;
+    const void *query, *offsets, *lengths, *block_table;
+    void *output;
+    float *lse;
+    void *workspace;
+    int64_t workspace_bytes, tokens, batch, heads, table_columns;
+    int64_t query_strides[3], output_strides[3], lse_strides[2]; /* token, head, element */
+    int64_t offsets_stride, lengths_stride, block_table_strides[2];
+    int64_t dtype, index_dtype;
+    double scale;
+} NtB200ChunkAttentionArgs;
+int nt_b200_chunk_attention(const NtB200ChunkAttentionArgs *args, void *stream);
+int64_t nt_b200_chunk_attention_workspace_size(void);
+
+/*
  * Root-mean-square norm of the rows of `input` [rows, width], after the addition
  * of `residual` where it is not null: t = input + residual, rounded to `dtype` and
  * stored in `total` (which may be `residual` or `input`), or t = input; y = (t * r)

@@ -13,6 +13,7 @@ from ninetoothed_b200.programs import (
     add,
     addmm,
     attention,
+    chunk_attention,
     conv2d,
     dropout,
     int4_matmul,
@@ -36,6 +37,7 @@ __all__ = [
     "add",
     "addmm",
     "attention",
+    "chunk_attention",
     "conv2d",
     "device_status",
     "dropout",

@@ -40,8 +40,6 @@ NVCC_FLAGS = (
     # them and launch its kernels without their shared-memory opt-in
     "-Xcompiler",
     "-fno-gnu-unique",
-    # the one translation unit's kernels are optimised on all cores
-    "-split-compile=0",
     "-shared",
 )
 

@@ -104,6 +104,8 @@ SIGNATURES = {
     "nt_b200_paged_attention_workspace_size": (ctypes.c_int64, ()),
     "nt_b200_prompt_attention": (ctypes.c_int, (_S, _P)),
     "nt_b200_prompt_attention_workspace_size": (ctypes.c_int64, (_I, _I, _I, _I)),
+    "nt_b200_chunk_attention": (ctypes.c_int, (_S, _P)),
+    "nt_b200_chunk_attention_workspace_size": (ctypes.c_int64, ()),
     "nt_b200_rms_norm": (ctypes.c_int, (_S, _P)),
     "nt_b200_int4_matmul": (ctypes.c_int, (_S, _P)),
 }

@@ -1,0 +1,1088 @@
+// Causal attention of the next pieces of prompts, packed one after another, over the
+// paged 8-bit cache that holds them already:
+//     s = (q . k_code) * (scale * key_scale[page]),  o = sum_j softmax(s)_j * value_scale[page_j] * v_code_j,
+//     lse = ln sum_j exp(s_j)
+// Sequence b has the queries offsets[b] .. offsets[b+1] - 1 and lengths[b] cached
+// tokens, its last query standing at the last of them.  A query that sees no token gets
+// o = 0 and lse = -inf.  All math is base 2 in fp32.
+//
+// Bound by the tensor cores and, level with them, by the exponentials (a block of 128
+// keys costs 256 rows 2048 cycles of either); short pieces by reading the cache once.
+//
+// Rows of a tile are (query, head of the group) pairs, so that all query heads of a
+// key/value head share one pass over its keys: 128 / group queries a tile.  A unit of
+// work is a key/value head and two tiles of 128 rows; its blocks of 128 keys, with
+// UNIT_STEPS more for its start and end, are steps of one line: sequence by sequence,
+// head by head.  The line is cut into equal pieces, one a CTA, so that any mix of
+// lengths keeps every SM busy to the end, and a few rows over many keys as well.  Where a
+// cut falls into a unit, its pieces leave (o, m, l) in a workspace and a second kernel
+// joins them, in the line's order.
+//
+// Persistent, one CTA an SM, 12 warps:
+//   warp 0      tensor memory, and the MMAs from one thread: S_t = Q_t K_j^T, O_t +=
+//               P_t V_j with P_t read from tensor memory;
+//   warps 1-3   read pages, turn codes into fp16 (exact for both types) and store them
+//               into a ring of 5 blocks as the MMAs read them;
+//   warps 4-11  softmax, 4 warps a tile, a thread a row; a unit's queries at its start.
+// Both operands are fp16: a query row is scaled by a power of two to a largest element in
+// [2^14, 2^15), which leaves elements down to 2^-28 of it all their bits, and P is rounded
+// to fp16 (11 bits) relative to the largest weight p * value_scale of its row, 2^9 above
+// it, so neither scales far apart nor a long tail lose bits that count.
+#pragma once
+
+#include "attention_tc.cuh"
+#include "common.cuh"
+#include "paged_attention.cuh"
+#include "prompt_attention.cuh"
+#include "ptx.cuh"
+
+namespace nt {
+namespace chunk {
+
+using paged::exp2_fast;
+using paged::kLn2;
+using paged::log2_fast;
+using paged::reference;
+using prompt::store_shared16;
+
+struct Problem : paged::Attention {
+  IndexArray offsets;
+  int64_t tokens;
+  int per_tile;  // queries of a tile
+  uint8_t *workspace;
+};
+
+constexpr int BM = 128, BN = 128, TILES = 2, ROWS = TILES * BM;  // rows of a tile, keys of a block
+// What a unit's start and end (its queries, its output) count in the line, in key
+// blocks; steps of a piece at least.
+constexpr int UNIT_STEPS = 3, LEAST_STEPS = 4;
+
+// ---------------------------------------------------------------- any layout
+// A warp a query row.
+template <typename T, typename C>
+__global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ Problem p) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= p.tokens * p.heads) return;
+  const int64_t token = row / p.heads;
+  const int h = (int)(row % p.heads);
+  const int64_t b = paged::warp_search(p.batch, token, [&](int64_t i) { return p.offsets[i]; });
+  const int64_t q0 = p.offsets[b], n = p.offsets[b + 1] - q0;
+  if (q0 < 0 || n < 0 || q0 + n > p.tokens) {
+    record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
+    return;
+  }
+  if (token < q0 || token >= q0 + n) return;
+  const T *q = static_cast<const T *>(p.query) + token * p.q_token + h * p.q_head;
+  T *out = static_cast<T *>(p.out) + token * p.o_token + h * p.o_head;
+  paged::attend_row<T, C>(p, b, h, paged::cached_length(p, b) - n + 1 + (token - q0), q, out,
+                          p.lse ? p.lse + token * p.l_token + h * p.l_head : nullptr);
+}
+
+// ---------------------------------------------------------------- the line
+// sum of floor((a i + b) / m) for i in [0, n), by the steps of Euclid's algorithm
+// (a, b >= 0): pairs of whole numbers under a line, counted again with the axes
+// exchanged.
+__device__ __forceinline__ int64_t floor_sum(int64_t n, int32_t m, int32_t a, int64_t b) {
+  int64_t sum = 0;
+  while (n > 0) {
+    sum += (n - 1) * n / 2 * (a / m);
+    a %= m;
+    sum += n * (b / m);
+    b %= m;
+    const int64_t top = a * n + b;
+    if (top < m) break;
+    n = top / m;
+    b = top % m;
+    const int32_t x = m;
+    m = a;
+    a = x;
+  }
+  return sum;
+}
+
+// Key blocks of a unit whose last query sees `seen` tokens: one at least.
+__device__ __forceinline__ int blocks_of(int seen) { return seen <= 0 ? 1 : (seen - 1) / BN + 1; }
+
+// A sequence: `pairs` units a head, of 2 * per_tile queries each.
+struct Sequence {
+  int32_t q0, n, length, pairs;
+  // false where the offsets are out of order or leave the tensors
+  __device__ __forceinline__ bool load(const Problem &p, int64_t b) {
+    const int64_t o0 = p.offsets[b], count = p.offsets[b + 1] - o0;
+    pairs = 0;
+    if (o0 < 0 || count < 0 || o0 + count > p.tokens) {
+      record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
+      return false;
+    }
+    q0 = (int32_t)o0;
+    n = (int32_t)count;
+    length = count > 0 ? paged::cached_length(p, b) : 0;
+    pairs = (int32_t)((count + 2 * p.per_tile - 1) / (2 * p.per_tile));
+    return true;
+  }
+  // tokens that the queries before `queries` see
+  __device__ __forceinline__ int seen(int queries) const { return length - n + queries; }
+  __device__ __forceinline__ int blocks(int pair, int i) const { return blocks_of(seen(min((i + 1) * pair, n))); }
+  // steps of a head's units before unit i, i < pairs, and of all
+  __device__ __forceinline__ int64_t before(int pair, int64_t i) const {
+    const int64_t start = (int64_t)length - n;
+    int64_t none = start < 0 ? -start / pair : 0;  // units that see nothing: one block
+    if (none > i) none = i;
+    return i * UNIT_STEPS + none + floor_sum(i - none, BN, pair, start + (none + 1) * pair + BN - 1);
+  }
+  __device__ __forceinline__ int64_t steps(int pair) const {
+    return before(pair, pairs - 1) + blocks(pair, pairs - 1) + UNIT_STEPS;
+  }
+};
+
+// A CTA's piece of the line, and where its first unit lies.
+struct Piece {
+  int64_t total, start, end;  // steps of the line; the piece
+  int64_t pos;                // of its first unit
+  int64_t batch;              // the unit
+  int32_t head, pair;
+  int32_t pieces;
+};
+
+// Where a role stands in its CTA's piece.  All lanes of a warp walk together; the
+// sequences come 32 at a time.
+struct Walk {
+  Sequence mine, seq;  // of lane i: sequence base + i; the current one
+  int64_t base, batch, pos;
+  int32_t head, pair;
+  __device__ __forceinline__ void window(const Problem &p, int64_t from) {
+    base = from;
+    mine.pairs = 0;
+    const int64_t b = from + (threadIdx.x & 31);
+    if (b < p.batch) mine.load(p, b);
+  }
+  __device__ __forceinline__ void take(int lane) {
+    seq.q0 = __shfl_sync(0xffffffffu, mine.q0, lane);
+    seq.n = __shfl_sync(0xffffffffu, mine.n, lane);
+    seq.length = __shfl_sync(0xffffffffu, mine.length, lane);
+    seq.pairs = __shfl_sync(0xffffffffu, mine.pairs, lane);
+  }
+  __device__ __forceinline__ void begin(const Problem &p, const Piece &piece) {
+    batch = piece.batch;
+    head = piece.head;
+    pair = piece.pair;
+    pos = piece.pos;
+    window(p, batch);
+    take(0);
+  }
+  __device__ __forceinline__ int blocks(const Problem &p) const { return seq.blocks(2 * p.per_tile, pair); }
+  // to the next unit; the caller stops at the piece's end, before the line's
+  __device__ __forceinline__ void next(const Problem &p) {
+    pos += blocks(p) + UNIT_STEPS;
+    if (++pair < seq.pairs) return;
+    pair = 0;
+    if (++head < p.kv_heads) return;
+    head = 0;
+    ++batch;
+    for (;;) {
+      const int at = (int)(batch - base);
+      const unsigned some = at < 32 ? __ballot_sync(0xffffffffu, mine.pairs > 0) >> at : 0u;
+      if (some) {
+        batch += __ffs(some) - 1;
+        take((int)(batch - base));
+        return;
+      }
+      batch = base + 32;
+      if (batch >= p.batch) {
+        seq.pairs = 0;
+        return;
+      }
+      window(p, batch);
+    }
+  }
+};
+
+// A unit's share of a piece.
+struct Item {
+  int32_t q0, queries;   // first packed query, how many (at most two tiles')
+  int32_t limit0, keys;  // keys that the first query sees (may be negative); of the sequence
+  int32_t batch, head;
+  int32_t from, until, blocks;  // the share's key blocks, of the unit's
+  int64_t end;                  // of the unit in the line
+  __device__ __forceinline__ Item(const Problem &p, const Piece &piece, const Walk &w) {
+    const int pair = 2 * p.per_tile, first = w.pair * pair;
+    q0 = w.seq.q0 + first;
+    queries = min(w.seq.n - first, pair);
+    limit0 = w.seq.length - w.seq.n + 1 + first;
+    keys = w.seq.length;
+    batch = (int32_t)w.batch;
+    head = w.head;
+    blocks = w.blocks(p);
+    end = w.pos + UNIT_STEPS + blocks;
+    from = (int32_t)min(max(piece.start - w.pos - UNIT_STEPS, (int64_t)0), (int64_t)blocks);
+    until = (int32_t)min(max(piece.end - w.pos - UNIT_STEPS, (int64_t)0), (int64_t)blocks);
+  }
+  // the share's end for tile t, whose rows may see fewer keys; `from` or less: none
+  __device__ __forceinline__ int until_of(int t, int per_tile) const {
+    const int last = min(queries, (t + 1) * per_tile) - 1;
+    if (last < t * per_tile) return 0;
+    return min(until, blocks_of(min(limit0 + last, keys)));
+  }
+  __device__ __forceinline__ bool whole() const { return from == 0 && until == blocks; }
+};
+// The items of a piece, all lanes of a warp together: f(item) is false where a wait
+// gave up.
+template <typename F>
+__device__ __forceinline__ void each_item(const Problem &p, const Piece &piece, F f) {
+  if (piece.start >= piece.end) return;
+  Walk w;
+  for (w.begin(p, piece); w.pos < piece.end && w.seq.pairs > 0; w.next(p)) {
+    const Item item(p, piece, w);
+    if (item.from < item.until && !f(item)) return;
+  }
+}
+
+// ---------------------------------------------------------------- shared memory, workspace
+constexpr int RING = 5, CONVERTERS = 3, SOFTMAX_WARPS = 8, WARPS = 1 + CONVERTERS + SOFTMAX_WARPS, THREADS = WARPS * 32;
+constexpr int GROUPS = BN / 16;  // of 16 tokens in a block: a page's or a part of one
+constexpr int TMEM_COLS = 512, SCALE_SLOTS = 4, NOTE_SLOTS = 3;
+
+// What a group's 16 keys share.
+struct alignas(16) GroupScale {
+  float key, add;           // s = raw * key * (the row's factor) + add (-inf: a page outside the pool)
+  float value, log2_value;  // the value scale
+};
+
+template <int DP>  // head_dim padded to 64 or 128
+struct Layout {
+  static constexpr int ATOMS = DP / 64;         // 128-byte swizzle atoms along the head
+  static constexpr int Q_BYTES = BM * DP * 2;   // one Q tile
+  static constexpr int KV_BYTES = BN * DP * 2;  // one key or value block
+  static constexpr int RING_OFF = TILES * Q_BYTES;
+  static constexpr int SCALE_OFF = RING_OFF + RING * KV_BYTES;
+  static constexpr int BAR_OFF = SCALE_OFF + SCALE_SLOTS * GROUPS * (int)sizeof(GroupScale);
+  static constexpr int PIECE_OFF = BAR_OFF + 256;
+  static constexpr int SCAN_OFF = PIECE_OFF + 64;                   // int64 [WARPS + 1]
+  static constexpr int STAMP_OFF = SCAN_OFF + 8 * (WARPS + 1);      // int [NOTE_SLOTS][CONVERTERS]
+  static constexpr int SMEM_BYTES = STAMP_OFF + 4 * NOTE_SLOTS * CONVERTERS;
+  static_assert(sizeof(Piece) <= 64, "the piece's place");
+  static_assert(SMEM_BYTES <= 232448, "shared memory of a CTA");
+  // a part in the workspace: o [DP / 4][ROWS] float4, then (m, l, mo) [ROWS] float4
+  static constexpr int64_t PART = (int64_t)ROWS * (DP + 4) * 4;
+};
+
+// A unit that pieces share, as its first CTA leaves it for the join.
+struct alignas(16) Shared {
+  int32_t last;  // CTA with its last part, or -1: no such unit
+  int32_t q0, queries, head;
+};
+// The workspace: Shared [CTAs], notes int [CTAs][NOTE_SLOTS][CONVERTERS][128], two parts a
+// CTA: of the unit that was begun before its piece, and of the one that goes on after it.
+__host__ __device__ constexpr int64_t notes_offset(int64_t ctas) { return ctas * (int64_t)sizeof(Shared); }
+__host__ __device__ constexpr int64_t parts_offset(int64_t ctas) {
+  return notes_offset(ctas) + ctas * NOTE_SLOTS * CONVERTERS * 128 * 4;
+}
+
+template <int DP> struct Control {
+  using L = Layout<DP>;
+  uint8_t *smem;
+  uint32_t base, bars;
+  __device__ __forceinline__ explicit Control(uint8_t *s) : smem(s), base(ptx::smem_u32(s)), bars(base + L::BAR_OFF) {}
+#define NT_BARRIER __device__ __forceinline__ uint32_t
+  // of tile t
+  NT_BARRIER q_full(int t) const { return bars + 8u * t; }       // Q_t stored
+  NT_BARRIER s_full(int t) const { return bars + 16 + 8u * t; }  // S_t of a key block in tensor memory
+  NT_BARRIER p_full(int t) const { return bars + 32 + 8u * t; }  // P_t written, O_t rescaled
+  NT_BARRIER o_done(int t) const { return bars + 48 + 8u * t; }  // the item's last P_t V done
+  NT_BARRIER o_free(int t) const { return bars + 64 + 8u * t; }  // O_t read out
+  // of ring slot s
+  NT_BARRIER slot_full(int s) const { return bars + 80 + 8u * s; }
+  NT_BARRIER slot_empty(int s) const { return bars + 80 + 8u * RING + 8u * s; }
+  // of a block's scales; of an item's notes: read
+  NT_BARRIER scale_full(int s) const { return bars + 80 + 16u * RING + 8u * s; }
+  NT_BARRIER notes_free(int s) const { return bars + 80 + 16u * RING + 8u * SCALE_SLOTS + 8u * s; }
+  NT_BARRIER settled() const { return bars + 80 + 16u * RING + 8u * (SCALE_SLOTS + NOTE_SLOTS); }
+#undef NT_BARRIER
+  static_assert(80 + 16 * RING + 8 * (SCALE_SLOTS + NOTE_SLOTS + 1) <= 240, "barriers");
+  __device__ __forceinline__ volatile uint32_t *tmem_base() const {
+    return reinterpret_cast<volatile uint32_t *>(smem + L::BAR_OFF + 240);
+  }
+  __device__ __forceinline__ volatile int *abort_flag() const {
+    return reinterpret_cast<volatile int *>(smem + L::BAR_OFF + 244);
+  }
+  __device__ __forceinline__ GroupScale *scales(int slot) const {
+    return reinterpret_cast<GroupScale *>(smem + L::SCALE_OFF) + slot * GROUPS;
+  }
+  // items with notes: the number of the item that a converter's notes are of
+  __device__ __forceinline__ volatile int *stamp(int slot, int converter) const {
+    return reinterpret_cast<volatile int *>(smem + L::STAMP_OFF) + slot * CONVERTERS + converter;
+  }
+  __device__ __forceinline__ int *notes(const Problem &p, int slot, int converter) const {
+    return reinterpret_cast<int *>(p.workspace + notes_offset(gridDim.x)) +
+           ((blockIdx.x * NOTE_SLOTS + slot) * CONVERTERS + converter) * 128;
+  }
+};
+
+// ---------------------------------------------------------------- the cut
+// All threads: the CTA's piece, into shared memory.
+__device__ __noinline__ void find_piece(const Problem &p, Piece *out, int64_t *scan) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pair = 2 * p.per_tile;
+  const int64_t per = ((int64_t)p.batch + THREADS - 1) / THREADS;  // sequences of a thread
+  const int64_t b0 = threadIdx.x * per, b1 = min(b0 + per, (int64_t)p.batch);
+  Sequence s;
+  int64_t mine = 0;
+  for (int64_t b = b0; b < b1; ++b)
+    if (s.load(p, b) && s.pairs > 0) mine += p.kv_heads * s.steps(pair);
+  int64_t up = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, up, o);
+    if (lane >= o) up += x;
+  }
+  if (lane == 31) scan[warp] = up;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) before += scan[w];
+    total += scan[w];
+  }
+  before += up - mine;
+  const int64_t pieces = max(min(total / LEAST_STEPS, (int64_t)gridDim.x), (int64_t)1);
+  const int64_t c = blockIdx.x;
+  Piece piece{};
+  piece.total = total;
+  piece.pieces = (int32_t)pieces;
+  piece.start = c < pieces ? total * c / pieces : total;
+  piece.end = c < pieces ? total * (c + 1) / pieces : total;
+  if (threadIdx.x == 0 && piece.start >= piece.end) *out = piece;
+  if (piece.start < piece.end && piece.start >= before && piece.start < before + mine) {
+    for (int64_t b = b0; b < b1; ++b) {
+      if (!s.load(p, b) || s.pairs == 0) continue;
+      const int64_t steps = s.steps(pair);  // of a head
+      if (piece.start < before + p.kv_heads * steps) {
+        const int64_t into = piece.start - before;
+        piece.batch = b;
+        piece.head = (int32_t)(into / steps);
+        piece.pos = before + piece.head * steps;
+        *out = piece;
+        break;
+      }
+      before += p.kv_heads * steps;
+    }
+  }
+  __syncthreads();
+  if (warp == 0 && piece.start < piece.end) {
+    s.load(p, out->batch);
+    const int64_t into = piece.start - out->pos;
+    const int64_t i = paged::warp_search(s.pairs, into, [&](int64_t k) { return s.before(pair, k); });
+    if (lane == 0) {
+      out->pair = (int32_t)i;
+      out->pos += s.before(pair, i);
+    }
+  }
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------- pages to operands
+// A group of 16 tokens on its way: asked for, then converted.
+struct Asked {
+  int32_t group;      // of the sequence
+  int32_t page;       // -1: outside the pool
+  int32_t ring;       // block's place in the ring; odd: values
+  int32_t item, head;
+  int32_t keys;       // of the sequence
+};
+
+template <typename C> __device__ __forceinline__ bool has_nan(uint32_t w) {
+  return std::is_same<C, __nv_fp8_e4m3>::value && (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+}
+
+template <typename C, int DP>
+__device__ __forceinline__ void convert(const Control<DP> &c, const Problem &p, const Piece &piece) {
+  using L = Layout<DP>;
+  constexpr int WORDS = DP / 16, KEYS = 32 / WORDS, LOADS = 16 / KEYS;  // 16-byte words of a token; tokens a load of the warp
+  constexpr int AHEAD = 2;
+  const int lane = threadIdx.x & 31, me = (threadIdx.x >> 5) - 1;
+  const int word = lane % WORDS, sub = lane / WORDS;
+  const bool in_head = word * 16 < p.head_dim;
+
+  // The groups of the CTA's blocks, K_0, V_0, K_1, ... one after another through all its
+  // items, are dealt to the warps in turn.  First steps ahead come the pages' numbers,
+  // AHEAD tasks ahead the codes.
+  Asked table[AHEAD], coming[AHEAD];  // page number asked for; codes asked for
+  uint4 codes[AHEAD][LOADS];
+  float scale[AHEAD];                 // lane 0: the key scale, lane 1: the value scale
+  for (int i = 0; i < AHEAD; ++i) table[i].ring = coming[i].ring = -1;
+  int items = 0;
+
+  auto store = [&](const Asked &a, const uint4 (&x)[LOADS], float s) -> bool {
+    const int slot = a.ring % RING, g = a.group % GROUPS;
+    if (!ptx::mbar_wait_warp(c.slot_empty(slot), ((uint32_t)(a.ring / RING) & 1u) ^ 1u, c.abort_flag())) return false;
+    const bool values = a.ring & 1;
+    uint32_t taken = 0;  // NaN codes of a value are taken out and noted
+    const uint32_t to = c.base + L::RING_OFF + slot * L::KV_BYTES + (word / 4) * (BN * 128);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int key = g * 16 + i * KEYS + sub;
+      uint4 v = x[i];
+      if (values && (has_nan<C>(v.x) || has_nan<C>(v.y) || has_nan<C>(v.z) || has_nan<C>(v.w))) {
+        taken |= 1u << i;
+        uint32_t *w = &v.x;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] &= ~(((((w[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu);
+      }
+      uint4 lo, hi;
+      paged::to_halves<C>(v.x, lo.x, lo.y);
+      paged::to_halves<C>(v.y, lo.z, lo.w);
+      paged::to_halves<C>(v.z, hi.x, hi.y);
+      paged::to_halves<C>(v.w, hi.z, hi.w);
+      // a quarter warp's stores meet every bank once: the second atom's lanes store their halves the other way round
+      const int chunk = (word % 4) * 2, flip = word / 4;
+      const uint32_t row = to + key * 128;
+      const uint32_t a0 = row + (((chunk + flip) ^ (key & 7)) * 16), a1 = row + (((chunk + 1 - flip) ^ (key & 7)) * 16);
+      store_shared16(a0, flip ? hi : lo);
+      store_shared16(a1, flip ? lo : hi);
+    }
+    if (!values) {
+      const float other = __shfl_sync(0xffffffffu, s, 1);
+      if (lane == 0) {
+        const int block = a.ring / 2 % SCALE_SLOTS;
+        GroupScale e;
+        e.key = a.page < 0 ? 0.f : p.scale * s;
+        e.add = a.page < 0 ? -INFINITY : 0.f;
+        e.value = a.page < 0 ? 0.f : other;
+        e.log2_value = a.page < 0 ? -INFINITY : log2_fast(other);
+        c.scales(block)[g] = e;
+        ptx::mbar_arrive(c.scale_full(block));
+      }
+    }
+    if (std::is_same<C, __nv_fp8_e4m3>::value && __any_sync(0xffffffffu, taken != 0)) {
+      // (rare) the first key with a NaN for each element of the head
+      const int note = a.item % NOTE_SLOTS;
+      int *notes = c.notes(p, note, me);
+      if (*c.stamp(note, me) != a.item) {
+        if (!ptx::mbar_wait_warp(c.notes_free(note), ((uint32_t)(a.item / NOTE_SLOTS) & 1u) ^ 1u, c.abort_flag())) return false;
+        for (int d = lane; d < 128; d += 32) notes[d] = INT32_MAX;
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) *c.stamp(note, me) = a.item;
+        __syncwarp();
+      }
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        if (!(taken >> i & 1)) continue;
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          for (int e = 0; e < 4; ++e)
+            if ((w[k] >> 8 * e & 0x7fu) == 0x7fu) atomicMin(notes + word * 16 + k * 4 + e, a.group * 16 + i * KEYS + sub);
+      }
+      __threadfence();
+    }
+    ptx::fence_proxy_async_smem();  // the MMAs read what was written here
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(c.slot_full(slot));
+    return true;
+  };
+  auto load = [&](const Asked &a, uint4 (&x)[LOADS], float &s) {
+    const bool values = a.ring & 1;
+    const int count = a.page < 0 ? 0 : min(max(a.keys - a.group * 16, 0), 16);
+    const int in_page = a.group - (int)((uint64_t)(uint32_t)a.group * p.page_reciprocal >> 36) * p.page_groups;
+    const uint8_t *from = (values ? p.value + a.page * p.v_page + a.head * p.v_head + (int64_t)(in_page * 16) * p.v_token
+                                  : p.key + a.page * p.k_page + a.head * p.k_head + (int64_t)(in_page * 16) * p.k_token) +
+                          word * 16;
+    const int64_t stride = values ? p.v_token : p.k_token;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int token = i * KEYS + sub;
+      x[i] = in_head && token < count ? __ldg(reinterpret_cast<const uint4 *>(from + token * stride)) : make_uint4(0, 0, 0, 0);
+    }
+    s = 0.f;
+    if (!values && a.page >= 0) {
+      if (lane == 0) s = p.key_scale[a.page * p.ks_page + a.head * p.ks_head];
+      if (lane == 1) s = p.value_scale[a.page * p.vs_page + a.head * p.vs_head];
+    }
+  };
+  auto ask = [&](Asked &a, int batch) {
+    a.page = -1;
+    if (a.group * 16 < a.keys) {
+      a.page = paged::page_of(p, batch, (int64_t)((uint64_t)(uint32_t)a.group * p.page_reciprocal >> 36));
+    }
+  };
+  auto step = [&](const Asked &next, bool more) -> bool {
+    // the oldest codes are stored, the oldest page number's codes asked for
+    if (coming[0].ring >= 0 && !store(coming[0], codes[0], scale[0])) return false;
+#pragma unroll
+    for (int i = 0; i + 1 < AHEAD; ++i) {
+      coming[i] = coming[i + 1];
+      scale[i] = scale[i + 1];
+#pragma unroll
+      for (int k = 0; k < LOADS; ++k) codes[i][k] = codes[i + 1][k];
+    }
+    coming[AHEAD - 1] = table[0];
+    if (table[0].ring >= 0) {
+      if (table[0].page < 0 && table[0].group * 16 < table[0].keys) record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
+      load(table[0], codes[AHEAD - 1], scale[AHEAD - 1]);
+    }
+#pragma unroll
+    for (int i = 0; i + 1 < AHEAD; ++i) table[i] = table[i + 1];
+    table[AHEAD - 1] = next;
+    if (!more) table[AHEAD - 1].ring = -1;
+    return true;
+  };
+  bool good = true;
+  int ring = 0, skip = me;  // the item's K_0; groups until this warp's next
+  each_item(p, piece, [&](const Item &e) {
+    const int count = 2 * (e.until - e.from) * GROUPS;  // K and V in turn
+    int x = skip;
+    for (; x < count; x += CONVERTERS) {
+      const int block = x / GROUPS;
+      Asked a;
+      a.ring = ring + block;
+      a.group = (e.from + block / 2) * GROUPS + x % GROUPS;
+      a.item = items;
+      a.head = e.head;
+      a.keys = e.keys;
+      ask(a, e.batch);
+      if (!(good = step(a, true))) return false;
+    }
+    skip = x - count;
+    ring += 2 * (e.until - e.from);
+    ++items;
+    return true;
+  });
+  for (int i = 0; good && i < 2 * AHEAD; ++i) good = step(Asked{}, false);
+}
+
+// ---------------------------------------------------------------- MMA issuer
+// A full warp; lane 0 issues.  K, V and Q stand in shared memory as 128-byte-swizzled
+// tiles of 64 elements.
+struct Standing {
+  int ring;            // place of the item's K_0
+  int blocks[TILES];   // key blocks of tile t so far
+  int used[TILES];     // items that had tile t
+};
+
+template <int DP>
+__device__ __forceinline__ void issue(const Control<DP> &c, const Problem &p, const Piece &piece, uint32_t tmem_base,
+                                      Shared &open) {
+  using L = Layout<DP>;
+  constexpr uint32_t fmt = tc::umma_format<__half>();
+  constexpr uint32_t idesc_qk = ptx::f16_idesc(fmt, 0, 0, BM, BN);  // B = keys, K-major
+  constexpr uint32_t idesc_pv = ptx::f16_idesc(fmt, 0, 1, BM, DP);  // B = values, MN-major
+  const bool issues = (threadIdx.x & 31) == 0;
+  auto tmem_s = [&](int t) { return tmem_base + (uint32_t)(t * BN); };
+  auto tmem_o = [&](int t) { return tmem_base + (uint32_t)(TILES * BN + t * 128); };
+  auto slot_addr = [&](int r) { return c.base + L::RING_OFF + (r % RING) * L::KV_BYTES; };
+  auto wait = [&](uint32_t bar, uint32_t parity) { return ptx::mbar_wait_warp(bar, parity, c.abort_flag()); };
+  auto wait_slot = [&](int r) { return wait(c.slot_full(r % RING), (uint32_t)(r / RING) & 1u); };
+  auto commit = [&](uint32_t bar) {
+    if (issues) ptx::mma_commit(bar);
+  };
+  auto issue_qk = [&](int t, int r) {
+    if (!issues) return;
+    const uint32_t kb = slot_addr(r);
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+      const uint32_t qoff = (kk / 4) * (BM * 128) + (kk % 4) * 32, koff = (kk / 4) * (BN * 128) + (kk % 4) * 32;
+      ptx::mma_f16_ss(tmem_s(t), ptx::sw128_desc(c.base + t * L::Q_BYTES + qoff, 16, 1024),
+                      ptx::sw128_desc(kb + koff, 16, 1024), idesc_qk, kk > 0 ? 1u : 0u);
+    }
+    ptx::mma_commit(c.s_full(t));
+  };
+  auto issue_pv = [&](int t, int r, bool first) {
+    if (!issues) return;
+    const uint32_t vb = slot_addr(r);
+#pragma unroll
+    for (int kk = 0; kk < BN / 16; ++kk)
+      ptx::mma_f16_ts(tmem_o(t), tmem_s(t) + (uint32_t)(kk * 8), ptx::sw128_desc(vb + kk * 16 * 128, BN * 128, 1024),
+                      idesc_pv, (!first || kk > 0) ? 1u : 0u);
+  };
+  Standing at{};
+  each_item(p, piece, [&](const Item &e) {
+    if (e.from == 0 && e.until < e.blocks)
+      open = Shared{(int32_t)((e.end * piece.pieces - 1) / piece.total), e.q0, e.queries, e.head};
+    const int count = e.until - e.from;
+    const int n[TILES] = {max(e.until_of(0, p.per_tile) - e.from, 0), max(e.until_of(1, p.per_tile) - e.from, 0)};
+    if (!wait_slot(at.ring)) return false;  // K_0
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      if (n[t] == 0) continue;
+      if (!wait(c.q_full(t), (uint32_t)at.used[t] & 1u)) return false;
+      ptx::tc_fence_after();
+      issue_qk(t, at.ring);
+    }
+    commit(c.slot_empty(at.ring % RING));
+    for (int j = 0; j < count; ++j) {
+      const int rv = at.ring + 2 * j + 1, rk = rv + 1;
+      if (!wait_slot(rv)) return false;
+      const bool next_keys = j + 1 < count;
+      bool waited = false;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        if (j >= n[t]) continue;
+        // P_t written also means that S_t was read: Q K^T may overwrite it
+        if (!wait(c.p_full(t), (uint32_t)(at.blocks[t] + j) & 1u)) return false;
+        if (j == 0 && at.used[t] > 0 && !wait(c.o_free(t), (uint32_t)(at.used[t] - 1) & 1u)) return false;
+        ptx::tc_fence_after();
+        issue_pv(t, rv, j == 0);
+        if (j == n[t] - 1) commit(c.o_done(t));
+        if (j + 1 < n[t]) {
+          if (!waited) {
+            if (!wait_slot(rk)) return false;
+            waited = true;
+            ptx::tc_fence_after();
+          }
+          issue_qk(t, rk);
+        }
+      }
+      commit(c.slot_empty(rv % RING));
+      if (next_keys) {
+        // (a block that no tile needs was loaded all the same)
+        if (!waited && !wait_slot(rk)) return false;
+        commit(c.slot_empty(rk % RING));
+      }
+    }
+    at.ring += 2 * count;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      at.blocks[t] += n[t];
+      at.used[t] += n[t] > 0;
+    }
+    return true;
+  });
+}
+
+// ---------------------------------------------------------------- queries, softmax, output
+// A row's references move only when a block passes them by 2^kLead, so that O is rescaled
+// rarely, and P is kept 2^kRise above: its largest, 2^15, stays in fp16's range.
+constexpr float kLead = 6.f, kRise = 9.f;
+constexpr float kLeastKey = 1.1754943508222875e-38f;  // in place of a key scale of 0: -inf times it is -inf
+
+// A row of Q into shared memory, scaled by 2^e with its largest finite element then in
+// [2^14, 2^15); returns 2^-e.  `query` null: zeros.
+template <int DP>
+__device__ __forceinline__ float store_query(const Control<DP> &c, const Problem &p, int t, int row, const uint16_t *query) {
+  using L = Layout<DP>;
+  uint32_t w[DP / 2];  // two elements each
+  if (p.q_vector) {
+#pragma unroll
+    for (int x = 0; x < DP / 8; ++x) {
+      const uint4 v = query && x * 8 < p.head_dim ? __ldg(reinterpret_cast<const uint4 *>(query) + x) : make_uint4(0, 0, 0, 0);
+      w[4 * x] = v.x; w[4 * x + 1] = v.y; w[4 * x + 2] = v.z; w[4 * x + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int x = 0; x < DP / 2; ++x)
+      w[x] = query && 2 * x < p.head_dim ? query[2 * x * p.q_dim] | (uint32_t)query[(2 * x + 1) * p.q_dim] << 16 : 0u;
+  }
+  auto values = [&](uint32_t v) {
+    return p.bf16 ? make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u))
+                  : __half22float2(*reinterpret_cast<const __half2 *>(&v));
+  };
+  float top = 0.f;
+#pragma unroll
+  for (int x = 0; x < DP / 2; ++x) {
+    const float2 v = values(w[x]);
+    top = fmaxf(top, fmaxf(paged::finite_magnitude(v.x), paged::finite_magnitude(v.y)));
+  }
+  // 2^(14 - exponent); rows of less than 2^-112 as those of 2^-112
+  const int e = max((int)(__float_as_uint(top) >> 23) - 127, -112);
+  const float factor = __uint_as_float((uint32_t)(paged::Q_TOP - e + 127) << 23);
+  const uint32_t to = c.base + t * L::Q_BYTES + row * 128;
+#pragma unroll
+  for (int x = 0; x < DP / 8; ++x) {
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = values(w[4 * x + i]);
+      h[i] = paged::half2_bits(v.x * factor, v.y * factor);
+    }
+    store_shared16(to + (x / 8) * (BM * 128) + (((x % 8) ^ (row & 7)) * 16), make_uint4(h[0], h[1], h[2], h[3]));
+  }
+  return __uint_as_float((uint32_t)(e - paged::Q_TOP + 127) << 23);
+}
+
+template <int N> __device__ __forceinline__ void store_output(const Problem &p, int64_t token, int head, int d0, const float (&x)[N]) {
+  uint16_t *out = static_cast<uint16_t *>(p.out) + token * p.o_token + (int64_t)head * p.o_head + d0 * p.o_dim;
+  uint32_t w[N / 2];
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i)
+    w[i] = p.bf16 ? tc::attn::pack2<__nv_bfloat16>(x[2 * i], x[2 * i + 1]) : tc::attn::pack2<__half>(x[2 * i], x[2 * i + 1]);
+  if (p.o_dim == 1 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 8; ++i)
+      reinterpret_cast<uint4 *>(out)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i * p.o_dim] = (uint16_t)(w[i / 2] >> 16 * (i & 1));
+  }
+}
+
+template <int DP>
+__device__ __forceinline__ void attend(const Control<DP> &c, const Problem &p, const Piece &piece, uint32_t tmem_base) {
+  using L = Layout<DP>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = (warp - 1 - CONVERTERS) / 4, quarter = warp & 3;
+  const int row = quarter * 32 + lane;  // row of the tile = lane of tensor memory
+  const int row_query = row / p.group + t * p.per_tile, row_head = row % p.group;
+  const bool has_row = row / p.group < p.per_tile;
+  const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+  const uint32_t tmem_s = tmem_base + (uint32_t)(t * BN) + lane_base;
+  const uint32_t tmem_o = tmem_base + (uint32_t)(TILES * BN + t * 128) + lane_base;
+  auto arrive_warp = [&](uint32_t bar) {
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(bar);
+  };
+  int s_turn = 0, o_turn = 0, block0 = 0, items = 0;  // blocks and items of this tile; the item's first block, the item
+  each_item(p, piece, [&](const Item &e) {
+    const int until = e.until_of(t, p.per_tile), item = items++, first_block = block0;
+    block0 += e.until - e.from;
+    const bool mine = has_row && row_query < e.queries;
+    const int64_t token = e.q0 + row_query;
+    const int head = e.head * p.group + row_head;
+    float *part = nullptr;
+    if (!e.whole())
+      part = reinterpret_cast<float *>(p.workspace + parts_offset(gridDim.x) +
+                                       (2 * (int64_t)blockIdx.x + (e.from > 0 ? 0 : 1)) * L::PART);
+    float4 *stats = reinterpret_cast<float4 *>(part) + ROWS * (DP / 4) + t * BM + row;
+    if (until <= e.from) {  // nothing to see in this share
+      if (part && mine) *stats = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+      arrive_warp(c.notes_free(item % NOTE_SLOTS));
+      return true;
+    }
+    const float factor = store_query<DP>(
+        c, p, t, row,
+        mine ? static_cast<const uint16_t *>(p.query) + token * p.q_token + (int64_t)head * p.q_head : nullptr);
+    ptx::fence_proxy_async_smem();
+    arrive_warp(c.q_full(t));
+    const int limit = min(e.limit0 + row_query, e.keys);             // keys that the row sees
+    const int sure = min(e.limit0 + t * p.per_tile, e.keys);         // that all rows see
+
+    float m = -INFINITY, mo = -INFINITY, l = 0.f;
+    for (int j = e.from; j < until; ++j) {
+      const int block = first_block + j - e.from, slot = block % SCALE_SLOTS;
+      if (!ptx::mbar_wait_warp(c.scale_full(slot), (uint32_t)(block / SCALE_SLOTS) & 1u, c.abort_flag())) return false;
+      if (!ptx::mbar_wait_warp(c.s_full(t), (uint32_t)s_turn & 1u, c.abort_flag())) return false;
+      ++s_turn;
+      ptx::tc_fence_after();
+      uint32_t sr[BN];
+#pragma unroll
+      for (int x = 0; x < BN / 32; ++x)
+        ptx::tmem_ld_32x32b_x32(tmem_s + (uint32_t)(x * 32), *reinterpret_cast<uint32_t(*)[32]>(&sr[x * 32]));
+      ptx::tmem_ld_wait();
+      float *s = reinterpret_cast<float *>(sr);
+      const int seen = limit - j * BN;
+      const bool masked = sure - j * BN < BN;
+      if (masked) {
+#pragma unroll
+        for (int x = 0; x < BN; ++x) s[x] = x < seen ? s[x] : -INFINITY;
+      }
+      const GroupScale *scales = c.scales(slot);
+      // (a group that the row does not see takes no part, whatever its scales)
+      auto key_factor = [&](const GroupScale &g, int k) {
+        const float f = g.key * factor;
+        return f == 0.f || (masked && k * 16 >= seen) ? kLeastKey : f;
+      };
+      float top_s = -INFINITY, top_w = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < GROUPS; ++k) {
+        const GroupScale g = scales[k];
+        float top[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          top[u] = fmaxf(fmaxf(s[k * 16 + u], s[k * 16 + 4 + u]), fmaxf(s[k * 16 + 8 + u], s[k * 16 + 12 + u]));
+        const float high = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), key_factor(g, k), g.add);
+        top_s = fmaxf(top_s, high);
+        top_w = fmaxf(top_w, high + g.log2_value);
+      }
+      const bool move = top_s > m + kLead, move_o = top_w > mo + kLead;
+      const float m_new = move ? top_s : m, mo_new = move_o ? top_w : mo;
+      const float alpha = move ? exp2_fast(m - m_new) : 1.f, alpha_o = move_o ? exp2_fast(mo - mo_new) : 1.f;
+      const float ref = reference(m_new), rise = exp2_fast(fminf(ref - reference(mo_new) + kRise, 126.f));
+      float sum[4] = {};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t packed[32];
+#pragma unroll
+        for (int k = 0; k < GROUPS / 2; ++k) {
+          const GroupScale g = scales[half * (GROUPS / 2) + k];
+          const float by = key_factor(g, half * (GROUPS / 2) + k), add = g.add - ref;
+          const float weight = masked && (half * (GROUPS / 2) + k) * 16 >= seen ? 0.f : g.value * rise;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const int at = (half * (GROUPS / 2) + k) * 16 + 2 * x;
+            const float p0 = exp2_fast(fmaf(s[at], by, add)), p1 = exp2_fast(fmaf(s[at + 1], by, add));
+            sum[(2 * x) & 3] += p0;
+            sum[(2 * x + 1) & 3] += p1;
+            packed[k * 8 + x] = paged::half2_bits(p0 * weight, p1 * weight);
+          }
+        }
+        ptx::tmem_st_32x32b_x32(tmem_s + (uint32_t)(half * 32), packed);
+      }
+      if (j > e.from && __any_sync(0xffffffffu, move_o)) {
+        // O_t holds P(j-1) V(j-1): the commit of S_t(j) covers it
+        uint32_t o[DP];
+#pragma unroll
+        for (int x = 0; x < DP / 32; ++x)
+          ptx::tmem_ld_32x32b_x32(tmem_o + (uint32_t)(x * 32), *reinterpret_cast<uint32_t(*)[32]>(&o[x * 32]));
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int y = 0; y < DP; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * alpha_o);
+#pragma unroll
+        for (int x = 0; x < DP / 32; ++x)
+          ptx::tmem_st_32x32b_x32(tmem_o + (uint32_t)(x * 32), *reinterpret_cast<uint32_t(*)[32]>(&o[x * 32]));
+      }
+      m = m_new;
+      mo = mo_new;
+      l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before();
+      arrive_warp(c.p_full(t));
+    }
+    if (!ptx::mbar_wait_warp(c.o_done(t), (uint32_t)o_turn & 1u, c.abort_flag())) return false;
+    ++o_turn;
+    ptx::tc_fence_after();
+    uint32_t o[DP];
+#pragma unroll
+    for (int x = 0; x < DP / 32; ++x)
+      ptx::tmem_ld_32x32b_x32(tmem_o + (uint32_t)(x * 32), *reinterpret_cast<uint32_t(*)[32]>(&o[x * 32]));
+    ptx::tmem_ld_wait();
+    ptx::tc_fence_before();
+    arrive_warp(c.o_free(t));
+    // values' NaN, to the rows that see them
+    for (int w = 0; w < CONVERTERS; ++w) {
+      if (*c.stamp(item % NOTE_SLOTS, w) != item) continue;
+      const int *notes = c.notes(p, item % NOTE_SLOTS, w);
+#pragma unroll
+      for (int d = 0; d < DP; ++d)
+        if (__ldcg(notes + d) < limit) o[d] = 0x7fc00000u;
+    }
+    arrive_warp(c.notes_free(item % NOTE_SLOTS));
+    if (mine && !part) {
+      // (mo: -inf where all values stand for 0)
+      const float f = l == 0.f ? 0.f : exp2_fast(reference(mo) - reference(m) - kRise) / l;
+#pragma unroll
+      for (int x = 0; x < DP / 16; ++x) {
+        float v[16];
+#pragma unroll
+        for (int y = 0; y < 16; ++y) v[y] = __uint_as_float(o[x * 16 + y]) * f;
+        if (x * 16 < p.head_dim) store_output<16>(p, token, head, x * 16, v);
+      }
+      if (p.lse) p.lse[token * p.l_token + (int64_t)head * p.l_head] = l == 0.f ? -INFINITY : (m + log2_fast(l)) * kLn2;
+    } else if (part && mine) {
+      float4 *out = reinterpret_cast<float4 *>(part) + t * BM + row;
+#pragma unroll
+      for (int x = 0; x < DP / 4; ++x)
+        out[x * ROWS] = make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]), __uint_as_float(o[4 * x + 2]),
+                                    __uint_as_float(o[4 * x + 3]));
+      *stats = make_float4(m, l, mo, 0.f);
+    }
+    return true;
+  });
+}
+
+template <typename C, int DP>
+__global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_constant__ Problem p) {
+  using L = Layout<DP>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const Control<DP> c(smem);
+  Shared *shared = reinterpret_cast<Shared *>(p.workspace) + blockIdx.x;
+  if ((c.base & 1023u) != 0) {  // the swizzle needs it; there is no room to align by hand
+    record_error(NT_B200_ERR_INVALID_ARGUMENT);
+    wait_prior_grid();
+    if (threadIdx.x == 0) shared->last = -1;
+    return;
+  }
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < TILES; ++t) {
+      ptx::mbar_init(c.q_full(t), 4);  // a warp's lanes arrive as one
+      ptx::mbar_init(c.s_full(t), 1);
+      ptx::mbar_init(c.p_full(t), 4);
+      ptx::mbar_init(c.o_done(t), 1);
+      ptx::mbar_init(c.o_free(t), 4);
+    }
+    for (int s = 0; s < RING; ++s) {
+      ptx::mbar_init(c.slot_full(s), GROUPS);
+      ptx::mbar_init(c.slot_empty(s), 1);
+    }
+    for (int s = 0; s < SCALE_SLOTS; ++s) ptx::mbar_init(c.scale_full(s), GROUPS);
+    for (int s = 0; s < NOTE_SLOTS; ++s) {
+      ptx::mbar_init(c.notes_free(s), SOFTMAX_WARPS);
+      for (int w = 0; w < CONVERTERS; ++w) *c.stamp(s, w) = -1;
+    }
+    ptx::mbar_init(c.settled(), 1);
+    *c.abort_flag() = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == 0) {
+    ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t *>(c.tmem_base())), TMEM_COLS);
+    ptx::tmem_relinquish();
+  }
+  wait_prior_grid();
+  ptx::tc_fence_before();
+  find_piece(p, reinterpret_cast<Piece *>(smem + L::PIECE_OFF), reinterpret_cast<int64_t *>(smem + L::SCAN_OFF));
+  ptx::tc_fence_after();
+  const Piece piece = *reinterpret_cast<const Piece *>(smem + L::PIECE_OFF);
+  const uint32_t tmem_base = *c.tmem_base();
+  if (warp == 0) {
+    Shared open{-1, 0, 0, 0};  // the unit that goes on in the next piece, for the join
+    issue<DP>(c, p, piece, tmem_base, open);
+    if ((threadIdx.x & 31) == 0) *shared = open;
+  } else if (warp <= CONVERTERS) {
+    convert<C, DP>(c, p, piece);
+  } else {
+    attend<DP>(c, p, piece, tmem_base);
+  }
+  allow_dependent_launch();
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (*c.abort_flag()) {
+    // after a wait gave up: the MMAs in flight, so that shared and tensor memory are at rest
+    if (threadIdx.x == 0) {
+      volatile int over = 0;
+      ptx::mma_commit(c.settled());
+      ptx::mbar_wait(c.settled(), 0, &over, 1000000000ull);
+    }
+    __syncthreads();
+  }
+  if (warp == 0) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------- join
+// Block (a, y): 16 elements of the rows of the unit that CTA a left open; a thread a row.
+template <int DP>
+__global__ void __launch_bounds__(ROWS) join_kernel(const __grid_constant__ Problem p, int ctas) {
+  using L = Layout<DP>;
+  wait_prior_grid();
+  allow_dependent_launch();
+  const Shared s = reinterpret_cast<const Shared *>(p.workspace)[blockIdx.x];
+  if (s.last < 0) return;
+  const int row = threadIdx.x % BM, t = threadIdx.x / BM;
+  const int query = t * p.per_tile + row / p.group;
+  if (row / p.group >= p.per_tile || query >= s.queries) return;
+  // the parts: this CTA's second, then the first of those after it
+  const auto part = [&](int i) {
+    return reinterpret_cast<const float4 *>(p.workspace + parts_offset(ctas) +
+                                            (i == 0 ? 2 * (int64_t)blockIdx.x + 1 : 2 * ((int64_t)blockIdx.x + i)) * L::PART);
+  };
+  const int parts = s.last - (int)blockIdx.x + 1;
+  constexpr int STATS = ROWS * (DP / 4);
+  float top = -INFINITY, top_o = -INFINITY;
+  for (int i = 0; i < parts; ++i) {
+    const float4 st = part(i)[STATS + threadIdx.x];
+    top = fmaxf(top, st.x);
+    top_o = fmaxf(top_o, st.z);
+  }
+  float l = 0.f, o[16] = {};
+  for (int i = 0; i < parts; ++i) {
+    const float4 *from = part(i);
+    const float4 st = from[STATS + threadIdx.x];
+    l += st.y * exp2_fast(st.x - reference(top));
+    if (st.z == -INFINITY && st.y == 0.f) continue;  // a tile without keys in this part: nothing was written
+    const float f = exp2_fast(st.z - reference(top_o));
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float4 v = from[(blockIdx.y * 4 + x) * ROWS + threadIdx.x];
+      o[4 * x] = fmaf(v.x, f, o[4 * x]);
+      o[4 * x + 1] = fmaf(v.y, f, o[4 * x + 1]);
+      o[4 * x + 2] = fmaf(v.z, f, o[4 * x + 2]);
+      o[4 * x + 3] = fmaf(v.w, f, o[4 * x + 3]);
+    }
+  }
+  const int64_t token = s.q0 + query;
+  const int head = s.head * p.group + row % p.group;
+  const float f = l == 0.f ? 0.f : exp2_fast(reference(top_o) - reference(top) - kRise) / l;
+#pragma unroll
+  for (int x = 0; x < 16; ++x) o[x] *= f;
+  store_output<16>(p, token, head, blockIdx.y * 16, o);
+  if (p.lse && blockIdx.y == 0)
+    p.lse[token * p.l_token + (int64_t)head * p.l_head] = l == 0.f ? -INFINITY : (top + log2_fast(l)) * kLn2;
+}
+
+template <typename C, int DP> int launch_tiles(const Problem &p, cudaStream_t stream) {
+  using L = Layout<DP>;
+  cudaError_t e = smem_optin<attention_kernel<C, DP>>(L::SMEM_BYTES);
+  if (e != cudaSuccess) return (int)e;
+  const int ctas = sm_count();
+  const int rc = launch_overlapped(attention_kernel<C, DP>, dim3(ctas), dim3(THREADS), L::SMEM_BYTES, stream, p);
+  if (rc != 0) return rc;
+  return launch_overlapped(join_kernel<DP>, dim3(ctas, (unsigned)(p.head_dim / 16)), dim3(ROWS), 0, stream, p, ctas);
+}
+
+template <typename T, typename C> int launch(const Problem &p, cudaStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    if (p.head_dim <= 128 && p.group <= BM && p.scale > 0.f && p.tokens <= (1 << 30)) {
+      if (p.head_dim <= 64) return launch_tiles<C, 64>(p, stream);
+      return launch_tiles<C, 128>(p, stream);
+    }
+  }
+  const int64_t blocks = (p.tokens * p.heads + 3) / 4;
+  if (blocks > (1LL << 31) - 1) return NT_B200_ERR_INVALID_ARGUMENT;
+  rows_kernel<T, C><<<(unsigned)blocks, 128, 0, stream>>>(p);
+  return launch_status();
+}
+
+}  // namespace chunk
+}  // namespace nt
+
+extern "C" int64_t nt_b200_chunk_attention_workspace_size(void) {
+  using namespace nt::chunk;
+  const int64_t ctas = nt::sm_count();
+  return parts_offset(ctas) + 2 * ctas * Layout<128>::PART;
+}
+
+extern "C" int nt_b200_chunk_attention(const NtB200ChunkAttentionArgs *a, void *stream) {
+  using namespace nt;
+  if (!a || a->batch < 0 || a->tokens < 0 || a->heads < 0 || a->table_columns < 0) return NT_B200_ERR_INVALID_ARGUMENT;
+  if (!is_float_dtype((int)a->dtype) || !is_index_dtype(a->index_dtype)) return NT_B200_ERR_UNSUPPORTED_DTYPE;
+  if (a->batch == 0 || a->tokens == 0 || a->heads == 0) return 0;
+  const NtB200PagedCache &c = a->cache;
+  const int rc = paged::check_cache(c);
+  if (rc != 0) return rc;
+  if (c.kv_heads == 0 || a->heads % c.kv_heads != 0 || c.head_dim > paged::kMostDim) return NT_B200_ERR_SHAPE_MISMATCH;
+  if (!a->query || !a->output || !a->lengths || !a->offsets || (a->table_columns > 0 && !a->block_table) || !a->workspace ||
+      (reinterpret_cast<uintptr_t>(a->workspace) & 15u) != 0 ||
+      a->workspace_bytes < nt_b200_chunk_attention_workspace_size() || a->batch > (1 << 30) || a->heads > (1 << 30) ||
+      a->table_columns > (1LL << 40) || !(a->scale == a->scale))
+    return NT_B200_ERR_INVALID_ARGUMENT;
+  const int wide = a->index_dtype == NT_B200_INT64;
+  chunk::Problem p{};
+  p.query = a->query;
+  p.out = a->output;
+  p.lse = a->lse;
+  p.key = static_cast<const uint8_t *>(c.key);
+  p.value = static_cast<const uint8_t *>(c.value);
+  p.key_scale = c.key_scale;
+  p.value_scale = c.value_scale;
+  p.lengths = {a->lengths, a->lengths_stride, wide};
+  p.offsets = {a->offsets, a->offsets_stride, wide};
+  p.block_table = {a->block_table, a->block_table_strides[1], wide};
+  p.table_row_stride = a->block_table_strides[0];
+  p.q_token = a->query_strides[0]; p.q_head = a->query_strides[1]; p.q_dim = a->query_strides[2];
+  p.o_token = a->output_strides[0]; p.o_head = a->output_strides[1]; p.o_dim = a->output_strides[2];
+  p.l_token = a->lse_strides[0]; p.l_head = a->lse_strides[1];
+  p.k_page = c.key_strides[0]; p.k_head = c.key_strides[1]; p.k_token = c.key_strides[2];
+  p.v_page = c.value_strides[0]; p.v_head = c.value_strides[1]; p.v_token = c.value_strides[2];
+  p.ks_page = c.key_scale_strides[0]; p.ks_head = c.key_scale_strides[1];
+  p.vs_page = c.value_scale_strides[0]; p.vs_head = c.value_scale_strides[1];
+  p.pages = c.pages;
+  const int64_t capacity = a->table_columns * c.page;
+  p.capacity = (int)(capacity < paged::MOST_TOKENS ? capacity : paged::MOST_TOKENS);
+  p.page_groups = (int)(c.page / 16);
+  p.page_reciprocal = ((1ull << 36) + p.page_groups - 1) / p.page_groups;
+  p.batch = (int)a->batch; p.heads = (int)a->heads; p.kv_heads = (int)c.kv_heads;
+  p.group = (int)(a->heads / c.kv_heads);
+  p.head_dim = (int)c.head_dim;
+  p.page = (int)c.page;
+  p.per_tile = p.group > chunk::BM ? 1 : chunk::BM / p.group;
+  p.bf16 = a->dtype == NT_B200_BFLOAT16;
+  p.q_vector = p.q_dim == 1 && p.q_token % 8 == 0 && p.q_head % 8 == 0 && rotary::aligned16(p.query);
+  p.scale = (float)(a->scale * 1.4426950408889634);
+  p.tokens = a->tokens;
+  p.workspace = static_cast<uint8_t *>(a->workspace);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return NT_DISPATCH_FLOAT((int)a->dtype, [&] {
+    if (c.code_dtype == NT_B200_INT8) return chunk::launch<scalar_t, int8_t>(p, s);
+    return chunk::launch<scalar_t, __nv_fp8_e4m3>(p, s);
+  });
+}

@@ -18,12 +18,13 @@
 // make the pairs (0, 4), (1, 5), (2, 6), (3, 7): a shift, a mask and a
 // subtraction for two weights, and one permute for two elements of x.
 //
-// A block has 8 warps and 32 * WR weight rows; a stage of its ring holds KS = 1024
-// / WR columns of them, 16 KB at any WR, and x's columns beside it.  A warp takes
-// 32 rows and 128 columns of a stage.  More rows of x take more weight rows a
-// block, so that x is never more than the weights.  Where the weight rows are too
-// few for the SMs, a cluster's blocks share the columns and join their sums
-// through distributed shared memory, always in the same order.
+// A block has 8 warps and 64 or 128 weight rows; a stage of its ring holds 512 or 256
+// columns of them, 16 KB, and x's columns beside it, of which a warp takes 64 rows by
+// 64 columns, or 32 by 128.  More rows of x take more weight rows a block, so that x
+// is never more than the weights.  Blocks go on from one set of rows to the next with
+// the copies running ahead.  Where the weight rows are too few for the SMs, a
+// cluster's blocks share the columns and join their sums through distributed shared
+// memory, always in the same order.
 #pragma once
 
 #include "common.cuh"
@@ -45,8 +46,11 @@ struct Params {
   int parts;          // of the columns: blocks of a cluster
   int stages;         // of the columns, all parts together
   uint32_t group32;   // 32-column steps of a group
-  int scale_words, zero_words;           // 4-byte words of a weight row in a stage
-  int x_bytes, stage_bytes;              // x's part of a stage; the whole
+  // scales and zero points of a weight row in a stage: bytes of a copy, of all, from row to row
+  int s_copy, z_copy, s_span, z_span, s_pitch, z_pitch;
+  int copiers;                             // threads that copy them
+  int x_rows, x_bytes, stage_bytes, ring, join, control;  // x's part of a stage; the whole; stages in shared memory; what follows them
+  int64_t row_blocks;
 };
 
 __device__ __forceinline__ float any_float(const uint8_t *at, int dtype) {
@@ -97,285 +101,453 @@ __global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ Param
 }
 
 // ---------------------------------------------------------------- tensor cores
-constexpr int WARPS = 8, THREADS = WARPS * 32, RING = 4;
+constexpr int WARPS = 8, THREADS = WARPS * 32;
+constexpr int MOST_RING = 8, CONTROL_BYTES = 16 * MOST_RING + 16;  // the stages' barriers and the abort flag
 
-// Two 16-bit floats from the low four bits of w's halves, less the zero point.
+// Two 16-bit floats from four bits of w's halves, less the zero point: `low` takes
+// bits 0-3, `high` bits 4-7 of each half.  The zero point comes as prepared.
 template <typename F> struct Codes;
 template <> struct Codes<__half> {
-  static constexpr uint32_t ONE = 0x64006400u;  // 1024, twice
-  static __device__ __forceinline__ uint32_t pair(uint32_t w, uint32_t zero) {
-    const uint32_t bits = (w & 0x000f000fu) | ONE;
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&bits), *reinterpret_cast<const __half2 *>(&zero));
+  // the zero point as `low` and `high` take it: 1024 + zero, -(64 + zero), twice each
+  static __device__ __forceinline__ uint32_t zero_low(uint32_t zero) { return 0x64006400u + zero * 0x10001u; }
+  static __device__ __forceinline__ uint32_t zero_high(uint32_t zero) { return 0xd400d400u + zero * 0x100010u; }
+  static __device__ __forceinline__ __half2 as(uint32_t v) { return *reinterpret_cast<const __half2 *>(&v); }
+  static __device__ __forceinline__ uint32_t low(uint32_t w, uint32_t z) {
+    const __half2 v = __hsub2(as((w & 0x000f000fu) | 0x64006400u), as(z));
     return *reinterpret_cast<const uint32_t *>(&v);
   }
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    paged::mma16816(d, a[0], a[1], a[2], a[3], b0, b1);
+  // (1024 + 16 code) / 16 - (64 + zero): nothing to round
+  static __device__ __forceinline__ uint32_t high(uint32_t w, uint32_t z) {
+    const __half2 v = __hfma2(as((w & 0x00f000f0u) | 0x64006400u), as(0x2c002c00u), as(z));
+    return *reinterpret_cast<const uint32_t *>(&v);
+  }
+  static __device__ __forceinline__ void mma(float (&d)[4], const float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                             uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   }
 };
 template <> struct Codes<__nv_bfloat16> {
-  static constexpr uint32_t ONE = 0x43004300u;  // 128, twice
-  static __device__ __forceinline__ uint32_t pair(uint32_t w, uint32_t zero) {
-    const uint32_t bits = (w & 0x000f000fu) | ONE;
-    const __nv_bfloat162 v =
-        __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&bits), *reinterpret_cast<const __nv_bfloat162 *>(&zero));
+  // 128 + zero, twice
+  static __device__ __forceinline__ uint32_t zero_low(uint32_t zero) { return 0x43004300u + zero * 0x10001u; }
+  static __device__ __forceinline__ uint32_t zero_high(uint32_t zero) { return zero_low(zero); }
+  static __device__ __forceinline__ __nv_bfloat162 as(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162 *>(&v); }
+  static __device__ __forceinline__ uint32_t low(uint32_t w, uint32_t z) {
+    const __nv_bfloat162 v = __hsub2(as((w & 0x000f000fu) | 0x43004300u), as(z));
     return *reinterpret_cast<const uint32_t *>(&v);
   }
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  static __device__ __forceinline__ uint32_t high(uint32_t w, uint32_t z) { return low(w >> 4, z); }
+  static __device__ __forceinline__ void mma(float (&d)[4], const float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                             uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   }
 };
 template <typename X> struct Operand { using type = __half; };  // 8-bit x
 template <> struct Operand<__nv_bfloat16> { using type = __nv_bfloat16; };
 
-__device__ __forceinline__ uint32_t load_shared4(uint32_t from) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
-  return v;
+// Copies `span` bytes of a row's scales or zero points from `from` on, BYTES a thread
+// and time.  Four at a time start with the word that holds the first.  What is past
+// the row, `until`, is not read: zeros.
+template <int BYTES>
+__device__ __forceinline__ void copy_row(uint32_t to, const uint8_t *array, int64_t from, int64_t until, int span, int first,
+                                         int step) {
+  if (BYTES == 4) from &= ~(int64_t)3;
+  for (int at = first * BYTES; at < span; at += step * BYTES) {
+    const int64_t left = until - from - at;
+    const int bytes = left >= BYTES ? BYTES : left > 0 ? (int)left : 0;
+    const uint8_t *source = left > 0 ? array + from + at : array;
+    if constexpr (BYTES == 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + at), "l"(source), "r"(bytes) : "memory");
+    else
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to + at), "l"(source), "n"(BYTES), "r"(bytes) : "memory");
+  }
 }
-__device__ __forceinline__ void copy_async4(uint32_t to, const void *from, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+// Arrives on the barrier once this thread's copies so far are done.
+__device__ __forceinline__ void arrive_after_copies(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 template <typename X, int NT> struct Layout {
-  static constexpr int WR = NT, WK = WARPS / WR;
-  static constexpr int R = 32 * WR, KS = 128 * WK;  // weight rows; columns of a stage
-  static constexpr int M = 8 * NT;                  // rows of x
-  static constexpr int CODES = R * KS / 2;
-  // x's rows in a stage, moved so that the rows a quarter (8-bit x: half) of a warp
-  // loads at once start in different banks
-  static constexpr int X_PITCH = KS * (int)sizeof(X) + 32 * (int)sizeof(X);
-  static constexpr int JOIN = WARPS * 32 * M * 4;  // the warps' sums, at the end
+  // Row tiles of a warp and steps of its slice of a stage: more rows where that leaves
+  // registers, as each step of x is loaded and unpacked once for all of them.
+  static constexpr int RT = NT == 4 ? 2 : 4, WSTEPS = 8 / RT;
+  static constexpr int WR = NT == 4 ? 4 : 1, WK = WARPS / WR;
+  static constexpr int R = 16 * RT * WR, KS = 32 * WSTEPS * WK;  // weight rows; columns of a stage
+  static constexpr int STEPS = KS / 32;                          // of 32 columns
+  static constexpr int M = 8 * NT;                               // rows of x
+  static constexpr int CODES = R * KS / 2, BOX = R * 128, BOXES = CODES / BOX;  // 128-byte columns of all rows
+  static constexpr int PITCH = R + 4, JOIN = WK * M * PITCH * 4;  // the warps' sums: lanes' stores in different banks
+  static constexpr int FACTORS = 16 * RT * WSTEPS * 16;           // a warp's scales and zero points, see Factor
   static_assert(CODES == 16384, "a stage's codes");
 };
 
-template <typename X, int NT>
-__global__ void __launch_bounds__(THREADS, 2) tiles_kernel(const __grid_constant__ Params p) {
+// What a row's group needs at its products: the scale, and the zero point as Codes takes it.
+struct alignas(16) Factor {
+  float scale;
+  uint32_t zero_low, zero_high, unused;
+};
+
+// Where the steps of a warp (or a stage) stand among the groups.
+struct Group {
+  uint32_t index, into;  // the group; steps into it
+  __device__ __forceinline__ Group(uint32_t step, uint32_t group32) : index(step / group32), into(step % group32) {}
+  __device__ __forceinline__ void advance(uint32_t quotient, uint32_t rest, uint32_t group32) {
+    index += quotient;
+    into += rest;
+    if (into >= group32) {
+      into -= group32;
+      ++index;
+    }
+  }
+};
+
+// After a wait gave up: the copies in flight, so that the block's shared memory is at
+// rest when it ends.  Nothing tells how far each stage's barrier went: both phases are
+// waited for, the later one until the limit.
+__device__ __noinline__ void settle(uint32_t full0, int ring) {
+  constexpr uint64_t limit_ns = 100000000ull;
+  if (threadIdx.x < (unsigned)ring) {
+    volatile int over = 0;
+    ptx::mbar_wait(full0 + 8u * threadIdx.x, 0, &over, limit_ns);
+    over = 0;
+    ptx::mbar_wait(full0 + 8u * threadIdx.x, 1, &over, limit_ns);
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ void add(float4 &a, const float4 &b) {
+  a.x += b.x;
+  a.y += b.y;
+  a.z += b.z;
+  a.w += b.w;
+}
+
+// GS: steps between two applications of a scale, a divisor of a group's and of a slice's
+template <typename X, int NT, int GS>
+__global__ void __launch_bounds__(THREADS, NT == 4 ? 1 : 2)
+tiles_kernel(const __grid_constant__ CUtensorMap tmap_codes, const __grid_constant__ CUtensorMap tmap_x,
+             const __grid_constant__ Params p) {
   using L = Layout<X, NT>;
   using F = typename Operand<X>::type;
-  constexpr int XS = sizeof(X);
-  extern __shared__ __align__(128) uint8_t smem[];
-  const uint32_t base = ptx::smem_u32(smem);
+  constexpr int XS = sizeof(X), RT = L::RT, SCALES = L::WSTEPS / GS;  // bytes of an element of x; scales of a row in a warp's slice
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = ptx::smem_u32(smem), bar0 = base + p.control;
+  if ((base & 1023u) != 0) {  // the swizzle needs it
+    record_error(NT_B200_ERR_INVALID_ARGUMENT);
+    return;
+  }
+  const auto full = [&](int slot) { return bar0 + 8u * slot; };
+  const auto empty = [&](int slot) { return bar0 + 8u * (MOST_RING + slot); };
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + p.control + CONTROL_BYTES - 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wr = warp % L::WR, wk = warp / L::WR, g = lane >> 2, c = lane & 3;
   const int part = (int)(blockIdx.x % (unsigned)p.parts);
-  const int64_t n0 = (int64_t)(blockIdx.x / (unsigned)p.parts) * L::R, m0 = (int64_t)blockIdx.y * L::M;
+  const uint32_t unit0 = blockIdx.x / (unsigned)p.parts;  // of weight rows; the next are the grid's clusters further on
+  const uint32_t units = (uint32_t)p.row_blocks, unit_step = gridDim.x / (uint32_t)p.parts;
+  const int64_t m0 = (int64_t)blockIdx.y * L::M;
   const int m_count = (int)(p.rows - m0 < L::M ? p.rows - m0 : L::M);
-  const int first = (int)((int64_t)p.stages * part / p.parts), last = (int)((int64_t)p.stages * (part + 1) / p.parts);
+  const int first = p.stages / p.parts * part + min(part, p.stages % p.parts);
+  const int last = first + p.stages / p.parts + (part < p.stages % p.parts ? 1 : 0);
   const int scale_size = float_size(p.scale_dtype);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.ring; ++s) {
+      ptx::mbar_init(full(s), 1 + p.copiers);
+      ptx::mbar_init(empty(s), WARPS);
+    }
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tmap(&tmap_codes);
+    ptx::prefetch_tmap(&tmap_x);
+  }
+  __syncthreads();
   wait_prior_grid();
 
-  // ---- copies of a stage
-  const auto copy = [&](int stage) {
-    const uint32_t slot = base + (uint32_t)((stage - first) % RING) * (uint32_t)p.stage_bytes;
-    const int64_t k0 = (int64_t)stage * L::KS;
-    constexpr int CHUNKS = L::KS / 32;  // 16-byte chunks of a weight row
+  // ---- copies of a stage: codes and x by TMA, scales and zero points by the first threads
+  const uint32_t stage_quotient = L::STEPS / p.group32, stage_rest = L::STEPS % p.group32;
+  const Group stage0((uint32_t)first * L::STEPS, p.group32), slice0((uint32_t)first * L::STEPS + wk * L::WSTEPS, p.group32);
+  uint32_t fill_unit = unit0, fill_phase = 1;
+  int fill_stage = first, fill_slot = 0;
+  Group fill_at = stage0;
+  const auto fill = [&]() {
+    if (fill_unit >= units || !ptx::mbar_wait(empty(fill_slot), fill_phase, abort_flag)) return;
+    const uint32_t to = base + (uint32_t)fill_slot * (uint32_t)p.stage_bytes, bar = full(fill_slot);
+    if (threadIdx.x == 0) {
+      ptx::mbar_arrive_expect_tx(bar, (uint32_t)(L::CODES + p.x_bytes));
 #pragma unroll
-    for (int i = 0; i < L::CODES / 16 / THREADS; ++i) {
-      const int at = threadIdx.x + i * THREADS, row = at / CHUNKS, q = at % CHUNKS;
-      const bool valid = n0 + row < p.outer && k0 + q * 32 < p.inner;
-      const uint8_t *from = valid ? p.codes + (n0 + row) * p.c_row + k0 / 2 + q * 16 : p.codes;
-      paged::copy_async16(slot + row * (L::KS / 2) + ((q & ~7) | ((q ^ row) & 7)) * 16, from, valid);
+      for (int b = 0; b < L::BOXES; ++b)
+        ptx::tma_load_2d(to + b * L::BOX, &tmap_codes, bar, fill_stage * (L::KS / 2) + b * 128, (int32_t)(fill_unit * L::R));
+      ptx::tma_load_3d(to + L::CODES, &tmap_x, bar, 0, (int32_t)m0, fill_stage * L::STEPS);
     }
-    constexpr int X_CHUNKS = L::KS * XS / 16;  // of a row of x
-    for (int at = threadIdx.x; at < m_count * X_CHUNKS; at += THREADS) {
-      const int m = at / X_CHUNKS, q = at % X_CHUNKS;
-      const int64_t k = k0 + q * (16 / XS);
-      const bool valid = k < p.inner;
-      const uint8_t *from = static_cast<const uint8_t *>(p.x) + ((m0 + m) * p.x_row + (valid ? k : 0)) * XS;
-      paged::copy_async16(slot + L::CODES + m * L::X_PITCH + q * 16, from, valid);
+    const int g0 = (int)fill_at.index;
+    fill_at.advance(stage_quotient, stage_rest, p.group32);
+    const int r = threadIdx.x % L::R, copier = threadIdx.x / L::R;
+    const int64_t row = (int64_t)fill_unit * L::R + r;
+    if (row < p.outer) {
+      const uint32_t s_to = to + L::CODES + p.x_bytes + r * p.s_pitch;
+      const int64_t s_from = (row * p.s_row + g0) * scale_size, s_until = (row * p.s_row + p.groups) * scale_size;
+      constexpr int STEP = THREADS / L::R;
+      if (p.s_copy == 16) copy_row<16>(s_to, p.scales, s_from, s_until, p.s_span, copier, STEP);
+      else if (p.s_copy == 8) copy_row<8>(s_to, p.scales, s_from, s_until, p.s_span, copier, STEP);
+      else copy_row<4>(s_to, p.scales, s_from, s_until, p.s_span, copier, STEP);
+      if (p.zeros) {
+        const uint32_t z_to = to + L::CODES + p.x_bytes + L::R * p.s_pitch + r * p.z_pitch;
+        const int64_t z_from = row * p.z_row + g0, z_until = row * p.z_row + p.groups;
+        if (p.z_copy == 16) copy_row<16>(z_to, p.zeros, z_from, z_until, p.z_span, copier, STEP);
+        else if (p.z_copy == 8) copy_row<8>(z_to, p.zeros, z_from, z_until, p.z_span, copier, STEP);
+        else copy_row<4>(z_to, p.zeros, z_from, z_until, p.z_span, copier, STEP);
+      }
     }
-    // scales and zero points: the words that hold a row's part, read no further
-    // than the row
-    const int row = threadIdx.x % L::R;
-    if (n0 + row < p.outer) {
-      const int g0 = (int)((uint32_t)k0 / (uint32_t)p.group);
-      const int g1 = min(p.groups, (int)((uint32_t)(k0 + L::KS + p.group - 1) / (uint32_t)p.group));
-      const auto words = [&](const uint8_t *array, int64_t row_stride, int size, int most, uint32_t to) {
-        const int64_t from = ((n0 + row) * row_stride + g0) * size, until = ((n0 + row) * row_stride + g1) * size;
-        const int64_t word0 = from & ~(int64_t)3;
-        for (int w = threadIdx.x / L::R; w < most; w += THREADS / L::R) {
-          const int64_t at = word0 + 4 * w;
-          if (at < until) copy_async4(to + 4 * w, array + at, (int)min((int64_t)4, until - at));
-        }
-      };
-      const uint32_t s_slot = slot + L::CODES + p.x_bytes;
-      words(p.scales, p.s_row, scale_size, p.scale_words, s_slot + 4 * row * p.scale_words);
-      if (p.zeros) words(p.zeros, p.z_row, 1, p.zero_words, s_slot + 4 * (L::R * p.scale_words + row * p.zero_words));
+    arrive_after_copies(bar);
+    if (++fill_slot == p.ring) {
+      fill_slot = 0;
+      fill_phase ^= 1u;
+    }
+    if (++fill_stage == last) {
+      fill_stage = first;
+      fill_unit += unit_step;
+      fill_at = stage0;
     }
   };
+  const bool copies = threadIdx.x < (unsigned)p.copiers;
+  if (copies)
+    for (int i = 0; i < p.ring - 1; ++i) fill();
 
-  float acc[2][NT][4] = {};
-  // ---- a warp's share of a stage
-  const auto consume = [&](int stage) {
-    const uint32_t slot_at = (uint32_t)((stage - first) % RING) * (uint32_t)p.stage_bytes;
-    const uint32_t slot = base + slot_at;
-    const int64_t k0 = (int64_t)stage * L::KS;
-    const uint32_t step0 = (uint32_t)(k0 / 32) + wk * 4;
-    uint32_t gi = step0 / p.group32, left = p.group32 - (step0 - gi * p.group32);  // steps to the group's end
-    const uint32_t g0 = (uint32_t)k0 / (uint32_t)p.group;
-    const uint8_t *s_slot = smem + slot_at + L::CODES + p.x_bytes;
-    const uint8_t *scale_at[4], *zero_at[4];
+  const uint32_t q0 = wk * L::WSTEPS;
+  const uint32_t code_row = (wr * 16 * RT + g) * 128 + (q0 / 8) * L::BOX + c * 4;
+  const uint32_t x_step = 32 * XS * p.x_rows, x_at = L::CODES + q0 * x_step + c * 8 * XS;
+  uint32_t x_row[NT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = wr * 32 + g + 8 * i;
-      const uint32_t s_mis = (uint32_t)(((n0 + row) * p.s_row + g0) * scale_size) & 3u;
-      scale_at[i] = s_slot + 4 * row * p.scale_words + s_mis;
-      const uint32_t z_mis = (uint32_t)((n0 + row) * p.z_row + g0) & 3u;
-      zero_at[i] = s_slot + 4 * (L::R * p.scale_words + row * p.zero_words) + z_mis;
-    }
-    uint32_t zero[4];
-    const auto load_zeros = [&]() {
+  for (int t = 0; t < NT; ++t) x_row[t] = min(t * 8 + g, p.x_rows - 1) * (32 * XS);  // (columns past the last are not written)
+  Factor *factors = reinterpret_cast<Factor *>(smem + p.join + L::JOIN + warp * L::FACTORS);  // [SCALES][16 * RT]
+  int slot = 0;
+  uint32_t phase = 0;
+  for (uint32_t unit = unit0; unit < units; unit += unit_step) {
+    const int64_t n0 = (int64_t)unit * L::R;
+    Group stage_at = stage0, slice_at = slice0;
+    float acc[RT][NT][4] = {};
+    // ---- a warp's slice of each stage: 16 RT rows, WSTEPS steps of 32 columns
+    for (int s = first; s < last; ++s) {
+      if (copies) fill();
+      if (!ptx::mbar_wait_warp(full(slot), phase, abort_flag)) break;
+      const uint8_t *stage = smem + (uint32_t)slot * (uint32_t)p.stage_bytes;
+      // a lane readies the factors of a row, or of two
+      {
+        constexpr int ROWS = RT / 2;
+        const auto ready = [&](auto value) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        zero[i] = Codes<F>::ONE | (p.zeros ? (uint32_t)zero_at[i][gi - g0] & 15u : 8u) * 0x10001u;
-    };
-    float sum[2][NT][4] = {};
-    load_zeros();
+          for (int i = 0; i < ROWS; ++i) {
+            const int r = wr * 16 * RT + lane + 32 * i;
+            const uint8_t *from = stage + L::CODES + p.x_bytes + r * p.s_pitch;
+            const uint8_t *zeros = stage + L::CODES + p.x_bytes + L::R * p.s_pitch + r * p.z_pitch;
+            // where a row's part starts in the first word of its copy
+            if (p.s_copy == 4) from += ((uint32_t)((n0 + r) * p.s_row) + stage_at.index) * (uint32_t)scale_size & 3u;
+            if (p.z_copy == 4) zeros += ((uint32_t)((n0 + r) * p.z_row) + stage_at.index) & 3u;
+            Group now = slice_at;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int q = wk * 4 + j;
-      // x: eight elements a lane, as the pairs (0, 4), (1, 5), (2, 6), (3, 7)
-      uint32_t b[NT][4];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int m = min(t * 8 + g, m_count - 1);  // columns past the last are not written
-        const uint32_t at = slot + L::CODES + m * L::X_PITCH + (q * 32 + c * 8) * XS;
-        uint4 v;
-        if constexpr (XS == 2) {
-          v = paged::load_shared16(at);
-        } else {
-          const uint2 w = paged::load_shared8(at);
-          paged::to_halves<X>(w.x, v.x, v.y);
-          paged::to_halves<X>(w.y, v.z, v.w);
-        }
-        b[t][0] = __byte_perm(v.x, v.z, 0x5410);
-        b[t][1] = __byte_perm(v.x, v.z, 0x7632);
-        b[t][2] = __byte_perm(v.y, v.w, 0x5410);
-        b[t][3] = __byte_perm(v.y, v.w, 0x7632);
+            for (int k = 0; k < SCALES; ++k) {
+              const uint32_t nth = now.index - stage_at.index;
+              const uint32_t zero = p.zeros ? zeros[nth] & 15u : 8u;
+              factors[k * 16 * RT + lane + 32 * i] =
+                  Factor{value(from + nth * scale_size), Codes<F>::zero_low(zero), Codes<F>::zero_high(zero), 0u};
+              now.advance(0, GS, p.group32);
+            }
+          }
+        };
+        if (p.scale_dtype == NT_B200_BFLOAT16)
+          ready([](const uint8_t *v) { return __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t *>(v) << 16); });
+        else if (p.scale_dtype == NT_B200_FLOAT16)
+          ready([](const uint8_t *v) { return __half2float(*reinterpret_cast<const __half *>(v)); });
+        else ready([](const uint8_t *v) { return *reinterpret_cast<const float *>(v); });
+        __syncwarp();
       }
+      float sum[RT][NT][4];
+      const float none[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = wr * 32 + r * 16 + g;
-        const uint32_t at = slot + row * (L::KS / 2) + ((q & ~7) | ((q ^ row) & 7)) * 16 + c * 4;
-        const uint32_t lo = load_shared4(at), hi = load_shared4(at + 8 * (L::KS / 2));
-        const uint32_t zl = zero[2 * r], zh = zero[2 * r + 1];
-        const uint32_t a0[4] = {Codes<F>::pair(lo, zl), Codes<F>::pair(hi, zh), Codes<F>::pair(lo >> 4, zl),
-                                Codes<F>::pair(hi >> 4, zh)};
-        const uint32_t a1[4] = {Codes<F>::pair(lo >> 8, zl), Codes<F>::pair(hi >> 8, zh), Codes<F>::pair(lo >> 12, zl),
-                                Codes<F>::pair(hi >> 12, zh)};
+      for (int j = 0; j < L::WSTEPS; ++j) {
+        // x: eight elements a lane, as the pairs (0, 4), (1, 5), (2, 6), (3, 7)
+        uint32_t b[NT][4];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          Codes<F>::mma(sum[r][t], a0, b[t][0], b[t][1]);
-          Codes<F>::mma(sum[r][t], a1, b[t][2], b[t][3]);
-        }
-      }
-      if (--left == 0 || j == 3) {
-        // (past the last column there are no scales, and all x are 0)
-        const bool some = gi < (uint32_t)p.groups;
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float lo = some ? any_float(scale_at[2 * r] + (gi - g0) * scale_size, p.scale_dtype) : 0.f;
-          const float hi = some ? any_float(scale_at[2 * r + 1] + (gi - g0) * scale_size, p.scale_dtype) : 0.f;
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            acc[r][t][0] = fmaf(lo, sum[r][t][0], acc[r][t][0]);
-            acc[r][t][1] = fmaf(lo, sum[r][t][1], acc[r][t][1]);
-            acc[r][t][2] = fmaf(hi, sum[r][t][2], acc[r][t][2]);
-            acc[r][t][3] = fmaf(hi, sum[r][t][3], acc[r][t][3]);
-            sum[r][t][0] = sum[r][t][1] = sum[r][t][2] = sum[r][t][3] = 0.f;
+          const uint8_t *from = stage + x_at + j * x_step + x_row[t];
+          if constexpr (XS == 2) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(from);
+            b[t][0] = __byte_perm(x.x, x.z, 0x5410);
+            b[t][1] = __byte_perm(x.x, x.z, 0x7632);
+            b[t][2] = __byte_perm(x.y, x.w, 0x5410);
+            b[t][3] = __byte_perm(x.y, x.w, 0x7632);
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2 *>(from);
+            paged::to_halves<X>(__byte_perm(x.x, x.y, 0x5140), b[t][0], b[t][1]);
+            paged::to_halves<X>(__byte_perm(x.x, x.y, 0x7362), b[t][2], b[t][3]);
           }
         }
-        if (left == 0) {
-          left = p.group32;
-          ++gi;
-          if (j < 3) load_zeros();
+        const uint8_t *codes = stage + code_row + (((q0 + j) ^ g) & 7) * 16;  // TMA's 128-byte swizzle of a row's 16-byte words
+        const Factor *factor = factors + (j / GS) * 16 * RT + g;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const uint32_t lo = *reinterpret_cast<const uint32_t *>(codes + r * 2048);
+          const uint32_t hi = *reinterpret_cast<const uint32_t *>(codes + r * 2048 + 1024);
+          const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
+          const Factor fl = factor[r * 16], fh = factor[r * 16 + 8];
+          const uint32_t a0[4] = {Codes<F>::low(lo, fl.zero_low), Codes<F>::low(hi, fh.zero_low),
+                                  Codes<F>::high(lo, fl.zero_high), Codes<F>::high(hi, fh.zero_high)};
+          const uint32_t a1[4] = {Codes<F>::low(lo8, fl.zero_low), Codes<F>::low(hi8, fh.zero_low),
+                                  Codes<F>::high(lo8, fl.zero_high), Codes<F>::high(hi8, fh.zero_high)};
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if (j % GS == 0) Codes<F>::mma(sum[r][t], none, a0, b[t][0], b[t][1]);
+            else Codes<F>::mma(sum[r][t], sum[r][t], a0, b[t][0], b[t][1]);
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t) Codes<F>::mma(sum[r][t], sum[r][t], a1, b[t][2], b[t][3]);
+          if (j % GS == GS - 1) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[r][t][e] = fmaf(e < 2 ? fl.scale : fh.scale, sum[r][t][e], acc[r][t][e]);
+          }
         }
       }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(empty(slot));
+      stage_at.advance(stage_quotient, stage_rest, p.group32);
+      slice_at.advance(stage_quotient, stage_rest, p.group32);
+      if (++slot == p.ring) {
+        slot = 0;
+        phase ^= 1u;
+      }
     }
-  };
+    if (unit + unit_step >= units) allow_dependent_launch();
 
-  for (int s = first; s < first + RING - 1; ++s) {
-    if (s < last) copy(s);
-    paged::copy_commit();
-  }
-  for (int s = first; s < last; ++s) {
-    paged::copy_wait<RING - 2>();
+    // ---- the warps' sums, [WK][M][R + 4], then the cluster's
+    float *joined = reinterpret_cast<float *>(smem + p.join);
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int m = t * 8 + 2 * c + (e & 1), row = wr * 16 * RT + r * 16 + g + (e >> 1) * 8;
+          joined[(wk * L::M + m) * L::PITCH + row] = acc[r][t][e];
+        }
     __syncthreads();
-    if (s + RING - 1 < last) copy(s + RING - 1);
-    paged::copy_commit();
-    consume(s);
-  }
-  allow_dependent_launch();
-  paged::copy_wait<0>();
-  __syncthreads();
-
-  // ---- the warps' sums, [WK][M][R], then the cluster's
-  float *joined = reinterpret_cast<float *>(smem);
+    const auto sum_of = [&](int at) {
+      float4 v = *reinterpret_cast<const float4 *>(joined + at);
 #pragma unroll
-  for (int r = 0; r < 2; ++r)
+      for (int k = 1; k < L::WK; ++k) add(v, *reinterpret_cast<const float4 *>(joined + k * L::M * L::PITCH + at));
+      return v;
+    };
+    const auto store = [&](int m, int row, const float4 &v) {
+      const float f[4] = {v.x, v.y, v.z, v.w};
+      const float by = p.x_scale ? p.x_scale[(m0 + m) * p.xs_stride] : 1.f;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int m = t * 8 + 2 * c + (e & 1), row = wr * 32 + r * 16 + g + (e >> 1) * 8;
-        joined[(wk * L::M + m) * L::R + row] = acc[r][t][e];
-      }
-  __syncthreads();
-  for (int at = threadIdx.x; at < L::M * L::R; at += THREADS) {
-    float v = joined[at];
-#pragma unroll
-    for (int w = 1; w < L::WK; ++w) v += joined[w * L::M * L::R + at];
-    joined[at] = v;
-  }
-  if (p.parts > 1) ptx::cluster_sync();
-  else __syncthreads();
-  for (int at = threadIdx.x + part * THREADS; at < L::M * L::R; at += THREADS * p.parts) {
-    const int m = at / L::R;
-    const int64_t n = n0 + at % L::R;
-    float v;
+      for (int e = 0; e < 4; ++e)
+        if (n0 + row + e < p.outer)
+          store_any(p.y, (m0 + m) * p.y_row + (n0 + row + e) * p.y_col, p.y_dtype, p.x_scale ? f[e] * by : f[e]);
+    };
+    constexpr int QUADS = L::R / 4;
     if (p.parts == 1) {
-      v = joined[at];
+      for (int i = threadIdx.x; i < m_count * QUADS; i += THREADS)
+        store(i / QUADS, i % QUADS * 4, sum_of(i / QUADS * L::PITCH + i % QUADS * 4));
+      __syncthreads();  // the sums are read: the next unit's may come
     } else {
-      v = 0.f;
-      for (int r = 0; r < p.parts; ++r) {
-        float other;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other) : "r"(ptx::mapa(base + 4 * at, r)) : "memory");
-        v += other;
+      // (a grid with parts has one unit a cluster)
+      for (int i = threadIdx.x; i < m_count * QUADS; i += THREADS) {
+        const int at = i / QUADS * L::PITCH + i % QUADS * 4;
+        *reinterpret_cast<float4 *>(joined + at) = sum_of(at);
       }
+      ptx::cluster_sync();
+      for (int i = threadIdx.x + part * THREADS; i < m_count * QUADS; i += THREADS * p.parts) {
+        const uint32_t from = base + p.join + 4 * (i / QUADS * L::PITCH + i % QUADS * 4);
+        float4 v[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r < p.parts)
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v[r].x), "=f"(v[r].y), "=f"(v[r].z), "=f"(v[r].w)
+                         : "r"(ptx::mapa(from, r)));
+#pragma unroll
+        for (int r = 1; r < 8; ++r)
+          if (r < p.parts) add(v[0], v[r]);
+        store(i / QUADS, i % QUADS * 4, v[0]);
+      }
+      ptx::cluster_sync();  // no block ends while another reads its sums
     }
-    if (m < m_count && n < p.outer)
-      store_any(p.y, (m0 + m) * p.y_row + n * p.y_col, p.y_dtype, p.x_scale ? v * p.x_scale[(m0 + m) * p.xs_stride] : v);
+    if (*abort_flag) break;  // (read by all after the same barrier)
   }
-  if (p.parts > 1) ptx::cluster_sync();  // no block ends while another reads its sums
+  __syncthreads();
+  if (*abort_flag) settle(bar0, p.ring);
 }
 
-template <typename X, int NT> int launch_tiles(Params p, cudaStream_t stream) {
+template <typename X, int NT, int GS> int launch_tiles(Params p, cudaStream_t stream) {
   using L = Layout<X, NT>;
-  const int size = float_size(p.scale_dtype);
-  const int in_stage = (L::KS + p.group - 1) / p.group + 1;  // groups that a stage can touch
-  p.scale_words = ((in_stage * size + 3) / 4 + 1) | 1;       // odd: rows in different banks
-  p.zero_words = p.zeros ? ((in_stage + 3) / 4 + 1) | 1 : 0;
-  const int64_t most = p.rows < L::M ? p.rows : L::M;
-  p.x_bytes = (int)most * L::X_PITCH;
-  p.stage_bytes = (L::CODES + p.x_bytes + 4 * L::R * (p.scale_words + p.zero_words) + 127) / 128 * 128;
+  constexpr int XS = sizeof(X);
+  tc::EncodeTiledFn encode = tc::encode_tiled_fn();
+  if (!encode) return tc::kNotEligible;
+  p.x_rows = (int)(p.rows < L::M ? p.rows : L::M);
+  p.x_bytes = p.x_rows * L::KS * XS;
+  // A row's scales in a stage: as wide a copy as every row and stage starts on; an odd
+  // number of 16 bytes apart, so that the rows that a warp reads lie in different banks.
+  const auto part = [&](const uint8_t *array, int64_t row_bytes, int size, int &copy, int &span, int &pitch) {
+    const int whole = L::KS % p.group == 0 ? L::KS / p.group * size : 0;  // 0: stages start within groups
+    copy = 16;
+    while (copy > 4 && (whole == 0 || whole % copy || row_bytes % copy || reinterpret_cast<uintptr_t>(array) % copy)) copy /= 2;
+    span = copy > 4 ? whole : ((L::KS + p.group - 1) / p.group + 1) * size + 3;
+    pitch = ((span + 18) / 16 | 1) * 16;
+    const int copies = (span + copy - 1) / copy;
+    return (copies < THREADS / L::R ? copies : THREADS / L::R) * L::R;
+  };
+  p.copiers = part(p.scales, p.s_row * float_size(p.scale_dtype), float_size(p.scale_dtype), p.s_copy, p.s_span, p.s_pitch);
+  if (p.zeros) {
+    const int more = part(p.zeros, p.z_row, 1, p.z_copy, p.z_span, p.z_pitch);
+    if (more > p.copiers) p.copiers = more;
+  }
+  p.stage_bytes = (L::CODES + p.x_bytes + L::R * (p.s_pitch + p.z_pitch) + 1023) / 1024 * 1024;
   p.stages = (int)((p.inner + L::KS - 1) / L::KS);
-  const int ring = RING * p.stage_bytes, bytes = ring > L::JOIN ? ring : L::JOIN;
-  constexpr int most_bytes = 232448;
+  // Stages on their way: what half of an SM's shared memory holds.
+  constexpr int half_bytes = 113 * 1024 - CONTROL_BYTES - L::JOIN - WARPS * L::FACTORS;
+  p.ring = half_bytes / p.stage_bytes;
+  if (p.ring > MOST_RING) p.ring = MOST_RING;
+  if (p.ring < 2) p.ring = 2;
+  p.join = p.ring * p.stage_bytes;
+  p.control = p.join + L::JOIN + WARPS * L::FACTORS;
+  const int bytes = p.control + CONTROL_BYTES;
+  constexpr int most_bytes = 220 * 1024;
   if (bytes > most_bytes) return tc::kNotEligible;
-  cudaError_t e = smem_optin<tiles_kernel<X, NT>>(most_bytes);
+  cudaError_t e = smem_optin<tiles_kernel<X, NT, GS>>(most_bytes);
   if (e != cudaSuccess) return (int)e;
+
+  CUtensorMap tmap_codes, tmap_x;
+  const cuuint32_t ones[3] = {1, 1, 1};
+  const cuuint64_t code_dims[2] = {(cuuint64_t)(p.inner / 2), (cuuint64_t)p.outer}, code_strides[1] = {(cuuint64_t)p.c_row};
+  const cuuint32_t code_box[2] = {128, (cuuint32_t)L::R};
+  // x as [steps][rows][32 columns]: a warp then reads its rows of a step side by side
+  const cuuint64_t x_dims[3] = {32, (cuuint64_t)p.rows, (cuuint64_t)(p.inner / 32)};
+  const cuuint64_t x_strides[2] = {(cuuint64_t)p.x_row * XS, 32 * XS};
+  const cuuint32_t x_box[3] = {32, (cuuint32_t)p.x_rows, (cuuint32_t)L::STEPS};
+  if (encode(&tmap_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(p.codes), code_dims, code_strides, code_box,
+             ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
+      encode(&tmap_x, XS == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(p.x),
+             x_dims, x_strides, x_box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return tc::kNotEligible;
+
   const int64_t row_blocks = (p.outer + L::R - 1) / L::R, m_blocks = (p.rows + L::M - 1) / L::M;
-  // Parts of the columns: as many as bring the grid to two blocks an SM, of two
-  // stages at least.
+  // Parts of the columns: as many as leave the grid in two blocks an SM.
+  const int64_t room = 2 * (int64_t)sm_count();
   int parts = 1;
-  while (parts < 8 && row_blocks * m_blocks * parts < 2 * sm_count() && p.stages >= 4 * parts) parts *= 2;
+  while (parts < 8 && row_blocks * m_blocks * parts * 2 <= room && p.stages >= 2 * parts) parts *= 2;
   p.parts = parts;
-  if (row_blocks * parts > (1LL << 31) - 1 || m_blocks > 65535) return NT_B200_ERR_INVALID_ARGUMENT;
+  p.row_blocks = row_blocks;
+  int64_t grid = row_blocks;
+  if (grid * m_blocks > room) grid = (room + m_blocks - 1) / m_blocks < grid ? (room + m_blocks - 1) / m_blocks : grid;
+  if (m_blocks > 65535) return NT_B200_ERR_INVALID_ARGUMENT;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(row_blocks * parts), (unsigned)m_blocks);
+  cfg.gridDim = dim3((unsigned)(grid * parts), (unsigned)m_blocks);
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = stream;
@@ -383,22 +555,33 @@ template <typename X, int NT> int launch_tiles(Params p, cudaStream_t stream) {
   attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attrs[0].val.programmaticStreamSerializationAllowed = 1;
   attrs[1].id = cudaLaunchAttributeClusterDimension;
-  attrs[1].val.clusterDim = {(unsigned)parts, 1, 1};
+  attrs[1].val.clusterDim.x = (unsigned)parts;
+  attrs[1].val.clusterDim.y = 1;
+  attrs[1].val.clusterDim.z = 1;
   cfg.attrs = attrs;
   cfg.numAttrs = parts > 1 ? 2 : 1;
-  return (int)cudaLaunchKernelEx(&cfg, tiles_kernel<X, NT>, p);
+  return (int)cudaLaunchKernelEx(&cfg, tiles_kernel<X, NT, GS>, tmap_codes, tmap_x, p);
+}
+template <typename X, int NT> int launch_groups(const Params &p, cudaStream_t stream) {
+  if constexpr (Layout<X, NT>::WSTEPS % 4 == 0)
+    if (p.group32 % 4 == 0) return launch_tiles<X, NT, 4>(p, stream);
+  if (p.group32 % 2 == 0) return launch_tiles<X, NT, 2>(p, stream);
+  return launch_tiles<X, NT, 1>(p, stream);
 }
 
-template <typename X> int launch(const Params &p, cudaStream_t stream) {
+template <typename X> int launch(Params p, cudaStream_t stream) {
   if constexpr (sizeof(X) <= 2) {
+    // (a single row's stride is never used)
+    if (p.rows == 1) p.x_row = p.inner;
+    if (p.outer == 1) p.c_row = p.inner / 2;
     const bool aligned = rotary::aligned16(p.x) && rotary::aligned16(p.codes) && p.x_col == 1 && p.c_col == 1 &&
                          p.s_col == 1 && (!p.zeros || p.z_col == 1) && (p.x_row * (int64_t)sizeof(X)) % 16 == 0 &&
-                         p.c_row % 16 == 0 && p.c_row >= 0 && p.s_row >= 0 && p.z_row >= 0 &&
+                         p.c_row % 16 == 0 && p.c_row > 0 && p.x_row > 0 && p.s_row >= 0 && p.z_row >= 0 &&
                          reinterpret_cast<uintptr_t>(p.scales) % 4 == 0 && reinterpret_cast<uintptr_t>(p.zeros) % 4 == 0;
-    if (aligned && p.inner <= (1LL << 30) && (p.rows + 31) / 32 <= 65535) {
-      const int rc = p.rows <= 8    ? launch_tiles<X, 1>(p, stream)
-                     : p.rows <= 16 ? launch_tiles<X, 2>(p, stream)
-                                    : launch_tiles<X, 4>(p, stream);
+    if (aligned && p.inner <= (1LL << 30) && p.outer <= (1LL << 30) && (p.rows + 31) / 32 <= 65535) {
+      const int rc = p.rows <= 8    ? launch_groups<X, 1>(p, stream)
+                     : p.rows <= 16 ? launch_groups<X, 2>(p, stream)
+                                    : launch_groups<X, 4>(p, stream);
       if (rc != tc::kNotEligible) return rc;
     }
   }

@@ -13,6 +13,7 @@
 #include "paged_append.cuh"
 #include "paged_attention.cuh"
 #include "prompt_attention.cuh"
+#include "chunk_attention.cuh"
 #include "rms_norm.cuh"
 #include "int4_matmul.cuh"
 #include "conv_no_alloc.cu"

@@ -118,15 +118,10 @@ __device__ __forceinline__ int page_of(const Attention &a, int64_t b, int64_t co
 // Every FAR_KEYS keys the sums go over to others: beside a weight of 1, what weights
 // of 2^-25 and less add one by one is lost.
 constexpr int kMostDim = 256, FAR_KEYS = 256;
+// The row of query head h in sequence b, which sees the first `limit` tokens; a warp.
 template <typename T, typename C>
-__global__ void __launch_bounds__(128) attention_rows_kernel(Attention a) {
+__device__ __forceinline__ void attend_row(const Attention &a, int64_t b, int h, int64_t limit, const T *q, T *out, float *lse) {
   const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= (int64_t)a.batch * a.queries * a.heads) return;
-  const int h = (int)(row % a.heads), i = (int)(row / a.heads % a.queries);
-  const int64_t b = row / a.heads / a.queries;
-  const int64_t limit = cached_length(a, b) - a.queries + 1 + i;
-  const T *q = static_cast<const T *>(a.query) + b * a.q_batch + i * a.q_token + h * a.q_head;
   constexpr int E = kMostDim / 32;
   float qv[E], acc[E], far[E];
 #pragma unroll
@@ -180,13 +175,23 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(Attention a) {
     }
   }
   l += l_far;
-  T *out = static_cast<T *>(a.out) + b * a.o_batch + i * a.o_token + h * a.o_head;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int d = lane + 32 * e;
     if (d < a.head_dim) out[d * a.o_dim] = from_f<T>(l == 0.f ? 0.f : (acc[e] + far[e]) / l);
   }
-  if (a.lse && lane == 0) a.lse[b * a.l_batch + i * a.l_token + h * a.l_head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (lse && lane == 0) *lse = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+template <typename T, typename C>
+__global__ void __launch_bounds__(128) attention_rows_kernel(Attention a) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= (int64_t)a.batch * a.queries * a.heads) return;
+  const int h = (int)(row % a.heads), i = (int)(row / a.heads % a.queries);
+  const int64_t b = row / a.heads / a.queries;
+  attend_row<T, C>(a, b, h, cached_length(a, b) - a.queries + 1 + i,
+                   static_cast<const T *>(a.query) + b * a.q_batch + i * a.q_token + h * a.q_head,
+                   static_cast<T *>(a.out) + b * a.o_batch + i * a.o_token + h * a.o_head,
+                   a.lse ? a.lse + b * a.l_batch + i * a.l_token + h * a.l_head : nullptr);
 }
 
 // ---------------------------------------------------------------- tensor cores

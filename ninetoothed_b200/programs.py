@@ -550,6 +550,8 @@ def copy(dst, src):
 
 # --------------------------------------------------------------------- serving operators
 from ninetoothed_b200.serving import (  # noqa: E402
+    chunk_attention,
+    chunk_attention_kernel,
     int4_matmul,
     int4_matmul_kernel,
     int4_quantize,
@@ -581,6 +583,8 @@ __all__ = [
     "to_padded_tensor",
     "attention",
     "attention_kernel",
+    "chunk_attention",
+    "chunk_attention_kernel",
     "conv2d",
     "conv2d_kernel",
     "conv2d_max_pool2d",

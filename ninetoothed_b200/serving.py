@@ -438,6 +438,84 @@ def prompt_attention(query, key, value, offsets, key_offsets=None, is_causal=Tru
     return (output, lse) if return_lse else output
 
 
+# --------------------------------------------------------------------- attention of chunks over the cache
+_chunk_values = itemgetter("query", "output", "lse", "offsets", "lengths", "block_table")
+
+
+def _launch_chunk_attention(v, stream):
+    query, out, lse, offsets, lengths, table = _chunk_values(v)
+    check_same_dtype(v, ("query", "output"))
+    check_same_dtype(v, ("offsets", "lengths", "block_table"))
+    cache = _cache_args(v)
+    tokens, heads, dim = query.shape
+    kv_heads, cache_dim = cache[5], cache[7]
+    batch = lengths.shape[0]
+    if out.shape != query.shape or dim != cache_dim or not kv_heads or heads % kv_heads:
+        raise TypeError(
+            f"chunk_attention query {tuple(query.shape)}, cache {tuple(v['key_cache'].shape)} and output "
+            f"{tuple(out.shape)} disagree."
+        )
+    if dim > 256:
+        raise TypeError("Kernel argument `query` has head dimension above the upper bound 256.")
+    if offsets.shape[0] != batch + 1 or table.shape[0] != batch:
+        raise TypeError(f"chunk_attention needs {batch + 1} offsets and {batch} block table rows.")
+    if lse is not None and lse.shape != query.shape[:2]:
+        raise TypeError("chunk_attention lse must have the query's shape without the head dimension.")
+    lib = _lib.library()
+    nbytes = lib.nt_b200_chunk_attention_workspace_size()
+    workspace = query.new_empty(nbytes, dtype=torch.uint8)
+    args = _lib.pack_args(
+        *cache, query.data_ptr(), offsets.data_ptr(), lengths.data_ptr(), table.data_ptr(), out.data_ptr(),
+        0 if lse is None else lse.data_ptr(), workspace.data_ptr(), nbytes, tokens, batch, heads, table.shape[1],
+        *query.stride(), *out.stride(), *((0, 0) if lse is None else lse.stride()), offsets.stride(0),
+        lengths.stride(0), *table.stride(), dtype_code(query.dtype), dtype_code(lengths.dtype),
+        scale=_scale(v["scale"], dim),
+    )
+    return lib.nt_b200_chunk_attention(args, stream)
+
+
+chunk_attention_kernel = Kernel(
+    name="chunk_attention",
+    args=(
+        TensorArg("query", 3),
+        *_CACHE_ARGS,
+        TensorArg("block_table", 2, INDEX_DTYPES),
+        TensorArg("offsets", 1, INDEX_DTYPES),
+        TensorArg("lengths", 1, INDEX_DTYPES),
+        TensorArg("output", 3),
+        TensorArg("lse", 2, _F32, optional=True),
+    ),
+    outputs=("output",),
+    launch=_launch_chunk_attention,
+    meta=("scale",),
+    meta_defaults={"scale": None, "lse": None},
+)
+
+
+def chunk_attention(query, key_cache, value_cache, key_scale, value_scale, block_table, offsets, lengths, scale=None,
+                    return_lse=False):
+    """Causal attention of the next pieces of prompts over the paged 8-bit cache that
+    holds them (`paged_append`); tokens of a page outside the pool are not seen.
+
+    `query` [tokens, heads, head_dim]: the new tokens of all sequences one after
+    another, sequence s from offsets[s] to offsets[s + 1] (`offsets`: batch + 1
+    entries); they are the last of its lengths[s] cached tokens, and each sees the
+    tokens up to itself.  Query head h reads key/value head h // (heads // kv_heads).
+    `scale` is 1 / sqrt(head_dim) by default.  Returns the output, in the query's
+    shape and dtype, or with `return_lse` (output, lse): the fp32 natural logarithm
+    of each query's sum of exponentials [tokens, heads].  A query that sees no token
+    gets 0, and -inf as its lse; tokens that belong to no sequence are not written."""
+    result = _bound("chunk_attention", query, key_cache, value_cache, key_scale, value_scale, block_table, offsets,
+                    lengths, scale, return_lse)
+    if result is not None:
+        return result
+    output = torch.empty_like(query, memory_format=torch.contiguous_format)
+    lse = query.new_empty(query.shape[:2], dtype=torch.float32) if return_lse else None
+    chunk_attention_kernel(query, key_cache, value_cache, key_scale, value_scale, block_table, offsets, lengths, output,
+                           lse, scale=scale)
+    return (output, lse) if return_lse else output
+
+
 # --------------------------------------------------------------------- norm
 _norm_values = itemgetter("input", "residual", "weight", "output", "total", "scale")
 
@@ -632,6 +710,8 @@ def int4_matmul(input, codes, scales, zeros=None, input_scale=None):
 __all__ = [
     "CODE_DTYPES",
     "INDEX_DTYPES",
+    "chunk_attention",
+    "chunk_attention_kernel",
     "int4_matmul",
     "int4_matmul_kernel",
     "int4_quantize",
