@@ -168,8 +168,9 @@ def binding():
                 if module is None:
                     _binding = False
                 else:
-                    names = ("rotary", "paged_append", "paged_attention", "prompt_attention",
-                             "paged_attention_workspace_size", "prompt_attention_workspace_size")
+                    names = ("rotary", "paged_append", "paged_attention", "prompt_attention", "chunk_attention",
+                             "rms_norm", "int4_matmul", "paged_attention_workspace_size",
+                             "prompt_attention_workspace_size", "chunk_attention_workspace_size")
                     module.bind(*(ctypes.cast(getattr(lib, f"nt_b200_{name}"), _P).value for name in names))
                     _binding = module
     return _binding or None

@@ -11,6 +11,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -22,8 +23,12 @@ decltype(&nt_b200_rotary) rotary_entry;
 decltype(&nt_b200_paged_append) append_entry;
 decltype(&nt_b200_paged_attention) paged_entry;
 decltype(&nt_b200_prompt_attention) prompt_entry;
+decltype(&nt_b200_chunk_attention) chunk_entry;
+decltype(&nt_b200_rms_norm) norm_entry;
+decltype(&nt_b200_int4_matmul) int4_entry;
 decltype(&nt_b200_paged_attention_workspace_size) paged_workspace;
 decltype(&nt_b200_prompt_attention_workspace_size) prompt_workspace;
+decltype(&nt_b200_chunk_attention_workspace_size) chunk_workspace;
 
 // The tensors of a call: all strided CUDA tensors of the current device.
 struct Call {
@@ -288,14 +293,169 @@ PyObject *prompt_attention(PyObject *, PyObject *const *o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// chunk_attention(query, key_cache, value_cache, key_scale, value_scale,
+// block_table, offsets, lengths, scale, return_lse)
+PyObject *chunk_attention(PyObject *, PyObject *const *o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  bool return_lse;
+  if (n != 10 || !chunk_entry || !flag(o[9], return_lse)) return none();
+  Call call;
+  const at::Tensor &q = call.tensor(o[0], 3), &table = call.tensor(o[5], 2), &offsets = call.tensor(o[6], 1);
+  const at::Tensor &lengths = call.tensor(o[7], 1);
+  NtB200ChunkAttentionArgs a{};
+  if (!cache_of(call, o + 1, a.cache) || !is_float(q) || q.numel() == 0 || q.size(2) != a.cache.head_dim || q.size(2) > 256 ||
+      q.size(1) % a.cache.kv_heads || !is_index(lengths) || table.scalar_type() != lengths.scalar_type() ||
+      offsets.scalar_type() != lengths.scalar_type() || offsets.size(0) != lengths.size(0) + 1 ||
+      table.size(0) != lengths.size(0) || !scale_of(o[8], q.size(2), a.scale))
+    return none();
+  Released released;
+  at::Tensor out = like(q), lse;
+  if (return_lse) {
+    lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+    a.lse = static_cast<float *>(lse.data_ptr());
+    strides(lse, a.lse_strides);
+  }
+  a.workspace_bytes = chunk_workspace();
+  at::Tensor workspace = at::empty({a.workspace_bytes}, q.options().dtype(at::kByte));
+  a.query = q.data_ptr(); a.offsets = offsets.data_ptr(); a.lengths = lengths.data_ptr(); a.block_table = table.data_ptr();
+  a.output = out.data_ptr(); a.workspace = workspace.data_ptr();
+  a.tokens = q.size(0); a.batch = lengths.size(0); a.heads = q.size(1); a.table_columns = table.size(1);
+  strides(q, a.query_strides); strides(out, a.output_strides); strides(table, a.block_table_strides);
+  a.offsets_stride = offsets.stride(0); a.lengths_stride = lengths.stride(0);
+  a.dtype = code_of(q); a.index_dtype = code_of(lengths);
+  const int code = chunk_entry(&a, call.stream());
+  released.reset();
+  return code ? PyLong_FromLong(code) : with_lse(out, lse);
+  END_HANDLE_TH_ERRORS
+}
+
+// A whole number, or none; false if it is neither.
+bool whole(PyObject *o, int64_t none, int64_t &value) {
+  if (o == Py_None) {
+    value = none;
+    return true;
+  }
+  if (!PyLong_CheckExact(o)) return false;
+  value = PyLong_AsLongLong(o);
+  if (value == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return true;
+}
+
+// rms_norm(input, weight, residual, eps, code_dtype, group)
+PyObject *rms_norm(PyObject *, PyObject *const *o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !norm_entry || !PyFloat_Check(o[3])) return none();
+  Call call;
+  const bool adds = o[2] != Py_None, codes = o[4] != Py_None;
+  const at::Tensor &x = call.tensor(o[0], 2), &w = call.tensor(o[1], 1);
+  if (!call.good || !is_float(x) || x.numel() == 0 || w.size(0) != x.size(1) || x.size(1) > 131072 ||
+      (w.scalar_type() != x.scalar_type() && w.scalar_type() != at::kFloat))
+    return none();
+  NtB200RmsNormArgs a{};
+  a.eps = PyFloat_AS_DOUBLE(o[3]);
+  at::ScalarType out_type = x.scalar_type();
+  const int64_t width = x.size(1);
+  if (!(a.eps >= 0) || !whole(o[5], 0, a.group) || a.group < 0 || (!codes && o[5] != Py_None)) return none();
+  if (codes) {
+    if (!THPDtype_Check(o[4])) return none();
+    out_type = reinterpret_cast<THPDtype *>(o[4])->scalar_type;
+    if (out_type != at::kChar && out_type != at::kFloat8_e4m3fn) return none();
+    if (o[5] != Py_None && a.group < width && (a.group == 0 || a.group % 16)) return none();
+  }
+  if (o[5] == Py_None || a.group > width) a.group = width;
+  const at::Tensor *residual = nullptr;
+  if (adds) {
+    const at::Tensor &r = call.tensor(o[2], 2);
+    if (!call.good || r.scalar_type() != x.scalar_type() || r.sizes() != x.sizes()) return none();
+    residual = &r;
+  }
+  Released released;
+  at::Tensor out = at::empty(x.sizes(), x.options().dtype(out_type)), scale, total;
+  if (codes) {
+    scale = at::empty({x.size(0), (width + a.group - 1) / a.group}, x.options().dtype(at::kFloat));
+    a.scale = static_cast<float *>(scale.data_ptr());
+    strides(scale, a.scale_strides);
+  }
+  if (residual) {
+    total = like(x);
+    a.residual = residual->data_ptr(); a.total = total.data_ptr();
+    strides(*residual, a.residual_strides); strides(total, a.total_strides);
+  }
+  a.input = x.data_ptr(); a.weight = w.data_ptr(); a.output = out.data_ptr();
+  a.rows = x.size(0); a.width = width;
+  strides(x, a.input_strides); strides(out, a.output_strides);
+  a.weight_stride = w.stride(0);
+  a.dtype = code_of(x); a.weight_dtype = code_of(w); a.output_dtype = code_of(out);
+  const int code = norm_entry(&a, call.stream());
+  released.reset();
+  if (code) return PyLong_FromLong(code);
+  if (!codes && !residual) return THPVariable_Wrap(out);
+  PyObject *parts[3] = {THPVariable_Wrap(out), nullptr, nullptr};
+  int count = 1;
+  if (codes) parts[count++] = THPVariable_Wrap(scale);
+  if (residual) parts[count++] = THPVariable_Wrap(total);
+  PyObject *all = nullptr;
+  if (parts[0] && parts[1] && (count < 3 || parts[2]))
+    all = count == 2 ? PyTuple_Pack(2, parts[0], parts[1]) : PyTuple_Pack(3, parts[0], parts[1], parts[2]);
+  for (PyObject *part : parts) Py_XDECREF(part);
+  return all;
+  END_HANDLE_TH_ERRORS
+}
+
+// int4_matmul(input, codes, scales, zeros, input_scale)
+PyObject *int4_matmul(PyObject *, PyObject *const *o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5 || !int4_entry) return none();
+  Call call;
+  const at::Tensor &x = call.tensor(o[0], 2), &codes = call.tensor(o[1], 2), &scales = call.tensor(o[2], 2);
+  if (!call.good || x.numel() == 0 || codes.numel() == 0 || scales.numel() == 0 || codes.scalar_type() != at::kByte ||
+      !is_float(scales))
+    return none();
+  const bool eight = x.scalar_type() == at::kChar || x.scalar_type() == at::kFloat8_e4m3fn;
+  const int64_t inner = x.size(1), groups = scales.size(1);
+  if ((!eight && !is_float(x)) || codes.size(0) != scales.size(0) || codes.size(1) != inner / 2 || inner % groups ||
+      inner / groups % 32)
+    return none();
+  NtB200Int4MatmulArgs a{};
+  if (o[3] != Py_None) {
+    const at::Tensor &zeros = call.tensor(o[3], 2);
+    if (!call.good || zeros.scalar_type() != at::kByte || zeros.sizes() != scales.sizes()) return none();
+    a.zeros = zeros.data_ptr();
+    strides(zeros, a.zeros_strides);
+  }
+  if (o[4] != Py_None) {
+    if (!THPVariable_Check(o[4])) return none();
+    const int64_t dim = THPVariable_Unpack(o[4]).dim();
+    const at::Tensor &by = call.tensor(o[4], dim);
+    if (!call.good || by.scalar_type() != at::kFloat || dim < 1 || dim > 2 || by.size(0) != x.size(0) ||
+        (dim == 2 && by.size(1) != 1))
+      return none();
+    a.input_scale = static_cast<const float *>(by.data_ptr());
+    a.input_scale_stride = by.stride(0);
+  }
+  Released released;
+  at::Tensor out = at::empty({x.size(0), scales.size(0)}, x.options().dtype(eight ? scales.scalar_type() : x.scalar_type()));
+  a.input = x.data_ptr(); a.codes = codes.data_ptr(); a.scales = scales.data_ptr(); a.output = out.data_ptr();
+  a.rows = x.size(0); a.inner = inner; a.outer = scales.size(0); a.group = inner / groups;
+  strides(x, a.input_strides); strides(codes, a.codes_strides); strides(scales, a.scales_strides); strides(out, a.output_strides);
+  a.dtype = code_of(x); a.scales_dtype = code_of(scales); a.output_dtype = code_of(out);
+  const int code = int4_entry(&a, call.stream());
+  released.reset();
+  return code ? PyLong_FromLong(code) : THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(addresses of the library's entry points, in the order above)
 PyObject *bind(PyObject *, PyObject *const *o, Py_ssize_t n) {
-  if (n != 6) {
-    PyErr_SetString(PyExc_TypeError, "bind takes six addresses");
+  if (n != 10) {
+    PyErr_SetString(PyExc_TypeError, "bind takes ten addresses");
     return nullptr;
   }
-  void *at[6];
-  for (int i = 0; i < 6; ++i) {
+  void *at[10];
+  for (int i = 0; i < 10; ++i) {
     at[i] = PyLong_AsVoidPtr(o[i]);
     if (PyErr_Occurred()) return nullptr;
   }
@@ -303,8 +463,12 @@ PyObject *bind(PyObject *, PyObject *const *o, Py_ssize_t n) {
   append_entry = reinterpret_cast<decltype(append_entry)>(at[1]);
   paged_entry = reinterpret_cast<decltype(paged_entry)>(at[2]);
   prompt_entry = reinterpret_cast<decltype(prompt_entry)>(at[3]);
-  paged_workspace = reinterpret_cast<decltype(paged_workspace)>(at[4]);
-  prompt_workspace = reinterpret_cast<decltype(prompt_workspace)>(at[5]);
+  chunk_entry = reinterpret_cast<decltype(chunk_entry)>(at[4]);
+  norm_entry = reinterpret_cast<decltype(norm_entry)>(at[5]);
+  int4_entry = reinterpret_cast<decltype(int4_entry)>(at[6]);
+  paged_workspace = reinterpret_cast<decltype(paged_workspace)>(at[7]);
+  prompt_workspace = reinterpret_cast<decltype(prompt_workspace)>(at[8]);
+  chunk_workspace = reinterpret_cast<decltype(chunk_workspace)>(at[9]);
   Py_RETURN_NONE;
 }
 
@@ -314,6 +478,9 @@ PyMethodDef methods[] = {
     {"paged_append", reinterpret_cast<PyCFunction>(paged_append), METH_FASTCALL, nullptr},
     {"paged_attention", reinterpret_cast<PyCFunction>(paged_attention), METH_FASTCALL, nullptr},
     {"prompt_attention", reinterpret_cast<PyCFunction>(prompt_attention), METH_FASTCALL, nullptr},
+    {"chunk_attention", reinterpret_cast<PyCFunction>(chunk_attention), METH_FASTCALL, nullptr},
+    {"rms_norm", reinterpret_cast<PyCFunction>(rms_norm), METH_FASTCALL, nullptr},
+    {"int4_matmul", reinterpret_cast<PyCFunction>(int4_matmul), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -18,12 +18,12 @@
 // cut falls into a unit, its pieces leave (o, m, l) in a workspace and a second kernel
 // joins them, in the line's order.
 //
-// Persistent, one CTA an SM, 12 warps:
+// Persistent, one CTA an SM, 16 warps:
 //   warp 0      tensor memory, and the MMAs from one thread: S_t = Q_t K_j^T, O_t +=
 //               P_t V_j with P_t read from tensor memory;
-//   warps 1-3   read pages, turn codes into fp16 (exact for both types) and store them
+//   warps 1-7   read pages, turn codes into fp16 (exact for both types) and store them
 //               into a ring of 5 blocks as the MMAs read them;
-//   warps 4-11  softmax, 4 warps a tile, a thread a row; a unit's queries at its start.
+//   warps 8-15  softmax, 4 warps a tile, a thread a row; a unit's queries at its start.
 // Both operands are fp16: a query row is scaled by a power of two to a largest element in
 // [2^14, 2^15), which leaves elements down to 2^-28 of it all their bits, and P is rounded
 // to fp16 (11 bits) relative to the largest weight p * value_scale of its row, 2^9 above
@@ -204,7 +204,7 @@ struct Item {
   int32_t batch, head;
   int32_t from, until, blocks;  // the share's key blocks, of the unit's
   int64_t end;                  // of the unit in the line
-  __device__ __forceinline__ Item(const Problem &p, const Piece &piece, const Walk &w) {
+  __device__ __forceinline__ void take(const Problem &p, const Piece &piece, const Walk &w) {
     const int pair = 2 * p.per_tile, first = w.pair * pair;
     q0 = w.seq.q0 + first;
     queries = min(w.seq.n - first, pair);
@@ -225,20 +225,37 @@ struct Item {
   }
   __device__ __forceinline__ bool whole() const { return from == 0 && until == blocks; }
 };
-// The items of a piece, all lanes of a warp together: f(item) is false where a wait
-// gave up.
+// The items of a piece, all lanes of a warp together.  Where a walk stands lies in
+// memory: in registers it would take them from the roles' loops.
+__device__ __noinline__ void begin_items(const Problem &p, const Piece &piece, Walk *w) {
+  w->seq.pairs = 0;
+  if (piece.start < piece.end) w->begin(p, piece);
+}
+__device__ __noinline__ bool next_item(const Problem &p, const Piece &piece, Walk *state, Item *item) {
+  Walk w = *state;
+  bool some = false;
+  while (!some && w.seq.pairs > 0 && w.pos < piece.end) {
+    item->take(p, piece, w);
+    w.next(p);
+    some = item->from < item->until;
+  }
+  *state = w;
+  return some;
+}
+// f(item) is false where a wait gave up.
 template <typename F>
 __device__ __forceinline__ void each_item(const Problem &p, const Piece &piece, F f) {
-  if (piece.start >= piece.end) return;
-  Walk w;
-  for (w.begin(p, piece); w.pos < piece.end && w.seq.pairs > 0; w.next(p)) {
-    const Item item(p, piece, w);
-    if (item.from < item.until && !f(item)) return;
+  Walk walk;
+  Item next;
+  begin_items(p, piece, &walk);
+  while (next_item(p, piece, &walk, &next)) {
+    const Item item = next;  // (a copy that no address is taken of stays in registers)
+    if (!f(item)) return;
   }
 }
 
 // ---------------------------------------------------------------- shared memory, workspace
-constexpr int RING = 5, CONVERTERS = 3, SOFTMAX_WARPS = 8, WARPS = 1 + CONVERTERS + SOFTMAX_WARPS, THREADS = WARPS * 32;
+constexpr int RING = 5, CONVERTERS = 7, SOFTMAX_WARPS = 8, WARPS = 1 + CONVERTERS + SOFTMAX_WARPS, THREADS = WARPS * 32;
 constexpr int GROUPS = BN / 16;  // of 16 tokens in a block: a page's or a part of one
 constexpr int TMEM_COLS = 512, SCALE_SLOTS = 4, NOTE_SLOTS = 3;
 
@@ -379,174 +396,191 @@ __device__ __noinline__ void find_piece(const Problem &p, Piece *out, int64_t *s
 }
 
 // ---------------------------------------------------------------- pages to operands
-// A group of 16 tokens on its way: asked for, then converted.
-struct Asked {
-  int32_t group;      // of the sequence
-  int32_t page;       // -1: outside the pool
-  int32_t ring;       // block's place in the ring; odd: values
-  int32_t item, head;
-  int32_t keys;       // of the sequence
-};
+// Four E4M3 codes: the top bit of each byte that is NaN, among others; the codes with 0
+// for NaN.
+__device__ __forceinline__ uint32_t nan_bits(uint32_t w) { return (w & 0x7f7f7f7fu) + 0x01010101u; }
+__device__ __forceinline__ uint32_t without_nan(uint32_t w) { return w & ~(((nan_bits(w) & 0x80808080u) >> 7) * 0xffu); }
 
-template <typename C> __device__ __forceinline__ bool has_nan(uint32_t w) {
-  return std::is_same<C, __nv_fp8_e4m3>::value && (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+// Takes the NaN codes out of a lane's word of a token's value, and notes the first key
+// with one for each element of the head.  A full warp; false where a wait gave up.
+template <int DP, int LOADS>
+__device__ __noinline__ bool take_out(const Control<DP> &c, const Problem &p, uint4 (&x)[LOADS], int item, int key0, int key_step,
+                                      int element0) {
+  const int lane = threadIdx.x & 31, me = (threadIdx.x >> 5) - 1, slot = item % NOTE_SLOTS;
+  int *notes = c.notes(p, slot, me);
+  if (*c.stamp(slot, me) != item) {
+    if (!ptx::mbar_wait_warp(c.notes_free(slot), ((uint32_t)(item / NOTE_SLOTS) & 1u) ^ 1u, c.abort_flag())) return false;
+    for (int d = lane; d < 128; d += 32) notes[d] = INT32_MAX;
+    __threadfence();
+    __syncwarp();
+    if (lane == 0) *c.stamp(slot, me) = item;
+    __syncwarp();
+  }
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    uint32_t *w = &x[i].x;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll 1
+      for (int e = 0; e < 4; ++e)
+        if ((w[k] >> 8 * e & 0x7fu) == 0x7fu) atomicMin(notes + element0 + k * 4 + e, key0 + i * key_step);
+      w[k] = without_nan(w[k]);
+    }
+  }
+  __threadfence();
+  return true;
 }
 
+// A group of 16 tokens, of which `count` are the sequence's.
+struct Group {
+  int64_t page;        // as the block table has it (to look at it is to wait for it), then -1: outside the pool
+  int32_t at, count;   // the group of the sequence
+  int32_t ring, item;  // its keys' place in the ring
+  int32_t head;
+};
+
+// The groups of the CTA's items are dealt to the warps in turn.  A warp stores a group's
+// keys, asks for those of its next, stores its values, asks for the next's values: so two
+// loads of 2 KB are always on their way, 28 KB an SM.  Pages' numbers come two groups ahead.
 template <typename C, int DP>
 __device__ __forceinline__ void convert(const Control<DP> &c, const Problem &p, const Piece &piece) {
   using L = Layout<DP>;
   constexpr int WORDS = DP / 16, KEYS = 32 / WORDS, LOADS = 16 / KEYS;  // 16-byte words of a token; tokens a load of the warp
-  constexpr int AHEAD = 2;
   const int lane = threadIdx.x & 31, me = (threadIdx.x >> 5) - 1;
-  const int word = lane % WORDS, sub = lane / WORDS;
+  // A quarter warp takes the four words of one 64-element atom of two tokens: its stores
+  // of their first halves, and of the second, then meet every bank once.
+  const int word = DP == 128 ? (lane & 3) | (lane >> 1 & 4) : lane & 3;
+  const int sub = DP == 128 ? (lane >> 2 & 1) | (lane >> 3 & 2) : lane >> 2;
   const bool in_head = word * 16 < p.head_dim;
+  const uint32_t base = c.base + L::RING_OFF + (word / 4) * (BN * 128) + sub * 128;
+  uint32_t place[2][2];  // of the halves of a word, for a load's even and odd turns
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) place[i][h] = base + i * KEYS * 128 + (((word % 4) * 2 + h) ^ ((i * KEYS + sub) & 7)) * 16;
 
-  // The groups of the CTA's blocks, K_0, V_0, K_1, ... one after another through all its
-  // items, are dealt to the warps in turn.  First steps ahead come the pages' numbers,
-  // AHEAD tasks ahead the codes.
-  Asked table[AHEAD], coming[AHEAD];  // page number asked for; codes asked for
-  uint4 codes[AHEAD][LOADS];
-  float scale[AHEAD];                 // lane 0: the key scale, lane 1: the value scale
-  for (int i = 0; i < AHEAD; ++i) table[i].ring = coming[i].ring = -1;
-  int items = 0;
-
-  auto store = [&](const Asked &a, const uint4 (&x)[LOADS], float s) -> bool {
-    const int slot = a.ring % RING, g = a.group % GROUPS;
-    if (!ptx::mbar_wait_warp(c.slot_empty(slot), ((uint32_t)(a.ring / RING) & 1u) ^ 1u, c.abort_flag())) return false;
-    const bool values = a.ring & 1;
-    uint32_t taken = 0;  // NaN codes of a value are taken out and noted
-    const uint32_t to = c.base + L::RING_OFF + slot * L::KV_BYTES + (word / 4) * (BN * 128);
+  auto store = [&](const uint4 (&x)[LOADS], int ring, int at) {
+    const uint32_t to = (ring % RING) * L::KV_BYTES + (at % GROUPS) * (16 * 128);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int key = g * 16 + i * KEYS + sub;
-      uint4 v = x[i];
-      if (values && (has_nan<C>(v.x) || has_nan<C>(v.y) || has_nan<C>(v.z) || has_nan<C>(v.w))) {
-        taken |= 1u << i;
-        uint32_t *w = &v.x;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] &= ~(((((w[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu);
-      }
       uint4 lo, hi;
-      paged::to_halves<C>(v.x, lo.x, lo.y);
-      paged::to_halves<C>(v.y, lo.z, lo.w);
-      paged::to_halves<C>(v.z, hi.x, hi.y);
-      paged::to_halves<C>(v.w, hi.z, hi.w);
-      // a quarter warp's stores meet every bank once: the second atom's lanes store their halves the other way round
-      const int chunk = (word % 4) * 2, flip = word / 4;
-      const uint32_t row = to + key * 128;
-      const uint32_t a0 = row + (((chunk + flip) ^ (key & 7)) * 16), a1 = row + (((chunk + 1 - flip) ^ (key & 7)) * 16);
-      store_shared16(a0, flip ? hi : lo);
-      store_shared16(a1, flip ? lo : hi);
-    }
-    if (!values) {
-      const float other = __shfl_sync(0xffffffffu, s, 1);
-      if (lane == 0) {
-        const int block = a.ring / 2 % SCALE_SLOTS;
-        GroupScale e;
-        e.key = a.page < 0 ? 0.f : p.scale * s;
-        e.add = a.page < 0 ? -INFINITY : 0.f;
-        e.value = a.page < 0 ? 0.f : other;
-        e.log2_value = a.page < 0 ? -INFINITY : log2_fast(other);
-        c.scales(block)[g] = e;
-        ptx::mbar_arrive(c.scale_full(block));
-      }
-    }
-    if (std::is_same<C, __nv_fp8_e4m3>::value && __any_sync(0xffffffffu, taken != 0)) {
-      // (rare) the first key with a NaN for each element of the head
-      const int note = a.item % NOTE_SLOTS;
-      int *notes = c.notes(p, note, me);
-      if (*c.stamp(note, me) != a.item) {
-        if (!ptx::mbar_wait_warp(c.notes_free(note), ((uint32_t)(a.item / NOTE_SLOTS) & 1u) ^ 1u, c.abort_flag())) return false;
-        for (int d = lane; d < 128; d += 32) notes[d] = INT32_MAX;
-        __threadfence();
-        __syncwarp();
-        if (lane == 0) *c.stamp(note, me) = a.item;
-        __syncwarp();
-      }
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        if (!(taken >> i & 1)) continue;
-        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          for (int e = 0; e < 4; ++e)
-            if ((w[k] >> 8 * e & 0x7fu) == 0x7fu) atomicMin(notes + word * 16 + k * 4 + e, a.group * 16 + i * KEYS + sub);
-      }
-      __threadfence();
+      paged::to_halves<C>(x[i].x, lo.x, lo.y);
+      paged::to_halves<C>(x[i].y, lo.z, lo.w);
+      paged::to_halves<C>(x[i].z, hi.x, hi.y);
+      paged::to_halves<C>(x[i].w, hi.z, hi.w);
+      store_shared16(place[i % 2][0] + to + (i / 2) * (2 * KEYS * 128), lo);
+      store_shared16(place[i % 2][1] + to + (i / 2) * (2 * KEYS * 128), hi);
     }
     ptx::fence_proxy_async_smem();  // the MMAs read what was written here
     __syncwarp();
-    if (lane == 0) ptx::mbar_arrive(c.slot_full(slot));
+    if (lane == 0) ptx::mbar_arrive(c.slot_full(ring % RING));
+  };
+  auto wait_empty = [&](int ring) {
+    return ptx::mbar_wait_warp(c.slot_empty(ring % RING), ((uint32_t)(ring / RING) & 1u) ^ 1u, c.abort_flag());
+  };
+  auto load = [&](uint4 (&x)[LOADS], const Group &g, const uint8_t *codes, int64_t page, int64_t head, int64_t token) {
+    const int in_page = g.at - (int)((uint64_t)(uint32_t)g.at * p.page_reciprocal >> 36) * p.page_groups;
+    const uint8_t *from = codes + g.page * page + g.head * head + (in_page * 16 + sub) * token + word * 16;
+    const int count = g.page < 0 || !in_head ? 0 : g.count - sub;
+    if (__all_sync(0xffffffffu, count > 16 - KEYS)) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) x[i] = __ldg(reinterpret_cast<const uint4 *>(from + i * KEYS * token));
+    } else {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i)
+        x[i] = i * KEYS < count ? __ldg(reinterpret_cast<const uint4 *>(from + i * KEYS * token)) : make_uint4(0, 0, 0, 0);
+    }
+  };
+
+  Walk walk;
+  Item next_of_walk;
+  begin_items(p, piece, &walk);
+  bool more = next_item(p, piece, &walk, &next_of_walk);
+  Item e = next_of_walk;  // (in registers: no address is taken of it)
+  int ring = 0, item = 0, x = me;  // the item's K_0; the next group
+  auto ask = [&](Group &g) -> bool {
+    while (more && x >= (e.until - e.from) * GROUPS) {
+      x -= (e.until - e.from) * GROUPS;
+      ring += 2 * (e.until - e.from);
+      ++item;
+      more = next_item(p, piece, &walk, &next_of_walk);
+      e = next_of_walk;
+    }
+    if (!more) return false;
+    g.ring = ring + x / GROUPS * 2;
+    g.at = e.from * GROUPS + x;
+    g.item = item;
+    g.head = e.head;
+    g.count = min(max(e.keys - g.at * 16, 0), 16);
+    g.page = -1;
+    if (g.count > 0) {
+      const int64_t column = (int64_t)((uint64_t)(uint32_t)g.at * p.page_reciprocal >> 36);
+      const int64_t entry = e.batch * p.table_row_stride + column * p.block_table.stride;
+      if (p.block_table.wide) g.page = static_cast<const int64_t *>(p.block_table.data)[entry];
+      else g.page = static_cast<const int32_t *>(p.block_table.data)[entry];
+    }
+    x += CONVERTERS;
     return true;
   };
-  auto load = [&](const Asked &a, uint4 (&x)[LOADS], float &s) {
-    const bool values = a.ring & 1;
-    const int count = a.page < 0 ? 0 : min(max(a.keys - a.group * 16, 0), 16);
-    const int in_page = a.group - (int)((uint64_t)(uint32_t)a.group * p.page_reciprocal >> 36) * p.page_groups;
-    const uint8_t *from = (values ? p.value + a.page * p.v_page + a.head * p.v_head + (int64_t)(in_page * 16) * p.v_token
-                                  : p.key + a.page * p.k_page + a.head * p.k_head + (int64_t)(in_page * 16) * p.k_token) +
-                          word * 16;
-    const int64_t stride = values ? p.v_token : p.k_token;
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int token = i * KEYS + sub;
-      x[i] = in_head && token < count ? __ldg(reinterpret_cast<const uint4 *>(from + token * stride)) : make_uint4(0, 0, 0, 0);
+  uint4 keys[LOADS], values[LOADS];
+  float key_scale = 0.f, value_scale = 0.f;
+  Group now, next;
+  bool has = ask(now), has_next = has && ask(next);
+  auto load_keys = [&](Group &g) {
+    if (g.page < 0 || g.page >= p.pages) {
+      if (g.count > 0) record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
+      g.page = -1;
     }
-    s = 0.f;
-    if (!values && a.page >= 0) {
-      if (lane == 0) s = p.key_scale[a.page * p.ks_page + a.head * p.ks_head];
-      if (lane == 1) s = p.value_scale[a.page * p.vs_page + a.head * p.vs_head];
+    load(keys, g, p.key, p.k_page, p.k_head, p.k_token);
+    if (g.page >= 0) {
+      key_scale = p.key_scale[g.page * p.ks_page + g.head * p.ks_head];
+      value_scale = p.value_scale[g.page * p.vs_page + g.head * p.vs_head];
     }
   };
-  auto ask = [&](Asked &a, int batch) {
-    a.page = -1;
-    if (a.group * 16 < a.keys) {
-      a.page = paged::page_of(p, batch, (int64_t)((uint64_t)(uint32_t)a.group * p.page_reciprocal >> 36));
+  if (has) {
+    load_keys(now);
+    load(values, now, p.value, p.v_page, p.v_head, p.v_token);
+  }
+#pragma unroll 1
+  while (has) {
+    const Group g = now;
+    if (!wait_empty(g.ring)) return;
+    const float scale = value_scale;
+    if (lane == 0) {
+      const int block = g.ring / 2 % SCALE_SLOTS;
+      GroupScale s{p.scale * key_scale, 0.f, scale, log2_fast(scale)};
+      if (g.page < 0) s = GroupScale{0.f, -INFINITY, 0.f, -INFINITY};
+      c.scales(block)[g.at % GROUPS] = s;
+      ptx::mbar_arrive(c.scale_full(block));
     }
-  };
-  auto step = [&](const Asked &next, bool more) -> bool {
-    // the oldest codes are stored, the oldest page number's codes asked for
-    if (coming[0].ring >= 0 && !store(coming[0], codes[0], scale[0])) return false;
+    store(keys, g.ring, g.at);
+    has = has_next;
+    now = next;
+    if (has) {
+      load_keys(now);
+      has_next = ask(next);
+    }
+    if (std::is_same<C, __nv_fp8_e4m3>::value) {
+      uint32_t nan = 0;
 #pragma unroll
-    for (int i = 0; i + 1 < AHEAD; ++i) {
-      coming[i] = coming[i + 1];
-      scale[i] = scale[i + 1];
+      for (int i = 0; i < LOADS; ++i)
+        nan |= nan_bits(values[i].x) | nan_bits(values[i].y) | nan_bits(values[i].z) | nan_bits(values[i].w);
+      if (__any_sync(0xffffffffu, (nan & 0x80808080u) != 0)) {
+        uint4 box[LOADS];
 #pragma unroll
-      for (int k = 0; k < LOADS; ++k) codes[i][k] = codes[i + 1][k];
-    }
-    coming[AHEAD - 1] = table[0];
-    if (table[0].ring >= 0) {
-      if (table[0].page < 0 && table[0].group * 16 < table[0].keys) record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
-      load(table[0], codes[AHEAD - 1], scale[AHEAD - 1]);
-    }
+        for (int i = 0; i < LOADS; ++i) box[i] = values[i];
+        if (!take_out<DP, LOADS>(c, p, box, g.item, g.at * 16 + sub, KEYS, word * 16)) return;
 #pragma unroll
-    for (int i = 0; i + 1 < AHEAD; ++i) table[i] = table[i + 1];
-    table[AHEAD - 1] = next;
-    if (!more) table[AHEAD - 1].ring = -1;
-    return true;
-  };
-  bool good = true;
-  int ring = 0, skip = me;  // the item's K_0; groups until this warp's next
-  each_item(p, piece, [&](const Item &e) {
-    const int count = 2 * (e.until - e.from) * GROUPS;  // K and V in turn
-    int x = skip;
-    for (; x < count; x += CONVERTERS) {
-      const int block = x / GROUPS;
-      Asked a;
-      a.ring = ring + block;
-      a.group = (e.from + block / 2) * GROUPS + x % GROUPS;
-      a.item = items;
-      a.head = e.head;
-      a.keys = e.keys;
-      ask(a, e.batch);
-      if (!(good = step(a, true))) return false;
+        for (int i = 0; i < LOADS; ++i) values[i] = box[i];
+      }
     }
-    skip = x - count;
-    ring += 2 * (e.until - e.from);
-    ++items;
-    return true;
-  });
-  for (int i = 0; good && i < 2 * AHEAD; ++i) good = step(Asked{}, false);
+    if (scale == 0.f)  // they stand for 0, however small their weights are kept
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) values[i] = make_uint4(0, 0, 0, 0);
+    if (!wait_empty(g.ring + 1)) return;
+    store(values, g.ring + 1, g.at);
+    if (has) load(values, now, p.value, p.v_page, p.v_head, p.v_token);
+  }
 }
 
 // ---------------------------------------------------------------- MMA issuer
@@ -651,7 +685,7 @@ __device__ __forceinline__ void issue(const Control<DP> &c, const Problem &p, co
 // ---------------------------------------------------------------- queries, softmax, output
 // A row's references move only when a block passes them by 2^kLead, so that O is rescaled
 // rarely, and P is kept 2^kRise above: its largest, 2^15, stays in fp16's range.
-constexpr float kLead = 6.f, kRise = 9.f;
+constexpr float kLead = 6.f, kRise = 9.f, kLeastShift = -60.f;
 constexpr float kLeastKey = 1.1754943508222875e-38f;  // in place of a key scale of 0: -inf times it is -inf
 
 // A row of Q into shared memory, scaled by 2^e with its largest finite element then in
@@ -761,76 +795,109 @@ __device__ __forceinline__ void attend(const Control<DP> &c, const Problem &p, c
       if (!ptx::mbar_wait_warp(c.s_full(t), (uint32_t)s_turn & 1u, c.abort_flag())) return false;
       ++s_turn;
       ptx::tc_fence_after();
-      uint32_t sr[BN];
-#pragma unroll
-      for (int x = 0; x < BN / 32; ++x)
-        ptx::tmem_ld_32x32b_x32(tmem_s + (uint32_t)(x * 32), *reinterpret_cast<uint32_t(*)[32]>(&sr[x * 32]));
-      ptx::tmem_ld_wait();
-      float *s = reinterpret_cast<float *>(sr);
       const int seen = limit - j * BN;
-      const bool masked = sure - j * BN < BN;
-      if (masked) {
+      bool move_o;
+      float alpha_o;
+      auto take_block = [&](auto with_mask) {
+      constexpr bool MASKED = decltype(with_mask)::value;
+      // 32 scores at a time, read twice: 128 would fill the registers.  The next are on
+      // their way while these are worked on.
+      auto ask_scores = [&](int quarter, uint32_t (&s)[32]) { ptx::tmem_ld_32x32b_x32(tmem_s + (uint32_t)(quarter * 32), s); };
+      auto mask_scores = [&](int quarter, float (&s)[32]) {
+        if constexpr (!MASKED) return;
+        const int in_quarter = seen - quarter * 32;
 #pragma unroll
-        for (int x = 0; x < BN; ++x) s[x] = x < seen ? s[x] : -INFINITY;
-      }
+        for (int x = 0; x < 32; ++x) s[x] = x < in_quarter ? s[x] : -INFINITY;
+      };
+      // f(quarter, its scores), the first half's and then the second's
+      auto each_quarter = [&](auto f) {
+        uint32_t a[32], b[32];
+        ask_scores(0, a);
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          ptx::tmem_ld_wait();
+          ask_scores(2 * half + 1, b);
+          f(2 * half, *reinterpret_cast<float(*)[32]>(&a));
+          ptx::tmem_ld_wait();
+          if (half == 0) ask_scores(2, a);
+          f(2 * half + 1, *reinterpret_cast<float(*)[32]>(&b));
+        }
+      };
       const GroupScale *scales = c.scales(slot);
       // (a group that the row does not see takes no part, whatever its scales)
-      auto key_factor = [&](const GroupScale &g, int k) {
-        const float f = g.key * factor;
-        return f == 0.f || (masked && k * 16 >= seen) ? kLeastKey : f;
+      auto unseen = [&](int k) { return MASKED && k * 16 >= seen; };
+      auto key_factor = [&](float key, int k) {
+        const float f = key * factor;
+        return MASKED && (f == 0.f || unseen(k)) ? kLeastKey : f;
       };
       float top_s = -INFINITY, top_w = -INFINITY;
+      each_quarter([&](int quarter, float (&s)[32]) {
+        mask_scores(quarter, s);
 #pragma unroll
-      for (int k = 0; k < GROUPS; ++k) {
-        const GroupScale g = scales[k];
-        float top[4];
+        for (int k = 0; k < 2; ++k) {
+          const int group = quarter * 2 + k;
+          const float4 g = *reinterpret_cast<const float4 *>(scales + group);
+          float top[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          top[u] = fmaxf(fmaxf(s[k * 16 + u], s[k * 16 + 4 + u]), fmaxf(s[k * 16 + 8 + u], s[k * 16 + 12 + u]));
-        const float high = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), key_factor(g, k), g.add);
-        top_s = fmaxf(top_s, high);
-        top_w = fmaxf(top_w, high + g.log2_value);
+          for (int u = 0; u < 4; ++u)
+            top[u] = fmaxf(fmaxf(s[k * 16 + u], s[k * 16 + 4 + u]), fmaxf(s[k * 16 + 8 + u], s[k * 16 + 12 + u]));
+          const float high = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), key_factor(g.x, group), g.y);
+          top_s = fmaxf(top_s, high);
+          top_w = fmaxf(top_w, high + g.w);
+        }
+      });
+      const bool move = top_s > m + kLead;
+      move_o = top_w > mo + kLead;
+      alpha_o = move_o ? exp2_fast(mo - top_w) : 1.f;
+      if (move) {
+        l *= exp2_fast(m - top_s);
+        m = top_s;
       }
-      const bool move = top_s > m + kLead, move_o = top_w > mo + kLead;
-      const float m_new = move ? top_s : m, mo_new = move_o ? top_w : mo;
-      const float alpha = move ? exp2_fast(m - m_new) : 1.f, alpha_o = move_o ? exp2_fast(mo - mo_new) : 1.f;
-      const float ref = reference(m_new), rise = exp2_fast(fminf(ref - reference(mo_new) + kRise, 126.f));
-      float sum[4] = {};
+      if (move_o) mo = top_w;
+      // P = 2^(s - m + shift) with the group's shift = log2 value_scale + m - mo + kRise, and
+      // l takes a group's sum of them times 2^-shift.  Where a group's values are so small
+      // that its P would leave fp32, P is kept at 2^kLeastShift: too large, but nothing beside the others.
+      const float ref = reference(m), rise = ref - reference(mo) + kRise;
+      each_quarter([&](int quarter, float (&s)[32]) {
+        mask_scores(quarter, s);
+        uint32_t packed[16];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t packed[32];
-#pragma unroll
-        for (int k = 0; k < GROUPS / 2; ++k) {
-          const GroupScale g = scales[half * (GROUPS / 2) + k];
-          const float by = key_factor(g, half * (GROUPS / 2) + k), add = g.add - ref;
-          const float weight = masked && (half * (GROUPS / 2) + k) * 16 >= seen ? 0.f : g.value * rise;
+        for (int k = 0; k < 2; ++k) {
+          const int group = quarter * 2 + k;
+          const float4 g = *reinterpret_cast<const float4 *>(scales + group);
+          const float by = key_factor(g.x, group);
+          float shift = g.w + rise;
+          shift = shift < kLeastShift || unseen(group) ? kLeastShift : shift;  // (a NaN scale stays)
+          const float add = g.y - ref + shift;
+          float sum[4] = {};
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
-            const int at = (half * (GROUPS / 2) + k) * 16 + 2 * x;
+            const int at = k * 16 + 2 * x;
             const float p0 = exp2_fast(fmaf(s[at], by, add)), p1 = exp2_fast(fmaf(s[at + 1], by, add));
             sum[(2 * x) & 3] += p0;
             sum[(2 * x + 1) & 3] += p1;
-            packed[k * 8 + x] = paged::half2_bits(p0 * weight, p1 * weight);
+            packed[k * 8 + x] = paged::half2_bits(p0, p1);
           }
+          l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), exp2_fast(-shift), l);
         }
-        ptx::tmem_st_32x32b_x32(tmem_s + (uint32_t)(half * 32), packed);
-      }
+        // (P's 16 columns lie among scores that were read before)
+        ptx::tmem_st_32x32b_x16(tmem_s + (uint32_t)(quarter * 16), packed);
+      });
+      };
+      if (sure - j * BN < BN) take_block(std::true_type{});
+      else take_block(std::false_type{});
       if (j > e.from && __any_sync(0xffffffffu, move_o)) {
         // O_t holds P(j-1) V(j-1): the commit of S_t(j) covers it
-        uint32_t o[DP];
+#pragma unroll 1
+        for (int x = 0; x < DP; x += 32) {
+          uint32_t o[32];
+          ptx::tmem_ld_32x32b_x32(tmem_o + (uint32_t)x, o);
+          ptx::tmem_ld_wait();
 #pragma unroll
-        for (int x = 0; x < DP / 32; ++x)
-          ptx::tmem_ld_32x32b_x32(tmem_o + (uint32_t)(x * 32), *reinterpret_cast<uint32_t(*)[32]>(&o[x * 32]));
-        ptx::tmem_ld_wait();
-#pragma unroll
-        for (int y = 0; y < DP; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * alpha_o);
-#pragma unroll
-        for (int x = 0; x < DP / 32; ++x)
-          ptx::tmem_st_32x32b_x32(tmem_o + (uint32_t)(x * 32), *reinterpret_cast<uint32_t(*)[32]>(&o[x * 32]));
+          for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * alpha_o);
+          ptx::tmem_st_32x32b_x32(tmem_o + (uint32_t)x, o);
+        }
       }
-      m = m_new;
-      mo = mo_new;
-      l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
       ptx::tmem_st_wait();
       ptx::tc_fence_before();
       arrive_warp(c.p_full(t));
@@ -838,41 +905,44 @@ __device__ __forceinline__ void attend(const Control<DP> &c, const Problem &p, c
     if (!ptx::mbar_wait_warp(c.o_done(t), (uint32_t)o_turn & 1u, c.abort_flag())) return false;
     ++o_turn;
     ptx::tc_fence_after();
-    uint32_t o[DP];
+    // (mo: -inf where all values stand for 0)
+    const float f = l == 0.f ? 0.f : exp2_fast(reference(mo) - reference(m) - kRise) / l;
+#pragma unroll 1
+    for (int x = 0; x < DP; x += 32) {
+      uint32_t o[32];
+      ptx::tmem_ld_32x32b_x32(tmem_o + (uint32_t)x, o);
+      ptx::tmem_ld_wait();
+      // values' NaN, to the rows that see them
+#pragma unroll 1
+      for (int w = 0; w < CONVERTERS; ++w) {
+        if (*c.stamp(item % NOTE_SLOTS, w) != item) continue;
+        const int *notes = c.notes(p, item % NOTE_SLOTS, w) + x;
 #pragma unroll
-    for (int x = 0; x < DP / 32; ++x)
-      ptx::tmem_ld_32x32b_x32(tmem_o + (uint32_t)(x * 32), *reinterpret_cast<uint32_t(*)[32]>(&o[x * 32]));
-    ptx::tmem_ld_wait();
+        for (int d = 0; d < 32; ++d)
+          if (__ldcg(notes + d) < limit) o[d] = 0x7fc00000u;
+      }
+      if (mine && !part) {
+#pragma unroll
+        for (int y = 0; y < 32; y += 16) {
+          float v[16];
+#pragma unroll
+          for (int z = 0; z < 16; ++z) v[z] = __uint_as_float(o[y + z]) * f;
+          if (x + y < p.head_dim) store_output<16>(p, token, head, x + y, v);
+        }
+      } else if (part && mine) {
+        float4 *out = reinterpret_cast<float4 *>(part) + (x / 4) * ROWS + t * BM + row;
+#pragma unroll
+        for (int y = 0; y < 8; ++y)
+          out[y * ROWS] = make_float4(__uint_as_float(o[4 * y]), __uint_as_float(o[4 * y + 1]), __uint_as_float(o[4 * y + 2]),
+                                      __uint_as_float(o[4 * y + 3]));
+      }
+    }
     ptx::tc_fence_before();
     arrive_warp(c.o_free(t));
-    // values' NaN, to the rows that see them
-    for (int w = 0; w < CONVERTERS; ++w) {
-      if (*c.stamp(item % NOTE_SLOTS, w) != item) continue;
-      const int *notes = c.notes(p, item % NOTE_SLOTS, w);
-#pragma unroll
-      for (int d = 0; d < DP; ++d)
-        if (__ldcg(notes + d) < limit) o[d] = 0x7fc00000u;
-    }
     arrive_warp(c.notes_free(item % NOTE_SLOTS));
-    if (mine && !part) {
-      // (mo: -inf where all values stand for 0)
-      const float f = l == 0.f ? 0.f : exp2_fast(reference(mo) - reference(m) - kRise) / l;
-#pragma unroll
-      for (int x = 0; x < DP / 16; ++x) {
-        float v[16];
-#pragma unroll
-        for (int y = 0; y < 16; ++y) v[y] = __uint_as_float(o[x * 16 + y]) * f;
-        if (x * 16 < p.head_dim) store_output<16>(p, token, head, x * 16, v);
-      }
-      if (p.lse) p.lse[token * p.l_token + (int64_t)head * p.l_head] = l == 0.f ? -INFINITY : (m + log2_fast(l)) * kLn2;
-    } else if (part && mine) {
-      float4 *out = reinterpret_cast<float4 *>(part) + t * BM + row;
-#pragma unroll
-      for (int x = 0; x < DP / 4; ++x)
-        out[x * ROWS] = make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]), __uint_as_float(o[4 * x + 2]),
-                                    __uint_as_float(o[4 * x + 3]));
-      *stats = make_float4(m, l, mo, 0.f);
-    }
+    if (mine && part) *stats = make_float4(m, l, mo, 0.f);
+    if (mine && !part && p.lse)
+      p.lse[token * p.l_token + (int64_t)head * p.l_head] = l == 0.f ? -INFINITY : (m + log2_fast(l)) * kLn2;
     return true;
   });
 }
@@ -919,7 +989,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
   ptx::tc_fence_before();
   find_piece(p, reinterpret_cast<Piece *>(smem + L::PIECE_OFF), reinterpret_cast<int64_t *>(smem + L::SCAN_OFF));
   ptx::tc_fence_after();
-  const Piece piece = *reinterpret_cast<const Piece *>(smem + L::PIECE_OFF);
+  const Piece &piece = *reinterpret_cast<const Piece *>(smem + L::PIECE_OFF);
   const uint32_t tmem_base = *c.tmem_base();
   if (warp == 0) {
     Shared open{-1, 0, 0, 0};  // the unit that goes on in the next piece, for the join

@@ -34,10 +34,7 @@ def _bound(name, *args):
     binding = _lib.binding()
     if binding is None:
         return None
-    call = getattr(binding, name, None)
-    if call is None:
-        return None
-    result = call(*args)
+    result = getattr(binding, name)(*args)
     if result.__class__ is int:
         raise KernelLaunchError(result)
     return result
