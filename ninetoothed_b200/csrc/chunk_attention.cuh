@@ -54,8 +54,11 @@ struct Problem : paged::Attention {
 
 constexpr int BM = 128, BN = 128, TILES = 2, ROWS = TILES * BM;  // rows of a tile, keys of a block
 // What a unit's start and end (its queries, its output) count in the line, in key
-// blocks; steps of a piece at least.
-constexpr int UNIT_STEPS = 3, LEAST_STEPS = 4;
+// blocks: 8 pieces of up to 512 tokens over up to 8192 took 357 us at 2, 336 at 3, 321 at
+// 5; units of few rows, 6 pieces of up to 300 over up to 4000, 73, 74 and 76.  Steps of a
+// piece at least: 4 pieces of up to 16 tokens over up to 1000 took 34 us at 8, 27 at 4, 23
+// at 2.
+constexpr int UNIT_STEPS = 4, LEAST_STEPS = 2;
 
 // ---------------------------------------------------------------- any layout
 // A warp a query row.
@@ -748,6 +751,12 @@ template <int N> __device__ __forceinline__ void store_output(const Problem &p, 
   }
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
 template <int DP>
 __device__ __forceinline__ void attend(const Control<DP> &c, const Problem &p, const Piece &piece, uint32_t tmem_base) {
   using L = Layout<DP>;
@@ -837,11 +846,10 @@ __device__ __forceinline__ void attend(const Control<DP> &c, const Problem &p, c
         for (int k = 0; k < 2; ++k) {
           const int group = quarter * 2 + k;
           const float4 g = *reinterpret_cast<const float4 *>(scales + group);
-          float top[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            top[u] = fmaxf(fmaxf(s[k * 16 + u], s[k * 16 + 4 + u]), fmaxf(s[k * 16 + 8 + u], s[k * 16 + 12 + u]));
-          const float high = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), key_factor(g.x, group), g.y);
+          const float *x = s + k * 16;
+          const float a = max3(max3(x[0], x[1], x[2]), x[3], x[4]), b = max3(max3(x[5], x[6], x[7]), x[8], x[9]);
+          const float d = max3(max3(x[10], x[11], x[12]), x[13], x[14]);
+          const float high = fmaf(fmaxf(max3(a, b, d), x[15]), key_factor(g.x, group), g.y);
           top_s = fmaxf(top_s, high);
           top_w = fmaxf(top_w, high + g.w);
         }
