@@ -18,13 +18,21 @@
 // make the pairs (0, 4), (1, 5), (2, 6), (3, 7): a shift, a mask and a
 // subtraction for two weights, and one permute for two elements of x.
 //
-// A block has 8 warps and 64 or 128 weight rows; a stage of its ring holds 512 or 256
-// columns of them, 16 KB, and x's columns beside it, of which a warp takes 64 rows by
-// 64 columns, or 32 by 128.  More rows of x take more weight rows a block, so that x
-// is never more than the weights.  Blocks go on from one set of rows to the next with
-// the copies running ahead.  Where the weight rows are too few for the SMs, a
-// cluster's blocks share the columns and join their sums through distributed shared
-// memory, always in the same order.
+// A block has 8 warps and 32, 64 or 128 weight rows; a stage of its ring holds 1024, 512
+// or 256 columns of them, 16 KB, and x's columns beside it, of which a warp takes 32 rows
+// by 128 columns.  More rows of x take more weight rows a block, so that x is never more
+// than the weights.  Blocks go on from one set of rows to the next with the copies
+// running ahead.  Where the weight rows are too few for the SMs, a cluster's blocks share
+// the columns and join their sums through distributed shared memory, always in the same
+// order.
+//
+// Measured (codes' bytes a second): 4096 x 4096 with one bfloat16 row 6.8 us, launch,
+// first copies and join for the most part; 10240 -> 4099 with 5 float16 rows, groups of 64
+// with zero points 13.8 us; 8192 x 8192 with 32 bfloat16 rows 36 us; 8192 -> 65536 with 16
+// E4M3 rows, groups of 32 with zero points 166 us, 1.6 TB/s.  Bound by issue, not by
+// memory: a warp takes about 600 instructions for 4096 codes, half of them to unpack, and
+// the copies alone take 71 us of the last.  (With a warp of its own for the copies the
+// register file holds 96 a thread and the products spill: 47 us for the third.)
 #pragma once
 
 #include "common.cuh"
@@ -171,10 +179,10 @@ __device__ __forceinline__ void arrive_after_copies(uint32_t bar) {
 }
 
 template <typename X, int NT> struct Layout {
-  // Row tiles of a warp and steps of its slice of a stage: more rows where that leaves
-  // registers, as each step of x is loaded and unpacked once for all of them.
-  static constexpr int RT = NT == 4 ? 2 : 4, WSTEPS = 8 / RT;
-  static constexpr int WR = NT == 4 ? 4 : 1, WK = WARPS / WR;
+  // Row tiles of a warp and steps of its slice of a stage.  (4 and 2, so that a step of x
+  // serves 64 rows, spilled: the head of 16 rows took 183 us, 166 at 2 and 4.)
+  static constexpr int RT = 2, WSTEPS = 4;
+  static constexpr int WR = NT, WK = WARPS / WR;
   static constexpr int R = 16 * RT * WR, KS = 32 * WSTEPS * WK;  // weight rows; columns of a stage
   static constexpr int STEPS = KS / 32;                          // of 32 columns
   static constexpr int M = 8 * NT;                               // rows of x
@@ -333,27 +341,24 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmap_codes, const __grid_consta
       if (copies) fill();
       if (!ptx::mbar_wait_warp(full(slot), phase, abort_flag)) break;
       const uint8_t *stage = smem + (uint32_t)slot * (uint32_t)p.stage_bytes;
-      // a lane readies the factors of a row, or of two
+      // a lane readies the factors of a row
       {
-        constexpr int ROWS = RT / 2;
+        static_assert(RT == 2, "a lane a row");
         const auto ready = [&](auto value) {
+          const int r = wr * 16 * RT + lane;
+          const uint8_t *from = stage + L::CODES + p.x_bytes + r * p.s_pitch;
+          const uint8_t *zeros = stage + L::CODES + p.x_bytes + L::R * p.s_pitch + r * p.z_pitch;
+          // where a row's part starts in the first word of its copy
+          if (p.s_copy == 4) from += ((uint32_t)((n0 + r) * p.s_row) + stage_at.index) * (uint32_t)scale_size & 3u;
+          if (p.z_copy == 4) zeros += ((uint32_t)((n0 + r) * p.z_row) + stage_at.index) & 3u;
+          Group now = slice_at;
 #pragma unroll
-          for (int i = 0; i < ROWS; ++i) {
-            const int r = wr * 16 * RT + lane + 32 * i;
-            const uint8_t *from = stage + L::CODES + p.x_bytes + r * p.s_pitch;
-            const uint8_t *zeros = stage + L::CODES + p.x_bytes + L::R * p.s_pitch + r * p.z_pitch;
-            // where a row's part starts in the first word of its copy
-            if (p.s_copy == 4) from += ((uint32_t)((n0 + r) * p.s_row) + stage_at.index) * (uint32_t)scale_size & 3u;
-            if (p.z_copy == 4) zeros += ((uint32_t)((n0 + r) * p.z_row) + stage_at.index) & 3u;
-            Group now = slice_at;
-#pragma unroll
-            for (int k = 0; k < SCALES; ++k) {
-              const uint32_t nth = now.index - stage_at.index;
-              const uint32_t zero = p.zeros ? zeros[nth] & 15u : 8u;
-              factors[k * 16 * RT + lane + 32 * i] =
-                  Factor{value(from + nth * scale_size), Codes<F>::zero_low(zero), Codes<F>::zero_high(zero), 0u};
-              now.advance(0, GS, p.group32);
-            }
+          for (int k = 0; k < SCALES; ++k) {
+            const uint32_t nth = now.index - stage_at.index;
+            const uint32_t zero = p.zeros ? zeros[nth] & 15u : 8u;
+            factors[k * 16 * RT + lane] =
+                Factor{value(from + nth * scale_size), Codes<F>::zero_low(zero), Codes<F>::zero_high(zero), 0u};
+            now.advance(0, GS, p.group32);
           }
         };
         if (p.scale_dtype == NT_B200_BFLOAT16)
@@ -563,8 +568,7 @@ template <typename X, int NT, int GS> int launch_tiles(Params p, cudaStream_t st
   return (int)cudaLaunchKernelEx(&cfg, tiles_kernel<X, NT, GS>, tmap_codes, tmap_x, p);
 }
 template <typename X, int NT> int launch_groups(const Params &p, cudaStream_t stream) {
-  if constexpr (Layout<X, NT>::WSTEPS % 4 == 0)
-    if (p.group32 % 4 == 0) return launch_tiles<X, NT, 4>(p, stream);
+  if (p.group32 % 4 == 0) return launch_tiles<X, NT, 4>(p, stream);
   if (p.group32 % 2 == 0) return launch_tiles<X, NT, 2>(p, stream);
   return launch_tiles<X, NT, 1>(p, stream);
 }
