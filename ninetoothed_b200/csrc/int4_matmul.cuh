@@ -28,11 +28,12 @@
 //
 // Measured (codes' bytes a second): 4096 x 4096 with one bfloat16 row 6.8 us, launch,
 // first copies and join for the most part; 10240 -> 4099 with 5 float16 rows, groups of 64
-// with zero points 13.8 us; 8192 x 8192 with 32 bfloat16 rows 36 us; 8192 -> 65536 with 16
-// E4M3 rows, groups of 32 with zero points 166 us, 1.6 TB/s.  Bound by issue, not by
+// with zero points 13.8 us; 8192 x 8192 with 32 bfloat16 rows 24 us (weights in tensor
+// memory, see tall_kernel; 36 us with these steps); 8192 -> 65536 with 16 E4M3 rows,
+// groups of 32 with zero points 166 us, 1.6 TB/s.  Bound by issue, not by
 // memory: a warp takes about 600 instructions for 4096 codes, half of them to unpack, and
 // the copies alone take 71 us of the last.  (With a warp of its own for the copies the
-// register file holds 96 a thread and the products spill: 47 us for the third.)
+// register file holds 96 a thread and the products spill: 47 us for the third against 36.)
 #pragma once
 
 #include "common.cuh"
@@ -226,11 +227,77 @@ __device__ __noinline__ void settle(uint32_t full0, int ring) {
   __syncthreads();
 }
 
+// The eight warps that compute.
+__device__ __forceinline__ void sync_warps() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); }
+__device__ __forceinline__ bool any_of_warps(int flag) {
+  int any;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.s32 p, %1, 0;\n"
+      "barrier.cta.red.or.pred p, 1, %2, p;\n"
+      "selp.s32 %0, 1, 0, p;\n"
+      "}"
+      : "=r"(any)
+      : "r"(flag), "n"(WARPS * 32)
+      : "memory");
+  return any != 0;
+}
 __device__ __forceinline__ void add(float4 &a, const float4 &b) {
   a.x += b.x;
   a.y += b.y;
   a.z += b.z;
   a.w += b.w;
+}
+
+// The sums of the warps that share columns, [WK][M][PITCH] in shared memory at `joined`,
+// and of a cluster's blocks, into y; for the eight warps that have them.
+template <typename L>
+__device__ __forceinline__ void join_sums(const Params &p, float *joined, uint32_t address, int64_t n0, int64_t m0, int m_count,
+                                          int part) {
+  constexpr int COUNT = WARPS * 32, QUADS = L::R / 4;
+  sync_warps();
+  const auto sum_of = [&](int at) {
+    float4 v = *reinterpret_cast<const float4 *>(joined + at);
+#pragma unroll
+    for (int k = 1; k < L::WK; ++k) add(v, *reinterpret_cast<const float4 *>(joined + k * L::M * L::PITCH + at));
+    return v;
+  };
+  const auto store = [&](int m, int row, const float4 &v) {
+    const float f[4] = {v.x, v.y, v.z, v.w};
+    const float by = p.x_scale ? p.x_scale[(m0 + m) * p.xs_stride] : 1.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n0 + row + e < p.outer)
+        store_any(p.y, (m0 + m) * p.y_row + (n0 + row + e) * p.y_col, p.y_dtype, p.x_scale ? f[e] * by : f[e]);
+  };
+  if (p.parts == 1) {
+    for (int i = threadIdx.x; i < m_count * QUADS; i += COUNT)
+      store(i / QUADS, i % QUADS * 4, sum_of(i / QUADS * L::PITCH + i % QUADS * 4));
+    sync_warps();  // the sums are read: the next unit's may come
+    return;
+  }
+  // (a grid with parts has one unit a cluster)
+  for (int i = threadIdx.x; i < m_count * QUADS; i += COUNT) {
+    const int at = i / QUADS * L::PITCH + i % QUADS * 4;
+    *reinterpret_cast<float4 *>(joined + at) = sum_of(at);
+  }
+  ptx::cluster_sync();
+  for (int i = threadIdx.x + part * COUNT; i < m_count * QUADS; i += COUNT * p.parts) {
+    const uint32_t from = address + 4 * (i / QUADS * L::PITCH + i % QUADS * 4);
+    float4 v[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (r < p.parts)
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[r].x), "=f"(v[r].y), "=f"(v[r].z), "=f"(v[r].w)
+                     : "r"(ptx::mapa(from, r)));
+#pragma unroll
+    for (int r = 1; r < 8; ++r)
+      if (r < p.parts) add(v[0], v[r]);
+    store(i / QUADS, i % QUADS * 4, v[0]);
+  }
+  ptx::cluster_sync();  // no block ends while another reads its sums
 }
 
 // GS: steps between two applications of a scale, a divisor of a group's and of a slice's
@@ -438,53 +505,316 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmap_codes, const __grid_consta
           const int m = t * 8 + 2 * c + (e & 1), row = wr * 16 * RT + r * 16 + g + (e >> 1) * 8;
           joined[(wk * L::M + m) * L::PITCH + row] = acc[r][t][e];
         }
-    __syncthreads();
-    const auto sum_of = [&](int at) {
-      float4 v = *reinterpret_cast<const float4 *>(joined + at);
-#pragma unroll
-      for (int k = 1; k < L::WK; ++k) add(v, *reinterpret_cast<const float4 *>(joined + k * L::M * L::PITCH + at));
-      return v;
-    };
-    const auto store = [&](int m, int row, const float4 &v) {
-      const float f[4] = {v.x, v.y, v.z, v.w};
-      const float by = p.x_scale ? p.x_scale[(m0 + m) * p.xs_stride] : 1.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n0 + row + e < p.outer)
-          store_any(p.y, (m0 + m) * p.y_row + (n0 + row + e) * p.y_col, p.y_dtype, p.x_scale ? f[e] * by : f[e]);
-    };
-    constexpr int QUADS = L::R / 4;
-    if (p.parts == 1) {
-      for (int i = threadIdx.x; i < m_count * QUADS; i += THREADS)
-        store(i / QUADS, i % QUADS * 4, sum_of(i / QUADS * L::PITCH + i % QUADS * 4));
-      __syncthreads();  // the sums are read: the next unit's may come
-    } else {
-      // (a grid with parts has one unit a cluster)
-      for (int i = threadIdx.x; i < m_count * QUADS; i += THREADS) {
-        const int at = i / QUADS * L::PITCH + i % QUADS * 4;
-        *reinterpret_cast<float4 *>(joined + at) = sum_of(at);
-      }
-      ptx::cluster_sync();
-      for (int i = threadIdx.x + part * THREADS; i < m_count * QUADS; i += THREADS * p.parts) {
-        const uint32_t from = base + p.join + 4 * (i / QUADS * L::PITCH + i % QUADS * 4);
-        float4 v[8];
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-          if (r < p.parts)
-            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                         : "=f"(v[r].x), "=f"(v[r].y), "=f"(v[r].z), "=f"(v[r].w)
-                         : "r"(ptx::mapa(from, r)));
-#pragma unroll
-        for (int r = 1; r < 8; ++r)
-          if (r < p.parts) add(v[0], v[r]);
-        store(i / QUADS, i % QUADS * 4, v[0]);
-      }
-      ptx::cluster_sync();  // no block ends while another reads its sums
-    }
+    join_sums<L>(p, joined, base + p.join, n0, m0, m_count, part);
     if (*abort_flag) break;  // (read by all after the same barrier)
   }
   __syncthreads();
   if (*abort_flag) settle(bar0, p.ring);
+}
+
+// ---------------------------------------------------------------- weights through tensor memory
+// The same products for more rows of x, with the weights as tcgen05's 128 rows and x's as
+// its columns: a thread unpacks the codes of its row of 128 into tensor memory, where the
+// MMAs read them (x from shared memory), and takes a group's sums out of tensor memory.
+// Scale and zero point are then its own row's, x needs no permutes and the MMAs no
+// registers, so that two blocks an SM fit.  A block's two warpgroups take the halves of a
+// stage's 256 columns, which share a scale each: groups of 128 columns and their multiples.
+//
+// 8192 x 8192 with 32 bfloat16 rows: 24 us (36 with fragments), bound by latency: a
+// warpgroup's unpacking, MMAs and sums follow one another.  Without the unpacking 19 us,
+// without the scales' loads 23.  Tried: 64 columns at a time in two buffers each, the sums
+// taken while the next MMAs run, 29 us (twice the stores and loads of tensor memory, and
+// their waits).  Sums of two groups a half, for groups of 64, spill: 30 us, 34 with fragments.
+struct Tall {
+  static constexpr int N = 32, R = 128, KS = 256, HALF = 128;
+  static constexpr int CODES = R * KS / 2, X_BOX = N * 128, X = 4 * X_BOX;  // x: 64 columns a box
+  static constexpr int STAGE = CODES + X;
+  static constexpr int M = N, WK = 1, PITCH = R + 4, JOIN = WK * M * PITCH * 4;
+  static constexpr int A_COLS = HALF / 2, D_COLS = 64, TMEM_COLS = 2 * (A_COLS + D_COLS);  // a warpgroup's weights, its sums
+};
+constexpr int TALL_WARPS = 10, TALL_THREADS = TALL_WARPS * 32;  // 8 that unpack, one that copies, one that issues
+constexpr int TALL_CONTROL = 16 * MOST_RING + 48;               // the stages' and warpgroups' barriers, and two words
+
+template <typename F>
+__global__ void __launch_bounds__(TALL_THREADS, 2)
+tall_kernel(const __grid_constant__ CUtensorMap tmap_codes, const __grid_constant__ CUtensorMap tmap_x,
+            const __grid_constant__ Params p) {
+  using L = Tall;
+  constexpr int N = L::N;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = ptx::smem_u32(smem), bar0 = base + p.control;
+  if ((base & 1023u) != 0) {  // the swizzle needs it
+    record_error(NT_B200_ERR_INVALID_ARGUMENT);
+    return;
+  }
+  const auto full = [&](int slot) { return bar0 + 8u * slot; };
+  const auto empty = [&](int slot) { return bar0 + 8u * (MOST_RING + slot); };
+  const auto a_full = [&](int wg) { return bar0 + 16u * MOST_RING + 8u * wg; };       // weights in tensor memory, sums read
+  const auto d_full = [&](int wg) { return bar0 + 16u * MOST_RING + 16u + 8u * wg; }; // sums in tensor memory
+  const uint32_t settled = bar0 + 16u * MOST_RING + 32u;
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + p.control + 16 * MOST_RING + 40);
+  volatile uint32_t *tmem_at = reinterpret_cast<volatile uint32_t *>(smem + p.control + 16 * MOST_RING + 44);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = (int)(blockIdx.x % (unsigned)p.parts);
+  const uint32_t unit0 = blockIdx.x / (unsigned)p.parts, units = (uint32_t)p.row_blocks, unit_step = gridDim.x / (uint32_t)p.parts;
+  const int64_t m0 = (int64_t)blockIdx.y * N;
+  const int m_count = (int)(p.rows - m0 < N ? p.rows - m0 : N);
+  const int first = p.stages / p.parts * part + min(part, p.stages % p.parts);
+  const int last = first + p.stages / p.parts + (part < p.stages % p.parts ? 1 : 0);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.ring; ++s) {
+      ptx::mbar_init(full(s), 1);
+      ptx::mbar_init(empty(s), 8 + 1);
+    }
+    for (int wg = 0; wg < 2; ++wg) {
+      ptx::mbar_init(a_full(wg), 4);
+      ptx::mbar_init(d_full(wg), 1);
+    }
+    ptx::mbar_init(settled, 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tmap(&tmap_codes);
+    ptx::prefetch_tmap(&tmap_x);
+  }
+  if (warp == 9) {
+    ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t *>(tmem_at)), L::TMEM_COLS);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_at;
+  wait_prior_grid();
+
+  int slot = 0;
+  uint32_t phase = 0;
+  const auto next_slot = [&]() {
+    if (++slot == p.ring) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  };
+  if (warp == 8) {
+    // ---- copies
+    if (lane == 0) {
+      for (uint32_t unit = unit0; unit < units && !*abort_flag; unit += unit_step)
+        for (int s = first; s < last; ++s) {
+          if (!ptx::mbar_wait(empty(slot), phase ^ 1u, abort_flag)) break;
+          const uint32_t to = base + (uint32_t)slot * L::STAGE;
+          ptx::mbar_arrive_expect_tx(full(slot), L::STAGE);
+          ptx::tma_load_2d(to, &tmap_codes, full(slot), s * (L::KS / 2), (int32_t)(unit * L::R));
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+            ptx::tma_load_2d(to + L::CODES + b * L::X_BOX, &tmap_x, full(slot), s * L::KS + 64 * b, (int32_t)m0);
+          next_slot();
+        }
+    }
+  } else if (warp == 9) {
+    // ---- MMAs
+    constexpr uint32_t idesc = ptx::f16_idesc(tc::umma_format<F>(), 0, 0, L::R, N);
+    if (lane == 0) {
+      uint32_t turn = 0;
+      for (uint32_t unit = unit0; unit < units && !*abort_flag; unit += unit_step)
+        for (int s = first; s < last; ++s, ++turn) {
+          if (!ptx::mbar_wait(full(slot), phase, abort_flag)) break;
+          const uint32_t x = base + (uint32_t)slot * L::STAGE + L::CODES;
+          bool good = true;
+          for (int wg = 0; wg < 2 && good; ++wg) {
+            good = ptx::mbar_wait(a_full(wg), turn & 1u, abort_flag);
+            if (!good) break;
+            ptx::tc_fence_after();
+            const uint32_t a = tmem + (uint32_t)(wg * (L::A_COLS + L::D_COLS)), d = a + L::A_COLS;
+#pragma unroll
+            for (int kk = 0; kk < L::HALF / 16; ++kk)
+              ptx::mma_f16_ts(d, a + (uint32_t)(kk * 8), ptx::sw128_desc(x + (2 * wg + kk / 4) * L::X_BOX + (kk % 4) * 32, 16, 1024), idesc,
+                              kk > 0 ? 1u : 0u);
+            ptx::mma_commit(d_full(wg));
+          }
+          if (!good) break;
+          ptx::mma_commit(empty(slot));
+          next_slot();
+        }
+    }
+  } else {
+    // ---- a thread's row, half a stage at a time
+    const int wg = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t a_cols = tmem + (uint32_t)(wg * (L::A_COLS + L::D_COLS)) + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t d_cols = a_cols + L::A_COLS;
+    const int scale_size = float_size(p.scale_dtype);
+    uint32_t turn = 0;
+    for (uint32_t unit = unit0; unit < units; unit += unit_step) {
+      const int64_t n = (int64_t)unit * L::R + row;
+      const bool some_row = n < p.outer;
+      float acc[N] = {};
+      // raw scale and zero point of the next half stage: on their way while this one is worked on
+      uint32_t raw, zero;
+      const auto fetch = [&](int s) {
+        const uint32_t group = (uint32_t)(s * (L::KS / 32) + wg * (L::HALF / 32)) / p.group32;
+        raw = 0;  // (past the last column x is 0)
+        zero = 8;
+        if (!some_row || s >= last || group >= (uint32_t)p.groups) return;
+        const uint8_t *at = p.scales + (n * p.s_row + group * p.s_col) * scale_size;
+        raw = scale_size == 4 ? *reinterpret_cast<const uint32_t *>(at) : *reinterpret_cast<const uint16_t *>(at);
+        if (p.zeros) zero = p.zeros[n * p.z_row + group * p.z_col];
+      };
+      const auto value = [&](uint32_t v) {
+        if (p.scale_dtype == NT_B200_FLOAT32) return __uint_as_float(v);
+        return p.scale_dtype == NT_B200_BFLOAT16 ? __uint_as_float(v << 16) : __half2float(__ushort_as_half((uint16_t)v));
+      };
+      float scale = 0.f;  // of the sums that the MMAs are at
+      const auto take_sums = [&]() {
+#pragma unroll
+        for (int m = 0; m < N; m += 16) {
+          uint32_t d[16];
+          ptx::tmem_ld_32x32b_x16(d_cols + (uint32_t)m, d);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[m + e] = fmaf(scale, __uint_as_float(d[e]), acc[m + e]);
+        }
+      };
+      fetch(first);
+      bool good = true;
+      for (int s = first; s < last; ++s, ++turn) {
+        good = ptx::mbar_wait_warp(full(slot), phase, abort_flag);
+        if (!good) break;
+        const float next_scale = value(raw);
+        const uint32_t z0 = Codes<F>::zero_low(zero & 15u), z1 = Codes<F>::zero_high(zero & 15u);
+        fetch(s + 1);
+        if (s > first) {  // the weights before were read, and their sums are there
+          good = ptx::mbar_wait_warp(d_full(wg), (turn - 1) & 1u, abort_flag);
+          if (!good) break;
+          ptx::tc_fence_after();
+          take_sums();
+        }
+        const uint8_t *codes = smem + (uint32_t)slot * L::STAGE + row * 128;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // (at its place in TMA's 128-byte swizzle)
+          const uint4 w = *reinterpret_cast<const uint4 *>(codes + (((wg * 4 + i) ^ row) & 7) * 16);
+          const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+          uint32_t a[16];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t v = word[k], v8 = v >> 8;
+            const uint32_t e04 = Codes<F>::low(v, z0), e15 = Codes<F>::high(v, z1);
+            const uint32_t e26 = Codes<F>::low(v8, z0), e37 = Codes<F>::high(v8, z1);
+            a[4 * k] = __byte_perm(e04, e15, 0x5410);
+            a[4 * k + 1] = __byte_perm(e26, e37, 0x5410);
+            a[4 * k + 2] = __byte_perm(e04, e15, 0x7632);
+            a[4 * k + 3] = __byte_perm(e26, e37, 0x7632);
+          }
+          ptx::tmem_st_32x32b_x16(a_cols + (uint32_t)(i * 16), a);
+        }
+        ptx::tmem_st_wait();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          ptx::mbar_arrive(a_full(wg));
+          ptx::mbar_arrive(empty(slot));
+        }
+        scale = next_scale;
+        next_slot();
+      }
+      if (good && ptx::mbar_wait_warp(d_full(wg), (turn - 1) & 1u, abort_flag)) {
+        ptx::tc_fence_after();
+        take_sums();
+        ptx::tc_fence_before();
+      }
+      if (unit + unit_step >= units) allow_dependent_launch();
+      // the warpgroups' sums, [N][PITCH]
+      float *joined = reinterpret_cast<float *>(smem + p.join);
+      if (wg == 1) {
+#pragma unroll
+        for (int m = 0; m < N; ++m) joined[m * L::PITCH + row] = acc[m];
+      }
+      sync_warps();
+      if (wg == 0) {
+#pragma unroll
+        for (int m = 0; m < N; ++m) joined[m * L::PITCH + row] += acc[m];
+      }
+      join_sums<L>(p, joined, base + p.join, (int64_t)unit * L::R, m0, m_count, part);
+      if (any_of_warps(*abort_flag)) break;  // (the other warps may set it at any time: one answer for all)
+    }
+  }
+  if (warp >= 8 && p.parts > 1) {  // the join's barriers are the whole cluster's
+    __syncwarp();
+    ptx::cluster_sync();
+    ptx::cluster_sync();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    // after a wait gave up: the MMAs in flight
+    if (threadIdx.x == 9 * 32) {
+      volatile int over = 0;
+      ptx::mma_commit(settled);
+      ptx::mbar_wait(settled, 0, &over, 100000000ull);
+    }
+    settle(bar0, p.ring);
+  }
+  if (warp == 9) {
+    __syncwarp();
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, L::TMEM_COLS);
+  }
+}
+
+// Launches a kernel over the row blocks, x's blocks of rows and parts of the columns.
+template <typename L, typename K>
+int launch_blocks(K kernel, Params &p, int threads, int bytes, const CUtensorMap &tmap_codes, const CUtensorMap &tmap_x,
+                  cudaStream_t stream) {
+  const int64_t row_blocks = (p.outer + L::R - 1) / L::R, m_blocks = (p.rows + L::M - 1) / L::M;
+  // Parts of the columns: as many as leave the grid in two blocks an SM.
+  const int64_t room = 2 * (int64_t)sm_count();
+  int parts = 1;
+  while (parts < 8 && row_blocks * m_blocks * parts * 2 <= room && p.stages >= 2 * parts) parts *= 2;
+  p.parts = parts;
+  p.row_blocks = row_blocks;
+  int64_t grid = row_blocks;
+  if (grid * m_blocks > room) grid = (room + m_blocks - 1) / m_blocks < grid ? (room + m_blocks - 1) / m_blocks : grid;
+  if (m_blocks > 65535) return NT_B200_ERR_INVALID_ARGUMENT;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(grid * parts), (unsigned)m_blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = (unsigned)parts;
+  attrs[1].val.clusterDim.y = 1;
+  attrs[1].val.clusterDim.z = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = parts > 1 ? 2 : 1;
+  return (int)cudaLaunchKernelEx(&cfg, kernel, tmap_codes, tmap_x, p);
+}
+
+template <typename F> int launch_tall(Params p, cudaStream_t stream) {
+  using L = Tall;
+  tc::EncodeTiledFn encode = tc::encode_tiled_fn();
+  if (!encode) return tc::kNotEligible;
+  p.stage_bytes = L::STAGE;
+  p.stages = (int)((p.inner + L::KS - 1) / L::KS);
+  constexpr int half_bytes = 113 * 1024 - TALL_CONTROL - L::JOIN;
+  p.ring = half_bytes / L::STAGE < MOST_RING ? half_bytes / L::STAGE : MOST_RING;
+  static_assert(half_bytes / L::STAGE >= 2, "a ring");
+  p.join = p.ring * L::STAGE;
+  p.control = p.join + L::JOIN;
+  const int bytes = p.control + TALL_CONTROL;
+  cudaError_t e = smem_optin<tall_kernel<F>>(bytes);
+  if (e != cudaSuccess) return (int)e;
+  CUtensorMap tmap_codes, tmap_x;
+  const cuuint32_t ones[2] = {1, 1}, code_box[2] = {128, (cuuint32_t)L::R}, x_box[2] = {64, (cuuint32_t)L::N};
+  const cuuint64_t code_dims[2] = {(cuuint64_t)(p.inner / 2), (cuuint64_t)p.outer}, code_strides[1] = {(cuuint64_t)p.c_row};
+  const cuuint64_t x_dims[2] = {(cuuint64_t)p.inner, (cuuint64_t)p.rows}, x_strides[1] = {(cuuint64_t)p.x_row * 2};
+  if (encode(&tmap_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(p.codes), code_dims, code_strides, code_box,
+             ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
+      encode(&tmap_x, tc::tmap_dtype<F>(), 2, const_cast<void *>(p.x), x_dims, x_strides, x_box, ones,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return tc::kNotEligible;
+  return launch_blocks<L>(tall_kernel<F>, p, TALL_THREADS, bytes, tmap_codes, tmap_x, stream);
 }
 
 template <typename X, int NT, int GS> int launch_tiles(Params p, cudaStream_t stream) {
@@ -541,31 +871,7 @@ template <typename X, int NT, int GS> int launch_tiles(Params p, cudaStream_t st
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return tc::kNotEligible;
 
-  const int64_t row_blocks = (p.outer + L::R - 1) / L::R, m_blocks = (p.rows + L::M - 1) / L::M;
-  // Parts of the columns: as many as leave the grid in two blocks an SM.
-  const int64_t room = 2 * (int64_t)sm_count();
-  int parts = 1;
-  while (parts < 8 && row_blocks * m_blocks * parts * 2 <= room && p.stages >= 2 * parts) parts *= 2;
-  p.parts = parts;
-  p.row_blocks = row_blocks;
-  int64_t grid = row_blocks;
-  if (grid * m_blocks > room) grid = (room + m_blocks - 1) / m_blocks < grid ? (room + m_blocks - 1) / m_blocks : grid;
-  if (m_blocks > 65535) return NT_B200_ERR_INVALID_ARGUMENT;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(grid * parts), (unsigned)m_blocks);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = bytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attrs[2];
-  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attrs[0].val.programmaticStreamSerializationAllowed = 1;
-  attrs[1].id = cudaLaunchAttributeClusterDimension;
-  attrs[1].val.clusterDim.x = (unsigned)parts;
-  attrs[1].val.clusterDim.y = 1;
-  attrs[1].val.clusterDim.z = 1;
-  cfg.attrs = attrs;
-  cfg.numAttrs = parts > 1 ? 2 : 1;
-  return (int)cudaLaunchKernelEx(&cfg, tiles_kernel<X, NT, GS>, tmap_codes, tmap_x, p);
+  return launch_blocks<L>(tiles_kernel<X, NT, GS>, p, THREADS, bytes, tmap_codes, tmap_x, stream);
 }
 template <typename X, int NT> int launch_groups(const Params &p, cudaStream_t stream) {
   if (p.group32 % 4 == 0) return launch_tiles<X, NT, 4>(p, stream);
@@ -583,6 +889,15 @@ template <typename X> int launch(Params p, cudaStream_t stream) {
                          p.c_row % 16 == 0 && p.c_row > 0 && p.x_row > 0 && p.s_row >= 0 && p.z_row >= 0 &&
                          reinterpret_cast<uintptr_t>(p.scales) % 4 == 0 && reinterpret_cast<uintptr_t>(p.zeros) % 4 == 0;
     if (aligned && p.inner <= (1LL << 30) && p.outer <= (1LL << 30) && (p.rows + 31) / 32 <= 65535) {
+      // Through tensor memory from 17 rows on, in groups of whole 128 columns: 24 us to 36 at
+      // 32 x 8192 -> 8192, 10.5 to 21 at 17 x 4096 -> 4096, equal at 32 x 1024 -> 4096 (below,
+      // the fragments' shorter start wins: 4.3 us to 6.0 at 256 columns); at 16 rows 23.9 to
+      // 22.8 and 144 to 148 (8192 -> 8192, 8192 -> 65536), at 9 x 4096 -> 4096 10.5 to 8.3.
+      if constexpr (sizeof(X) == 2)
+        if (p.rows > 16 && p.group32 % 4 == 0 && p.inner >= 1024) {
+          const int rc = launch_tall<X>(p, stream);
+          if (rc != tc::kNotEligible) return rc;
+        }
       const int rc = p.rows <= 8    ? launch_groups<X, 1>(p, stream)
                      : p.rows <= 16 ? launch_groups<X, 2>(p, stream)
                                     : launch_groups<X, 4>(p, stream);
