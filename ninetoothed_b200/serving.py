@@ -617,10 +617,12 @@ def int4_quantize(weight, group=128, symmetric=True):
     share a scale, in the weight's dtype, and without `symmetric` a zero point:
     element = (code - zero) * scale with codes from 0 to 15; symmetric groups are
     centred at 8 and have no zeros (None)."""
+    if weight.dim() != 2 or weight.dtype not in FLOAT_DTYPES:
+        raise TypeError(f"int4_quantize needs a matrix of float16, bfloat16 or float32; got {weight.dtype} {tuple(weight.shape)}.")
     outer, inner = weight.shape
     if group <= 0 or group % 32 or inner % group:
         raise ValueError(f"group must be a multiple of 32 that divides {inner}; got {group}.")
-    w = weight.float().view(outer, -1, group) if weight.is_contiguous() else weight.float().reshape(outer, -1, group)
+    w = weight.detach().float().reshape(outer, inner // group, group)
     if symmetric:
         scales = (w.abs().amax(dim=2) / 7).to(weight.dtype)
         zero = torch.full_like(scales, 8, dtype=torch.float32)

@@ -81,3 +81,16 @@ def test_quantized_weights_stand_for_the_weights():
         assert off.max() <= (0.5001 if symmetric else 1.0001)
     with pytest.raises(ValueError):
         programs.int4_quantize(w, 48)
+
+
+def test_quantized_weights_of_parameters_strides_and_no_elements():
+    w = torch.randn(64, 6)
+    want = programs.int4_quantize(w.t().contiguous(), 32, False)
+    got = programs.int4_quantize(torch.nn.Parameter(w).t(), 32, False)
+    assert all(torch.equal(a, b) and not a.requires_grad for a, b in zip(got, want))
+    for shape in ((0, 64), (5, 0), (0, 0)):
+        codes, scales, zeros = programs.int4_quantize(torch.zeros(shape), 32, False)
+        assert codes.shape == (shape[0], shape[1] // 2) and scales.shape == zeros.shape == (shape[0], shape[1] // 32)
+    for bad in (w[0], w[None], w.to(torch.int8), w.double()):
+        with pytest.raises(TypeError):
+            programs.int4_quantize(bad, 32)

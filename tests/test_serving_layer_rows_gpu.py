@@ -99,3 +99,16 @@ def test_two_streams_a_graph_and_other_kernels_between():
         outs.append([t.clone() for t in captured])
     assert all(torch.equal(p, q) for out in outs for p, q in zip(out, want))
     assert device_status() == 0
+
+
+def test_offsets_past_32_bits():
+    outer, inner = 1_100_000, 8192  # 4.5 GB of codes
+    codes = torch.zeros(outer, inner // 2, dtype=torch.uint8, device="cuda")
+    codes[-300:] = torch.randint(0, 256, (300, inner // 2), dtype=torch.uint8, device="cuda")
+    scales = torch.ones(outer, 64, dtype=torch.float16, device="cuda")
+    scales[-300:] = torch.rand(300, 64, device="cuda").half()
+    x = torch.randn(17, inner).half()
+    got = programs.int4_matmul(dev(x), codes, scales)[:, -300:].cpu()
+    want, size = product(x, codes[-300:].cpu(), scales[-300:].cpu(), None)
+    assert ((got.double() - want).abs() <= product_limit(want, size, torch.float16, inner, 128)).all()
+    assert device_status() == 0
