@@ -769,6 +769,17 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return y;
 }
 
+// A warp is done with an item's notes; false where a wait gave up.  A tile that has nothing
+// in its items would run through them all: a warp arrives for a slot's use only after all
+// arrived for the one before, so that a phase is one use by every warp, and what waits for
+// it by parity (here and in take_out) is never two phases off.
+__device__ __noinline__ bool leave_notes(uint32_t bar, int item, volatile int *abort_flag) {
+  if (!ptx::mbar_wait_warp(bar, ((uint32_t)(item / NOTE_SLOTS) & 1u) ^ 1u, abort_flag)) return false;
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(bar);
+  return true;
+}
+
 template <int DP>
 __device__ __forceinline__ void attend(const Control<DP> &c, const Problem &p, const Piece &piece, uint32_t tmem_base) {
   using L = Layout<DP>;
@@ -784,16 +795,6 @@ __device__ __forceinline__ void attend(const Control<DP> &c, const Problem &p, c
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(bar);
   };
-  // The warp is done with an item's notes.  A tile that has nothing in its items would run
-  // through them all: a warp arrives for a slot's use only after all arrived for the one
-  // before, so that a phase is one use by every warp, and what waits for it by parity
-  // (here and in take_out) is never two phases off.
-  auto leave_notes = [&](int item) {
-    const uint32_t bar = c.notes_free(item % NOTE_SLOTS);
-    if (!ptx::mbar_wait_warp(bar, ((uint32_t)(item / NOTE_SLOTS) & 1u) ^ 1u, c.abort_flag())) return false;
-    arrive_warp(bar);
-    return true;
-  };
   int s_turn = 0, o_turn = 0, block0 = 0, items = 0;  // blocks and items of this tile; the item's first block, the item
   each_item(p, piece, [&](const Item &e) {
     const int until = e.until_of(t, p.per_tile), item = items++, first_block = block0;
@@ -808,7 +809,7 @@ __device__ __forceinline__ void attend(const Control<DP> &c, const Problem &p, c
     float4 *stats = reinterpret_cast<float4 *>(part) + ROWS * (DP / 4) + t * BM + row;
     if (until <= e.from) {  // nothing to see in this share
       if (part && mine) *stats = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
-      return leave_notes(item);
+      return leave_notes(c.notes_free(item % NOTE_SLOTS), item, c.abort_flag());
     }
     const float factor = store_query<DP>(
         c, p, t, row,
@@ -821,10 +822,10 @@ __device__ __forceinline__ void attend(const Control<DP> &c, const Problem &p, c
     float m = -INFINITY, mo = -INFINITY, l = 0.f;
     for (int j = e.from; j < until; ++j) {
       const int block = first_block + j - e.from, slot = block % SCALE_SLOTS;
-      // (scores first: for a tile that is items ahead the slot's phase may be two back, which
-      // looks the same; with this block's scores there it is this block's)
-      if (!ptx::mbar_wait_warp(c.s_full(t), (uint32_t)s_turn & 1u, c.abort_flag())) return false;
+      // (for a tile that is items ahead the scales' phase may be two back, which looks the
+      // same: they are there with the scores, as a group's are written before its keys)
       if (!ptx::mbar_wait_warp(c.scale_full(slot), (uint32_t)(block / SCALE_SLOTS) & 1u, c.abort_flag())) return false;
+      if (!ptx::mbar_wait_warp(c.s_full(t), (uint32_t)s_turn & 1u, c.abort_flag())) return false;
       ++s_turn;
       ptx::tc_fence_after();
       const int seen = limit - j * BN;
@@ -973,7 +974,7 @@ __device__ __forceinline__ void attend(const Control<DP> &c, const Problem &p, c
     if (mine && part) *stats = make_float4(m, l, mo, 0.f);
     if (mine && !part && p.lse)
       p.lse[token * p.l_token + (int64_t)head * p.l_head] = l == 0.f ? -INFINITY : (m + log2_fast(l)) * kLn2;
-    return leave_notes(item);
+    return leave_notes(c.notes_free(item % NOTE_SLOTS), item, c.abort_flag());
   });
 }
 
