@@ -27,7 +27,9 @@
 // Both operands are fp16: a query row is scaled by a power of two to a largest element in
 // [2^14, 2^15), which leaves elements down to 2^-28 of it all their bits, and P is rounded
 // to fp16 (11 bits) relative to the largest weight p * value_scale of its row, 2^9 above
-// it, so neither scales far apart nor a long tail lose bits that count.
+// it, so neither scales far apart nor a long tail lose bits that count.  l is kept in two
+// floats.  O's fp32 sums in tensor memory take 16 keys a step, and a step loses what is
+// less than 2^-24 of the sum so far.
 //
 // Measured (32 query heads on 8 of 128 elements, e4m3, 64-token pages): two pieces of
 // 2048 tokens over 24576 2.07 ms, 763 TFLOP/s; one of 256 over 100000 0.55-0.57 ms, 769;
@@ -291,7 +293,8 @@ struct Layout {
   static constexpr int PIECE_OFF = BAR_OFF + 256;
   static constexpr int SCAN_OFF = PIECE_OFF + 64;                   // int64 [WARPS + 1]
   static constexpr int STAMP_OFF = SCAN_OFF + 8 * (WARPS + 1);      // int [NOTE_SLOTS][CONVERTERS]
-  static constexpr int SMEM_BYTES = STAMP_OFF + 4 * NOTE_SLOTS * CONVERTERS;
+  static constexpr int LOW_OFF = STAMP_OFF + 4 * NOTE_SLOTS * CONVERTERS;  // float [SOFTMAX_WARPS * 32]
+  static constexpr int SMEM_BYTES = LOW_OFF + 4 * SOFTMAX_WARPS * 32;
   static_assert(sizeof(Piece) <= 64, "the piece's place");
   static_assert(SMEM_BYTES <= 232448, "shared memory of a CTA");
   // a part in the workspace: o [DP / 4][ROWS] float4, then (m, l, mo) [ROWS] float4
@@ -791,6 +794,8 @@ __device__ __forceinline__ void attend(const Control<DP> &c, const Problem &p, c
   const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
   const uint32_t tmem_s = tmem_base + (uint32_t)(t * BN) + lane_base;
   const uint32_t tmem_o = tmem_base + (uint32_t)(TILES * BN + t * 128) + lane_base;
+  // what the row's sum of weights has beside l; a register for it would spill others
+  volatile float *l_low = reinterpret_cast<volatile float *>(c.smem + L::LOW_OFF) + (warp - 1 - CONVERTERS) * 32 + lane;
   auto arrive_warp = [&](uint32_t bar) {
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(bar);
@@ -820,6 +825,7 @@ __device__ __forceinline__ void attend(const Control<DP> &c, const Problem &p, c
     const int sure = min(e.limit0 + t * p.per_tile, e.keys);         // that all rows see
 
     float m = -INFINITY, mo = -INFINITY, l = 0.f;
+    *l_low = 0.f;
     for (int j = e.from; j < until; ++j) {
       const int block = first_block + j - e.from, slot = block % SCALE_SLOTS;
       // (for a tile that is items ahead the scales' phase may be two back, which looks the
@@ -830,7 +836,7 @@ __device__ __forceinline__ void attend(const Control<DP> &c, const Problem &p, c
       ptx::tc_fence_after();
       const int seen = limit - j * BN;
       bool move_o;
-      float alpha_o;
+      float alpha_o, near = 0.f;  // near: the block's part of the sum of weights
       auto take_block = [&](auto with_mask) {
       constexpr bool MASKED = decltype(with_mask)::value;
       // 32 scores at a time, read twice: 128 would fill the registers.  The next are on
@@ -882,12 +888,14 @@ __device__ __forceinline__ void attend(const Control<DP> &c, const Problem &p, c
       move_o = top_w > mo + kLead;
       alpha_o = move_o ? exp2_fast(mo - top_w) : 1.f;
       if (move) {
-        l *= exp2_fast(m - top_s);
+        const float f = exp2_fast(m - top_s);
+        l *= f;
+        *l_low *= f;
         m = top_s;
       }
       if (move_o) mo = top_w;
       // P = 2^(s - m + shift) with the group's shift = log2 value_scale + m - mo + kRise, and
-      // l takes a group's sum of them times 2^-shift.  Where a group's values are so small
+      // near takes a group's sum of them times 2^-shift.  Where a group's values are so small
       // that its P would leave fp32, P is kept at 2^kLeastShift: too large, but nothing beside the others.
       const float ref = reference(m), rise = ref - reference(mo) + kRise;
       each_quarter([&](int quarter, float (&s)[32]) {
@@ -910,7 +918,7 @@ __device__ __forceinline__ void attend(const Control<DP> &c, const Problem &p, c
             sum[(2 * x + 1) & 3] += p1;
             packed[k * 8 + x] = paged::half2_bits(p0, p1);
           }
-          l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), exp2_fast(-shift), l);
+          near = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), exp2_fast(-shift), near);
         }
         // (P's 16 columns lie among scores that were read before)
         ptx::tmem_st_32x32b_x16(tmem_s + (uint32_t)(quarter * 16), packed);
@@ -933,10 +941,17 @@ __device__ __forceinline__ void attend(const Control<DP> &c, const Problem &p, c
       ptx::tmem_st_wait();
       ptx::tc_fence_before();
       arrive_warp(c.p_full(t));
+      // l + near, and what fp32 cuts off it: beside a weight of 1, 2^18 weights of 2^-28 were
+      // lost 16 at a time (1e-3 of the lse).  (While the MMAs run it takes no time: 2024 us
+      // for two pieces of 2048 tokens over 24576, 2018 with one sum.)
+      const float both = __fadd_rn(l, near), added = __fsub_rn(both, l);
+      *l_low += __fadd_rn(__fsub_rn(l, __fsub_rn(both, added)), __fsub_rn(near, added));
+      l = both;
     }
     if (!ptx::mbar_wait_warp(c.o_done(t), (uint32_t)o_turn & 1u, c.abort_flag())) return false;
     ++o_turn;
     ptx::tc_fence_after();
+    l += *l_low;
     // (mo: -inf where all values stand for 0)
     const float f = l == 0.f ? 0.f : exp2_fast(reference(mo) - reference(m) - kRise) / l;
 #pragma unroll 1
