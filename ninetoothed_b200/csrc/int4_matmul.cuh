@@ -506,7 +506,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmap_codes, const __grid_consta
           joined[(wk * L::M + m) * L::PITCH + row] = acc[r][t][e];
         }
     join_sums<L>(p, joined, base + p.join, n0, m0, m_count, part);
-    if (*abort_flag) break;  // (read by all after the same barrier)
+    if (any_of_warps(*abort_flag)) break;  // (a warp ahead may set it at any time: one answer for all)
   }
   __syncthreads();
   if (*abort_flag) settle(bar0, p.ring);
