@@ -498,7 +498,8 @@ int nt_b200_rms_norm(const NtB200RmsNormArgs *args, void *stream);
  * output[m, n] = input_scale[m] * sum_k input[m, k] (q[n, k] - z[n, k / group])
  * scales[n, k / group] for input [rows, inner] and 4-bit weights q, two a byte of
  * `codes` [outer, inner / 2], the even k in the low half.  z = 8 where `zeros` is
- * null, else the low four bits of zeros (uint8) [outer, inner / group]; scales
+ * null, else zeros (uint8) [outer, inner / group], 0 to 63 (larger ones are recorded as
+ * NT_B200_ERR_INDEX_OUT_OF_RANGE, and what they give is not specified); scales
  * [outer, inner / group] of scales_dtype; input_scale (fp32, [rows]) may be null.
  * `group` is a multiple of 32 and divides inner.  Products and sums are fp32, the
  * result is rounded once to output_dtype.  dtype: FLOAT16, BFLOAT16, FLOAT32,

@@ -74,6 +74,14 @@ __device__ __forceinline__ void store_any(void *y, int64_t at, int dtype, float 
 }
 __host__ __device__ constexpr int float_size(int dtype) { return dtype == NT_B200_FLOAT32 ? 4 : 2; }
 
+// Zero points are whole numbers up to 63, which both unpackings take off without rounding
+// (formats that store them less one hold 16); larger ones are an error.  `seen`: a thread's,
+// joined by or.
+constexpr uint32_t MOST_ZERO = 63;
+__device__ __forceinline__ void check_zeros(uint32_t seen) {
+  if (seen > MOST_ZERO) record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
+}
+
 // ---------------------------------------------------------------- any layout
 // A warp a weight row and 8 rows of x: 32-bit floats, strides off the 16-byte grid.
 template <typename X>
@@ -85,11 +93,14 @@ __global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ Param
   const X *x = static_cast<const X *>(p.x) + m0 * p.x_row;
   const int count = (int)(p.rows - m0 < M ? p.rows - m0 : M);
   float sum[M] = {};
+  uint32_t seen = 0;
   for (int64_t b = lane; b < p.inner / 2; b += 32) {
     const int64_t g = 2 * b / p.group;
     const uint8_t code = p.codes[n * p.c_row + b * p.c_col];
     const float s = any_float(p.scales + (n * p.s_row + g * p.s_col) * float_size(p.scale_dtype), p.scale_dtype);
-    const float z = p.zeros ? (float)(p.zeros[n * p.z_row + g * p.z_col] & 15) : 8.f;
+    const uint32_t zero = p.zeros ? p.zeros[n * p.z_row + g * p.z_col] : 8u;
+    seen |= zero;
+    const float z = (float)zero;
     const float w0 = ((float)(code & 15) - z) * s, w1 = ((float)(code >> 4) - z) * s;
 #pragma unroll
     for (int m = 0; m < M; ++m)
@@ -98,6 +109,7 @@ __global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ Param
         sum[m] = fmaf(to_f(at[0]), w0, fmaf(to_f(at[p.x_col]), w1, sum[m]));
       }
   }
+  check_zeros(seen);
 #pragma unroll
   for (int m = 0; m < M; ++m) {
 #pragma unroll
@@ -403,6 +415,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmap_codes, const __grid_consta
     const int64_t n0 = (int64_t)unit * L::R;
     Group stage_at = stage0, slice_at = slice0;
     float acc[RT][NT][4] = {};
+    uint32_t seen = 0;
     // ---- a warp's slice of each stage: 16 RT rows, WSTEPS steps of 32 columns
     for (int s = first; s < last; ++s) {
       if (copies) fill();
@@ -422,7 +435,8 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmap_codes, const __grid_consta
 #pragma unroll
           for (int k = 0; k < SCALES; ++k) {
             const uint32_t nth = now.index - stage_at.index;
-            const uint32_t zero = p.zeros ? zeros[nth] & 15u : 8u;
+            uint32_t zero = 8;
+            if (p.zeros) seen |= zero = zeros[nth];
             factors[k * 16 * RT + lane] =
                 Factor{value(from + nth * scale_size), Codes<F>::zero_low(zero), Codes<F>::zero_high(zero), 0u};
             now.advance(0, GS, p.group32);
@@ -492,6 +506,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmap_codes, const __grid_consta
         phase ^= 1u;
       }
     }
+    if (n0 + wr * 16 * RT + lane < p.outer) check_zeros(seen);  // (nothing was copied for other rows)
     if (unit + unit_step >= units) allow_dependent_launch();
 
     // ---- the warps' sums, [WK][M][R + 4], then the cluster's
@@ -678,7 +693,8 @@ tall_kernel(const __grid_constant__ CUtensorMap tmap_codes, const __grid_constan
         good = ptx::mbar_wait_warp(full(slot), phase, abort_flag);
         if (!good) break;
         const float next_scale = value(raw);
-        const uint32_t z0 = Codes<F>::zero_low(zero & 15u), z1 = Codes<F>::zero_high(zero & 15u);
+        const uint32_t z0 = Codes<F>::zero_low(zero), z1 = Codes<F>::zero_high(zero);
+        check_zeros(zero);
         fetch(s + 1);
         if (s > first) {  // the weights before were read, and their sums are there
           good = ptx::mbar_wait_warp(d_full(wg), (turn - 1) & 1u, abort_flag);

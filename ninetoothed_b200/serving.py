@@ -690,7 +690,8 @@ def int4_matmul(input, codes, scales, zeros=None, input_scale=None):
     weights (code - zero) * scale: `codes` uint8 [outer, inner / 2], two a byte with
     the even element in the low half; `scales` [outer, groups], each for inner /
     groups neighbouring elements (a multiple of 32); `zeros` uint8 [outer, groups],
-    0 to 15, or 8 throughout (`int4_quantize` makes all three).  Made for the few
+    0 to 63, or 8 throughout (`int4_quantize` makes all three); larger zeros are
+    an error that `device_status` tells of.  Made for the few
     rows of a decoding step: every 32 rows read the weights once.
 
     The input is float16, bfloat16 or float32, and so is the output; or
