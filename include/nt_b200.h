@@ -450,7 +450,9 @@ int64_t nt_b200_prompt_attention_workspace_size(int64_t query_tokens, int64_t ba
  * (probabilities rounded to fp16 there) for head_dim up to 128, up to 128 query heads to
  * a key/value head and a positive scale; the rest, FLOAT32 and head_dim up to 256, on
  * CUDA cores.  Tokens that belong to no sequence are not written, nor those of a sequence
- * whose offsets are out of order or leave the tensors.  `workspace`: 16-byte aligned
+ * whose offsets are out of order or leave the tensors (recorded as
+ * NT_B200_ERR_INDEX_OUT_OF_RANGE; on CUDA cores, which search the offsets, tokens of other
+ * sequences may then be left out too).  `workspace`: 16-byte aligned
  * device memory of nt_b200_chunk_attention_workspace_size() bytes (the current
  * device's), for this call alone.
  */

@@ -80,14 +80,16 @@ template <typename T, typename C>
 __global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ Problem p) {
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= p.tokens * p.heads) return;
+  // All sequences' offsets are looked at: among ones out of order the search below may miss
+  // sequences, whose tokens would be left out without a word.
+  for (int64_t i = row * 32 + (threadIdx.x & 31); i < p.batch; i += p.tokens * p.heads * 32)
+    if (p.offsets[i] < 0 || p.offsets[i + 1] < p.offsets[i] || p.offsets[i + 1] > p.tokens)
+      record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
   const int64_t token = row / p.heads;
   const int h = (int)(row % p.heads);
   const int64_t b = paged::warp_search(p.batch, token, [&](int64_t i) { return p.offsets[i]; });
   const int64_t q0 = p.offsets[b], n = p.offsets[b + 1] - q0;
-  if (q0 < 0 || n < 0 || q0 + n > p.tokens) {
-    record_error(NT_B200_ERR_INDEX_OUT_OF_RANGE);
-    return;
-  }
+  if (q0 < 0 || n < 0 || q0 + n > p.tokens) return;
   if (token < q0 || token >= q0 + n) return;
   const T *q = static_cast<const T *>(p.query) + token * p.q_token + h * p.q_head;
   T *out = static_cast<T *>(p.out) + token * p.o_token + h * p.o_head;
