@@ -584,7 +584,10 @@ rms_norm_kernel = Kernel(
 )
 
 
-def rms_norm(input, weight, residual=None, eps=1e-6, code_dtype=None, group=None):
+_NOT_GIVEN = object()
+
+
+def rms_norm(input, weight, residual=None, eps=1e-6, code_dtype=_NOT_GIVEN, group=None):
     """Root-mean-square norm of the rows of `input` [rows, width]: with t = input
     + residual (or input), t / sqrt(mean(t^2) + eps) * weight (`weight`: [width],
     in the input's dtype or float32).
@@ -595,7 +598,15 @@ def rms_norm(input, weight, residual=None, eps=1e-6, code_dtype=None, group=None
     shorter; one for the row by default).  E4M3 scales are the least power of two
     that brings a group's largest element to 448 or less, int8 ones that element /
     127.  With a `residual` the last of the outputs is the sum t in the input's
-    dtype, the next residual; the norm is that of t as it is stored."""
+    dtype, the next residual; the norm is that of t as it is stored.
+
+    `code_dtype` None is no code_dtype: a caller that switches the 8-bit output off so
+    leaves `group` as it is, where it has no meaning.  A `group` with no word of
+    `code_dtype` is refused."""
+    if code_dtype is _NOT_GIVEN or code_dtype is None:
+        if code_dtype is _NOT_GIVEN and group is not None:
+            raise TypeError("rms_norm has groups with an 8-bit output only.")
+        code_dtype = group = None
     result = _bound("rms_norm", input, weight, residual, eps, code_dtype, group)
     if result is not None:
         return result
