@@ -201,8 +201,7 @@ def _own_norm(s):
 
     case = s["case"]
     return _named(case, programs.rms_norm(s["input"], s["weight"], residual=s["residual"], eps=s["eps"],
-                                          code_dtype=CODES.get(case["code"]),
-                                          group=(case["group"] or None) if case["code"] else None))
+                                          code_dtype=CODES.get(case["code"]), group=case["group"] or None))
 
 
 def _own_int4(s):
