@@ -446,7 +446,8 @@ int64_t nt_b200_prompt_attention_workspace_size(int64_t query_tokens, int64_t ba
  * outside the pool.  With s = scale * (q . k) over the tokens seen, output = softmax(s)
  * v and, where `lse` is not null, lse [tokens, heads] = ln sum exp(s) (fp32); a query
  * that sees nothing gets 0 and -inf.  Scores, softmax and sums are fp32; the cache's
- * scales must not be negative.  FLOAT16 and BFLOAT16 queries run on tcgen05 tensor cores
+ * scales must not be negative, and a value scale that is not finite makes output and, on
+ * tensor cores, lse of who sees it NaN.  FLOAT16 and BFLOAT16 queries run on tcgen05 tensor cores
  * (probabilities rounded to fp16 there) for head_dim up to 128, up to 128 query heads to
  * a key/value head and a positive scale; the rest, FLOAT32 and head_dim up to 256, on
  * CUDA cores.  Tokens that belong to no sequence are not written, nor those of a sequence
@@ -508,7 +509,8 @@ int nt_b200_rms_norm(const NtB200RmsNormArgs *args, void *stream);
  * FLOAT8_E4M3FN or INT8; scales and output: FLOAT16, BFLOAT16, FLOAT32.  Tensor
  * cores take all but FLOAT32 inputs where element strides are 1, rows of input and
  * codes (and both bases) on the 16-byte grid and the bases of scales and zeros on
- * the 4-byte one; the rest runs on CUDA cores.
+ * the 4-byte one, for up to 65535 * 32 rows; the rest runs on CUDA cores, for up to
+ * 65535 * 8.
  */
 typedef struct NtB200Int4MatmulArgs {
     const void *input, *codes, *scales, *zeros; /* zeros may be null */
