@@ -32,9 +32,9 @@
 // less than 2^-24 of the sum so far.
 //
 // Measured (32 query heads on 8 of 128 elements, e4m3, 64-token pages): two pieces of
-// 2048 tokens over 24576 2.07 ms, 763 TFLOP/s; one of 256 over 100000 0.55-0.57 ms, 769;
-// eight of up to 512 over up to 8192 0.33 ms.  Bound by a block's way through a tile, 3.3 us:
-// the softmax's 3500 cycles with 16 warps at 0.42 of the issue rate, then P V and the next
+// 2048 tokens over 24576 2.03 ms, 780 TFLOP/s; one of 256 over 100000 0.55-0.58 ms, 720-760;
+// eight of up to 512 over up to 8192 0.32 ms.  Bound by a block's way through a tile, 3.2 us:
+// the softmax's 3500 cycles with 16 warps at 0.43 of the issue rate, then P V and the next
 // Q K^T, 850 each where 512 are dense; the seven converting warps wait half of their time.
 // Measured and not kept: 3 and 5 converting warps (2.74 and 2.16 ms where 7 took 2.10);
 // two buffers of scores of 64-key blocks, so that Q K^T runs ahead (2.79 ms: Q is read
@@ -68,10 +68,10 @@ struct Problem : paged::Attention {
 
 constexpr int BM = 128, BN = 128, TILES = 2, ROWS = TILES * BM;  // rows of a tile, keys of a block
 // What a unit's start and end (its queries, its output) count in the line, in key
-// blocks: 8 pieces of up to 512 tokens over up to 8192 took 357 us at 2, 336 at 3, 321 at
-// 5; units of few rows, 6 pieces of up to 300 over up to 4000, 73, 74 and 76.  Steps of a
-// piece at least: 4 pieces of up to 16 tokens over up to 1000 took 34 us at 8, 27 at 4, 23
-// at 2.
+// blocks: 8 pieces of up to 512 tokens over up to 8192 took 354 us at 2, 335 at 3, 324 at
+// 4, 317 at 5; units of few rows, 6 pieces of up to 300 over up to 4000, 75.2, 75.5, 75.9
+// and 76.5; 4 of up to 16 over up to 1000 22.6, 23.6, 22.9 and 23.7.  Steps of a piece at
+// least: the last took 32 us at 8, 26 at 4, 23 at 2.
 constexpr int UNIT_STEPS = 4, LEAST_STEPS = 2;
 
 // ---------------------------------------------------------------- any layout
@@ -100,7 +100,8 @@ __global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ Probl
 // ---------------------------------------------------------------- the line
 // sum of floor((a i + b) / m) for i in [0, n), by the steps of Euclid's algorithm
 // (a, b >= 0): pairs of whole numbers under a line, counted again with the axes
-// exchanged.
+// exchanged (floor sums and their reciprocity: Graham, Knuth and Patashnik, Concrete
+// Mathematics, 3.5).
 __device__ __forceinline__ int64_t floor_sum(int64_t n, int32_t m, int32_t a, int64_t b) {
   int64_t sum = 0;
   while (n > 0) {
@@ -280,8 +281,8 @@ constexpr int TMEM_COLS = 512, SCALE_SLOTS = 4, NOTE_SLOTS = 3;
 
 // What a group's 16 keys share.
 struct alignas(16) GroupScale {
-  float key, add;           // s = raw * key * (the row's factor) + add (-inf: a page outside the pool)
-  float value, log2_value;  // the value scale
+  float key, add;  // s = raw * key * (the row's factor) + add (-inf: a page outside the pool)
+  float unused, log2_value;
 };
 
 template <int DP>  // head_dim padded to 64 or 128
@@ -568,7 +569,7 @@ __device__ __forceinline__ void convert(const Control<DP> &c, const Problem &p, 
     const float scale = value_scale;
     if (lane == 0) {
       const int block = g.ring / 2 % SCALE_SLOTS;
-      GroupScale s{p.scale * key_scale, 0.f, scale, log2_fast(scale)};
+      GroupScale s{p.scale * key_scale, 0.f, 0.f, log2_fast(scale)};
       if (g.page < 0) s = GroupScale{0.f, -INFINITY, 0.f, -INFINITY};
       c.scales(block)[g.at % GROUPS] = s;
       ptx::mbar_arrive(c.scale_full(block));

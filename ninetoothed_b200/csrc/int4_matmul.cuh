@@ -3,8 +3,9 @@
 // with two codes a byte, the even element in the low half, and a zero point of 8
 // where none are given.
 //
-// Bound by memory: a weight is half a byte and serves every row of x, 4 flops a
-// byte and row.  The weights go through shared memory once; x comes from L2.
+// A weight is half a byte and serves every row of x, 4 flops a byte and row: reading the
+// weights is the floor.  They go through shared memory once for every 8, 16 or 32 rows of
+// x; x comes from L2.
 //
 // Codes become 16-bit floats without rounding (their bits set into the mantissa
 // of 1024, or of 128 in bfloat16, and the zero point taken off, which leaves a
@@ -26,12 +27,12 @@
 // the columns and join their sums through distributed shared memory, always in the same
 // order.
 //
-// Measured (codes' bytes a second): 4096 x 4096 with one bfloat16 row 6.8 us, launch,
+// Measured (codes' bytes a second): 4096 x 4096 with one bfloat16 row 7.0 us, launch,
 // first copies and join for the most part; 10240 -> 4099 with 5 float16 rows, groups of 64
-// with zero points 13.8 us; 8192 x 8192 with 32 bfloat16 rows 24 us (weights in tensor
-// memory, see tall_kernel; 36 us with these steps); 8192 -> 65536 with 16 E4M3 rows,
-// groups of 32 with zero points 166 us, 1.6 TB/s.  Bound by issue, not by
-// memory: a warp takes about 600 instructions for 4096 codes, half of them to unpack, and
+// with zero points 14.0 us; 8192 x 8192 with 32 bfloat16 rows 24.7 us (weights in tensor
+// memory, see tall_kernel; in groups of 64 or of 8-bit rows, with these steps, 35); 8192 ->
+// 65536 with 16 E4M3 rows, groups of 32 with zero points 166 us, 1.6 TB/s.  Bound by issue,
+// not by the floor: a warp takes about 600 instructions for 4096 codes, half of them to unpack, and
 // the copies alone take 71 us of the last.  (With a warp of its own for the copies the
 // register file holds 96 a thread and the products spill: 47 us for the third against 36.)
 #pragma once
@@ -535,7 +536,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmap_codes, const __grid_consta
 // registers, so that two blocks an SM fit.  A block's two warpgroups take the halves of a
 // stage's 256 columns, which share a scale each: groups of 128 columns and their multiples.
 //
-// 8192 x 8192 with 32 bfloat16 rows: 24 us (36 with fragments), bound by latency: a
+// 8192 x 8192 with 32 bfloat16 rows: 24.7 us (36 with fragments), bound by latency: a
 // warpgroup's unpacking, MMAs and sums follow one another.  Without the unpacking 19 us,
 // without the scales' loads 23.  Tried: 64 columns at a time in two buffers each, the sums
 // taken while the next MMAs run, 29 us (twice the stores and loads of tensor memory, and
@@ -779,7 +780,8 @@ template <typename L, typename K>
 int launch_blocks(K kernel, Params &p, int threads, int bytes, const CUtensorMap &tmap_codes, const CUtensorMap &tmap_x,
                   cudaStream_t stream) {
   const int64_t row_blocks = (p.outer + L::R - 1) / L::R, m_blocks = (p.rows + L::M - 1) / L::M;
-  // Parts of the columns: as many as leave the grid in two blocks an SM.
+  // Parts of the columns: as many as leave the grid in two blocks an SM.  (tiles_kernel with
+  // 32 rows of x fits once: it goes through such a grid in two turns.)
   const int64_t room = 2 * (int64_t)sm_count();
   int parts = 1;
   while (parts < 8 && row_blocks * m_blocks * parts * 2 <= room && p.stages >= 2 * parts) parts *= 2;

@@ -702,8 +702,11 @@ def int4_matmul(input, codes, scales, zeros=None, input_scale=None):
     the even element in the low half; `scales` [outer, groups], each for inner /
     groups neighbouring elements (a multiple of 32); `zeros` uint8 [outer, groups],
     0 to 63, or 8 throughout (`int4_quantize` makes all three); larger zeros are
-    an error that `device_status` tells of.  Made for the few
-    rows of a decoding step: every 32 rows read the weights once.
+    an error that `device_status` tells of.  Made for the few rows of a decoding
+    step: on tensor cores up to 8, up to 16, or else every 32 rows read the weights
+    once.  float32 inputs and strides off the 16-byte grid run on CUDA cores, where
+    every 8 do, 8 to 24 times as long; from some 150 rows on `matmul` with weights of
+    16 bits is the faster one.
 
     The input is float16, bfloat16 or float32, and so is the output; or
     float8_e4m3fn or int8 with `input_scale` fp32 [rows] or [rows, 1] (`rms_norm`'s
